@@ -200,9 +200,6 @@ def _prepare_logprobs(case, dev, g, normal):
     s = {"case": case, "logits": x, "tokens": tokens,
          "logprob": torch.empty(rows, device=dev), "entropy": torch.empty(rows, device=dev),
          "top_logprob": torch.empty(rows, top, device=dev), "top_id": torch.empty(rows, top, dtype=torch.int64, device=dev)}
-    if own:
-        import leafcutterllm_b200 as lc
-        s["workspace"] = torch.empty(lc.token_logprobs_workspace(x, top), dtype=torch.uint8, device=dev)
     return s
 
 
@@ -225,7 +222,7 @@ def run(s):
         return _attention(s)
     if own:
         import leafcutterllm_b200 as lc
-        out = lc.token_logprobs_dev(s["logits"], s["tokens"], s["logprob"], s["entropy"], s["top_logprob"], s["top_id"], workspace=s["workspace"])
+        out = lc.token_logprobs_dev(s["logits"], s["tokens"], s["logprob"], s["entropy"], s["top_logprob"], s["top_id"])
     else:
         out = _logprobs(s)
     return dict(zip(("logprob", "entropy", "top_logprob", "top_id"), out))
