@@ -137,6 +137,80 @@ int32_t lc_attention_decode_dev(const float* q_dev, const void* k_pool_dev, cons
 int32_t lc_attention_decode_static(const float* q_dev, const void* k_pool_dev, const void* v_pool_dev, const int32_t* page_table_dev,
                                    int32_t n_pages, int32_t ctx_len, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                    int32_t page_tokens, int32_t kv_f32, float* out_dev);
+/* ---- A key/value cache in 8 bits (no counterpart in the reference, whose cache is f16: rust/src/cache/mod.rs:33-61) ----
+ * The pools hold integers of 8 bits, [page][kv head][page_tokens][head_dim], 16-byte aligned; the scales are f32, [page][kv head],
+ * one for the keys and one for the values.  A cached element is its integer times the scale of its page and head.
+ * page_tokens: 16, 32, 64, 128 or 256; head_dim: a multiple of 16, 256 at most; the pools may pass 2^32 bytes. */
+typedef struct lc_kv8_cache {
+    void* k_dev;
+    void* v_dev;
+    float* k_scale_dev;
+    float* v_scale_dev;
+    int32_t n_pages, n_kv_heads, page_tokens, head_dim;
+} lc_kv8_cache;
+/* Which positions of which sequences the rows of a call are.  Row r of sequence i, row_start[i] <= r < row_start[i + 1], stands at
+ * position ctx[i] + (r - row_start[i]); its page is page_table[i][position / page_tokens].  Everything is read on the device when the
+ * kernels run, so a captured graph follows what these arrays hold when it is replayed.  Sequences may have no rows, and row_start[0]
+ * may be positive; rows of a tensor outside all sequences are neither read nor written.
+ * max_rows: the most rows that a sequence is expected to have; it chooses between kernels and sizes their grids, and a call whose
+ * sequences have more is slower, not wrong.
+ * status_dev (may be NULL): a word that a call raises to i + 1, for the highest such i, where sequence i cannot be served: its row_start is
+ * not ascending within the call's rows (its rows are left alone), or its positions leave the table or a page that it needs is not
+ * in 0 .. n_pages - 1 (appends skip that page, reads and attention give NaN in those rows).  No call clears it.
+ * n_seqs: 4096 at most. */
+typedef struct lc_kv8_rows {
+    const int32_t* page_table_dev; /* [n_seqs][table_width] */
+    const int32_t* ctx_dev;        /* [n_seqs] */
+    const int32_t* row_start_dev;  /* [n_seqs + 1] */
+    int32_t* status_dev;
+    int32_t n_seqs, table_width, max_rows, reserved;
+} lc_kv8_rows;
+/* These calls take device pointers of ONE device, which need not be the current one, and queue on `stream` (a cudaStream_t of that
+ * device; cudaStreamLegacy and cudaStreamPerThread are accepted as such), or on the library's stream of that device where it is NULL.  They neither wait nor
+ * allocate, so they can be captured into a graph.  typ: LC_TYPE_F32, LC_TYPE_F16 or LC_TYPE_BF16, of all activations of the call; n_rows: rows
+ * of its tensors; a stride is the distance between two rows in elements (heads and dims of a row are contiguous).
+ *
+ * Rotation table of a rotary embedding over the first rot_dim dims of a head, pairs (d, d + rot_dim / 2) as lc_rope has them: out[d] is the
+ * fraction of a full turn per position, theta^(-2 d / rot_dim) / (2 pi), in units of 2^-64.  Host arithmetic; a caller with frequencies of its
+ * own fills such a table itself.  Positions times entries wrap around, so far positions lose nothing. */
+int32_t lc_rope_turns(double theta, int32_t rot_dim, uint64_t* out);
+/* Appends rows of keys and values, each [n_rows][n_kv_heads][head_dim], at their positions, the keys rotated by turns_dev (rot_dim / 2
+ * entries; rot_dim 0: no rotation).  Rotations and quotients are taken in 64 bits.  Per page and head that receives rows: the scale becomes the largest finite
+ * magnitude among the new rows / 127 (rounded to f32) or, where the page already holds rows of the sequence, the larger of that and the scale before; if it grows,
+ * the integers of the earlier rows are rounded once more, to the new scale.  New integers are round(x / scale) to the nearest even, infinities
+ * become +-127 and NaN 0 (all 0 where the scale is 0).  Slots behind the last row keep what they hold.
+ * q_dev (may be NULL), [n_rows][n_heads][head_dim], is rotated likewise into q_out_dev, which may be q_dev.
+ * A page that receives rows in a call must belong to one sequence of it; pages that several sequences share may only be read. */
+int32_t lc_kv8_append_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, const void* k_dev,
+                          int64_t k_stride, const void* v_dev, int64_t v_stride, const void* q_dev, int64_t q_stride, void* q_out_dev,
+                          int64_t q_out_stride, int32_t n_heads, const uint64_t* turns_dev, int32_t rot_dim, void* stream);
+/* The cached rows as values (integer * scale, rounded to typ): k_out_dev and v_out_dev are [n_rows][n_kv_heads][head_dim]; either may be NULL. */
+int32_t lc_kv8_read_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, void* k_out_dev,
+                        int64_t k_stride, void* v_out_dev, int64_t v_stride, void* stream);
+/* Attention of the rows over the cache (the core of rust/src/inference/attention.rs:69-113, as lc_attention_decode_dev): each row of q_dev
+ * [n_rows][n_heads][head_dim], already rotated, attends to the positions up to its own, which the cache already holds (append first), and
+ * with window > 0 only to the last `window` of them.  Scores are q . k * scale (0: 1 / sqrt(head_dim)).  Queries of any finite size are taken.
+ * The workspace is the caller's: lc_attention_kv8_workspace says how many bytes, for any contexts and any rows of at most
+ * these arguments' sizes; it needs no initial value and keeps nothing between calls.  Calls that may run at the same time (graphs that may be replayed at the
+ * same time among them) need a workspace each. */
+int32_t lc_attention_kv8_workspace(const lc_kv8_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, int32_t n_heads,
+                                   size_t* out_bytes);
+int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, const void* q_dev,
+                             int64_t q_stride, int32_t n_heads, float scale, int32_t window, void* out_dev, int64_t out_stride,
+                             void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* Log probabilities (no counterpart in the reference).  For each row of logits [rows][vocab] (stride elements apart): logprob[r] = log softmax of the row at tokens[r]
+ * (NaN where tokens[r] is outside 0 .. vocab - 1), entropy[r] in nats, and the `top` (0 .. 32, vocab at most) likeliest tokens with their log probabilities,
+ * the larger logit first, equal logits by the lower index (-0 equals 0).  logprob, entropy, top_logprob / top_id may be NULL (tokens with logprob, and the last
+ * two together).  Logits of minus infinity have probability 0; a row of nothing else has logprob and top_logprob of minus infinity and entropy 0.  A row
+ * with a NaN or plus infinity has NaN everywhere and top_id -1.  Sums are in 64 bits.
+ * The _dev form: streams and types as above. */
+int32_t lc_token_logprobs(const float* logits, size_t rows, size_t vocab, const int64_t* tokens, int32_t top, float* logprob,
+                          float* entropy, float* top_logprob, int64_t* top_id);
+int32_t lc_token_logprobs_dev(uint32_t typ, const void* logits_dev, int32_t rows, int32_t vocab, int64_t stride, const int64_t* tokens_dev,
+                              int32_t top, float* logprob_dev, float* entropy_dev, float* top_logprob_dev, int64_t* top_id_dev,
+                              void* stream);
+
 /* CUDA-event stopwatch on the library's stream: begin, queue work, end -> milliseconds. */
 int32_t lc_timer_begin(void);
 int32_t lc_timer_end(float* out_ms);

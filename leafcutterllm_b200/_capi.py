@@ -48,6 +48,16 @@ class GgufReport(C.Structure):
                 ("total_blocks_checked", C.c_uint64), ("total_bad_blocks", C.c_uint64), ("config", ModelConfig)]
 
 
+class Kv8CacheStruct(C.Structure):
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("k_scale_dev", C.c_void_p), ("v_scale_dev", C.c_void_p),
+                ("n_pages", C.c_int32), ("n_kv_heads", C.c_int32), ("page_tokens", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class Kv8RowsStruct(C.Structure):
+    _fields_ = [("page_table_dev", C.c_void_p), ("ctx_dev", C.c_void_p), ("row_start_dev", C.c_void_p), ("status_dev", C.c_void_p),
+                ("n_seqs", C.c_int32), ("table_width", C.c_int32), ("max_rows", C.c_int32), ("reserved", C.c_int32)]
+
+
 TOKEN_CB = C.CFUNCTYPE(None, C.c_int64, C.c_void_p)
 
 _f = C.POINTER(C.c_float)
@@ -56,6 +66,7 @@ _vp = C.c_void_p
 _i32 = C.c_int32
 _u32 = C.c_uint32
 _u64 = C.c_uint64
+_i64 = C.c_int64
 
 # name -> (restype, argtypes); every name here is declared in include/leafcutter_b200.h
 SIGNATURES = {
@@ -88,6 +99,13 @@ SIGNATURES = {
     "lc_dequantize_dev": (_i32, [_u32, _vp, _sz, _vp]),
     "lc_attention_decode_dev": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
     "lc_attention_decode_static": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "lc_rope_turns": (_i32, [C.c_double, _i32, _vp]),
+    "lc_kv8_append_dev": (_i32, [_vp, _vp, _u32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp]),
+    "lc_kv8_read_dev": (_i32, [_vp, _vp, _u32, _i32, _vp, _i64, _vp, _i64, _vp]),
+    "lc_attention_kv8_workspace": (_i32, [_vp, _vp, _u32, _i32, _i32, C.POINTER(_sz)]),
+    "lc_attention_kv8_dev": (_i32, [_vp, _vp, _u32, _i32, _vp, _i64, _i32, C.c_float, _i32, _vp, _i64, _vp, _sz, _vp]),
+    "lc_token_logprobs": (_i32, [_vp, _sz, _sz, _vp, _i32, _vp, _vp, _vp, _vp]),
+    "lc_token_logprobs_dev": (_i32, [_u32, _vp, _i32, _i32, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
     "lc_timer_begin": (_i32, []),
     "lc_timer_end": (_i32, [_f]),
     "lc_flush_l2": (_i32, []),

@@ -188,6 +188,23 @@ def sample_top_p(logits, temperature: float, top_p: float, u: float = None) -> i
     return int(out.value)
 
 
+def token_logprobs(logits, tokens, top: int = 0):
+    """Log probabilities of `tokens` under rows of logits, entropies (nats), and the `top` likeliest tokens with their log probabilities (larger logit
+    first, equal ones by the lower index): (logprob [rows], entropy [rows], top_logprob [rows, top], top_id [rows, top]).  A token
+    outside the vocabulary has NaN."""
+    v = _f32(logits)
+    if v.ndim != 2:
+        raise ValueError("token_logprobs: logits [rows, vocab] expected")
+    tok = np.ascontiguousarray(tokens, np.int64).ravel()
+    if tok.size != v.shape[0]:
+        raise ValueError("token_logprobs: one token per row expected")
+    rows = v.shape[0]
+    lp, ent = np.empty(rows, np.float32), np.empty(rows, np.float32)
+    tl, ti = np.empty((rows, max(top, 0)), np.float32), np.empty((rows, max(top, 0)), np.int64)
+    check(load().lc_token_logprobs(_p(v), rows, v.shape[1], _p(tok), top, _p(lp), _p(ent), _p(tl), _p(ti)))
+    return lp, ent, tl, ti
+
+
 def seeded_uniform(seed: int, index: int) -> float:
     """Draw `index` of a seeded generation (see Engine.generate(seed=...))."""
     return float(load().lc_seeded_uniform(seed, index))

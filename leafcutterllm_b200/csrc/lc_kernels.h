@@ -12,6 +12,12 @@ int32_t launch_dequant(uint32_t typ, const void* w, size_t n_elems, float* out, 
 int32_t launch_sample_top_p(const float* logits_dev, size_t n, float temperature, float top_p, float u, int64_t* token_dev, cudaStream_t s);
 int32_t sample_top_p_sync(const float* logits_dev, size_t n, float temperature, float top_p, float u, int64_t* token_host, cudaStream_t s);
 float seeded_uniform(uint64_t seed, uint64_t index);
+// Log probabilities of given tokens, entropies and the likeliest tokens of rows of logits (logprobs.cu): f32, f16 or bf16; the check is the host
+// form's
+int32_t launch_token_logprobs(uint32_t typ, const void* x, int32_t rows, int32_t vocab, int64_t stride, const int64_t* tokens, int32_t top,
+                              float* logprob, float* entropy, float* top_logprob, int64_t* top_id, cudaStream_t s);
+int32_t check_token_logprobs(const char* call, size_t rows, size_t vocab, const float* logits, const int64_t* tokens, int32_t top, const float* logprob,
+                             const float* top_logprob, const int64_t* top_id);
 // Block-scale scan (scan.cu): geometry of every block type the reference's type table knows and how its scales are
 // read; the launch adds the number of bad blocks to one 64-bit word on the device.
 bool scan_geom(uint32_t typ, uint32_t* block_elems, uint32_t* block_bytes, int* kind);

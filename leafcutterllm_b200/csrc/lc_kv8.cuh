@@ -1,0 +1,94 @@
+// What the kernels over the 8-bit key/value cache share: views of the cache and of a call's rows, the sequence of a row, activations of
+// three types, and on the host the checks of arguments and the device that a call runs on.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_bf16.h>
+#include "lc_common.cuh"
+
+namespace lc {
+
+constexpr int kKv8MaxSeqs = 4096;
+
+struct Kv8Pool {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int n_pages, n_kv, page_shift, hd;  // page_tokens = 1 << page_shift
+};
+struct Kv8Seqs {
+    const int32_t* table;
+    const int32_t* ctx;
+    const int32_t* row_start;
+    int32_t* status;
+    int n_seqs, width, n_rows;
+};
+
+// Device of the call's pointers, current while this lives.
+struct DeviceScope {
+    int before = -1;
+    int32_t enter(const void* dev_ptr, const char* what);
+    ~DeviceScope() {
+        if (before >= 0) (void)cudaSetDevice(before);
+    }
+};
+inline cudaStream_t stream_or_own(void* s) { return s ? (cudaStream_t)s : stream(); }
+// kv8.cu: the arguments that all calls over the cache have; `view` and `seqs` are filled
+int32_t kv8_check(const char* call, const lc_kv8_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, Kv8Pool* view, Kv8Seqs* seqs);
+// nothing but a cache line's worth of alignment is asked of activations: 16-byte accesses where pointer and stride (in bytes) allow them
+inline bool rows_aligned(const void* p, int64_t stride_elems, size_t elem, size_t to) {
+    return ((uintptr_t)p % to) == 0 && ((size_t)stride_elems * elem) % to == 0;
+}
+
+#ifdef __CUDACC__
+template <typename T> __device__ __forceinline__ float elem_f(T v);
+template <> __device__ __forceinline__ float elem_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float elem_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float elem_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T to_elem(float v);
+template <> __device__ __forceinline__ float to_elem<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half to_elem<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 to_elem<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Rows [first, first + n) of sequence i; false where row_start is not ascending within the call's rows.
+__device__ __forceinline__ bool kv8_span(const Kv8Seqs& s, int i, int& first, int& n) {
+    const int a = s.row_start[i], b = s.row_start[i + 1];
+    first = a;
+    n = b - a;
+    return a >= 0 && b >= a && b <= s.n_rows;
+}
+// Whether positions ctx .. ctx + n - 1 lie in the table.
+__device__ __forceinline__ bool kv8_in_table(const Kv8Seqs& s, const Kv8Pool& p, int ctx, int n) {
+    return ctx >= 0 && (long long)ctx + n <= ((long long)s.width << p.page_shift);
+}
+__device__ __forceinline__ void kv8_raise(const Kv8Seqs& s, int i) {
+    if (s.status) atomicMax(s.status, i + 1);
+}
+// By one whole block: raises the status for sequences that the arrays themselves rule out.
+__device__ __forceinline__ void kv8_check_seqs(const Kv8Seqs& s, const Kv8Pool& p) {
+    if (!s.status) return;
+    for (int i = threadIdx.x; i < s.n_seqs; i += blockDim.x) {
+        int first, n;
+        if (!kv8_span(s, i, first, n) || (n > 0 && !kv8_in_table(s, p, s.ctx[i], n))) kv8_raise(s, i);
+    }
+}
+// By one whole warp: the sequence whose rows row `r` is one of (-1: none), 32 probes a step.
+__device__ __forceinline__ int kv8_seq_of_row(const Kv8Seqs& s, int r) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, len = s.n_seqs + 1;
+    for (;;) {
+        const int step = (len + 31) >> 5, at = lane * step;
+        const bool le = at < len && s.row_start[lo + at] <= r;
+        const int cnt = __popc(__ballot_sync(0xffffffffu, le));
+        if (cnt == 0) return -1;
+        lo += (cnt - 1) * step;
+        len = min(step, len - (cnt - 1) * step);
+        if (step == 1) break;
+    }
+    if (lo >= s.n_seqs) return -1;
+    int first, n;
+    return kv8_span(s, lo, first, n) && r - first < n && r >= first ? lo : -1;
+}
+#endif
+
+}  // namespace lc

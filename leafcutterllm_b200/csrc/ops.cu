@@ -543,5 +543,30 @@ int32_t lc_argmax(const float* v, size_t n, int64_t* out_index) {
     LC_TRY(launch_argmax((float*)S->a.p, n, 1, (int64_t*)S->c.p, stream()));
     return down(out_index, S->c, 8);
 }
+int32_t lc_token_logprobs(const float* logits, size_t rows, size_t vocab, const int64_t* tokens, int32_t top, float* logprob, float* entropy,
+                          float* top_logprob, int64_t* top_id) {
+    LC_TRY(check_token_logprobs("lc_token_logprobs", rows, vocab, logits, tokens, top, logprob, top_logprob, top_id));
+    if (rows == 0) return LC_OK;
+    L1_ENTER();
+    // outputs in a row: identifiers, then log probabilities and entropies
+    const size_t ids = rows * (size_t)top * 8, tops = rows * (size_t)top * 4;
+    LC_TRY(up(S->a, logits, rows * vocab * 4));
+    if (logprob) LC_TRY(up(S->b, tokens, rows * 8));
+    LC_TRY(S->c.reserve(ids + tops + rows * 8));
+    unsigned char* c = (unsigned char*)S->c.p;
+    int64_t* d_id = (int64_t*)c;
+    float* d_top = (float*)(c + ids);
+    float* d_lp = (float*)(c + ids + tops);
+    LC_TRY(launch_token_logprobs(LC_TYPE_F32, S->a.p, (int32_t)rows, (int32_t)vocab, (int64_t)vocab, (const int64_t*)S->b.p, top,
+                                 logprob ? d_lp : nullptr, entropy ? d_lp + rows : nullptr, d_top, d_id, stream()));
+    if (top > 0) {
+        LC_CUDA(cudaMemcpyAsync(top_id, d_id, ids, cudaMemcpyDeviceToHost, stream()));
+        LC_CUDA(cudaMemcpyAsync(top_logprob, d_top, tops, cudaMemcpyDeviceToHost, stream()));
+    }
+    if (logprob) LC_CUDA(cudaMemcpyAsync(logprob, d_lp, rows * 4, cudaMemcpyDeviceToHost, stream()));
+    if (entropy) LC_CUDA(cudaMemcpyAsync(entropy, d_lp + rows, rows * 4, cudaMemcpyDeviceToHost, stream()));
+    LC_CUDA(cudaStreamSynchronize(stream()));
+    return LC_OK;
+}
 
 }  // extern "C"
