@@ -18,14 +18,14 @@ namespace {
 
 constexpr int kStep = 16;            // keys of a warp's step: one page's, or a part of one page's
 constexpr int kRunWarps = 4;
-constexpr int kChunk = kStep * kRunWarps;  // keys of a block's step
 constexpr float kNegInf = -INFINITY;
 
 struct AttnArgs {
     const void* q;
     void* out;
     int64_t q_stride, out_stride;
-    int n_heads, group, window;
+    int typ, n_heads, group, window;
+    bool q_vec, out_vec;             // 16-byte accesses
     float scale_log2;                // scale * log2(e)
     float* part;                     // partial results of runs that end inside a unit
 };
@@ -64,6 +64,52 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// sixteen elements in a row as f32, and back
+template <typename T> __device__ __forceinline__ void load16(const T* p, bool vec, float* v) {
+    constexpr int E = 16 / sizeof(T);
+    if (vec) {
+#pragma unroll
+        for (int u = 0; u < 16 / E; u++) {
+            __align__(16) T t[E];
+            *reinterpret_cast<uint4*>(t) = reinterpret_cast<const uint4*>(p)[u];
+#pragma unroll
+            for (int e = 0; e < E; e++) v[u * E + e] = elem_f(t[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) v[e] = elem_f(p[e]);
+    }
+}
+__device__ __forceinline__ void load16(const void* p, int64_t at, int typ, bool vec, float* v) {
+    if (typ == LC_TYPE_F32) load16((const float*)p + at, vec, v);
+    else if (typ == LC_TYPE_F16) load16((const __half*)p + at, vec, v);
+    else load16((const __nv_bfloat16*)p + at, vec, v);
+}
+template <typename T> __device__ __forceinline__ void store16(T* p, bool vec, const float* v) {
+    constexpr int E = 16 / sizeof(T);
+    if (vec) {
+#pragma unroll
+        for (int u = 0; u < 16 / E; u++) {
+            __align__(16) T t[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) t[e] = to_elem<T>(v[u * E + e]);
+            reinterpret_cast<uint4*>(p)[u] = *reinterpret_cast<const uint4*>(t);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) p[e] = to_elem<T>(v[e]);
+    }
+}
+__device__ __forceinline__ void store16(void* p, int64_t at, int typ, bool vec, const float* v) {
+    if (typ == LC_TYPE_F32) store16((float*)p + at, vec, v);
+    else if (typ == LC_TYPE_F16) store16((__half*)p + at, vec, v);
+    else store16((__nv_bfloat16*)p + at, vec, v);
+}
+__device__ __forceinline__ void store1(void* p, int64_t at, int typ, float v) {
+    if (typ == LC_TYPE_F32) ((float*)p)[at] = v;
+    else if (typ == LC_TYPE_F16) ((__half*)p)[at] = to_elem<__half>(v);
+    else ((__nv_bfloat16*)p)[at] = to_elem<__nv_bfloat16>(v);
+}
 // a power of two that brings the largest magnitude of a row into [2^14, 2^15), and its inverse; 1 for a row of zeros or with infinities
 __device__ __forceinline__ void row_scale(float top, float& up, float& down) {
     const int e = (__float_as_int(top) >> 23) & 0xff;
@@ -76,43 +122,46 @@ __device__ __forceinline__ void row_scale(float top, float& up, float& down) {
 
 // ------------------------------------------------------------------------------------------------------------------------------------
 // Runs: few rows per sequence.  A unit is (sequence, kv head, row block of RB rows = tokens x heads of the group); its keys are cut into
-// chunks of 64.  All chunks of all units stand in one line, which is cut into equal runs, one per block, so that
-// contexts of any lengths keep all blocks equally long at work.  A unit that lies in several runs leaves partial results, which the next kernel
-// joins.  A warp takes 16 keys of a chunk; keys and values come through a ring of its own in shared memory (cp.async, no block-wide waits).
+// steps of 16.  All steps of all units stand in one line, which is cut into equal runs, one per WARP, so that contexts of any lengths
+// keep all warps equally long at work and none waits for another.  A unit that lies in several runs leaves partial results, which the next kernel
+// joins.  Keys and values come through a ring of the warp's own in shared memory (cp.async).
+//
+// Operand layouts, so that nothing is transposed: the dims of a score and the keys of a weighted sum are sums' indexes and may stand in any
+// order, so a thread takes 16 neighbouring dims of its key (one 16-byte read) for four steps of the scores, and its columns of
+// the weighted sum are 16 neighbouring dims of its four keys.  What it ends with is 32 neighbouring dims (HD 64: 16) of its row.
 // ------------------------------------------------------------------------------------------------------------------------------------
 
-// The line: chunks before each sequence, its chunks per unit and first chunk follow from ctx and rows.
 struct SeqWork {
-    int first, n, ctx, blocks, chunk0, chunks;  // rows, context, row blocks, first chunk, chunks per unit
+    int first, n, ctx, blocks, step0, steps;  // rows, context, row blocks, first step, steps per unit
     bool inside;
 };
 template <int RB>
 __device__ __forceinline__ SeqWork seq_work(const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, int i) {
     SeqWork w;
     w.inside = false;
-    w.blocks = w.chunk0 = w.chunks = 0;
+    w.blocks = w.step0 = w.steps = 0;
     w.ctx = s.ctx[i];
     if (!kv8_span(s, i, w.first, w.n) || w.n == 0) { w.n = 0; return w; }
     w.blocks = (w.n * a.group + RB - 1) / RB;
     w.inside = kv8_in_table(s, p, w.ctx, w.n);
     if (w.inside) {
         const int lo = a.window > 0 ? max(0, w.ctx - a.window + 1) : 0;
-        w.chunk0 = lo / kChunk;
-        w.chunks = (w.ctx + w.n + kChunk - 1) / kChunk - w.chunk0;
+        w.step0 = lo / kStep;
+        w.steps = (w.ctx + w.n + kStep - 1) / kStep - w.step0;
     } else {
-        w.chunks = 1;  // one step that writes NaN
+        w.steps = 1;  // one step that writes NaN
     }
     return w;
 }
-// cum[i] = chunks of the sequences before i, cum[n_seqs] = all; by one block, returns the total
+// cum[i] = steps of the sequences before i, cum[n_seqs] = all; by one block, returns the total
 template <int RB>
 __device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, uint32_t* cum, uint32_t* warp_sums) {
-    const int per = (s.n_seqs + blockDim.x - 1) / blockDim.x, i0 = threadIdx.x * per, i1 = min(i0 + per, s.n_seqs);
+    const int per = (s.n_seqs + blockDim.x - 1) / blockDim.x, i0 = min((int)threadIdx.x * per, s.n_seqs), i1 = min(i0 + per, s.n_seqs);
     uint32_t sum = 0;
     for (int i = i0; i < i1; i++) {
         const SeqWork w = seq_work<RB>(s, p, a, i);
         cum[i] = sum;
-        sum += (uint32_t)w.blocks * (uint32_t)p.n_kv * (uint32_t)w.chunks;
+        sum += (uint32_t)w.blocks * (uint32_t)p.n_kv * (uint32_t)w.steps;
     }
     uint32_t incl = sum;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -132,7 +181,7 @@ __device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, 
     __syncthreads();
     return total;
 }
-__device__ __forceinline__ int seq_at(const uint32_t* cum, int n_seqs, uint32_t t) {  // the sequence whose chunks t is one of
+__device__ __forceinline__ int seq_at(const uint32_t* cum, int n_seqs, uint32_t t) {  // the sequence whose steps t is one of
     int lo = 0, hi = n_seqs;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -140,410 +189,476 @@ __device__ __forceinline__ int seq_at(const uint32_t* cum, int n_seqs, uint32_t 
     }
     return lo;
 }
-__device__ __forceinline__ uint32_t run_start(uint32_t total, int b, int blocks) { return (uint32_t)((unsigned long long)total * b / blocks); }
+// The line of `total` steps in equal runs, none of them empty, and none shorter than kLeast where that leaves warps without one.
+constexpr uint32_t kLeast = 4;
+struct Runs {
+    uint32_t n, per, more;  // the first `more` runs have a step more than `per`
+    __device__ __forceinline__ Runs(uint32_t total, uint32_t warps) {
+        n = min((total + kLeast - 1) / kLeast, warps);
+        per = n ? total / n : 0;
+        more = total - per * n;
+    }
+    __device__ __forceinline__ uint32_t start(uint32_t b) const { return b * per + min(b, more); }
+    __device__ __forceinline__ uint32_t run_of(uint32_t t) const {  // the run that step t is in
+        const uint32_t longer = more * (per + 1);
+        return t < longer ? t / (per + 1) : more + (t - longer) / per;
+    }
+};
 
 // floats of one partial result: maxima, sums and rows of HD
 template <int HD, int RB> __host__ __device__ constexpr int part_floats() { return RB * (HD + 2); }
 
 // Where a place of the line lies.
 struct Place {
-    int seq, kvh, rb, chunk;       // chunk: index within the unit
+    int seq, kvh, rb, step;        // step: index within the unit
     SeqWork w;
-    uint32_t unit_start;           // place of the unit's first chunk
+    uint32_t unit_start;           // place of the unit's first step
 };
 template <int RB>
 __device__ __forceinline__ void place_at(Place& at, const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, const uint32_t* cum, uint32_t t) {
     at.seq = seq_at(cum, s.n_seqs, t);
     at.w = seq_work<RB>(s, p, a, at.seq);
-    const uint32_t in = t - cum[at.seq], unit = in / at.w.chunks;
-    at.chunk = in - unit * at.w.chunks;
-    at.unit_start = t - at.chunk;
+    const uint32_t in = t - cum[at.seq], unit = in / at.w.steps;
+    at.step = in - unit * at.w.steps;
+    at.unit_start = t - at.step;
     at.kvh = unit / at.w.blocks;
     at.rb = unit - at.kvh * at.w.blocks;
 }
 
-template <typename T, int HD, int RB> struct RunShape {
+// MT tiles of 16 rows: 8 MT rows in the split form, 16 MT in the plain one
+template <int HD, int MT, bool SPLIT> struct RunShape {
+    static constexpr int kRows = MT * (SPLIT ? 8 : 16);
     static constexpr int kStageBytes = 2 * kStep * HD + 16;   // keys, values, their two scales
     static constexpr int kStages = HD == 64 ? 4 : 3;
-    static constexpr int kRing = kRunWarps * kStages * kStageBytes;
-    static constexpr int kJoin = kRunWarps * part_floats<HD, RB>() * 4;
+    static constexpr bool kQueriesShared = HD == 256 || MT > 1;  // operand fragments of the queries in shared memory, not in registers
+    static constexpr int kQueries = kQueriesShared ? MT * (HD / 16) * 512 : 0;
+    static constexpr int kWarp = kStages * kStageBytes + kQueries;
+    static constexpr int kBlocks = HD == 256 || MT > 1 ? 2 : SPLIT ? 4 : 3;
 };
 
-template <typename T, int HD, int RB>
-__global__ void __launch_bounds__(kRunWarps * 32, HD == 256 ? 2 : RB == 8 ? 4 : 3)
+template <int HD, int MT, bool SPLIT, bool FULL>
+__global__ void __launch_bounds__(kRunWarps * 32, RunShape<HD, MT, SPLIT>::kBlocks)
 kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
-    constexpr bool SPLIT = RB == 8;
+    using Shape = RunShape<HD, MT, SPLIT>;
+    constexpr int RB = Shape::kRows;
     constexpr int NT = HD / 8;              // tiles of 8 dims of the output; a thread's values of a key are NT in a row
     constexpr int KS = HD / 16;             // k steps of the scores
-    constexpr int OC = SPLIT ? 2 : 4;
-    using Shape = RunShape<T, HD, RB>;
+    constexpr int HF = SPLIT ? 1 : 2;       // rows of a tile that a thread has a part in
+    constexpr int OC = 2 * HF;
+    constexpr int S = Shape::kStages;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint32_t warp_sums[kRunWarps];
-    float* join = reinterpret_cast<float*>(smem);                 // shares its place with the ring between segments' ends
-    uint32_t* cum = reinterpret_cast<uint32_t*>(smem + (Shape::kRing > Shape::kJoin ? Shape::kRing : Shape::kJoin));
+    uint32_t* cum = reinterpret_cast<uint32_t*>(smem + kRunWarps * Shape::kWarp);
     pdl_launch_dependents();
     if (blockIdx.x == 0) kv8_check_seqs(seqs, pool);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const uint32_t total = line_up<RB>(seqs, pool, a, cum, warp_sums);
-    uint32_t t = run_start(total, blockIdx.x, gridDim.x);
-    const uint32_t t_end = run_start(total, blockIdx.x + 1, gridDim.x);
-    const uint32_t ring = smem_u32(smem) + warp * Shape::kStages * Shape::kStageBytes;
-    const int hd = pool.hd, page_mask = (1 << pool.page_shift) - 1;
+    const Runs runs(total, gridDim.x * kRunWarps);
+    const uint32_t run = blockIdx.x * kRunWarps + warp;
+    if (run >= runs.n) return;
+    uint32_t t = runs.start(run);
+    const uint32_t t_end = runs.start(run + 1);
+    unsigned char* const mine = smem + warp * Shape::kWarp;
+    const uint32_t ring = smem_u32(mine);
+    uint4* const qs = reinterpret_cast<uint4*>(mine + S * Shape::kStageBytes);
+    const int hd = FULL ? HD : pool.hd, page_mask = (1 << pool.page_shift) - 1;
+    // a lane's part of every copy: chunk lch of rows lrow, lrow + kRowsPer, ...; chunks behind hd repeat the last one (their queries are 0, their sums not stored)
+    constexpr int kChunks = HD / 16, kRowsPer = 32 / kChunks;
+    const int lrow = lane / kChunks, lch = lane % kChunks;
+    const int lsrc = lrow * hd + (FULL ? lch : min(lch, (hd >> 4) - 1)) * 16;
 
     while (t < t_end) {
-        // a segment: this run's chunks of one unit
+        // a segment: this run's steps of one unit
         Place at;
         place_at<RB>(at, seqs, pool, a, cum, t);
         const SeqWork& w = at.w;
-        const int c0 = at.chunk, c1 = min(w.chunks, c0 + (int)(t_end - t));
+        const int s0 = at.step, s1 = min(w.steps, s0 + (int)(t_end - t));
         const int32_t* table = seqs.table + (size_t)at.seq * seqs.width;
         const int row_lo = at.rb * RB, row_n = min(RB, w.n * a.group - row_lo);
-        const int key_end = w.ctx + w.n;    // exclusive
 
-        auto page_of = [&](int chunk) -> int {  // the page of this warp's keys of a chunk
-            const int key = (w.chunk0 + chunk) * kChunk + warp * kStep;
-            if (!w.inside || chunk >= c1 || key >= key_end) return -1;
-            return table[key >> pool.page_shift];
+        // pages of 32 steps on, one per lane
+        int pages_at = s0, pages = -1;
+        auto look_up = [&]() {
+            const int st = pages_at + lane;
+            pages = w.inside && st < s1 ? table[((w.step0 + st) * kStep) >> pool.page_shift] : -1;
         };
-        auto fetch = [&](int chunk, int number) {
-            const int key = (w.chunk0 + chunk) * kChunk + warp * kStep;
-            if (w.inside && chunk < c1 && key < key_end) {
-                const uint32_t st = ring + (uint32_t)(chunk % Shape::kStages) * Shape::kStageBytes;
-                const bool held = number >= 0 && number < pool.n_pages;
-                if (!held) { if (lane == 0) kv8_raise(seqs, at.seq); }
-                else {
+        look_up();
+        bool poisoned = !w.inside;
+        auto fetch = [&](int st) {
+            if (st - pages_at == 32) { pages_at += 32; look_up(); }
+            if (st < s1 && w.inside) {
+                const int number = __shfl_sync(0xffffffffu, pages, st - pages_at);
+                if (number < 0 || number >= pool.n_pages) {
+                    poisoned = true;
+                    if (lane == 0) kv8_raise(seqs, at.seq);
+                } else {
+                    const uint32_t dst = ring + (uint32_t)(st % S) * Shape::kStageBytes;
                     const size_t ph = (size_t)number * pool.n_kv + at.kvh;
-                    const size_t off = ((ph << pool.page_shift) + (key & page_mask)) * hd;
-                    const int pieces = hd >> 4;
+                    const size_t off = ((ph << pool.page_shift) + (((w.step0 + st) * kStep) & page_mask)) * hd + lsrc;
+                    const int8_t* ks = pool.k + off;
+                    const int8_t* vs = pool.v + off;
 #pragma unroll
-                    for (int e = lane; e < kStep * (HD / 16); e += 32) {
-                        const int row = e / (HD / 16), ch = e % (HD / 16);
-                        if (ch < pieces) {
-                            cp_async16(st + row * HD + ((ch ^ ((row & 1) << 2)) & (HD / 16 - 1)) * 16, pool.k + off + (size_t)row * hd + ch * 16);
-                            cp_async16(st + kStep * HD + row * HD + ((ch ^ (row & 6)) & (HD / 16 - 1)) * 16, pool.v + off + (size_t)row * hd + ch * 16);
-                        }
+                    for (int i = 0; i < kStep / kRowsPer; i++) {
+                        const int row = lrow + i * kRowsPer;
+                        cp_async16(dst + row * HD + ((lch ^ ((row & 1) << 2)) & (kChunks - 1)) * 16, ks + i * kRowsPer * hd);
+                        cp_async16(dst + kStep * HD + row * HD + ((lch ^ (row & 6)) & (kChunks - 1)) * 16, vs + i * kRowsPer * hd);
                     }
-                    if (lane < 2) cp_async4(st + 2 * kStep * HD + lane * 4, (lane ? pool.v_scale : pool.k_scale) + ph);
+                    if (lane < 2) cp_async4(dst + 2 * kStep * HD + lane * 4, (lane ? pool.v_scale : pool.k_scale) + ph);
                 }
             }
             cp_async_commit();
         };
+#pragma unroll
+        for (int k = 0; k < S - 1; k++) fetch(s0 + k);
 
-        int next_page = page_of(c0);
+        // the queries as operand fragments: step ks = 4 j + wd of the scores takes dims 64 j + 16 c + 4 wd .. + 3
+        uint32_t qf[Shape::kQueriesShared ? 1 : KS][4];
+        float rf[MT][HF];
+        int limit[MT][HF];                   // last position that the row sees (-1: no row)
 #pragma unroll
-        for (int k = 0; k < Shape::kStages - 1; k++) {
-            const int now = next_page;
-            next_page = page_of(c0 + k + 1);
-            fetch(c0 + k, now);
-        }
-
-        // the queries as operand fragments: dims of step ks = 4 j + wd: chunk j of 64, 16 c .. in it, word wd
-        uint32_t qf[KS][4];
-        float rf[SPLIT ? 1 : 2];
-        int limit[SPLIT ? 1 : 2];            // last position that the row sees (-1: no row)
+        for (int mt = 0; mt < MT; mt++) {
+            uint32_t f[KS][4];
 #pragma unroll
-        for (int hf = 0; hf < (SPLIT ? 1 : 2); hf++) {
-            const int r = g + 8 * hf;
-            const bool has = r < row_n;
-            const int tok = has ? (row_lo + r) / a.group : 0, hq = has ? (row_lo + r) % a.group : 0;
-            const T* src = (const T*)a.q + (int64_t)(w.first + tok) * a.q_stride + (int64_t)(at.kvh * a.group + hq) * hd;
-            limit[hf] = has ? w.ctx + tok : -1;
-            float top = 0.0f;
-            if (has)
-                for (int j = 0; j < HD / 64; j++)
+            for (int hf = 0; hf < HF; hf++) {
+                const int r = (SPLIT ? 8 : 16) * mt + g + 8 * hf;
+                const bool has = r < row_n;
+                const int tok = has ? (row_lo + r) / a.group : 0, hq = has ? (row_lo + r) - tok * a.group : 0;
+                const int64_t src = (int64_t)(w.first + tok) * a.q_stride + (int64_t)(at.kvh * a.group + hq) * hd;
+                limit[mt][hf] = has ? w.ctx + tok : -1;
+                float v[KS][4], top = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int d = 64 * j + 16 * c + e;
-                        if (d < hd) top = fmaxf(top, fabsf(elem_f(src[d])));
+                for (int j = 0; j < KS / 4; j++) {
+                    const int d = 64 * j + 16 * c;
+                    if (has && (FULL || d < hd)) load16(a.q, src + d, a.typ, a.q_vec, &v[4 * j][0]);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 16; e++) v[4 * j + (e >> 2)][e & 3] = 0.0f;
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(v[ks][e]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                float up, down;
+                row_scale(top, up, down);
+                rf[mt][hf] = a.scale_log2 * down;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    if (SPLIT) {
+                        h2_split(v[ks][0] * up, v[ks][1] * up, f[ks][0], f[ks][1]);
+                        h2_split(v[ks][2] * up, v[ks][3] * up, f[ks][2], f[ks][3]);
+                    } else {
+                        f[ks][hf] = h2_pack(v[ks][0] * up, v[ks][1] * up);
+                        f[ks][2 + hf] = h2_pack(v[ks][2] * up, v[ks][3] * up);
                     }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            float up, down;
-            row_scale(top, up, down);
-            rf[hf] = a.scale_log2 * down;
+                }
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                const int d = 64 * (ks >> 2) + 16 * c + 4 * (ks & 3);
-                float v[4];
+                if (Shape::kQueriesShared) qs[(mt * KS + ks) * 32 + lane] = make_uint4(f[ks][0], f[ks][1], f[ks][2], f[ks][3]);
+                else
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = has && d + e < hd ? elem_f(src[d + e]) * up : 0.0f;
-                if (SPLIT) {
-                    h2_split(v[0], v[1], qf[ks][0], qf[ks][1]);
-                    h2_split(v[2], v[3], qf[ks][2], qf[ks][3]);
-                } else {
-                    qf[ks][hf] = h2_pack(v[0], v[1]);
-                    qf[ks][2 + hf] = h2_pack(v[2], v[3]);
-                }
+                    for (int e = 0; e < 4; e++) qf[Shape::kQueriesShared ? 0 : ks][e] = f[ks][e];
             }
         }
 
-        float o[NT][OC];
+        float o[MT][NT][OC], m[MT][HF], l[MT][HF];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int mt = 0; mt < MT; mt++) {
 #pragma unroll
-            for (int e = 0; e < OC; e++) o[n][e] = 0.0f;
-        float m[SPLIT ? 1 : 2], l[SPLIT ? 1 : 2];
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int hf = 0; hf < (SPLIT ? 1 : 2); hf++) { m[hf] = kNegInf; l[hf] = 0.0f; }
-        bool poisoned = !w.inside;
+                for (int e = 0; e < OC; e++) o[mt][n][e] = 0.0f;
+#pragma unroll
+            for (int hf = 0; hf < HF; hf++) { m[mt][hf] = kNegInf; l[mt][hf] = 0.0f; }
+        }
 
-        for (int chunk = c0; chunk < c1; chunk++) {
-            const int now = next_page;
-            next_page = page_of(chunk + Shape::kStages);
-            cp_async_wait<Shape::kStages - 2>();
+        for (int st = s0; st < s1; st++) {
+            cp_async_wait<S - 2>();
             __syncwarp();
-            const int key0 = (w.chunk0 + chunk) * kChunk + warp * kStep;
-            const unsigned char* st = smem + (warp * Shape::kStages + chunk % Shape::kStages) * Shape::kStageBytes;
-            const bool any = w.inside && key0 < key_end;
-            if (any) {
-                const int number = table[key0 >> pool.page_shift];
-                if (number < 0 || number >= pool.n_pages) poisoned = true;
-                else {
-                    const float ksc = *reinterpret_cast<const float*>(st + 2 * kStep * HD), vsc = *reinterpret_cast<const float*>(st + 2 * kStep * HD + 4);
-                    float s[2][4];
+            const int key0 = (w.step0 + st) * kStep;
+            const unsigned char* kp = mine + (st % S) * Shape::kStageBytes;
+            const float ksc = *reinterpret_cast<const float*>(kp + 2 * kStep * HD), vsc = *reinterpret_cast<const float*>(kp + 2 * kStep * HD + 4);
+            float s[MT][2][4];
 #pragma unroll
-                    for (int tl = 0; tl < 2; tl++) {
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[tl][e] = 0.0f;
+                for (int tl = 0; tl < 2; tl++)
 #pragma unroll
-                        for (int j = 0; j < HD / 64; j++) {
-                            const int row = 8 * tl + g, ch = 4 * j + c;
-                            uint4 kw = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                            if (ch * 16 < hd) {
-                                kw = *reinterpret_cast<const uint4*>(st + row * HD + ((ch ^ ((row & 1) << 2)) & (HD / 16 - 1)) * 16);
-                                kw.x ^= 0x80808080u; kw.y ^= 0x80808080u; kw.z ^= 0x80808080u; kw.w ^= 0x80808080u;
-                            }
-                            mma_f16(s[tl], qf[4 * j + 0], ints01(kw.x), ints23(kw.x));
-                            mma_f16(s[tl], qf[4 * j + 1], ints01(kw.y), ints23(kw.y));
-                            mma_f16(s[tl], qf[4 * j + 2], ints01(kw.z), ints23(kw.z));
-                            mma_f16(s[tl], qf[4 * j + 3], ints01(kw.w), ints23(kw.w));
-                        }
-                    }
-                    uint32_t pf[4];
+                    for (int e = 0; e < 4; e++) s[mt][tl][e] = 0.0f;
 #pragma unroll
-                    for (int hf = 0; hf < (SPLIT ? 1 : 2); hf++) {
-                        float v[4];
-                        const float f = rf[hf] * ksc;
+            for (int j = 0; j < HD / 64; j++) {
+                uint32_t kw[2][4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int tl = e >> 1, k = e & 1, key = key0 + 8 * tl + 2 * c + k;
-                            v[e] = (SPLIT ? s[tl][k] + s[tl][2 + k] : s[tl][2 * hf + k]) * f;
-                            if (key > limit[hf] || (a.window > 0 && key <= limit[hf] - a.window)) v[e] = kNegInf;
-                        }
-                        float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        mx = fmaxf(mx, m[hf]);
-                        const float ref = mx == kNegInf ? 0.0f : mx;
-                        if (__any_sync(0xffffffffu, mx > m[hf])) {
-                            const float corr = exp2_fast(m[hf] - ref);
-                            l[hf] *= corr;
+                for (int tl = 0; tl < 2; tl++) {
+                    const int row = 8 * tl + g, ch = 4 * j + c;
+                    const uint4 u = *reinterpret_cast<const uint4*>(kp + row * HD + ((ch ^ ((row & 1) << 2)) & (kChunks - 1)) * 16);
+                    kw[tl][0] = u.x ^ 0x80808080u; kw[tl][1] = u.y ^ 0x80808080u; kw[tl][2] = u.z ^ 0x80808080u; kw[tl][3] = u.w ^ 0x80808080u;
+                }
 #pragma unroll
-                            for (int n = 0; n < NT; n++) { o[n][2 * hf] *= corr; o[n][2 * hf + 1] *= corr; }
-                            m[hf] = mx;
-                        }
-                        float p[4];
+                for (int wd = 0; wd < 4; wd++) {
+                    const int ks = 4 * j + wd;
+                    const uint32_t b00 = ints01(kw[0][wd]), b01 = ints23(kw[0][wd]), b10 = ints01(kw[1][wd]), b11 = ints23(kw[1][wd]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) p[e] = exp2_fast(v[e] - ref + 8.0f);
-                        l[hf] += (p[0] + p[1]) + (p[2] + p[3]);
-                        if (SPLIT) {
-                            h2_split(p[0], p[1], pf[0], pf[1]);
-                            h2_split(p[2], p[3], pf[2], pf[3]);
+                    for (int mt = 0; mt < MT; mt++) {
+                        uint32_t f[4];
+                        if (Shape::kQueriesShared) {
+                            const uint4 u = qs[(mt * KS + ks) * 32 + lane];
+                            f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
                         } else {
-                            pf[hf] = h2_pack(p[0], p[1]);
-                            pf[2 + hf] = h2_pack(p[2], p[3]);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) f[e] = qf[Shape::kQueriesShared ? 0 : ks][e];
                         }
+                        mma_f16(s[mt][0], f, b00, b01);
+                        mma_f16(s[mt][1], f, b10, b11);
                     }
-                    // values: a thread's keys are 2c, 2c + 1, 8 + 2c, 9 + 2c; its dims NT in a row (HD 256: 16 and 16 more 128 further)
-                    const unsigned char* vs = st + kStep * HD;
-                    constexpr int WORDS = HD == 64 ? 2 : 4;
+                }
+            }
+            uint32_t pf[MT][4];
 #pragma unroll
-                    for (int gr = 0; gr < (HD == 256 ? 2 : 1); gr++) {
-                        const int ch = HD == 64 ? g >> 1 : 8 * gr + g;
-                        uint32_t kv[4][WORDS];
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                        for (int x = 0; x < 4; x++) {
-                            const int row = (x >> 1) * 8 + 2 * c + (x & 1);
-                            const unsigned char* at16 = vs + row * HD + ((ch ^ (row & 6)) & (HD / 16 - 1)) * 16;
-                            if (HD == 64) {
-                                uint2 u = make_uint2(0, 0);
-                                if (ch * 16 < hd) u = *reinterpret_cast<const uint2*>(at16 + (g & 1) * 8);
-                                kv[x][0] = u.x ^ 0x80808080u; kv[x][1] = u.y ^ 0x80808080u;
+                for (int hf = 0; hf < HF; hf++) {
+                    float v[4];
+                    const float f = rf[mt][hf] * ksc;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int tl = e >> 1, k = e & 1, key = key0 + 8 * tl + 2 * c + k;
+                        v[e] = (SPLIT ? s[mt][tl][k] + s[mt][tl][2 + k] : s[mt][tl][2 * hf + k]) * f;
+                        if (key > limit[mt][hf] || (a.window > 0 && key <= limit[mt][hf] - a.window)) v[e] = kNegInf;
+                    }
+                    float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    mx = fmaxf(mx, m[mt][hf]);
+                    const float ref = mx == kNegInf ? 0.0f : mx;
+                    if (__any_sync(0xffffffffu, mx > m[mt][hf])) {
+                        const float corr = exp2_fast(m[mt][hf] - ref);
+                        l[mt][hf] *= corr;
+#pragma unroll
+                        for (int n = 0; n < NT; n++) { o[mt][n][2 * hf] *= corr; o[mt][n][2 * hf + 1] *= corr; }
+                        m[mt][hf] = mx;
+                    }
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) p[e] = exp2_fast(v[e] - ref + 8.0f);
+                    l[mt][hf] += (p[0] + p[1]) + (p[2] + p[3]);
+                    if (SPLIT) {
+                        h2_split(p[0], p[1], pf[mt][0], pf[mt][1]);
+                        h2_split(p[2], p[3], pf[mt][2], pf[mt][3]);
+                    } else {
+                        pf[mt][hf] = h2_pack(p[0], p[1]);
+                        pf[mt][2 + hf] = h2_pack(p[2], p[3]);
+                    }
+                }
+            // values: a thread's keys are 2c, 2c + 1, 8 + 2c, 9 + 2c; its dims NT in a row (HD 256: 16 and 16 more 128 further)
+            const unsigned char* vp = kp + kStep * HD;
+            constexpr int WORDS = HD == 64 ? 2 : 4;
+#pragma unroll
+            for (int gr = 0; gr < (HD == 256 ? 2 : 1); gr++) {
+                const int ch = HD == 64 ? g >> 1 : 8 * gr + g;
+                uint32_t kv[4][WORDS];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int row = (x >> 1) * 8 + 2 * c + (x & 1);
+                    const unsigned char* at16 = vp + row * HD + ((ch ^ (row & 6)) & (kChunks - 1)) * 16;
+                    if (HD == 64) {
+                        const uint2 u = *reinterpret_cast<const uint2*>(at16 + (g & 1) * 8);
+                        kv[x][0] = u.x ^ 0x80808080u; kv[x][1] = u.y ^ 0x80808080u;
+                    } else {
+                        const uint4 u = *reinterpret_cast<const uint4*>(at16);
+                        kv[x][0] = u.x ^ 0x80808080u; kv[x][1] = u.y ^ 0x80808080u;
+                        kv[x][WORDS - 2] = u.z ^ 0x80808080u; kv[x][WORDS - 1] = u.w ^ 0x80808080u;
+                    }
+                }
+#pragma unroll
+                for (int wd = 0; wd < WORDS; wd++) {
+                    const uint32_t a01 = __byte_perm(kv[0][wd], kv[1][wd], 0x5140), a23 = __byte_perm(kv[0][wd], kv[1][wd], 0x7362);
+                    const uint32_t b01 = __byte_perm(kv[2][wd], kv[3][wd], 0x5140), b23 = __byte_perm(kv[2][wd], kv[3][wd], 0x7362);
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        const uint32_t va = b < 2 ? a01 : a23, vb = b < 2 ? b01 : b23;
+                        const uint32_t v0 = b & 1 ? ints23(va) : ints01(va), v1 = b & 1 ? ints23(vb) : ints01(vb);
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_f16(acc, pf[mt], v0, v1);
+                            float(&oo)[OC] = o[mt][16 * gr + 4 * wd + b];
+                            if (SPLIT) {
+                                oo[0] = fmaf(acc[0] + acc[2], vsc, oo[0]);
+                                oo[1] = fmaf(acc[1] + acc[3], vsc, oo[1]);
                             } else {
-                                uint4 u = make_uint4(0, 0, 0, 0);
-                                if (ch * 16 < hd) u = *reinterpret_cast<const uint4*>(at16);
-                                kv[x][0] = u.x ^ 0x80808080u; kv[x][1] = u.y ^ 0x80808080u;
-                                kv[x][WORDS - 2] = u.z ^ 0x80808080u; kv[x][WORDS - 1] = u.w ^ 0x80808080u;
-                            }
-                        }
 #pragma unroll
-                        for (int wd = 0; wd < WORDS; wd++) {
-                            const uint32_t a01 = __byte_perm(kv[0][wd], kv[1][wd], 0x5140), a23 = __byte_perm(kv[0][wd], kv[1][wd], 0x7362);
-                            const uint32_t b01 = __byte_perm(kv[2][wd], kv[3][wd], 0x5140), b23 = __byte_perm(kv[2][wd], kv[3][wd], 0x7362);
-#pragma unroll
-                            for (int b = 0; b < 4; b++) {
-                                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                const uint32_t va = b < 2 ? a01 : a23, vb = b < 2 ? b01 : b23;
-                                mma_f16(acc, pf, b & 1 ? ints23(va) : ints01(va), b & 1 ? ints23(vb) : ints01(vb));
-                                float(&oo)[OC] = o[16 * gr + 4 * wd + b];
-                                if (SPLIT) {
-                                    oo[0] = fmaf(acc[0] + acc[2], vsc, oo[0]);
-                                    oo[1] = fmaf(acc[1] + acc[3], vsc, oo[1]);
-                                } else {
-#pragma unroll
-                                    for (int e = 0; e < OC; e++) oo[e] = fmaf(acc[e], vsc, oo[e]);
-                                }
+                                for (int e = 0; e < OC; e++) oo[e] = fmaf(acc[e], vsc, oo[e]);
                             }
                         }
                     }
                 }
             }
             __syncwarp();
-            fetch(chunk + Shape::kStages - 1, now);
+            fetch(st + S - 1);
         }
         cp_async_wait<0>();
 
-        // join the warps: maxima, sums, rows
-        if (poisoned) {
+        const bool starts = s0 == 0, ends = s1 == w.steps;
+        float* part = a.part + (size_t)(2 * run + (starts ? 1 : 0)) * part_floats<HD, RB>();
 #pragma unroll
-            for (int hf = 0; hf < (SPLIT ? 1 : 2); hf++) l[hf] = __int_as_float(0x7fffffff);
-        }
+        for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-        for (int hf = 0; hf < (SPLIT ? 1 : 2); hf++) {
-            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
-            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
-        }
-        __syncthreads();  // all warps have done with the ring
-        float* mine = join + warp * part_floats<HD, RB>();
+            for (int hf = 0; hf < HF; hf++) {
+                float sum = l[mt][hf];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (poisoned) sum = __int_as_float(0x7fffffff);
+                const int r = (SPLIT ? 8 : 16) * mt + g + 8 * hf;
+                if (r >= row_n) continue;
+                const bool whole = starts && ends;
+                // a NaN sum makes all of the row NaN
+                const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+                const int tok = (row_lo + r) / a.group, hq = (row_lo + r) - tok * a.group;
+                const int64_t dst = (int64_t)(w.first + tok) * a.out_stride + (int64_t)(at.kvh * a.group + hq) * hd;
+                if (!whole && c == 0) { part[r] = m[mt][hf]; part[RB + r] = sum; }
+                constexpr int GR = HD == 256 ? 2 : 1, W = HD == 64 ? 1 : 2;  // W runs of 16 dims
 #pragma unroll
-        for (int hf = 0; hf < (SPLIT ? 1 : 2); hf++) {
-            const int r = g + 8 * hf;
-            if (c == 0) { mine[r] = m[hf]; mine[RB + r] = l[hf]; }
+                for (int gr = 0; gr < GR; gr++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                // tile n = byte n of the dims that a thread's column owns
-                const int gr = HD == 256 ? n >> 4 : 0, byte = HD == 256 ? n & 15 : n;
-                const int width = HD == 64 ? 8 : 16;
-                mine[2 * RB + r * HD + 128 * gr + (2 * c) * width + byte] = o[n][2 * hf];
-                mine[2 * RB + r * HD + 128 * gr + (2 * c + 1) * width + byte] = o[n][2 * hf + 1];
+                    for (int x = 0; x < W; x++) {
+                        float v[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            // HD 64: dims 8 (2c) + e of the first column, then of the second
+                            const int tile = HD == 64 ? e & 7 : 16 * gr + e, col = HD == 64 ? e >> 3 : x;
+                            v[e] = o[mt][tile][2 * hf + col] * inv;
+                        }
+                        const int d = HD == 64 ? 16 * c : 128 * gr + 32 * c + 16 * x;
+                        if (!whole) store16(part + 2 * RB + r * HD + d, true, v);
+                        else if (FULL || d < hd) store16(a.out, dst + d, a.typ, a.out_vec, v);
+                    }
             }
-        }
-        __syncthreads();
-        const bool starts = c0 == 0, ends = c1 == w.chunks;
-        float* part = a.part + (size_t)(2 * blockIdx.x + (starts ? 1 : 0)) * part_floats<HD, RB>();
-        for (int e = tid; e < RB * HD; e += kRunWarps * 32) {
-            const int r = e / HD, d = e % HD;
-            if (r >= row_n) continue;
-            float mx = kNegInf;
-#pragma unroll
-            for (int x = 0; x < kRunWarps; x++) mx = fmaxf(mx, join[x * part_floats<HD, RB>() + r]);
-            const float ref = mx == kNegInf ? 0.0f : mx;
-            float sum = 0.0f, val = 0.0f;
-#pragma unroll
-            for (int x = 0; x < kRunWarps; x++) {
-                const float* px = join + x * part_floats<HD, RB>();
-                const float f = exp2_fast(px[r] - ref);
-                // a warp without a key has weight 0 and sum 0; a poisoned one has a NaN sum
-                sum += px[RB + r] == 0.0f ? 0.0f : isnan(px[RB + r]) ? px[RB + r] : f * px[RB + r];
-                val = fmaf(f, px[2 * RB + r * HD + d], val);
-            }
-            if (starts && ends) {
-                if (d < hd) {
-                    const int tok = (row_lo + r) / a.group, hq = (row_lo + r) % a.group;
-                    const float y = sum == 0.0f ? 0.0f : val / sum;
-                    ((T*)a.out)[(int64_t)(w.first + tok) * a.out_stride + (int64_t)(at.kvh * a.group + hq) * hd + d] = to_elem<T>(isnan(sum) ? sum : y);
-                }
-            } else {
-                if (d == 0) { part[r] = mx; part[RB + r] = sum; }
-                part[2 * RB + e] = val;
-            }
-        }
-        __syncthreads();
-        t += (uint32_t)(c1 - c0);
+        __syncwarp();
+        t += (uint32_t)(s1 - s0);
     }
 }
 
-// Joins the partial results of units that lie in several runs.  Block b looks at the border between runs b and b + 1 and serves the unit
-// across it, if run b is where that unit begins.
-template <typename T, int HD, int RB>
-__global__ void __launch_bounds__(128) kv8_join_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a, int runs) {
+// Joins the partial results of units that lie in several runs.  A border between runs b and b + 1 stands for the unit across it, if
+// run b is where that unit begins; a block looks at kRunWarps borders, one after the other.
+constexpr int kJoinThreads = 128;
+template <int HD, int RB>
+__global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a, int warps) {
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint32_t warp_sums[4];
+    __shared__ uint32_t warp_sums[kJoinThreads / 32];
+    __shared__ float4 s_val[kJoinThreads];
+    __shared__ float s_m[kJoinThreads], s_sum[kJoinThreads];
     uint32_t* cum = reinterpret_cast<uint32_t*>(smem);
     const uint32_t total = line_up<RB>(seqs, pool, a, cum, warp_sums);
     pdl_wait();  // every block: this kernel's end then means that of the one before
-    const int b = blockIdx.x;
-    const uint32_t border = run_start(total, b + 1, runs), start = run_start(total, b, runs);
-    if (border >= total || border == start) return;  // no unit there, or the run is empty
-    Place at;
-    place_at<RB>(at, seqs, pool, a, cum, border - 1);
-    const uint32_t u0 = at.unit_start, u1 = u0 + at.w.chunks;
-    if (u1 <= border || u0 < start) return;          // ends with the run; or began in an earlier one
-    int last = b + 1;                                // the run with the unit's last chunk
-    while (run_start(total, last + 1, runs) < u1) last++;
-    const int row_lo = at.rb * RB, row_n = min(RB, at.w.n * a.group - row_lo);
-    constexpr int P = part_floats<HD, RB>();
-    for (int e = threadIdx.x; e < row_n * HD; e += blockDim.x) {
-        const int r = e / HD, d = e % HD;
-        if (d >= pool.hd) continue;
-        const float* p = a.part + (size_t)(2 * b + 1) * P;
-        float mx = p[r], sum = p[RB + r], val = p[2 * RB + e];
-        for (int x = b + 1; x <= last; x++) {
-            if (run_start(total, x, runs) == run_start(total, x + 1, runs)) continue;  // an empty run leaves nothing
-            p = a.part + (size_t)(2 * x) * P;
-            const float m2 = fmaxf(mx, p[r]), ref = m2 == kNegInf ? 0.0f : m2;
-            const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(p[r] - ref);
-            sum = (isnan(sum) ? sum : f0 * sum) + (isnan(p[RB + r]) ? p[RB + r] : f1 * p[RB + r]);
-            val = fmaf(f0, val, f1 * p[2 * RB + e]);
-            mx = m2;
+    const Runs runs(total, warps);
+    constexpr int P = part_floats<HD, RB>(), Q = HD / 4;
+    for (uint32_t b = blockIdx.x * kRunWarps; b < (blockIdx.x + 1) * kRunWarps && b + 1 < runs.n; b++) {
+        const uint32_t border = runs.start(b + 1), start = runs.start(b);
+        Place at;
+        place_at<RB>(at, seqs, pool, a, cum, border - 1);
+        const uint32_t u0 = at.unit_start, u1 = u0 + at.w.steps;
+        if (u1 <= border || u0 < start) continue;        // ends with the run; or began in an earlier one
+        const uint32_t last = runs.run_of(u1 - 1);
+        const int row_lo = at.rb * RB, row_n = min(RB, at.w.n * a.group - row_lo);
+        // threads: four dims of a row each, as many shares of the partial results as there are threads for
+        const int cells = row_n * Q, per = min(cells, kJoinThreads), shares = kJoinThreads / per;
+        const int share = threadIdx.x / per;
+        for (int e0 = 0; e0 < cells; e0 += per) {
+            const int e = e0 + threadIdx.x - share * per, r = e / Q, d = (e - r * Q) * 4;
+            float mx = kNegInf, sum = 0.0f;
+            float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (share < shares && e < cells) {
+#pragma unroll 4
+                for (uint32_t x = b + share; x <= last; x += shares) {
+                    const float* p = a.part + (size_t)(2 * x + (x == b ? 1 : 0)) * P;
+                    const float pm = p[r], ps = p[RB + r];
+                    const float4 v = *reinterpret_cast<const float4*>(p + 2 * RB + r * HD + d);
+                    const float m2 = fmaxf(mx, pm), ref = m2 == kNegInf ? 0.0f : m2;
+                    const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(pm - ref);
+                    sum = f0 * sum + (isnan(ps) ? ps : f1 * ps);
+                    val.x = fmaf(f0, val.x, f1 * v.x); val.y = fmaf(f0, val.y, f1 * v.y);
+                    val.z = fmaf(f0, val.z, f1 * v.z); val.w = fmaf(f0, val.w, f1 * v.w);
+                    mx = m2;
+                }
+            }
+            if (shares > 1) {
+                __syncthreads();
+                s_val[threadIdx.x] = val; s_m[threadIdx.x] = mx; s_sum[threadIdx.x] = sum;
+                __syncthreads();
+                if (share == 0) {
+                    for (int x = 1; x < shares; x++) {
+                        const int i = x * per + threadIdx.x;
+                        const float m2 = fmaxf(mx, s_m[i]), ref = m2 == kNegInf ? 0.0f : m2;
+                        const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(s_m[i] - ref);
+                        const float4 v = s_val[i];
+                        sum = f0 * sum + f1 * s_sum[i];
+                        val.x = fmaf(f0, val.x, f1 * v.x); val.y = fmaf(f0, val.y, f1 * v.y);
+                        val.z = fmaf(f0, val.z, f1 * v.z); val.w = fmaf(f0, val.w, f1 * v.w);
+                        mx = m2;
+                    }
+                }
+            }
+            if (share == 0 && e < cells && d < pool.hd) {
+                const int tok = (row_lo + r) / a.group, hq = (row_lo + r) - tok * a.group;
+                const int64_t dst = (int64_t)(at.w.first + tok) * a.out_stride + (int64_t)(at.kvh * a.group + hq) * pool.hd + d;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                store1(a.out, dst, a.typ, val.x * inv);
+                store1(a.out, dst + 1, a.typ, val.y * inv);
+                store1(a.out, dst + 2, a.typ, val.z * inv);
+                store1(a.out, dst + 3, a.typ, val.w * inv);
+            }
         }
-        const int tok = (row_lo + r) / a.group, hq = (row_lo + r) % a.group;
-        const float y = isnan(sum) ? sum : sum == 0.0f ? 0.0f : val / sum;
-        ((T*)a.out)[(int64_t)(at.w.first + tok) * a.out_stride + (int64_t)(at.kvh * a.group + hq) * pool.hd + d] = to_elem<T>(y);
+        __syncthreads();
     }
 }
 
 struct RunPlan {
-    int hd, rb, blocks;
+    int hd, mt, blocks;
+    bool split;
     size_t bytes;
+    int rows() const { return mt * (split ? 8 : 16); }
 };
-// Rows of at most 8 per unit, and everything in f32, in the split form: its 22 bits come at no more products.
+// f32 is always in the split form, for its 22 bits; 16-bit types where a unit has 8 rows at most, since it costs no more products there.  Two
+// tiles share a step's keys and values where a unit has rows for them (heads of 256: their sums have no room in registers).
 RunPlan plan_runs(const Kv8Pool& pool, uint32_t typ, int group, int max_rows) {
     RunPlan p;
     p.hd = pool.hd <= 64 ? 64 : pool.hd <= 128 ? 128 : 256;
-    p.rb = typ == LC_TYPE_F32 || group * (max_rows < 1 ? 1 : max_rows) <= 8 ? 8 : 16;
-    p.blocks = sm_count() * (p.hd == 256 ? 2 : p.rb == 8 ? 4 : 3);
-    p.bytes = (size_t)2 * p.blocks * p.rb * (p.hd + 2) * sizeof(float);
+    const int64_t rows = (int64_t)group * (max_rows < 1 ? 1 : max_rows);
+    p.split = typ == LC_TYPE_F32 || rows <= 8;
+    p.mt = rows > (p.split ? 8 : 16) && p.hd < 256 ? 2 : 1;
+    p.blocks = sm_count() * (p.hd == 256 || p.mt > 1 ? 2 : p.split ? 4 : 3);
+    p.bytes = (size_t)2 * p.blocks * kRunWarps * p.rows() * (p.hd + 2) * sizeof(float);
     return p;
 }
 
-template <typename T, int HD, int RB>
+template <int HD, int MT, bool SPLIT, bool FULL>
 int32_t runs_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int blocks, cudaStream_t s) {
-    using Shape = RunShape<T, HD, RB>;
-    const size_t cum = (size_t)(seqs.n_seqs + 1) * 4;
-    const size_t smem = (Shape::kRing > Shape::kJoin ? Shape::kRing : Shape::kJoin) + cum;
-    LC_CUDA(ensure_smem_limit((const void*)kv8_runs_kernel<T, HD, RB>, smem));
-    kv8_runs_kernel<T, HD, RB><<<blocks, kRunWarps * 32, smem, s>>>(pool, seqs, a);
+    using Shape = RunShape<HD, MT, SPLIT>;
+    const size_t cum = (size_t)(seqs.n_seqs + 1) * 4, smem = kRunWarps * Shape::kWarp + cum;
+    LC_CUDA(ensure_smem_limit((const void*)kv8_runs_kernel<HD, MT, SPLIT, FULL>, smem));
+    kv8_runs_kernel<HD, MT, SPLIT, FULL><<<blocks, kRunWarps * 32, smem, s>>>(pool, seqs, a);
     LC_CUDA(cudaGetLastError());
-    LC_CUDA(launch_pdl(kv8_join_kernel<T, HD, RB>, dim3((unsigned)(blocks - 1)), dim3(128), cum, s, pool, seqs, a, blocks));
+    LC_CUDA(launch_pdl(kv8_join_kernel<HD, Shape::kRows>, dim3((unsigned)blocks), dim3(kJoinThreads), cum, s, pool, seqs, a, blocks * kRunWarps));
     return LC_OK;
 }
-template <typename T>
+template <int HD, int MT, bool SPLIT>
+int32_t runs_full(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int blocks, cudaStream_t s) {
+    return pool.hd == HD ? runs_as<HD, MT, SPLIT, true>(pool, seqs, a, blocks, s) : runs_as<HD, MT, SPLIT, false>(pool, seqs, a, blocks, s);
+}
+template <int HD>
 int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const RunPlan& p, cudaStream_t s) {
-    if (p.rb == 8) {
-        if (p.hd == 64) return runs_as<T, 64, 8>(pool, seqs, a, p.blocks, s);
-        if (p.hd == 128) return runs_as<T, 128, 8>(pool, seqs, a, p.blocks, s);
-        return runs_as<T, 256, 8>(pool, seqs, a, p.blocks, s);
-    }
-    if (p.hd == 64) return runs_as<T, 64, 16>(pool, seqs, a, p.blocks, s);
-    if (p.hd == 128) return runs_as<T, 128, 16>(pool, seqs, a, p.blocks, s);
-    return runs_as<T, 256, 16>(pool, seqs, a, p.blocks, s);
+    if constexpr (HD < 256)
+        if (p.mt == 2) return p.split ? runs_full<HD, 2, true>(pool, seqs, a, p.blocks, s) : runs_full<HD, 2, false>(pool, seqs, a, p.blocks, s);
+    return p.split ? runs_full<HD, 1, true>(pool, seqs, a, p.blocks, s) : runs_full<HD, 1, false>(pool, seqs, a, p.blocks, s);
 }
 
 int32_t check_heads(const char* call, const Kv8Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {
     LC_CHECK(n_heads > 0 && n_heads <= 65536 && n_heads % pool.n_kv == 0, LC_ERR_INVALID, "%s: %d heads over %d kv heads", call, n_heads, pool.n_kv);
     // places of the line, row blocks of 8 at worst, in 31 bits
-    const double chunks = (double)((int64_t)seqs.width << pool.page_shift) / kChunk + 2, blocks = (double)seqs.n_rows * (n_heads / pool.n_kv) / 8 + seqs.n_seqs;
+    const double chunks = (double)((int64_t)seqs.width << pool.page_shift) / kStep + 2, blocks = (double)seqs.n_rows * (n_heads / pool.n_kv) / 8 + seqs.n_seqs;
     LC_CHECK(chunks * blocks * pool.n_kv < 2147483648.0, LC_ERR_INVALID, "%s: %d rows of %d heads over tables of %d pages are too many for one call", call, seqs.n_rows, n_heads, seqs.width);
     return LC_OK;
 }
@@ -587,11 +702,13 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
     LC_CHECK(workspace_dev && workspace_bytes >= plan.bytes && (uintptr_t)workspace_dev % 16 == 0, LC_ERR_INVALID,
              "lc_attention_kv8_dev: needs a workspace of %zu bytes, 16-byte aligned (got %zu)", plan.bytes, workspace_bytes);
     if (scale == 0.0f) scale = 1.0f / sqrtf((float)pool.hd);
-    AttnArgs a{q_dev, out_dev, q_stride, out_stride, n_heads, group, window, scale * 1.44269504088896f, (float*)workspace_dev};
+    const size_t elem = typ == LC_TYPE_F32 ? 4 : 2;
+    AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, n_heads, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16),
+               scale * 1.44269504088896f, (float*)workspace_dev};
     cudaStream_t s = stream_or_own(stream_);
-    if (typ == LC_TYPE_F32) return runs_of<float>(pool, seqs, a, plan, s);
-    if (typ == LC_TYPE_F16) return runs_of<__half>(pool, seqs, a, plan, s);
-    return runs_of<__nv_bfloat16>(pool, seqs, a, plan, s);
+    if (plan.hd == 64) return runs_of<64>(pool, seqs, a, plan, s);
+    if (plan.hd == 128) return runs_of<128>(pool, seqs, a, plan, s);
+    return runs_of<256>(pool, seqs, a, plan, s);
 }
 
 }  // extern "C"

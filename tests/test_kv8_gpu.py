@@ -289,10 +289,14 @@ def test_bad_pages_and_rows_are_kept_out(gpu, dtype, new):
     the highest such sequence, and the others come out as ever."""
     seqs = [(50, new), (40, new), (30, new), (20, new)]
     good = Setup(gpu, seqs, 2, 64, 16, seed=11)
-    q, _ = good.normal(4, dtype)
+    q, q64 = good.normal(4, dtype)
     (k, _), (v, _) = good.normal(2, dtype), good.normal(2, dtype)
-    want = host(good.cache.attention(good.batch, q))
+    exact, mass, big, keys = good.plain.attention(good.table, good.ctx, good.start, q64)
+    bound = plain.attention_bound(exact, mass, big, keys, 64, dtype, dtype == "float32")
     n = lambda i: slice(int(good.start[i]), int(good.start[i + 1]))  # noqa: E731
+
+    def as_ever(out, i):  # within the bound of any call: where contexts are cut, and with it the order of sums, goes by all sequences of a call
+        return (np.abs(out[n(i)].astype(np.float64) - exact[n(i)]) <= bound[n(i)]).all()
 
     def attempt(table=None, ctx=None, start=None):
         s = Setup(gpu, seqs, 2, 64, 16, seed=11)
@@ -315,7 +319,7 @@ def test_bad_pages_and_rows_are_kept_out(gpu, dtype, new):
         assert status == (2, 2, 2)
         assert np.isnan(out[n(1)][-1]).all() and np.isnan(ko[n(1)][-1]).all()
         for i in (0, 2, 3):
-            assert np.array_equal(out[n(i)], want[n(i)])
+            assert as_ever(out, i)
     for bad in (-1, 10 ** 6, 2 ** 31 - 1, -2 ** 31):
         ctx = good.ctx.copy()
         ctx[2] = bad
@@ -323,14 +327,14 @@ def test_bad_pages_and_rows_are_kept_out(gpu, dtype, new):
         assert status == (3, 3, 3)
         assert np.isnan(out[n(2)]).all() and np.isnan(ko[n(2)]).all()
         for i in (0, 1, 3):
-            assert np.array_equal(out[n(i)], want[n(i)])
+            assert as_ever(out, i)
         for x, y in zip(before, after):                  # its pages stay as they were
             used = [int(p) for p in good.table[2] if p >= 0]
             assert torch.equal(x[used], y[used])
     for start in ([0, new, 2 * new, 3 * new, 2 ** 31 - 1], [-5, new, 2 * new, 3 * new, 4 * new], [0, new, 2 * new, 4 * new + 1, 4 * new]):
         out, ko, status, before, after = attempt(start=np.array(start, np.int32))
         assert min(status) > 0
-        assert np.array_equal(out[n(1)], want[n(1)])
+        assert as_ever(out, 1)
     # without a status word
     b = gpu.Kv8Rows(cuda(table), cuda(ctx), cuda(good.start), new)
     good.cache.attention(b, q)
