@@ -8,6 +8,7 @@
 // 2^(s - max + 8).  In the split form (RB = 8 rows to a tile of 16) rows 0 .. 7 of the tile hold the f16 value and rows 8 .. 15 what its
 // rounding lost, 22 bits together: the two halves of a sum lie in the same thread.  In the plain form (RB = 16) a tile holds 16 rows, weights
 // rounded to f16 (2^-12 of each).
+#include <algorithm>
 #include "lc_kv8.cuh"
 #include "lc_kernels.h"
 #include "lc_tma.cuh"
@@ -153,31 +154,41 @@ __device__ __forceinline__ SeqWork seq_work(const Kv8Seqs& s, const Kv8Pool& p, 
     }
     return w;
 }
-// cum[i] = steps of the sequences before i, cum[n_seqs] = all; by one block, returns the total
+// cum[i] = steps of the sequences before i, cum[n_seqs] = all; units[i] (if wanted) the units before i; by one block, returns the total
 template <int RB>
-__device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, uint32_t* cum, uint32_t* warp_sums) {
+__device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, uint32_t* cum, uint32_t* units, uint2* warp_sums) {
     const int per = (s.n_seqs + blockDim.x - 1) / blockDim.x, i0 = min((int)threadIdx.x * per, s.n_seqs), i1 = min(i0 + per, s.n_seqs);
-    uint32_t sum = 0;
+    uint32_t sum = 0, usum = 0;
     for (int i = i0; i < i1; i++) {
         const SeqWork w = seq_work<RB>(s, p, a, i);
         cum[i] = sum;
+        if (units) units[i] = usum;
         sum += (uint32_t)w.blocks * (uint32_t)p.n_kv * (uint32_t)w.steps;
+        usum += (uint32_t)w.blocks * (uint32_t)p.n_kv;
     }
-    uint32_t incl = sum;
+    uint32_t incl = sum, uincl = usum;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
+        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, uincl, o);
+        if (lane >= o) { incl += v; uincl += u; }
     }
-    if (lane == 31) warp_sums[warp] = incl;
+    if (lane == 31) warp_sums[warp] = make_uint2(incl, uincl);
     __syncthreads();
-    uint32_t before = incl - sum, total = 0;
+    uint32_t before = incl - sum, ubefore = uincl - usum, total = 0, utotal = 0;
     for (int w = 0; w < (int)(blockDim.x >> 5); w++) {
-        if (w < warp) before += warp_sums[w];
-        total += warp_sums[w];
+        const uint2 v = warp_sums[w];
+        if (w < warp) { before += v.x; ubefore += v.y; }
+        total += v.x;
+        utotal += v.y;
     }
-    for (int i = i0; i < i1; i++) cum[i] += before;
-    if (threadIdx.x == 0) cum[s.n_seqs] = total;
+    for (int i = i0; i < i1; i++) {
+        cum[i] += before;
+        if (units) units[i] += ubefore;
+    }
+    if (threadIdx.x == 0) {
+        cum[s.n_seqs] = total;
+        if (units) units[s.n_seqs] = utotal;
+    }
     __syncthreads();
     return total;
 }
@@ -247,12 +258,12 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
     constexpr int OC = 2 * HF;
     constexpr int S = Shape::kStages;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint32_t warp_sums[kRunWarps];
+    __shared__ uint2 warp_sums[kRunWarps];
     uint32_t* cum = reinterpret_cast<uint32_t*>(smem + kRunWarps * Shape::kWarp);
     pdl_launch_dependents();
     if (blockIdx.x == 0) kv8_check_seqs(seqs, pool);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const uint32_t total = line_up<RB>(seqs, pool, a, cum, warp_sums);
+    const uint32_t total = line_up<RB>(seqs, pool, a, cum, nullptr, warp_sums);
     const Runs runs(total, gridDim.x * kRunWarps);
     const uint32_t run = blockIdx.x * kRunWarps + warp;
     if (run >= runs.n) return;
@@ -541,77 +552,73 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
     }
 }
 
-// Joins the partial results of units that lie in several runs.  A border between runs b and b + 1 stands for the unit across it, if
-// run b is where that unit begins; a block looks at kRunWarps borders, one after the other.
+// Joins the partial results of units that lie in several runs.  grid: (units, slices of `per` groups of four dims of a unit's rows); what threads are
+// left over take shares of the partial results.
 constexpr int kJoinThreads = 128;
 template <int HD, int RB>
-__global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a, int warps) {
+__global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a, int warps, int per) {
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint32_t warp_sums[kJoinThreads / 32];
+    __shared__ uint2 warp_sums[kJoinThreads / 32];
     __shared__ float4 s_val[kJoinThreads];
     __shared__ float s_m[kJoinThreads], s_sum[kJoinThreads];
     uint32_t* cum = reinterpret_cast<uint32_t*>(smem);
-    const uint32_t total = line_up<RB>(seqs, pool, a, cum, warp_sums);
+    uint32_t* units = cum + seqs.n_seqs + 1;
+    const uint32_t total = line_up<RB>(seqs, pool, a, cum, units, warp_sums);
     pdl_wait();  // every block: this kernel's end then means that of the one before
     const Runs runs(total, warps);
     constexpr int P = part_floats<HD, RB>(), Q = HD / 4;
-    for (uint32_t b = blockIdx.x * kRunWarps; b < (blockIdx.x + 1) * kRunWarps && b + 1 < runs.n; b++) {
-        const uint32_t border = runs.start(b + 1), start = runs.start(b);
-        Place at;
-        place_at<RB>(at, seqs, pool, a, cum, border - 1);
-        const uint32_t u0 = at.unit_start, u1 = u0 + at.w.steps;
-        if (u1 <= border || u0 < start) continue;        // ends with the run; or began in an earlier one
-        const uint32_t last = runs.run_of(u1 - 1);
-        const int row_lo = at.rb * RB, row_n = min(RB, at.w.n * a.group - row_lo);
-        // threads: four dims of a row each, as many shares of the partial results as there are threads for
-        const int cells = row_n * Q, per = min(cells, kJoinThreads), shares = kJoinThreads / per;
-        const int share = threadIdx.x / per;
-        for (int e0 = 0; e0 < cells; e0 += per) {
-            const int e = e0 + threadIdx.x - share * per, r = e / Q, d = (e - r * Q) * 4;
-            float mx = kNegInf, sum = 0.0f;
-            float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (share < shares && e < cells) {
+    const int shares = kJoinThreads / per, share = threadIdx.x / per, e = blockIdx.y * per + threadIdx.x - share * per;
+    const int r = e / Q, d = (e - r * Q) * 4;
+    for (uint32_t u = blockIdx.x; u < units[seqs.n_seqs]; u += gridDim.x) {
+        const int i = seq_at(units, seqs.n_seqs, u);
+        const SeqWork w = seq_work<RB>(seqs, pool, a, i);
+        const uint32_t in = u - units[i], u0 = cum[i] + in * w.steps;
+        const uint32_t b = runs.run_of(u0), last = runs.run_of(u0 + w.steps - 1);
+        if (b == last) continue;                         // that run has written the rows
+        const int kvh = in / w.blocks, row_lo = (in - kvh * w.blocks) * RB, row_n = min(RB, w.n * a.group - row_lo);
+        const bool here = r < row_n;
+        float mx = kNegInf, sum = 0.0f;
+        float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (here) {
 #pragma unroll 4
-                for (uint32_t x = b + share; x <= last; x += shares) {
-                    const float* p = a.part + (size_t)(2 * x + (x == b ? 1 : 0)) * P;
-                    const float pm = p[r], ps = p[RB + r];
-                    const float4 v = *reinterpret_cast<const float4*>(p + 2 * RB + r * HD + d);
-                    const float m2 = fmaxf(mx, pm), ref = m2 == kNegInf ? 0.0f : m2;
-                    const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(pm - ref);
-                    sum = f0 * sum + (isnan(ps) ? ps : f1 * ps);
+            for (uint32_t x = b + share; x <= last; x += shares) {
+                const float* p = a.part + (size_t)(2 * x + (x == b ? 1 : 0)) * P;
+                const float pm = p[r], ps = p[RB + r];
+                const float4 v = *reinterpret_cast<const float4*>(p + 2 * RB + r * HD + d);
+                const float m2 = fmaxf(mx, pm), ref = m2 == kNegInf ? 0.0f : m2;
+                const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(pm - ref);
+                sum = f0 * sum + (isnan(ps) ? ps : f1 * ps);
+                val.x = fmaf(f0, val.x, f1 * v.x); val.y = fmaf(f0, val.y, f1 * v.y);
+                val.z = fmaf(f0, val.z, f1 * v.z); val.w = fmaf(f0, val.w, f1 * v.w);
+                mx = m2;
+            }
+        }
+        if (shares > 1) {
+            __syncthreads();
+            s_val[threadIdx.x] = val; s_m[threadIdx.x] = mx; s_sum[threadIdx.x] = sum;
+            __syncthreads();
+            if (share == 0 && here) {
+                for (int x = 1; x < shares; x++) {
+                    const int k = x * per + threadIdx.x;
+                    const float m2 = fmaxf(mx, s_m[k]), ref = m2 == kNegInf ? 0.0f : m2;
+                    const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(s_m[k] - ref);
+                    const float4 v = s_val[k];
+                    sum = f0 * sum + f1 * s_sum[k];
                     val.x = fmaf(f0, val.x, f1 * v.x); val.y = fmaf(f0, val.y, f1 * v.y);
                     val.z = fmaf(f0, val.z, f1 * v.z); val.w = fmaf(f0, val.w, f1 * v.w);
                     mx = m2;
                 }
             }
-            if (shares > 1) {
-                __syncthreads();
-                s_val[threadIdx.x] = val; s_m[threadIdx.x] = mx; s_sum[threadIdx.x] = sum;
-                __syncthreads();
-                if (share == 0) {
-                    for (int x = 1; x < shares; x++) {
-                        const int i = x * per + threadIdx.x;
-                        const float m2 = fmaxf(mx, s_m[i]), ref = m2 == kNegInf ? 0.0f : m2;
-                        const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(s_m[i] - ref);
-                        const float4 v = s_val[i];
-                        sum = f0 * sum + f1 * s_sum[i];
-                        val.x = fmaf(f0, val.x, f1 * v.x); val.y = fmaf(f0, val.y, f1 * v.y);
-                        val.z = fmaf(f0, val.z, f1 * v.z); val.w = fmaf(f0, val.w, f1 * v.w);
-                        mx = m2;
-                    }
-                }
-            }
-            if (share == 0 && e < cells && d < pool.hd) {
-                const int tok = (row_lo + r) / a.group, hq = (row_lo + r) - tok * a.group;
-                const int64_t dst = (int64_t)(at.w.first + tok) * a.out_stride + (int64_t)(at.kvh * a.group + hq) * pool.hd + d;
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                store1(a.out, dst, a.typ, val.x * inv);
-                store1(a.out, dst + 1, a.typ, val.y * inv);
-                store1(a.out, dst + 2, a.typ, val.z * inv);
-                store1(a.out, dst + 3, a.typ, val.w * inv);
-            }
         }
-        __syncthreads();
+        if (share == 0 && here && d < pool.hd) {
+            const int tok = (row_lo + r) / a.group, hq = (row_lo + r) - tok * a.group;
+            const int64_t dst = (int64_t)(w.first + tok) * a.out_stride + (int64_t)(kvh * a.group + hq) * pool.hd + d;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            store1(a.out, dst, a.typ, val.x * inv);
+            store1(a.out, dst + 1, a.typ, val.y * inv);
+            store1(a.out, dst + 2, a.typ, val.z * inv);
+            store1(a.out, dst + 3, a.typ, val.w * inv);
+        }
     }
 }
 
@@ -635,24 +642,30 @@ RunPlan plan_runs(const Kv8Pool& pool, uint32_t typ, int group, int max_rows) {
 }
 
 template <int HD, int MT, bool SPLIT, bool FULL>
-int32_t runs_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int blocks, cudaStream_t s) {
+int32_t runs_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, int blocks, cudaStream_t s) {
     using Shape = RunShape<HD, MT, SPLIT>;
     const size_t cum = (size_t)(seqs.n_seqs + 1) * 4, smem = kRunWarps * Shape::kWarp + cum;
     LC_CUDA(ensure_smem_limit((const void*)kv8_runs_kernel<HD, MT, SPLIT, FULL>, smem));
     kv8_runs_kernel<HD, MT, SPLIT, FULL><<<blocks, kRunWarps * 32, smem, s>>>(pool, seqs, a);
     LC_CUDA(cudaGetLastError());
-    LC_CUDA(launch_pdl(kv8_join_kernel<HD, Shape::kRows>, dim3((unsigned)blocks), dim3(kJoinThreads), cum, s, pool, seqs, a, blocks * kRunWarps));
+    // units by what max_rows says (the kernel goes on to more); few of them are cut into thinner slices, with more shares
+    const int64_t rows = std::min<int64_t>(Shape::kRows, (int64_t)a.group * std::max(1, max_rows));
+    const int64_t units = std::min<int64_t>(4096, ((int64_t)seqs.n_rows * a.group / Shape::kRows + seqs.n_seqs) * pool.n_kv);
+    int per = kJoinThreads;
+    while (per > 32 && units * ((rows * HD / 4 + per - 1) / per) < 2 * sm_count()) per /= 2;
+    const unsigned slices = (unsigned)((Shape::kRows * HD / 4 + per - 1) / per);
+    LC_CUDA(launch_pdl(kv8_join_kernel<HD, Shape::kRows>, dim3((unsigned)units, slices), dim3(kJoinThreads), 2 * cum, s, pool, seqs, a, blocks * kRunWarps, per));
     return LC_OK;
 }
 template <int HD, int MT, bool SPLIT>
-int32_t runs_full(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int blocks, cudaStream_t s) {
-    return pool.hd == HD ? runs_as<HD, MT, SPLIT, true>(pool, seqs, a, blocks, s) : runs_as<HD, MT, SPLIT, false>(pool, seqs, a, blocks, s);
+int32_t runs_full(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, int blocks, cudaStream_t s) {
+    return pool.hd == HD ? runs_as<HD, MT, SPLIT, true>(pool, seqs, a, max_rows, blocks, s) : runs_as<HD, MT, SPLIT, false>(pool, seqs, a, max_rows, blocks, s);
 }
 template <int HD>
-int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const RunPlan& p, cudaStream_t s) {
+int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, const RunPlan& p, cudaStream_t s) {
     if constexpr (HD < 256)
-        if (p.mt == 2) return p.split ? runs_full<HD, 2, true>(pool, seqs, a, p.blocks, s) : runs_full<HD, 2, false>(pool, seqs, a, p.blocks, s);
-    return p.split ? runs_full<HD, 1, true>(pool, seqs, a, p.blocks, s) : runs_full<HD, 1, false>(pool, seqs, a, p.blocks, s);
+        if (p.mt == 2) return p.split ? runs_full<HD, 2, true>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 2, false>(pool, seqs, a, max_rows, p.blocks, s);
+    return p.split ? runs_full<HD, 1, true>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 1, false>(pool, seqs, a, max_rows, p.blocks, s);
 }
 
 int32_t check_heads(const char* call, const Kv8Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {
@@ -706,9 +719,9 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
     AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, n_heads, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16),
                scale * 1.44269504088896f, (float*)workspace_dev};
     cudaStream_t s = stream_or_own(stream_);
-    if (plan.hd == 64) return runs_of<64>(pool, seqs, a, plan, s);
-    if (plan.hd == 128) return runs_of<128>(pool, seqs, a, plan, s);
-    return runs_of<256>(pool, seqs, a, plan, s);
+    if (plan.hd == 64) return runs_of<64>(pool, seqs, a, rows->max_rows, plan, s);
+    if (plan.hd == 128) return runs_of<128>(pool, seqs, a, rows->max_rows, plan, s);
+    return runs_of<256>(pool, seqs, a, rows->max_rows, plan, s);
 }
 
 }  // extern "C"

@@ -19,9 +19,9 @@
 namespace lc {
 
 int32_t DeviceScope::enter(const void* dev_ptr, const char* what) {
-    if (!have_device()) return LC_ERR_CUDA;
     cudaPointerAttributes a;
     const cudaError_t e = cudaPointerGetAttributes(&a, dev_ptr);
+    if (e != cudaSuccess && !have_device()) return LC_ERR_CUDA;
     if (e != cudaSuccess || (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)) {
         (void)cudaGetLastError();
         set_error("%s: not a device pointer", what);

@@ -15,44 +15,46 @@ from . import _capi
 from ._capi import TYPE_BF16, TYPE_F16, TYPE_F32, Kv8CacheStruct, Kv8RowsStruct, check, load
 
 _TYPES = {}
+_raw_stream = None
 
 
 def _torch():
+    global _raw_stream
     import torch
     if not _TYPES:
         _TYPES.update({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16})
+        # the handle of the current stream alone, where torch has a way to it: making a stream object costs 2 us
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
     return torch
 
 
-def _stream(device, stream):
-    """A cudaStream_t: the current stream of the device where none is given.  Handle 0 is the legacy stream there; the library takes 0 for its own."""
-    if stream is None:
-        stream = _torch().cuda.current_stream(device)
-    handle = getattr(stream, "cuda_stream", stream)
+def _stream(index, stream):
+    """A cudaStream_t: the current stream of device `index` where none is given.  Handle 0 is the legacy stream there; the library takes 0 for its own."""
+    handle = _raw_stream(index) if stream is None else getattr(stream, "cuda_stream", stream)
     return handle or 1  # cudaStreamLegacy
 
 
 def _typ(t):
-    torch = _torch()
+    if not _TYPES:
+        _torch()
     typ = _TYPES.get(t.dtype)
     if typ is None:
         raise ValueError(f"{t.dtype}: float32, float16 and bfloat16 are taken")
-    return torch, typ
+    return typ
 
 
-def _on(device, *tensors):
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"a tensor is on {t.device}, the others are on {device}")
+def _elsewhere(index, *tensors):
+    raise ValueError(f"tensors on one device expected: {['cuda:%d' % index if index >= 0 else 'cpu'] + [str(t.device) for t in tensors if t is not None]}")
 
 
 def _rows(t, heads, dim, what):
     """Rows [n][heads][dim] whose heads and dims are contiguous: the distance between rows, in elements."""
-    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{what}: [rows, {heads if heads is not None else 'heads'}, {dim}] expected, got {list(t.shape)}")
-    if t.shape[0] and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim)):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what}: [rows, {heads if heads is not None else 'heads'}, {dim}] expected, got {list(shape)}")
+    if shape[0] and (stride[2] != 1 or (shape[1] > 1 and stride[1] != dim)):
         raise ValueError(f"{what}: the heads of a row must be contiguous")
-    return max(t.stride(0), t.shape[1] * dim) if t.shape[0] <= 1 else t.stride(0)
+    return stride[0] if shape[0] > 1 else shape[1] * dim
 
 
 def _contiguous(what, dtype, *tensors):
@@ -85,8 +87,9 @@ class Kv8Rows:
             _contiguous("Kv8Rows", torch.int32, status)
             if status.numel() < 1:
                 raise ValueError("Kv8Rows: status has no element")
-        self.device = page_table.device
-        _on(self.device, ctx, row_start, status)
+        self.index = page_table.get_device()
+        if ctx.get_device() != self.index or row_start.get_device() != self.index or (status is not None and status.get_device() != self.index):
+            _elsewhere(self.index, ctx, row_start, status)
         self._kept = (page_table, ctx, row_start, status)
         self.struct = Kv8RowsStruct(page_table.data_ptr(), ctx.data_ptr(), row_start.data_ptr(), status.data_ptr() if status is not None else None,
                                     n, page_table.shape[1], max_rows, 0)
@@ -103,8 +106,9 @@ class Kv8Cache:
             raise ValueError("Kv8Cache: k and v [pages, kv heads, page_tokens, head_dim], scales [pages, kv heads] expected")
         _contiguous("Kv8Cache", torch.int8, k, v)
         _contiguous("Kv8Cache", torch.float32, k_scale, v_scale)
-        self.device = k.device
-        _on(self.device, v, k_scale, v_scale)
+        self.device, self.index = k.device, k.get_device()
+        if v.get_device() != self.index or k_scale.get_device() != self.index or v_scale.get_device() != self.index:
+            _elsewhere(self.index, v, k_scale, v_scale)
         self._kept = (k, v, k_scale, v_scale)
         self.n_kv_heads, self.page_tokens, self.head_dim = k.shape[1:]
         self.struct = Kv8CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
@@ -114,27 +118,31 @@ class Kv8Cache:
         """Appends rows of keys and values [rows, kv heads, head_dim] at their positions, the keys rotated by `turns` (rope_turns on the GPU; None: not
         rotated), q [rows, heads, head_dim] likewise into q_out (None: a new tensor; it may be q).  Returns q_out.  A page that receives rows
         must belong to one sequence of the call."""
-        torch, typ = _typ(k)
-        if v.dtype != k.dtype or v.shape[0] != k.shape[0]:
+        typ, n, index = _typ(k), k.shape[0], self.index
+        if v.dtype != k.dtype or v.shape[0] != n:
             raise ValueError("append: keys and values of one type and as many rows expected")
         ks, vs = _rows(k, self.n_kv_heads, self.head_dim, "k"), _rows(v, self.n_kv_heads, self.head_dim, "v")
-        _on(self.device, rows, k, v, turns, q, q_out)
-        qp = qs = op = os = heads = 0
+        if rows.index != index or k.get_device() != index or v.get_device() != index:
+            _elsewhere(index, k, v)
+        qp = qs = op = os = heads = tp = rot = 0
         if q is not None:
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            if q.dtype != k.dtype or q_out.dtype != k.dtype or q.shape[0] != k.shape[0] or q_out.shape != q.shape:
-                raise ValueError("append: queries of the keys' type and as many rows expected, q_out like q")
+                q_out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
             heads = q.shape[1]
+            if q.dtype != k.dtype or q_out.dtype != k.dtype or q.shape[0] != n or q_out.shape[0] != n:
+                raise ValueError("append: queries of the keys' type and as many rows expected, q_out like q")
             qs, os = _rows(q, None, self.head_dim, "q"), _rows(q_out, heads, self.head_dim, "q_out")
             qp, op = q.data_ptr(), q_out.data_ptr()
-        tp = rot = 0
+            if q.get_device() != index or q_out.get_device() != index:
+                _elsewhere(index, q, q_out)
         if turns is not None:
             if turns.element_size() != 8 or turns.is_floating_point() or not turns.is_contiguous() or turns.dim() != 1:
                 raise ValueError("append: turns are contiguous 64-bit integers")
+            if turns.get_device() != index:
+                _elsewhere(index, turns)
             tp, rot = turns.data_ptr(), 2 * turns.shape[0]
-        check(load().lc_kv8_append_dev(self._ref, rows._ref, typ, k.shape[0], k.data_ptr(), ks, v.data_ptr(), vs, qp, qs, op, os, heads, tp, rot,
-                                       _stream(self.device, stream)))
+        check(load().lc_kv8_append_dev(self._ref, rows._ref, typ, n, k.data_ptr(), ks, v.data_ptr(), vs, qp, qs, op, os, heads, tp, rot,
+                                       _stream(index, stream)))
         return q_out
 
     def read(self, rows: Kv8Rows, k_out=None, v_out=None, stream=None):
@@ -142,20 +150,21 @@ class Kv8Cache:
         some = k_out if k_out is not None else v_out
         if some is None:
             raise ValueError("read: nothing to read into")
-        _, typ = _typ(some)
-        _on(self.device, rows, k_out, v_out)
+        typ = _typ(some)
+        if rows.index != self.index or some.get_device() != self.index or (v_out is not None and v_out.get_device() != self.index):
+            _elsewhere(self.index, k_out, v_out)
         p, s = [0, 0], [0, 0]
         for i, t in enumerate((k_out, v_out)):
             if t is not None:
                 if t.dtype != some.dtype or t.shape[0] != some.shape[0]:
                     raise ValueError("read: k_out and v_out of one type and as many rows expected")
                 p[i], s[i] = t.data_ptr(), _rows(t, self.n_kv_heads, self.head_dim, "k_out" if i == 0 else "v_out")
-        check(load().lc_kv8_read_dev(self._ref, rows._ref, typ, some.shape[0], p[0], s[0], p[1], s[1], _stream(self.device, stream)))
+        check(load().lc_kv8_read_dev(self._ref, rows._ref, typ, some.shape[0], p[0], s[0], p[1], s[1], _stream(self.index, stream)))
         return k_out, v_out
 
     def attention_workspace(self, rows: Kv8Rows, q) -> int:
         """Bytes of workspace of attention over such rows."""
-        _, typ = _typ(q)
+        typ = _typ(q)
         out = C.c_size_t()
         check(load().lc_attention_kv8_workspace(self._ref, rows._ref, typ, q.shape[0], q.shape[1], C.byref(out)))
         return int(out.value)
@@ -164,23 +173,24 @@ class Kv8Cache:
         """Attention of q [rows, heads, head_dim], already rotated, over the cache: each row attends to the positions up to its own (with
         window > 0 to the last `window` of them), which the cache already holds.  scale None: 1 / sqrt(head_dim).  Returns out.  workspace: a uint8 tensor of
         attention_workspace bytes (None: a new one); calls that may run at the same time need one each."""
-        torch, typ = _typ(q)
+        typ, index = _typ(q), self.index
         qs = _rows(q, None, self.head_dim, "q")
+        n, heads = q.shape[:2]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if out.dtype != q.dtype or out.shape != q.shape:
+            out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+        if out.dtype != q.dtype or out.shape[0] != n:
             raise ValueError("attention: out like q expected")
-        os = _rows(out, q.shape[1], self.head_dim, "out")
+        os = _rows(out, heads, self.head_dim, "out")
         if workspace is None:
-            on = stream if hasattr(stream, "cuda_stream") else None
-            if stream is not None and on is None:
+            torch = _torch()
+            if stream is not None and not hasattr(stream, "cuda_stream"):
                 raise ValueError("attention: a stream given as a number needs a workspace of the caller's")
-            with torch.cuda.stream(on) if on is not None else torch.cuda.device(self.device):
+            with torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.device):
                 workspace = torch.empty(self.attention_workspace(rows, q), dtype=torch.uint8, device=self.device)
-        _on(self.device, rows, q, out, workspace)
-        check(load().lc_attention_kv8_dev(self._ref, rows._ref, typ, q.shape[0], q.data_ptr(), qs, q.shape[1], float(scale) if scale is not None else 0.0, window,
-                                          out.data_ptr(), os, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                                          _stream(self.device, stream)))
+        if rows.index != index or q.get_device() != index or out.get_device() != index or workspace.get_device() != index:
+            _elsewhere(index, q, out, workspace)
+        check(load().lc_attention_kv8_dev(self._ref, rows._ref, typ, n, q.data_ptr(), qs, heads, 0.0 if scale is None else scale, window, out.data_ptr(), os,
+                                          workspace.data_ptr(), workspace.nbytes, _stream(index, stream)))
         return out
 
 
@@ -188,25 +198,31 @@ def token_logprobs_dev(logits, tokens, logprob=None, entropy=None, top_logprob=N
     """Log probabilities of `tokens` (int64 [rows]) under logits [rows, vocab], entropies of the rows (nats), and the `top` likeliest tokens with theirs
     (larger logit first, equal ones by the lower index).  Outputs that are None are made; `top` (0 .. 32) is the width of
     top_id where that is given, else 0 unless said.  Returns (logprob, entropy, top_logprob, top_id)."""
-    torch, typ = _typ(logits)
-    if logits.dim() != 2 or (logits.shape[0] and logits.shape[1] > 1 and logits.stride(1) != 1):
+    typ, index = _typ(logits), logits.get_device()
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[0] and shape[1] > 1 and stride[1] != 1):
         raise ValueError("token_logprobs_dev: logits [rows, vocab] with contiguous rows expected")
-    rows, vocab = logits.shape
+    rows, vocab = shape
+    torch = _torch()
     if (top_logprob is None) != (top_id is None):
         raise ValueError("token_logprobs_dev: top_logprob and top_id go together")
     if top_id is not None and top is not None and top_id.shape[-1] != top:
         raise ValueError("token_logprobs_dev: top_id is not `top` wide")
     top = top_id.shape[-1] if top_id is not None else top or 0
-    new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=logits.device)  # noqa: E731
-    logprob = new(torch.float32, rows) if logprob is None else logprob
-    entropy = new(torch.float32, rows) if entropy is None else entropy
+    if logprob is None:
+        logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    if entropy is None:
+        entropy = torch.empty(rows, dtype=torch.float32, device=logits.device)
     if top_id is None:
-        top_logprob, top_id = new(torch.float32, rows, max(top, 0)), new(torch.int64, rows, max(top, 0))
-    _on(logits.device, tokens, logprob, entropy, top_logprob, top_id)
+        top_logprob = torch.empty(rows, max(top, 0), dtype=torch.float32, device=logits.device)
+        top_id = torch.empty(rows, max(top, 0), dtype=torch.int64, device=logits.device)
     _contiguous("token_logprobs_dev", torch.int64, tokens, top_id)
     _contiguous("token_logprobs_dev", torch.float32, logprob, entropy, top_logprob)
-    if tokens.shape != (rows,) or logprob.shape != (rows,) or entropy.shape != (rows,) or top_logprob.shape != (rows, top) or top_id.shape != (rows, top):
+    one, wide = (rows,), (rows, top)
+    if tokens.shape != one or logprob.shape != one or entropy.shape != one or top_logprob.shape != wide or top_id.shape != wide:
         raise ValueError("token_logprobs_dev: one token and one output per row expected")
-    check(load().lc_token_logprobs_dev(typ, logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, tokens.data_ptr(), top, logprob.data_ptr(),
-                                       entropy.data_ptr(), top_logprob.data_ptr(), top_id.data_ptr(), _stream(logits.device, stream)))
+    if any(t.get_device() != index for t in (tokens, logprob, entropy, top_logprob, top_id)):
+        _elsewhere(index, tokens, logprob, entropy, top_logprob, top_id)
+    check(load().lc_token_logprobs_dev(typ, logits.data_ptr(), rows, vocab, stride[0] if rows > 1 else vocab, tokens.data_ptr(), top, logprob.data_ptr(),
+                                       entropy.data_ptr(), top_logprob.data_ptr(), top_id.data_ptr(), _stream(index, stream)))
     return logprob, entropy, top_logprob, top_id
