@@ -11,115 +11,13 @@
 #include <algorithm>
 #include "lc_kv8.cuh"
 #include "lc_kernels.h"
-#include "lc_tma.cuh"
+#include "lc_kv8_attn.cuh"
 
 namespace lc {
 
 namespace {
 
-constexpr int kStep = 16;            // keys of a warp's step: one page's, or a part of one page's
 constexpr int kRunWarps = 4;
-constexpr float kNegInf = -INFINITY;
-
-struct AttnArgs {
-    const void* q;
-    void* out;
-    int64_t q_stride, out_stride;
-    int typ, n_heads, group, window;
-    bool q_vec, out_vec;             // 16-byte accesses
-    float scale_log2;                // scale * log2(e)
-    float* part;                     // partial results of runs that end inside a unit
-};
-
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t h2_pack(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-// (a, b) as f16 and what that rounding lost, as f16
-__device__ __forceinline__ void h2_split(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = h2_pack(a - __low2float(h), b - __high2float(h));
-}
-// Bytes 0, 1 (or 2, 3) of x = integers + 128 as f16 integers: 0x64 is the high byte of 1024.0, and 1152 = 1024 + 128.
-__device__ __forceinline__ uint32_t minus_1152(uint32_t v) {
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(1152.0f));
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t ints01(uint32_t x) { return minus_1152(__byte_perm(x, 0x64646464u, 0x4140u)); }
-__device__ __forceinline__ uint32_t ints23(uint32_t x) { return minus_1152(__byte_perm(x, 0x64646464u, 0x4342u)); }
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// sixteen elements in a row as f32, and back
-template <typename T> __device__ __forceinline__ void load16(const T* p, bool vec, float* v) {
-    constexpr int E = 16 / sizeof(T);
-    if (vec) {
-#pragma unroll
-        for (int u = 0; u < 16 / E; u++) {
-            __align__(16) T t[E];
-            *reinterpret_cast<uint4*>(t) = reinterpret_cast<const uint4*>(p)[u];
-#pragma unroll
-            for (int e = 0; e < E; e++) v[u * E + e] = elem_f(t[e]);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) v[e] = elem_f(p[e]);
-    }
-}
-__device__ __forceinline__ void load16(const void* p, int64_t at, int typ, bool vec, float* v) {
-    if (typ == LC_TYPE_F32) load16((const float*)p + at, vec, v);
-    else if (typ == LC_TYPE_F16) load16((const __half*)p + at, vec, v);
-    else load16((const __nv_bfloat16*)p + at, vec, v);
-}
-template <typename T> __device__ __forceinline__ void store16(T* p, bool vec, const float* v) {
-    constexpr int E = 16 / sizeof(T);
-    if (vec) {
-#pragma unroll
-        for (int u = 0; u < 16 / E; u++) {
-            __align__(16) T t[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) t[e] = to_elem<T>(v[u * E + e]);
-            reinterpret_cast<uint4*>(p)[u] = *reinterpret_cast<const uint4*>(t);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) p[e] = to_elem<T>(v[e]);
-    }
-}
-__device__ __forceinline__ void store16(void* p, int64_t at, int typ, bool vec, const float* v) {
-    if (typ == LC_TYPE_F32) store16((float*)p + at, vec, v);
-    else if (typ == LC_TYPE_F16) store16((__half*)p + at, vec, v);
-    else store16((__nv_bfloat16*)p + at, vec, v);
-}
-__device__ __forceinline__ void store1(void* p, int64_t at, int typ, float v) {
-    if (typ == LC_TYPE_F32) ((float*)p)[at] = v;
-    else if (typ == LC_TYPE_F16) ((__half*)p)[at] = to_elem<__half>(v);
-    else ((__nv_bfloat16*)p)[at] = to_elem<__nv_bfloat16>(v);
-}
-// a power of two that brings the largest magnitude of a row into [2^14, 2^15), and its inverse; 1 for a row of zeros or with infinities
-__device__ __forceinline__ void row_scale(float top, float& up, float& down) {
-    const int e = (__float_as_int(top) >> 23) & 0xff;
-    int s = 127 + 14 - (e - 127);
-    s = s < 1 ? 1 : s > 253 ? 253 : s;
-    if (top == 0.0f || e == 255) s = 127;
-    up = __int_as_float(s << 23);
-    down = __int_as_float((254 - s) << 23);
-}
 
 // ------------------------------------------------------------------------------------------------------------------------------------
 // Runs: few rows per sequence.  A unit is (sequence, kv head, row block of RB rows = tokens x heads of the group); its keys are cut into
@@ -132,74 +30,6 @@ __device__ __forceinline__ void row_scale(float top, float& up, float& down) {
 // the weighted sum are 16 neighbouring dims of its four keys.  What it ends with is 32 neighbouring dims (HD 64: 16) of its row.
 // ------------------------------------------------------------------------------------------------------------------------------------
 
-struct SeqWork {
-    int first, n, ctx, blocks, step0, steps;  // rows, context, row blocks, first step, steps per unit
-    bool inside;
-};
-template <int RB>
-__device__ __forceinline__ SeqWork seq_work(const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, int i) {
-    SeqWork w;
-    w.inside = false;
-    w.blocks = w.step0 = w.steps = 0;
-    w.ctx = s.ctx[i];
-    if (!kv8_span(s, i, w.first, w.n) || w.n == 0) { w.n = 0; return w; }
-    w.blocks = (w.n * a.group + RB - 1) / RB;
-    w.inside = kv8_in_table(s, p, w.ctx, w.n);
-    if (w.inside) {
-        const int lo = a.window > 0 ? max(0, w.ctx - a.window + 1) : 0;
-        w.step0 = lo / kStep;
-        w.steps = (w.ctx + w.n + kStep - 1) / kStep - w.step0;
-    } else {
-        w.steps = 1;  // one step that writes NaN
-    }
-    return w;
-}
-// cum[i] = steps of the sequences before i, cum[n_seqs] = all; units[i] (if wanted) the units before i; by one block, returns the total
-template <int RB>
-__device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, uint32_t* cum, uint32_t* units, uint2* warp_sums) {
-    const int per = (s.n_seqs + blockDim.x - 1) / blockDim.x, i0 = min((int)threadIdx.x * per, s.n_seqs), i1 = min(i0 + per, s.n_seqs);
-    uint32_t sum = 0, usum = 0;
-    for (int i = i0; i < i1; i++) {
-        const SeqWork w = seq_work<RB>(s, p, a, i);
-        cum[i] = sum;
-        if (units) units[i] = usum;
-        sum += (uint32_t)w.blocks * (uint32_t)p.n_kv * (uint32_t)w.steps;
-        usum += (uint32_t)w.blocks * (uint32_t)p.n_kv;
-    }
-    uint32_t incl = sum, uincl = usum;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, uincl, o);
-        if (lane >= o) { incl += v; uincl += u; }
-    }
-    if (lane == 31) warp_sums[warp] = make_uint2(incl, uincl);
-    __syncthreads();
-    uint32_t before = incl - sum, ubefore = uincl - usum, total = 0, utotal = 0;
-    for (int w = 0; w < (int)(blockDim.x >> 5); w++) {
-        const uint2 v = warp_sums[w];
-        if (w < warp) { before += v.x; ubefore += v.y; }
-        total += v.x;
-        utotal += v.y;
-    }
-    for (int i = i0; i < i1; i++) {
-        cum[i] += before;
-        if (units) units[i] += ubefore;
-    }
-    if (threadIdx.x == 0) {
-        cum[s.n_seqs] = total;
-        if (units) units[s.n_seqs] = utotal;
-    }
-    __syncthreads();
-    return total;
-}
-__device__ __forceinline__ int seq_at(const uint32_t* cum, int n_seqs, uint32_t t) {  // the sequence whose steps t is one of
-    int lo = 0, hi = n_seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cum[mid] <= t) lo = mid; else hi = mid;
-    }
-    return lo;
-}
 // The line of `total` steps in equal runs, none of them empty, and none shorter than kLeast where that leaves warps without one.
 constexpr uint32_t kLeast = 4;
 struct Runs {
@@ -692,7 +522,9 @@ int32_t lc_attention_kv8_workspace(const lc_kv8_cache* cache, const lc_kv8_rows*
     LC_TRY(check_heads("lc_attention_kv8_workspace", pool, seqs, n_heads));
     DeviceScope dev;
     LC_TRY(dev.enter(cache->k_dev, "lc_attention_kv8_workspace: cache"));
-    *out_bytes = plan_runs(pool, typ, n_heads / pool.n_kv, rows->max_rows).bytes;
+    TilePlan tiles;
+    const int group = n_heads / pool.n_kv;
+    *out_bytes = kv8_tiles_apply(pool, seqs, typ, group, rows->max_rows, &tiles) ? tiles.bytes : plan_runs(pool, typ, group, rows->max_rows).bytes;
     return LC_OK;
 }
 
@@ -712,13 +544,18 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
     LC_TRY(dev.enter(cache->k_dev, "lc_attention_kv8_dev: cache"));
     const int group = n_heads / pool.n_kv;
     const RunPlan plan = plan_runs(pool, typ, group, rows->max_rows);
-    LC_CHECK(workspace_dev && workspace_bytes >= plan.bytes && (uintptr_t)workspace_dev % 16 == 0, LC_ERR_INVALID,
-             "lc_attention_kv8_dev: needs a workspace of %zu bytes, 16-byte aligned (got %zu)", plan.bytes, workspace_bytes);
+    TilePlan tiles;
+    const bool by_tiles = kv8_tiles_apply(pool, seqs, typ, group, rows->max_rows, &tiles);
+    const size_t need = by_tiles ? tiles.bytes : plan.bytes;
+    LC_CHECK(workspace_dev && workspace_bytes >= need && (uintptr_t)workspace_dev % 16 == 0, LC_ERR_INVALID,
+             "lc_attention_kv8_dev: needs a workspace of %zu bytes, 16-byte aligned (got %zu)", need, workspace_bytes);
     if (scale == 0.0f) scale = 1.0f / sqrtf((float)pool.hd);
+    window = std::min(window, 1 << 30);  // the kernels' differences of positions stay in 32 bits
     const size_t elem = typ == LC_TYPE_F32 ? 4 : 2;
     AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, n_heads, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16),
                scale * 1.44269504088896f, (float*)workspace_dev};
     cudaStream_t s = stream_or_own(stream_);
+    if (by_tiles) return launch_kv8_tiles(pool, seqs, a, tiles, s);
     if (plan.hd == 64) return runs_of<64>(pool, seqs, a, rows->max_rows, plan, s);
     if (plan.hd == 128) return runs_of<128>(pool, seqs, a, rows->max_rows, plan, s);
     return runs_of<256>(pool, seqs, a, rows->max_rows, plan, s);

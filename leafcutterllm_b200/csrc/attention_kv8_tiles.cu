@@ -1,0 +1,563 @@
+// Attention over the 8-bit key/value cache for many rows per sequence (prompts), on tcgen05.
+//
+// A block has a unit: 256 rows (tokens x heads of the group, so that grouped heads share a tile's keys) of a sequence and kv head, in two tiles of 128, which
+// take turns on the matrix unit while the other's softmax runs.  It walks the keys in tiles of 128.
+//   warps 0-3, 4-7   the softmax of row tile 0, 1: a row per thread, scores and sums in tensor memory;
+//   warps 8-11       bring the next keys and values from the cache, as f16 integers, into shared memory (K as [key][dim], V as [dim][key], 128-byte
+//                    swizzle); one thread of warp 8 issues the products.
+// Scores: S = Q K^T, the queries times one power of two for the whole unit; f32 queries as f16 high and low parts, two products.
+// Weights: with f the key's scale factor (scale log2 e S_k) and S_v of the key's page, P_j = 2^(s_j f_j + log2 S_v,j - M + 8), M the row's largest exponent so far: the
+// value's scale is in the weight, so a page's scale costs an addition per 16 keys; the denominator is sum P_j / S_v,j.  P goes back into the place of S, as f16
+// (f32: high and low parts), and O = P V of a key tile is added to the row's sum in registers, in f32: what the matrix unit cuts off when it adds stays
+// within a tile of keys.
+//
+// What bounds it (a pair of row tiles x 128 keys, head dim 128): products 2,048 cycles (f32: 4,096), exponentials 2,048 on the special-function unit, and about
+// 2,500 issue cycles of softmax, sums and unpacking per scheduler.
+#include <algorithm>
+#include "lc_kernels.h"
+#include "lc_kv8_attn.cuh"
+#include "lc_umma.cuh"
+
+namespace lc {
+
+namespace {
+
+constexpr int kTileRows2 = 256, kKeys = 128, kTileThreads = 384;
+constexpr int kGroups = kKeys / 16;
+
+// what the softmax needs to know of 16 keys: score factor, log2 of the values' scale, its inverse
+struct GroupConst {
+    float f, lv, inv, pad;
+};
+struct TileShared {
+    uint64_t s_full[2], p_full[2], o_full[2], c_full[2];
+    GroupConst consts[2][kGroups];
+    uint2 sums[kTileThreads / 32];
+    uint32_t tmem;
+    int dead;
+    float top;
+};
+
+template <int HD, bool SPLIT> struct TileShape {
+    static constexpr int kPart = HD * 256;                    // 128 rows of HD f16
+    static constexpr int kQ = 2 * (SPLIT ? 2 : 1) * kPart;    // [row tile][high, low]
+    static constexpr int kK = HD * 256, kV = HD * 256;
+    static constexpr int kBytes = kQ + kK + kV + 1024;
+};
+
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    tmem_ld16(taddr, r);
+    tmem_ld16(taddr + 16, r + 16);
+}
+// The four warps that bring keys and values meet; true if all is well with every one of them, so that all go on or all stop.
+__device__ __forceinline__ bool conv_sync(bool ok) {
+    uint32_t all;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.and.pred p, 1, 128, q;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(all) : "r"((uint32_t)ok) : "memory");
+    return all != 0;
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 16-byte chunk `ch` (of 8) of a row of 128 bytes
+__device__ __forceinline__ int sw128(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
+
+template <int HD, bool SPLIT>
+__global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a, int splits) {
+    using Shape = TileShape<HD, SPLIT>;
+    constexpr int TERMS = SPLIT ? 2 : 1;
+    extern __shared__ unsigned char raw_smem[];
+    __shared__ TileShared sh;
+    unsigned char* const smem = (unsigned char*)(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
+    unsigned char* const sq = smem;
+    unsigned char* const sk = sq + Shape::kQ;
+    unsigned char* const sv = sk + Shape::kK;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if (blockIdx.x == 0 && blockIdx.y == 0) kv8_check_seqs(seqs, pool);
+
+    // the unit: sequences in order, the row blocks with most keys first
+    uint32_t* units = reinterpret_cast<uint32_t*>(smem);
+    uint32_t* cum = units + seqs.n_seqs + 1;
+    line_up<kTileRows2>(seqs, pool, a, cum, units, sh.sums);
+    if (blockIdx.x >= units[seqs.n_seqs]) return;
+    const int seq = seq_at(units, seqs.n_seqs, blockIdx.x);
+    const int in = blockIdx.x - units[seq];
+    __syncthreads();  // the arrays' place is the queries'
+    const SeqWork w = seq_work<kTileRows2>(seqs, pool, a, seq);
+    const int kvh = in % pool.n_kv, rb = w.blocks - 1 - in / pool.n_kv;
+    const int row_lo = rb * kTileRows2, row_n = min(kTileRows2, w.n * a.group - row_lo);
+    const int n_tiles = row_n > 128 ? 2 : 1;
+    const int hd = pool.hd;
+    const int64_t head0 = (int64_t)kvh * a.group * hd;
+    auto row_at = [&](int r, int64_t stride) {  // offset of the unit's row r
+        const int tok = (row_lo + r) / a.group;
+        return (int64_t)(w.first + tok) * stride + head0 + (int64_t)(row_lo + r - tok * a.group) * hd;
+    };
+    float* const part = a.part + (size_t)(blockIdx.x * gridDim.y + blockIdx.y) * (kTileRows2 * (HD + 2));
+    if (!w.inside) {
+        if (splits == 1) {
+            for (int e = tid; e < row_n * hd; e += kTileThreads) store1(a.out, row_at(e / hd, a.out_stride) + e % hd, a.typ, __int_as_float(0x7fffffff));
+        } else if (tid < kTileRows2) {
+            part[tid] = 0.0f;
+            part[kTileRows2 + tid] = __int_as_float(0x7fffffff);
+            for (int d = 0; d < HD; d++) part[2 * kTileRows2 + tid * HD + d] = 0.0f;
+        }
+        return;
+    }
+    // keys: from the first row's window to the last row's position; this block's share of their tiles
+    const int tok_first = row_lo / a.group, tok_last = (row_lo + row_n - 1) / a.group;
+    const int key_lo = a.window > 0 ? max(0, w.ctx + tok_first - a.window + 1) : 0, key_end = w.ctx + tok_last + 1;
+    const int tiles0 = key_lo / kKeys, all = (key_end + kKeys - 1) / kKeys - tiles0;
+    const int i0 = (int)((long long)all * blockIdx.y / splits), n = (int)((long long)all * (blockIdx.y + 1) / splits) - i0;
+    const int tile0 = tiles0 + i0;
+    if (n == 0) {  // only where a unit is cut
+        if (tid < kTileRows2) { part[tid] = kNegInf; part[kTileRows2 + tid] = 0.0f; }
+        return;
+    }
+
+    if (tid == 0) {
+        for (int t = 0; t < 2; t++) {
+            mbar_init(&sh.s_full[t], 1);
+            mbar_init(&sh.o_full[t], 1);
+            mbar_init(&sh.p_full[t], 128);
+            mbar_init(&sh.c_full[t], 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async();
+        sh.dead = 0;
+        sh.top = 0.0f;
+    }
+    if (warp == 0) tmem_alloc(&sh.tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    const uint32_t col_s[2] = {tmem, tmem + 128}, col_o[2] = {tmem + 256, tmem + 384};
+
+    // the queries: their largest magnitude, then f16 in place
+    {
+        constexpr int C = HD / 16;
+        const int chunks = n_tiles * 128 * C;
+        float top = 0.0f;
+        for (int e = tid; e < chunks; e += kTileThreads) {
+            const int r = e / C, ch = e % C;
+            if (r < row_n && ch * 16 < hd) {
+                float v[16];
+                load16(a.q, row_at(r, a.q_stride) + ch * 16, a.typ, a.q_vec, v);
+#pragma unroll
+                for (int x = 0; x < 16; x++) top = fabsf(v[x]) < INFINITY ? fmaxf(top, fabsf(v[x])) : top;
+            }
+        }
+        top = warp_max(top);
+        if (lane == 0) atomicMax(reinterpret_cast<int*>(&sh.top), __float_as_int(top));  // not negative: ordered as integers
+    }
+    __syncthreads();
+    float up, down;
+    row_scale(sh.top, up, down);
+    {
+        constexpr int C = HD / 16;
+        const int chunks = n_tiles * 128 * C;
+        for (int e = tid; e < chunks; e += kTileThreads) {
+            const int r = e / C, ch = e % C;
+            float v[16];
+            if (r < row_n && ch * 16 < hd) load16(a.q, row_at(r, a.q_stride) + ch * 16, a.typ, a.q_vec, v);
+            else
+#pragma unroll
+                for (int x = 0; x < 16; x++) v[x] = 0.0f;
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                if (SPLIT) h2_split(v[2 * x] * up, v[2 * x + 1] * up, hi[x], lo[x]);
+                else hi[x] = h2_pack(v[2 * x] * up, v[2 * x + 1] * up);
+            }
+            unsigned char* dst = sq + (r >> 7) * TERMS * Shape::kPart + (ch >> 2) * (128 * 128);
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int at = sw128(r & 127, 2 * (ch & 3) + x);
+                *reinterpret_cast<uint4*>(dst + at) = make_uint4(hi[4 * x], hi[4 * x + 1], hi[4 * x + 2], hi[4 * x + 3]);
+                if (SPLIT) *reinterpret_cast<uint4*>(dst + Shape::kPart + at) = make_uint4(lo[4 * x], lo[4 * x + 1], lo[4 * x + 2], lo[4 * x + 3]);
+            }
+        }
+    }
+    fence_async();
+    __syncthreads();
+
+    if (warp >= 8) {
+        // ------------------------------------------------------------------------------------- keys and values, products
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 152;");
+        const int ct = tid - 256, cw = warp - 8;
+        constexpr int KC = HD / 16, KP = 128 / KC, KN = kKeys / KP;   // K: chunks of a key, keys of a pass, passes
+        constexpr int LPK = HD / 4, VU = 4 * LPK / 32;                // V: lanes of a key, octets of keys per lane
+        const int32_t* table = seqs.table + (size_t)seq * seqs.width;
+        const int page_mask = (1 << pool.page_shift) - 1;
+        const float k_factor = a.scale_log2 * down;
+        // lane g < 8: the page of group g of a tile: -1 behind the end, -2 outside the pool
+        auto look_up = [&](int i) {
+            const int key = (tile0 + i) * kKeys + (lane & 7) * 16;
+            if (i >= n || key >= key_end) return -1;
+            const int p = table[key >> pool.page_shift];
+            return p >= 0 && p < pool.n_pages ? p : -2;
+        };
+        uint4 kr[KN];
+        uint32_t vr[VU][8];
+        float ksc = 0.0f, vsc = 0.0f, vsc_v = 0.0f;
+        int k_page = 0;
+        auto load_k = [&](int i, int pages) {
+            const int base = (tile0 + i) * kKeys;
+#pragma unroll
+            for (int u = 0; u < KN; u++) {
+                const int key = ct / KC + u * KP, ch = ct % KC;
+                const int p = __shfl_sync(0xffffffffu, pages, key >> 4);
+                kr[u] = make_uint4(0, 0, 0, 0);
+                if (p >= 0 && ch * 16 < hd)
+                    kr[u] = __ldg(reinterpret_cast<const uint4*>(pool.k + ((((size_t)p * pool.n_kv + kvh) << pool.page_shift) + ((base + key) & page_mask)) * hd + ch * 16));
+            }
+            k_page = pages;
+            if (lane < kGroups && pages >= 0) {
+                ksc = __ldg(pool.k_scale + (size_t)pages * pool.n_kv + kvh);
+                vsc = __ldg(pool.v_scale + (size_t)pages * pool.n_kv + kvh);
+            }
+        };
+        auto load_v = [&](int i, int pages) {
+            const int base = (tile0 + i) * kKeys;
+#pragma unroll
+            for (int u = 0; u < VU; u++) {
+                const int octet = 4 * cw + u * (32 / LPK) + lane / LPK, d = (lane % LPK) * 4;
+                const int p = __shfl_sync(0xffffffffu, pages, octet >> 1);
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    vr[u][x] = 0;
+                    if (p >= 0 && d < hd)
+                        vr[u][x] = __ldg(reinterpret_cast<const uint32_t*>(pool.v + ((((size_t)p * pool.n_kv + kvh) << pool.page_shift) + ((base + octet * 8 + x) & page_mask)) * hd + d));
+                }
+            }
+            vsc_v = 1.0f;
+            if (lane < kGroups && pages >= 0) vsc_v = __ldg(pool.v_scale + (size_t)pages * pool.n_kv + kvh);
+        };
+        auto put_k = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < KN; u++) {
+                const int key = ct / KC + u * KP, ch = ct % KC;
+                const uint32_t x[4] = {kr[u].x ^ 0x80808080u, kr[u].y ^ 0x80808080u, kr[u].z ^ 0x80808080u, kr[u].w ^ 0x80808080u};
+                unsigned char* dst = sk + (ch >> 2) * (128 * 128);
+                const uint4 first = make_uint4(ints01(x[0]), ints23(x[0]), ints01(x[1]), ints23(x[1]));
+                const uint4 second = make_uint4(ints01(x[2]), ints23(x[2]), ints01(x[3]), ints23(x[3]));
+                // the upper half of a row's chunks writes its second piece first: eight lanes then meet all banks
+                const bool swap = ch >= 4;
+                *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + (swap ? 1 : 0))) = swap ? second : first;
+                *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + (swap ? 0 : 1))) = swap ? first : second;
+            }
+            if (cw == 0) {
+                float lv = k_page >= 0 && vsc != 0.0f ? __log2f(vsc) : kNegInf, most = lv;
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                // a page of zeros counts in the denominator alone: its weights take the scale of its neighbours, its values are zeros
+                if (lv == kNegInf) lv = most == kNegInf ? 0.0f : most;
+                if (lane < kGroups) {
+                    GroupConst g;
+                    g.f = k_page >= 0 ? ksc * k_factor : k_page == -2 ? __int_as_float(0x7fffffff) : 0.0f;
+                    g.lv = lv;
+                    g.inv = exp2f(-lv);
+                    g.pad = 0.0f;
+                    sh.consts[i & 1][lane] = g;
+                    if (k_page == -2) kv8_raise(seqs, seq);
+                }
+            }
+        };
+        auto put_v = [&]() {
+#pragma unroll
+            for (int u = 0; u < VU; u++) {
+                const int octet = 4 * cw + u * (32 / LPK) + lane / LPK;
+                const bool zero = __shfl_sync(0xffffffffu, vsc_v, octet >> 1) == 0.0f;
+                uint32_t x[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = (zero ? 0u : vr[u][k]) ^ 0x80808080u;
+                uint32_t pairs01[4], pairs23[4];  // (keys 2k, 2k + 1) of dims 0, 1 and 2, 3
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    pairs01[k] = __byte_perm(x[2 * k], x[2 * k + 1], 0x5140);
+                    pairs23[k] = __byte_perm(x[2 * k], x[2 * k + 1], 0x7362);
+                }
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const uint32_t* p = b < 2 ? pairs01 : pairs23;
+                    uint4 out;
+                    out.x = b & 1 ? ints23(p[0]) : ints01(p[0]);
+                    out.y = b & 1 ? ints23(p[1]) : ints01(p[1]);
+                    out.z = b & 1 ? ints23(p[2]) : ints01(p[2]);
+                    out.w = b & 1 ? ints23(p[3]) : ints01(p[3]);
+                    // row b LPK + l holds dim 4 l + b: eight lanes write eight rows
+                    *reinterpret_cast<uint4*>(sv + (octet >> 3) * (HD * 128) + sw128(b * LPK + lane % LPK, octet & 7)) = out;
+                }
+            }
+        };
+        const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv);
+        auto scores = [&](int t) {
+#pragma unroll
+            for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ks++) {
+                    const uint32_t off = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
+                    umma_f16_ss(col_s[t], umma_desc_sw128(q_at + (t * TERMS + term) * Shape::kPart + off), umma_desc_sw128(k_at + off), idesc_f16(kKeys), term + ks > 0);
+                }
+            umma_commit(&sh.s_full[t]);
+        };
+        auto sums = [&](int t) {
+#pragma unroll
+            for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                for (int ks = 0; ks < kKeys / 16; ks++)
+                    umma_f16_ts(col_o[t], col_s[t] + 16 * ks + 8 * term, umma_desc_sw128(v_at + (ks >> 2) * (HD * 128) + (ks & 3) * 32), idesc_f16(HD), term + ks > 0);
+            umma_commit(&sh.o_full[t]);
+        };
+        bool ok = true;
+        int pages = look_up(0);
+        load_k(0, pages);
+        load_v(0, pages);
+        pages = look_up(1);
+        put_k(0);
+        fence_async();
+        conv_sync(true);
+        if (ct == 0) {
+            mbar_arrive(&sh.c_full[0]);
+            for (int t = 0; t < n_tiles; t++) scores(t);
+        }
+        __syncwarp();
+        load_k(1, pages);
+        put_v();
+        fence_async();
+        conv_sync(true);
+        load_v(1, pages);
+        pages = look_up(2);
+        const int last = n_tiles - 1;
+        for (int i = 0; i < n && ok; i++) {
+            const bool more = i + 1 < n;
+            if (more) {
+                ok = mbar_wait(&sh.s_full[last], i & 1);  // the keys' place is free
+                put_k(i + 1);
+                fence_async();
+                ok = conv_sync(ok);
+                if (!ok) break;
+                load_k(i + 2, pages);
+            }
+            if (warp == 8) {
+                if (lane == 0 && ok) {
+                    if (more) mbar_arrive(&sh.c_full[(i + 1) & 1]);
+                    for (int t = 0; t < n_tiles && ok; t++) {
+                        ok = mbar_wait(&sh.p_full[t], i & 1);
+                        tc_fence_after();
+                        if (!ok) break;
+                        sums(t);
+                        if (more) scores(t);
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            }
+            if (more) {
+                ok = ok && mbar_wait(&sh.o_full[last], i & 1);  // the values' place is free
+                put_v();
+                fence_async();
+                ok = conv_sync(ok);
+                load_v(i + 2, pages);
+                pages = look_up(i + 3);
+            }
+        }
+        if (!ok) sh.dead = 1;
+    } else {
+        // ------------------------------------------------------------------------------------------------------ softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t my_s = col_s[t] + lanes, my_o = col_o[t] + lanes;
+        const int limit = w.ctx + (row_lo + min(r, row_n - 1)) / a.group;      // last position that the row sees
+        const int least = __shfl_sync(0xffffffffu, limit, 0), most = __shfl_sync(0xffffffffu, limit, 31);
+        float o[HD], m = kNegInf, l = 0.0f, corr = 1.0f;
+#pragma unroll
+        for (int d = 0; d < HD; d++) o[d] = 0.0f;
+        bool ok = true;
+        auto add_up = [&](int i) {  // o = o corr + the key tile's sums
+            ok = mbar_wait(&sh.o_full[t], i & 1) && ok;
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t x[32];
+                tmem_ld32(my_o + c, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; e++) o[c + e] = fmaf(o[c + e], corr, __uint_as_float(x[e]));
+            }
+        };
+        if (t < n_tiles) {
+            for (int i = 0; i < n && ok; i++) {
+                if (i > 0) add_up(i - 1);
+                ok = mbar_wait(&sh.c_full[i & 1], (i >> 1) & 1) && mbar_wait(&sh.s_full[t], i & 1) && ok;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const GroupConst* gc = sh.consts[i & 1];
+                const int key0 = (tile0 + i) * kKeys;
+                const bool plain = key0 + kKeys - 1 <= least && (a.window == 0 || key0 > most - a.window);
+                // places of the tile that the row sees: [from, to]
+                const int to = limit - key0, from = a.window > 0 ? limit - a.window + 1 - key0 : 0;
+                float mx = m;
+#pragma unroll
+                for (int c = 0; c < kKeys; c += 32) {
+                    uint32_t x[32];
+                    tmem_ld32(my_s + c, x);
+                    tmem_wait_ld();
+                    if (!plain)
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (c + e > to || c + e < from) x[e] = __float_as_uint(kNegInf);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float g = __uint_as_float(x[16 * h]);
+#pragma unroll
+                        for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(x[16 * h + e]));
+                        const GroupConst k = gc[c / 16 + h];
+                        if (g != kNegInf) mx = fmaxf(mx, fmaf(g, k.f, k.lv));
+                    }
+                }
+                const float ref = mx == kNegInf ? 0.0f : mx;
+                corr = exp2_fast(m - ref);
+                m = mx;
+                float sum = 0.0f;
+                // 16 keys' weights take the first 8 columns of their scores' 16 (f32: their low parts the other 8)
+#pragma unroll
+                for (int c = 0; c < kKeys; c += 16) {
+                    uint32_t x[16], p[8], q[8];
+                    tmem_ld16(my_s + c, x);
+                    tmem_wait_ld();
+                    const GroupConst k = gc[c / 16];
+                    const float off = k.lv - ref + 8.0f;
+                    float gs = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float p0 = exp2_fast(fmaf(__uint_as_float(x[e]), k.f, off)), p1 = exp2_fast(fmaf(__uint_as_float(x[e + 1]), k.f, off));
+                        if (!plain) {
+                            if (c + e > to || c + e < from) p0 = 0.0f;
+                            if (c + e + 1 > to || c + e + 1 < from) p1 = 0.0f;
+                        }
+                        gs += p0 + p1;
+                        if (SPLIT) h2_split(p0, p1, p[e / 2], q[e / 2]);
+                        else p[e / 2] = h2_pack(p0, p1);
+                    }
+                    sum = fmaf(gs, k.inv, sum);
+                    tmem_st8(my_s + c, p);
+                    if (SPLIT) tmem_st8(my_s + c + 8, q);
+                }
+                l = fmaf(l, corr, sum);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&sh.p_full[t]);
+            }
+            if (ok) add_up(n - 1);
+            if (!ok) sh.dead = 1;
+            if (!ok || isnan(l)) l = __int_as_float(0x7fffffff);
+            if (!ok && lane == 0) kv8_raise(seqs, seq);
+            if (r < row_n) {
+                if (splits == 1) {
+                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                    const int64_t dst = row_at(r, a.out_stride);
+#pragma unroll
+                    for (int d = 0; d < HD; d += 16) {
+                        float v[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) v[e] = o[((d + e) >> 2) + ((d + e) & 3) * (HD / 4)] * inv;
+                        if (d < hd) store16(a.out, dst + d, a.typ, a.out_vec, v);
+                    }
+                } else {
+                    part[r] = m;
+                    part[kTileRows2 + r] = l;
+#pragma unroll
+                    for (int d = 0; d < HD; d += 16) {
+                        float v[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) v[e] = o[((d + e) >> 2) + ((d + e) & 3) * (HD / 4)];
+                        store16(part + 2 * kTileRows2 + (size_t)r * HD + d, true, v);
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) tmem_free(tmem, 512);
+}
+
+// Joins the parts of units whose keys are cut: a warp per row.
+template <int HD>
+__global__ void __launch_bounds__(256) kv8_tiles_join_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a, int splits) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint2 sums[8];
+    uint32_t* units = reinterpret_cast<uint32_t*>(smem);
+    uint32_t* cum = units + seqs.n_seqs + 1;
+    line_up<kTileRows2>(seqs, pool, a, cum, units, sums);
+    pdl_wait();
+    if (blockIdx.x >= units[seqs.n_seqs]) return;
+    const int seq = seq_at(units, seqs.n_seqs, blockIdx.x), in = blockIdx.x - units[seq];
+    const SeqWork w = seq_work<kTileRows2>(seqs, pool, a, seq);
+    const int kvh = in % pool.n_kv, row_lo = (w.blocks - 1 - in / pool.n_kv) * kTileRows2, row_n = min(kTileRows2, w.n * a.group - row_lo);
+    const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (r >= row_n) return;
+    constexpr int PER = HD / 32;
+    float mx = kNegInf, sum = 0.0f, v[PER];
+#pragma unroll
+    for (int e = 0; e < PER; e++) v[e] = 0.0f;
+    for (int s = 0; s < splits; s++) {
+        const float* p = a.part + (size_t)(blockIdx.x * splits + s) * (kTileRows2 * (HD + 2));
+        const float pm = p[r], ps = p[kTileRows2 + r];
+        if (pm == kNegInf && ps == 0.0f) continue;      // no keys: its sums are not there
+        const float m2 = fmaxf(mx, pm), ref = m2 == kNegInf ? 0.0f : m2;
+        const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(pm - ref);
+        sum = f0 * sum + (isnan(ps) ? ps : f1 * ps);
+#pragma unroll
+        for (int e = 0; e < PER; e++) v[e] = fmaf(f0, v[e], f1 * p[2 * kTileRows2 + (size_t)r * HD + lane * PER + e]);
+        mx = m2;
+    }
+    const int tok = (row_lo + r) / a.group;
+    const int64_t dst = (int64_t)(w.first + tok) * a.out_stride + ((int64_t)kvh * a.group + (row_lo + r - tok * a.group)) * pool.hd;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int e = 0; e < PER; e++)
+        if (lane * PER + e < pool.hd) store1(a.out, dst + lane * PER + e, a.typ, v[e] * inv);
+}
+
+template <int HD, bool SPLIT>
+int32_t tiles_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const TilePlan& plan, cudaStream_t s) {
+    using Shape = TileShape<HD, SPLIT>;
+    const void* kern = (const void*)kv8_tiles_kernel<HD, SPLIT>;
+    const size_t smem = std::max<size_t>(Shape::kBytes, (size_t)2 * (seqs.n_seqs + 1) * 4 + 1024);
+    LC_CUDA(ensure_smem_limit(kern, smem));
+    kv8_tiles_kernel<HD, SPLIT><<<dim3((unsigned)plan.units, (unsigned)plan.splits), kTileThreads, smem, s>>>(pool, seqs, a, plan.splits);
+    LC_CUDA(cudaGetLastError());
+    if (plan.splits > 1) {
+        const size_t cum = (size_t)2 * (seqs.n_seqs + 1) * 4;
+        LC_CUDA(launch_pdl(kv8_tiles_join_kernel<HD>, dim3((unsigned)plan.units, kTileRows2 / 8), dim3(256), cum, s, pool, seqs, a, plan.splits));
+    }
+    return LC_OK;
+}
+
+}  // namespace
+
+bool kv8_tiles_apply(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, TilePlan* plan) {
+    const int64_t rows = (int64_t)group * max_rows;
+    if (pool.hd > 128 || rows < 64) return false;
+    const int64_t units = ((int64_t)seqs.n_rows * group / kTileRows2 + seqs.n_seqs) * pool.n_kv;
+    if (units > 1 << 20) return false;
+    plan->units = (int)units;
+    plan->splits = 1;
+    plan->bytes = 16;
+    return true;
+}
+
+int32_t launch_kv8_tiles(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const TilePlan& plan, cudaStream_t s) {
+    if (pool.hd <= 64) return a.typ == LC_TYPE_F32 ? tiles_as<64, true>(pool, seqs, a, plan, s) : tiles_as<64, false>(pool, seqs, a, plan, s);
+    return a.typ == LC_TYPE_F32 ? tiles_as<128, true>(pool, seqs, a, plan, s) : tiles_as<128, false>(pool, seqs, a, plan, s);
+}
+
+}  // namespace lc
