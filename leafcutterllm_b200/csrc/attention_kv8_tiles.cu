@@ -3,13 +3,18 @@
 // A block has a unit: 256 rows (tokens x heads of the group, so that grouped heads share a tile's keys) of a sequence and kv head, in two tiles of 128, which
 // take turns on the matrix unit while the other's softmax runs.  It walks the keys in tiles of 128.
 //   warps 0-3, 4-7   the softmax of row tile 0, 1: a row per thread, scores and sums in tensor memory;
-//   warps 8-11       bring the next keys and values from the cache, as f16 integers, into shared memory (K as [key][dim], V as [dim][key], 128-byte
-//                    swizzle); one thread of warp 8 issues the products.
+//   warp 13          copies the next keys and values from the cache into shared memory (bulk copies of 16 keys);
+//   warps 8-11       unpack them to f16 (K as [key][dim], V as [dim][key], 128-byte swizzle);
+//   warp 12          one thread issues the products.  With the unpacking in the same warp an iteration took 9,500 cycles instead of 4,000: the issue waits
+//                    for the matrix unit's queue.
 // Scores: S = Q K^T, the queries times one power of two for the whole unit; f32 queries as f16 high and low parts, two products.
-// Weights: with f the key's scale factor (scale log2 e S_k) and S_v of the key's page, P_j = 2^(s_j f_j + log2 S_v,j - M + 8), M the row's largest exponent so far: the
+// Weights: with f the key's scale factor (scale log2 e S_k) and S_v of the key's page, P_j = 2^(s_j f_j + log2 S_v,j - M + 6), M the row's largest exponent so far: the
 // value's scale is in the weight, so a page's scale costs an addition per 16 keys; the denominator is sum P_j / S_v,j.  P goes back into the place of S, as f16
-// (f32: high and low parts), and O = P V of a key tile is added to the row's sum in registers, in f32: what the matrix unit cuts off when it adds stays
-// within a tile of keys.
+// (f32: high and low parts).  O = P V:
+//   f32             a key tile's sums are added to the row's in registers: what the matrix unit cuts off when it adds stays within a tile of keys (2,048 keys in
+//                   its own sums were off by 1e-5);
+//   16-bit types    O stays in tensor memory for all keys (the same error is a hundredth of the outputs' rounding), and so that it rarely
+//                   has to be scaled again, M is raised only when a row's largest exponent has grown by more than 8.
 //
 // What bounds it (a pair of row tiles x 128 keys, head dim 128): products 2,048 cycles (f32: 4,096), exponentials 2,048 on the special-function unit, and about
 // 2,500 issue cycles of softmax, sums and unpacking per scheduler.
@@ -22,16 +27,21 @@ namespace lc {
 
 namespace {
 
-constexpr int kTileRows2 = 256, kKeys = 128, kTileThreads = 384;
+constexpr int kTileRows2 = 256, kKeys = 128, kTileThreads = 512, kSlots = 4;
 constexpr int kGroups = kKeys / 16;
 
-// what the softmax needs to know of 16 keys: score factor, log2 of the values' scale, its inverse
+// what the softmax needs to know of 16 keys: score factor, log2 of the values' scale, its inverse; and what the unpacking does
+enum : int { kHere = 0, kAbsent = 1, kOutside = 2, kZeroValues = 4 };  // behind the end: zeros; outside the pool: keys of NaN
 struct GroupConst {
-    float f, lv, inv, pad;
+    float f, lv, inv;
+    int state;
 };
 struct TileShared {
-    uint64_t s_full[2], p_full[2], o_full[2], c_full[2];
-    GroupConst consts[2][kGroups];
+    uint64_t s_full[2], p_full[2], o_full[2];  // scores, weights, sums of a row tile
+    uint64_t c_full[kSlots];                   // consts of a key tile
+    uint64_t raw_full[2], raw_free[2];         // copied keys, values
+    uint64_t f16_full[2];                      // unpacked keys, values; their places are free when the last row tile's products are done
+    GroupConst consts[kSlots][kGroups];
     uint2 sums[kTileThreads / 32];
     uint32_t tmem;
     int dead;
@@ -42,7 +52,8 @@ template <int HD, bool SPLIT> struct TileShape {
     static constexpr int kPart = HD * 256;                    // 128 rows of HD f16
     static constexpr int kQ = 2 * (SPLIT ? 2 : 1) * kPart;    // [row tile][high, low]
     static constexpr int kK = HD * 256, kV = HD * 256;
-    static constexpr int kBytes = kQ + kK + kV + 1024;
+    static constexpr int kRaw = kKeys * HD;                   // keys, values as they are in the cache
+    static constexpr int kBytes = kQ + kK + kV + 2 * kRaw + 1024;
 };
 
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -50,12 +61,6 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
     tmem_ld16(taddr, r);
     tmem_ld16(taddr + 16, r + 16);
-}
-// The four warps that bring keys and values meet; true if all is well with every one of them, so that all go on or all stop.
-__device__ __forceinline__ bool conv_sync(bool ok) {
-    uint32_t all;
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.and.pred p, 1, 128, q;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(all) : "r"((uint32_t)ok) : "memory");
-    return all != 0;
 }
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
@@ -74,6 +79,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
     unsigned char* const sq = smem;
     unsigned char* const sk = sq + Shape::kQ;
     unsigned char* const sv = sk + Shape::kK;
+    unsigned char* const raw[2] = {sv + Shape::kV, sv + Shape::kV + Shape::kRaw};
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (blockIdx.x == 0 && blockIdx.y == 0) kv8_check_seqs(seqs, pool);
 
@@ -122,8 +128,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             mbar_init(&sh.s_full[t], 1);
             mbar_init(&sh.o_full[t], 1);
             mbar_init(&sh.p_full[t], 128);
-            mbar_init(&sh.c_full[t], 1);
+            mbar_init(&sh.raw_full[t], 1);
+            mbar_init(&sh.raw_free[t], 4);
+            mbar_init(&sh.f16_full[t], 4);
         }
+        for (int t = 0; t < kSlots; t++) mbar_init(&sh.c_full[t], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
         sh.dead = 0;
@@ -184,96 +193,156 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
     fence_async();
     __syncthreads();
 
-    if (warp >= 8) {
-        // ------------------------------------------------------------------------------------- keys and values, products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 152;");
+    const int last = n_tiles - 1;
+    if (warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 12) {
+            // ------------------------------------------------------------------------------------------------ products
+            if (lane == 0) {
+                const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv);
+                auto scores = [&](int t) {
+#pragma unroll
+                    for (int term = 0; term < TERMS; term++) {
+                        const uint64_t dq = umma_desc_sw128(q_at + (t * TERMS + term) * Shape::kPart), dk = umma_desc_sw128(k_at);
+#pragma unroll
+                        for (int ks = 0; ks < HD / 16; ks++) {
+                            const uint64_t off = ((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4;
+                            umma_f16_ss(col_s[t], dq + off, dk + off, idesc_f16(kKeys), term + ks > 0);
+                        }
+                    }
+                    umma_commit(&sh.s_full[t]);
+                };
+                auto sums = [&](int t, bool on) {
+                    const uint64_t dv = umma_desc_sw128(v_at);
+#pragma unroll
+                    for (int term = 0; term < TERMS; term++)
+#pragma unroll
+                        for (int ks = 0; ks < kKeys / 16; ks++)
+                            umma_f16_ts(col_o[t], col_s[t] + 16 * ks + 8 * term, dv + (((ks >> 2) * (HD * 128) + (ks & 3) * 32) >> 4), idesc_f16(HD), (uint32_t)(on || term + ks > 0));
+                    umma_commit(&sh.o_full[t]);
+                };
+                bool ok = mbar_wait(&sh.f16_full[0], 0);
+                tc_fence_after();
+                for (int t = 0; t < n_tiles && ok; t++) scores(t);
+                for (int i = 0; i < n && ok; i++) {
+                    const bool more = i + 1 < n;
+                    ok = mbar_wait(&sh.f16_full[1], i & 1);
+                    for (int t = 0; t < n_tiles && ok; t++) {
+                        ok = mbar_wait(&sh.p_full[t], i & 1);
+                        tc_fence_after();
+                        if (!ok) break;
+                        sums(t, !SPLIT && i > 0);
+                        if (more) {
+                            if (t == 0) ok = mbar_wait(&sh.f16_full[0], (i + 1) & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            scores(t);
+                        }
+                    }
+                }
+                if (!ok) sh.dead = 1;
+            }
+            __syncwarp();
+        } else if (warp == 13) {
+            // -------------------------------------------------------------------------------------------------- copies
+            const int32_t* table = seqs.table + (size_t)seq * seqs.width;
+            const int page_mask = (1 << pool.page_shift) - 1;
+            const float k_factor = a.scale_log2 * down;
+            const uint32_t bytes = 16 * hd;
+            auto look_up = [&](int i) {  // lane g < 8: the page of group g: -1 behind the end, -2 outside the pool
+                const int key = (tile0 + i) * kKeys + lane * 16;
+                if (lane >= kGroups || i >= n || key >= key_end) return -1;
+                const int p = table[key >> pool.page_shift];
+                return p >= 0 && p < pool.n_pages ? p : -2;
+            };
+            int page = look_up(0);
+            bool ok = true;
+            for (int i = 0; i < n && ok; i++) {
+                const int next = look_up(i + 1);
+                const size_t ph = (size_t)(page < 0 ? 0 : page) * pool.n_kv + kvh;
+                const size_t off = ((ph << pool.page_shift) + (((tile0 + i) * kKeys + lane * 16) & page_mask)) * hd;
+                const float ksc = page >= 0 ? pool.k_scale[ph] : 1.0f, vsc = page >= 0 ? pool.v_scale[ph] : 0.0f;
+                const uint32_t all = bytes * __popc(__ballot_sync(0xffffffffu, page >= 0));
+                for (int x = 0; x < 2; x++) {
+                    if (i > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.raw_free[x], (i - 1) & 1));
+                    if (!ok) break;
+                    if (x == 0) {
+                        float lv = page >= 0 && vsc != 0.0f ? log2f(vsc) : kNegInf, most = lv;
+#pragma unroll
+                        for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                        // a page of zeros counts in the denominator alone: its weights take the scale of its neighbours, its values are zeros
+                        if (lv == kNegInf) lv = most == kNegInf ? 0.0f : most;
+                        if (lane < kGroups) {
+                            // a score factor of 0 as 2^-100, so that a masked score of minus infinity stays one
+                            const float f = page < 0 ? 1.0f : ksc * k_factor;
+                            GroupConst g;
+                            g.f = f == 0.0f ? 0x1p-100f : f;
+                            g.lv = lv;
+                            g.inv = exp2f(-lv);
+                            g.state = page == -1 ? kAbsent : page == -2 ? kOutside : vsc == 0.0f ? kZeroValues : kHere;
+                            sh.consts[i % kSlots][lane] = g;
+                            if (page == -2) kv8_raise(seqs, seq);
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.c_full[i % kSlots]);
+                    }
+                    if (lane == 0) mbar_expect_tx(&sh.raw_full[x], all);
+                    __syncwarp();
+                    if (page >= 0) bulk_load(raw[x] + lane * bytes, (x ? pool.v : pool.k) + off, bytes, &sh.raw_full[x]);
+                }
+                page = next;
+            }
+            if (!ok) {  // whatever is under way lands before the block ends
+                sh.dead = 1;
+                for (int x = 0; x < 2; x++) (void)mbar_wait(&sh.raw_full[x], 0), (void)mbar_wait(&sh.raw_full[x], 1);
+            }
+        }
+    } else if (warp >= 8) {
+        // ---------------------------------------------------------------------------------------------------- unpacking
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         const int ct = tid - 256, cw = warp - 8;
         constexpr int KC = HD / 16, KP = 128 / KC, KN = kKeys / KP;   // K: chunks of a key, keys of a pass, passes
         constexpr int LPK = HD / 4, VU = 4 * LPK / 32;                // V: lanes of a key, octets of keys per lane
-        const int32_t* table = seqs.table + (size_t)seq * seqs.width;
-        const int page_mask = (1 << pool.page_shift) - 1;
-        const float k_factor = a.scale_log2 * down;
-        // lane g < 8: the page of group g of a tile: -1 behind the end, -2 outside the pool
-        auto look_up = [&](int i) {
-            const int key = (tile0 + i) * kKeys + (lane & 7) * 16;
-            if (i >= n || key >= key_end) return -1;
-            const int p = table[key >> pool.page_shift];
-            return p >= 0 && p < pool.n_pages ? p : -2;
-        };
-        uint4 kr[KN];
-        uint32_t vr[VU][8];
-        float ksc = 0.0f, vsc = 0.0f, vsc_v = 0.0f;
-        int k_page = 0;
-        auto load_k = [&](int i, int pages) {
-            const int base = (tile0 + i) * kKeys;
-#pragma unroll
+        bool ok = true;
+        for (int i = 0; i < n && ok; i++) {
+            const GroupConst* gc = sh.consts[i % kSlots];
+            ok = mbar_wait(&sh.c_full[i % kSlots], (i / kSlots) & 1) && mbar_wait(&sh.raw_full[0], i & 1);
+            if (i > 0) ok = ok && mbar_wait(&sh.s_full[last], (i - 1) & 1);  // the keys' place is free
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+#pragma unroll 4
             for (int u = 0; u < KN; u++) {
-                const int key = ct / KC + u * KP, ch = ct % KC;
-                const int p = __shfl_sync(0xffffffffu, pages, key >> 4);
-                kr[u] = make_uint4(0, 0, 0, 0);
-                if (p >= 0 && ch * 16 < hd)
-                    kr[u] = __ldg(reinterpret_cast<const uint4*>(pool.k + ((((size_t)p * pool.n_kv + kvh) << pool.page_shift) + ((base + key) & page_mask)) * hd + ch * 16));
-            }
-            k_page = pages;
-            if (lane < kGroups && pages >= 0) {
-                ksc = __ldg(pool.k_scale + (size_t)pages * pool.n_kv + kvh);
-                vsc = __ldg(pool.v_scale + (size_t)pages * pool.n_kv + kvh);
-            }
-        };
-        auto load_v = [&](int i, int pages) {
-            const int base = (tile0 + i) * kKeys;
-#pragma unroll
-            for (int u = 0; u < VU; u++) {
-                const int octet = 4 * cw + u * (32 / LPK) + lane / LPK, d = (lane % LPK) * 4;
-                const int p = __shfl_sync(0xffffffffu, pages, octet >> 1);
-#pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    vr[u][x] = 0;
-                    if (p >= 0 && d < hd)
-                        vr[u][x] = __ldg(reinterpret_cast<const uint32_t*>(pool.v + ((((size_t)p * pool.n_kv + kvh) << pool.page_shift) + ((base + octet * 8 + x) & page_mask)) * hd + d));
-                }
-            }
-            vsc_v = 1.0f;
-            if (lane < kGroups && pages >= 0) vsc_v = __ldg(pool.v_scale + (size_t)pages * pool.n_kv + kvh);
-        };
-        auto put_k = [&](int i) {
-#pragma unroll
-            for (int u = 0; u < KN; u++) {
-                const int key = ct / KC + u * KP, ch = ct % KC;
-                const uint32_t x[4] = {kr[u].x ^ 0x80808080u, kr[u].y ^ 0x80808080u, kr[u].z ^ 0x80808080u, kr[u].w ^ 0x80808080u};
+                const int key = ct / KC + u * KP, ch = ct % KC, state = gc[key >> 4].state;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (!(state & (kAbsent | kOutside)) && ch * 16 < hd) x = *reinterpret_cast<const uint4*>(raw[0] + key * hd + ch * 16);
+                x.x ^= 0x80808080u; x.y ^= 0x80808080u; x.z ^= 0x80808080u; x.w ^= 0x80808080u;
                 unsigned char* dst = sk + (ch >> 2) * (128 * 128);
-                const uint4 first = make_uint4(ints01(x[0]), ints23(x[0]), ints01(x[1]), ints23(x[1]));
-                const uint4 second = make_uint4(ints01(x[2]), ints23(x[2]), ints01(x[3]), ints23(x[3]));
+                uint4 first = make_uint4(ints01(x.x), ints23(x.x), ints01(x.y), ints23(x.y));
+                uint4 second = make_uint4(ints01(x.z), ints23(x.z), ints01(x.w), ints23(x.w));
+                if (state == kOutside) first = second = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);  // NaN
                 // the upper half of a row's chunks writes its second piece first: eight lanes then meet all banks
                 const bool swap = ch >= 4;
                 *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + (swap ? 1 : 0))) = swap ? second : first;
                 *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + (swap ? 0 : 1))) = swap ? first : second;
             }
-            if (cw == 0) {
-                float lv = k_page >= 0 && vsc != 0.0f ? __log2f(vsc) : kNegInf, most = lv;
-#pragma unroll
-                for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                // a page of zeros counts in the denominator alone: its weights take the scale of its neighbours, its values are zeros
-                if (lv == kNegInf) lv = most == kNegInf ? 0.0f : most;
-                if (lane < kGroups) {
-                    GroupConst g;
-                    g.f = k_page >= 0 ? ksc * k_factor : k_page == -2 ? __int_as_float(0x7fffffff) : 0.0f;
-                    g.lv = lv;
-                    g.inv = exp2f(-lv);
-                    g.pad = 0.0f;
-                    sh.consts[i & 1][lane] = g;
-                    if (k_page == -2) kv8_raise(seqs, seq);
-                }
-            }
-        };
-        auto put_v = [&]() {
+            fence_async();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&sh.f16_full[0]); mbar_arrive(&sh.raw_free[0]); }
+
+            ok = mbar_wait(&sh.raw_full[1], i & 1);
+            if (i > 0) ok = ok && mbar_wait(&sh.o_full[last], (i - 1) & 1);  // the values' place is free
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
 #pragma unroll
             for (int u = 0; u < VU; u++) {
-                const int octet = 4 * cw + u * (32 / LPK) + lane / LPK;
-                const bool zero = __shfl_sync(0xffffffffu, vsc_v, octet >> 1) == 0.0f;
+                const int octet = 4 * cw + u * (32 / LPK) + lane / LPK, d = (lane % LPK) * 4;
+                const bool none = gc[octet >> 1].state != kHere || d >= hd;
                 uint32_t x[8];
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = (zero ? 0u : vr[u][k]) ^ 0x80808080u;
+                for (int k = 0; k < 8; k++) {
+                    x[k] = none ? 0u : *reinterpret_cast<const uint32_t*>(raw[1] + (octet * 8 + k) * hd + d);
+                    x[k] ^= 0x80808080u;
+                }
                 uint32_t pairs01[4], pairs23[4];  // (keys 2k, 2k + 1) of dims 0, 1 and 2, 3
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -292,77 +361,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                     *reinterpret_cast<uint4*>(sv + (octet >> 3) * (HD * 128) + sw128(b * LPK + lane % LPK, octet & 7)) = out;
                 }
             }
-        };
-        const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv);
-        auto scores = [&](int t) {
-#pragma unroll
-            for (int term = 0; term < TERMS; term++)
-#pragma unroll
-                for (int ks = 0; ks < HD / 16; ks++) {
-                    const uint32_t off = (ks >> 2) * (128 * 128) + (ks & 3) * 32;
-                    umma_f16_ss(col_s[t], umma_desc_sw128(q_at + (t * TERMS + term) * Shape::kPart + off), umma_desc_sw128(k_at + off), idesc_f16(kKeys), term + ks > 0);
-                }
-            umma_commit(&sh.s_full[t]);
-        };
-        auto sums = [&](int t) {
-#pragma unroll
-            for (int term = 0; term < TERMS; term++)
-#pragma unroll
-                for (int ks = 0; ks < kKeys / 16; ks++)
-                    umma_f16_ts(col_o[t], col_s[t] + 16 * ks + 8 * term, umma_desc_sw128(v_at + (ks >> 2) * (HD * 128) + (ks & 3) * 32), idesc_f16(HD), term + ks > 0);
-            umma_commit(&sh.o_full[t]);
-        };
-        bool ok = true;
-        int pages = look_up(0);
-        load_k(0, pages);
-        load_v(0, pages);
-        pages = look_up(1);
-        put_k(0);
-        fence_async();
-        conv_sync(true);
-        if (ct == 0) {
-            mbar_arrive(&sh.c_full[0]);
-            for (int t = 0; t < n_tiles; t++) scores(t);
-        }
-        __syncwarp();
-        load_k(1, pages);
-        put_v();
-        fence_async();
-        conv_sync(true);
-        load_v(1, pages);
-        pages = look_up(2);
-        const int last = n_tiles - 1;
-        for (int i = 0; i < n && ok; i++) {
-            const bool more = i + 1 < n;
-            if (more) {
-                ok = mbar_wait(&sh.s_full[last], i & 1);  // the keys' place is free
-                put_k(i + 1);
-                fence_async();
-                ok = conv_sync(ok);
-                if (!ok) break;
-                load_k(i + 2, pages);
-            }
-            if (warp == 8) {
-                if (lane == 0 && ok) {
-                    if (more) mbar_arrive(&sh.c_full[(i + 1) & 1]);
-                    for (int t = 0; t < n_tiles && ok; t++) {
-                        ok = mbar_wait(&sh.p_full[t], i & 1);
-                        tc_fence_after();
-                        if (!ok) break;
-                        sums(t);
-                        if (more) scores(t);
-                    }
-                }
-                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-            }
-            if (more) {
-                ok = ok && mbar_wait(&sh.o_full[last], i & 1);  // the values' place is free
-                put_v();
-                fence_async();
-                ok = conv_sync(ok);
-                load_v(i + 2, pages);
-                pages = look_up(i + 3);
-            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(&sh.f16_full[1]); mbar_arrive(&sh.raw_free[1]); }
         }
         if (!ok) sh.dead = 1;
     } else {
@@ -374,85 +375,145 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         const int limit = w.ctx + (row_lo + min(r, row_n - 1)) / a.group;      // last position that the row sees
         const int least = __shfl_sync(0xffffffffu, limit, 0), most = __shfl_sync(0xffffffffu, limit, 31);
         float o[HD], m = kNegInf, l = 0.0f, corr = 1.0f;
-#pragma unroll
-        for (int d = 0; d < HD; d++) o[d] = 0.0f;
         bool ok = true;
         auto add_up = [&](int i) {  // o = o corr + the key tile's sums
             ok = mbar_wait(&sh.o_full[t], i & 1) && ok;
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < HD; c += 32) {
-                uint32_t x[32];
-                tmem_ld32(my_o + c, x);
+            for (int c = 0; c < HD; c += 16) {
+                uint32_t x[16];
+                tmem_ld16(my_o + c, x);
                 tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[c + e] = fmaf(o[c + e], corr, __uint_as_float(x[e]));
+                for (int e = 0; e < 16; e++) o[c + e] = fmaf(o[c + e], corr, __uint_as_float(x[e]));
             }
         };
         if (t < n_tiles) {
+            if (SPLIT)
+#pragma unroll
+                for (int d = 0; d < HD; d++) o[d] = 0.0f;
             for (int i = 0; i < n && ok; i++) {
-                if (i > 0) add_up(i - 1);
-                ok = mbar_wait(&sh.c_full[i & 1], (i >> 1) & 1) && mbar_wait(&sh.s_full[t], i & 1) && ok;
+                if (SPLIT && i > 0) add_up(i - 1);
+                ok = mbar_wait(&sh.c_full[i % kSlots], (i / kSlots) & 1) && mbar_wait(&sh.s_full[t], i & 1) && ok;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const GroupConst* gc = sh.consts[i & 1];
+                const GroupConst* gc = sh.consts[i % kSlots];
                 const int key0 = (tile0 + i) * kKeys;
                 const bool plain = key0 + kKeys - 1 <= least && (a.window == 0 || key0 > most - a.window);
                 // places of the tile that the row sees: [from, to]
                 const int to = limit - key0, from = a.window > 0 ? limit - a.window + 1 - key0 : 0;
-                float mx = m;
+                float mx = m, sum = 0.0f;
+                if constexpr (SPLIT) {
+#pragma unroll 1
+                    for (int c = 0; c < kKeys; c += 32) {
+                        uint32_t x[32];
+                        tmem_ld32(my_s + c, x);
+                        tmem_wait_ld();
+                        if (!plain)
 #pragma unroll
-                for (int c = 0; c < kKeys; c += 32) {
-                    uint32_t x[32];
-                    tmem_ld32(my_s + c, x);
+                            for (int e = 0; e < 32; e++)
+                                if (c + e > to || c + e < from) x[e] = __float_as_uint(kNegInf);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            float g = __uint_as_float(x[16 * h]);
+#pragma unroll
+                            for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(x[16 * h + e]));
+                            const GroupConst k = gc[c / 16 + h];
+                            mx = fmaxf(mx, fmaf(g, k.f, k.lv));
+                        }
+                    }
+                    const float ref = mx == kNegInf ? 0.0f : mx;
+                    corr = exp2_fast(m - ref);
+                    m = mx;
+                    // 16 keys' weights take the first 8 columns of their scores' 16, their low parts the other 8
+#pragma unroll 2
+                    for (int c = 0; c < kKeys; c += 16) {
+                        uint32_t x[16], p[8], q[8];
+                        tmem_ld16(my_s + c, x);
+                        tmem_wait_ld();
+                        const GroupConst k = gc[c / 16];
+                        const float off = k.lv - ref + 6.0f;
+                        if (!plain)
+#pragma unroll
+                            for (int e = 0; e < 16; e++)
+                                if (c + e > to || c + e < from) x[e] = __float_as_uint(kNegInf);
+                        float gs = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const float p0 = exp2_fast(fmaf(__uint_as_float(x[e]), k.f, off)), p1 = exp2_fast(fmaf(__uint_as_float(x[e + 1]), k.f, off));
+                            gs += p0 + p1;
+                            h2_split(p0, p1, p[e / 2], q[e / 2]);
+                        }
+                        sum = fmaf(gs, k.inv, sum);
+                        tmem_st8(my_s + c, p);
+                        tmem_st8(my_s + c + 8, q);
+                    }
+                    l = fmaf(l, corr, sum);
+                } else {
+                    uint32_t x[kKeys];
+#pragma unroll
+                    for (int c = 0; c < kKeys; c += 16) tmem_ld16(my_s + c, x + c);
                     tmem_wait_ld();
                     if (!plain)
 #pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            if (c + e > to || c + e < from) x[e] = __float_as_uint(kNegInf);
+                        for (int e = 0; e < kKeys; e++)
+                            if (e > to || e < from) x[e] = __float_as_uint(kNegInf);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        float g = __uint_as_float(x[16 * h]);
+                    for (int c = 0; c < kKeys; c += 16) {
+                        float g = __uint_as_float(x[c]);
 #pragma unroll
-                        for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(x[16 * h + e]));
-                        const GroupConst k = gc[c / 16 + h];
-                        if (g != kNegInf) mx = fmaxf(mx, fmaf(g, k.f, k.lv));
+                        for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(x[c + e]));
+                        const GroupConst k = gc[c / 16];
+                        mx = fmaxf(mx, fmaf(g, k.f, k.lv));
                     }
-                }
-                const float ref = mx == kNegInf ? 0.0f : mx;
-                corr = exp2_fast(m - ref);
-                m = mx;
-                float sum = 0.0f;
-                // 16 keys' weights take the first 8 columns of their scores' 16 (f32: their low parts the other 8)
+                    const bool raise = mx > m + 8.0f;  // also from minus infinity
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float f = raise ? exp2_fast(m - mx) : 1.0f;
+                        if (raise) m = mx;
+                        l *= f;
+                        if (i > 0) {
+                            ok = mbar_wait(&sh.o_full[t], (i - 1) & 1);
+                            ok = __all_sync(0xffffffffu, ok);
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < HD; c += 16) {
+                                uint32_t y[16];
+                                tmem_ld16(my_o + c, y);
+                                tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < kKeys; c += 16) {
-                    uint32_t x[16], p[8], q[8];
-                    tmem_ld16(my_s + c, x);
-                    tmem_wait_ld();
-                    const GroupConst k = gc[c / 16];
-                    const float off = k.lv - ref + 8.0f;
-                    float gs = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float p0 = exp2_fast(fmaf(__uint_as_float(x[e]), k.f, off)), p1 = exp2_fast(fmaf(__uint_as_float(x[e + 1]), k.f, off));
-                        if (!plain) {
-                            if (c + e > to || c + e < from) p0 = 0.0f;
-                            if (c + e + 1 > to || c + e + 1 < from) p1 = 0.0f;
+                                for (int e = 0; e < 16; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
+                                tmem_st16(my_o + c, y);
+                            }
                         }
-                        gs += p0 + p1;
-                        if (SPLIT) h2_split(p0, p1, p[e / 2], q[e / 2]);
-                        else p[e / 2] = h2_pack(p0, p1);
                     }
-                    sum = fmaf(gs, k.inv, sum);
-                    tmem_st8(my_s + c, p);
-                    if (SPLIT) tmem_st8(my_s + c + 8, q);
+                    const float ref = m == kNegInf ? 0.0f : m;
+#pragma unroll
+                    for (int c = 0; c < kKeys; c += 16) {
+                        uint32_t p[8];
+                        const GroupConst k = gc[c / 16];
+                        const float off = k.lv - ref + 6.0f;
+                        float g0 = 0.0f, g1 = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const float p0 = exp2_fast(fmaf(__uint_as_float(x[c + e]), k.f, off)), p1 = exp2_fast(fmaf(__uint_as_float(x[c + e + 1]), k.f, off));
+                            g0 += p0;
+                            g1 += p1;
+                            p[e / 2] = h2_pack(p0, p1);
+                        }
+                        sum = fmaf(g0 + g1, k.inv, sum);
+                        tmem_st8(my_s + c, p);
+                    }
+                    l += sum;
                 }
-                l = fmaf(l, corr, sum);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&sh.p_full[t]);
+            }
+            if constexpr (!SPLIT) {
+#pragma unroll
+                for (int d = 0; d < HD; d++) o[d] = 0.0f;
             }
             if (ok) add_up(n - 1);
             if (!ok) sh.dead = 1;
