@@ -1,12 +1,13 @@
 // Log probabilities of given tokens, entropies and the likeliest tokens of rows of logits, in one pass over them.
 //
 // With m the row's maximum, d = x - m, S = sum e^d and T = sum e^d d:   log p(x) = d - log S,   entropy = log S - T / S.
-// Every thread keeps a running m, S and T.  Sixteen logits at a time: their f32 sums are added to S and T in 64 bits, which a row of one
-// near-certain token needs (log S ~ 1e-3 is then S - 1).  A later maximum m' turns (S, T) into (f S, f (T + (m - m') S)), f = e^(m - m').
+// Every thread keeps a running S and T against its warp's m, sixteen logits at a time, whose f32 sums are added in 64 bits.  A later maximum m' turns
+// (S, T) into (f S, f (T + (m - m') S)), f = e^(m - m').  m is the warp's and not the lane's: some lane finds a new maximum of its own in most steps, a warp in
+// one of six (128,256 logits: 255 -> 130 us with the change, 2,048 rows).
 //
-// The best `top` are kept per warp, lane i holding the i-th as a key (logit in the order of whole numbers, then the lower index).  A logit below
-// the block's bound cannot be among them; the bound is the largest of the warps' last keys, and to begin with the top-th largest of
-// the lanes' maxima of the first sixteen.  Only logits above it take the way through the list.
+// The best `top`: a logit below the block's bound cannot be among them.  The bound is the top-th largest of the maxima of groups of
+// four threads after 1, 2, 4, ... steps, and every logit that reaches it goes to a list of its warp's; a full list is cut to its best `top` by counting,
+// for each, the larger ones.
 //
 // A row goes to a cluster of 1, 2, 4 or 8 blocks, which join over distributed shared memory: one launch, no workspace.
 #include <cooperative_groups.h>
@@ -20,19 +21,23 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kChunkElems = 16, kMaxCluster = 8, kMaxTop = 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kChunkElems = 16, kMaxCluster = 8, kMaxTop = 32, kList = 128, kGroups = kThreads / 4;
 
 struct Sums {
     float m;
     double s, t;
 };
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-    if (b.m == -INFINITY) return a;
-    if (a.m == -INFINITY) return b;
-    const float m = fmaxf(a.m, b.m);
-    const float da = a.m - m, db = b.m - m;
-    const double fa = expf(da), fb = expf(db);
-    return Sums{m, fa * a.s + fb * b.s, fa * (a.t + (double)da * a.s) + fb * (b.t + (double)db * b.s)};
+// Of the sums in the lanes of a warp (m minus infinity: none), in all lanes.
+__device__ __forceinline__ Sums join_lanes(Sums a) {
+    const float m = warp_max(a.m), d = a.m - m;
+    const double f = a.m == -INFINITY ? 0.0 : (double)expf(d);
+    double s = f * a.s, t = a.m == -INFINITY ? 0.0 : f * (a.t + (double)d * a.s);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    return Sums{m, s, t};
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -61,6 +66,7 @@ struct LogprobArgs {
     int64_t* top_id;
     int64_t stride;
     int vocab, top, vec;  // vec: rows are 16-byte aligned
+    int size_shift;       // blocks of a row = 1 << size_shift
 };
 
 // what a block leaves for its cluster
@@ -70,24 +76,79 @@ struct BlockPart {
     unsigned long long keys[kMaxTop];
 };
 
-// Sixteen logits of a thread: `per` pieces of 16 bytes, blockDim apart.  Places behind the end give minus infinity.
-template <typename T>
-__device__ __forceinline__ void load_chunk(const T* row, int piece0, int n, bool vec, float (&x)[kChunkElems]) {
-    constexpr int E = 16 / sizeof(T), U = kChunkElems / E;
+// Sixteen logits of a thread as they lie in memory: `U` pieces of 16 bytes, a block's width apart.  Places behind the end give minus infinity.
+template <typename T> struct Chunk {
+    static constexpr int E = 16 / sizeof(T), U = kChunkElems / E;
+    uint4 w[U];
+    __device__ __forceinline__ void load(const T* row, int piece0, int n, bool vec) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int at = (piece0 + u * kThreads) * E;
-        if (vec && at + E <= n) {
-            const uint4 w = __ldcs(reinterpret_cast<const uint4*>(row + at));
-            __align__(16) T t[E];
-            *reinterpret_cast<uint4*>(t) = w;
+        for (int u = 0; u < U; u++) {
+            const int at = (piece0 + u * kThreads) * E;
+            if (vec && at + E <= n) {
+                w[u] = __ldcs(reinterpret_cast<const uint4*>(row + at));
+            } else {
+                __align__(16) T t[E];
 #pragma unroll
-            for (int e = 0; e < E; e++) x[u * E + e] = elem_f(t[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; e++) x[u * E + e] = at + e < n ? elem_f(row[at + e]) : -INFINITY;
+                for (int e = 0; e < E; e++) t[e] = at + e < n ? row[at + e] : to_elem<T>(-INFINITY);
+                w[u] = *reinterpret_cast<const uint4*>(t);
+            }
         }
     }
+    __device__ __forceinline__ void values(float (&x)[kChunkElems]) const {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            __align__(16) T t[E];
+            *reinterpret_cast<uint4*>(t) = w[u];
+#pragma unroll
+            for (int e = 0; e < E; e++) x[u * E + e] = elem_f(t[e]);
+        }
+    }
+};
+// two f32 at a time
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}\n" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}\n"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+
+// By a whole warp: cuts its list to the best `top`; returns the last of them, or 0 where there are fewer.  Not inlined: one copy of it per place in the unrolled
+// search made the code so long that a step's way through it took 13,000 cycles.
+__device__ __noinline__ unsigned long long cut_list(unsigned long long* list, int listed, int top, uint32_t* bound) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    unsigned long long key[kList / 32];
+    int above[kList / 32];
+#pragma unroll
+    for (int k = 0; k < kList / 32; k++) {
+        key[k] = k * 32 + lane < listed ? list[k * 32 + lane] : 0ull;
+        above[k] = 0;
+    }
+#pragma unroll 4
+    for (int j = 0; j < listed; j++) {
+        const unsigned long long other = list[j];
+#pragma unroll
+        for (int k = 0; k < kList / 32; k++) above[k] += other > key[k];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kList / 32; k++)
+        if (key[k] != 0ull && above[k] < top) list[above[k]] = key[k];
+    __syncwarp();
+    if (listed < top) return 0ull;
+    const unsigned long long last = list[top - 1];
+    if (lane == 0) atomicMax(bound, (uint32_t)(last >> 32));
+    return last;
 }
 
 template <typename T, bool TOP>
@@ -97,87 +158,142 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(LogprobArgs
     __shared__ Sums warp_sums[kWarps];
     __shared__ int s_bad;
     __shared__ uint32_t s_bound;                       // order of a value that at least `top` logits reach
-    __shared__ unsigned long long s_keys[kMaxCluster > kWarps ? kMaxCluster * kMaxTop : kWarps * kMaxTop];
+    __shared__ unsigned long long s_list[kWarps][kList];
+    __shared__ int s_count[kWarps];
+    __shared__ __align__(16) uint32_t s_top[kGroups];                // maxima of four lanes each, in the order of whole numbers
+    __shared__ unsigned long long s_keys[kThreads];
+    static_assert(kMaxCluster * kMaxTop <= kThreads && kWarps * kMaxTop <= kThreads, "a thread for each of the keys that are joined");
     cg::cluster_group cluster = cg::this_cluster();
-    const int size = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int64_t r = blockIdx.x / size;
+    const int size = 1 << a.size_shift, rank = blockIdx.x & (size - 1);
+    const int64_t r = blockIdx.x >> a.size_shift;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const T* whole = (const T*)a.x + r * a.stride;
     // this block's slice, in pieces of 16 bytes
     const int pieces = (a.vocab + E - 1) / E;
-    const int p0 = (int)((long long)pieces * rank / size), p1 = (int)((long long)pieces * (rank + 1) / size);
+    const int p0 = (int)(((long long)pieces * rank) >> a.size_shift), p1 = (int)(((long long)pieces * (rank + 1)) >> a.size_shift);
     const int first = p0 * E, n = max(0, min(a.vocab, p1 * E) - first);
     const T* row = whole + first;
     if (threadIdx.x == 0) { s_bad = 0; s_bound = 0; }
     __syncthreads();
 
-    Sums mine{-INFINITY, 0.0, 0.0};
+    float m = -INFINITY;                               // the warp's
+    double sum_s = 0.0, sum_t = 0.0;
     bool bad = false;
-    unsigned long long best = 0;                       // lane i: the warp's i-th best key
+    float lane_top = -INFINITY;
+    int steps = 0;
+    unsigned long long* list = s_list[warp];           // the warp's candidates
+    int listed = 0;
+    unsigned long long last = 0;                       // what a candidate has to exceed: the top-th of the list when it was cut
     const int count = p1 - p0;                         // pieces
-    constexpr int U = kChunkElems / E;
+    constexpr int U = Chunk<T>::U;
+    // what the row's last step needs is under way from here on
+    float asked = __int_as_float(0x7fffffff);
+    if (rank == 0 && threadIdx.x == 0 && a.logprob) {
+        const int64_t tok = a.tokens[r];
+        if (tok >= 0 && tok < a.vocab) asked = elem_f(whole[tok]);
+    }
+    Chunk<T> next;
+    if (count > 0) next.load(row, (int)threadIdx.x, n, a.vec);
     for (int base = 0; base < count; base += kThreads * U) {
         float x[kChunkElems];
         const int piece0 = base + (int)threadIdx.x;
-        load_chunk<T>(row, piece0, n, a.vec, x);
+        next.values(x);
+        if (base + kThreads * U < count) next.load(row, piece0 + kThreads * U, n, a.vec);
         float top = x[0];
 #pragma unroll
         for (int e = 1; e < kChunkElems; e++) top = max_nan(top, x[e]);
         if (!(top < INFINITY)) bad = true;
-        if (top > mine.m) {
-            if (mine.m != -INFINITY) {
-                const float dm = mine.m - top;
+        if (__any_sync(0xffffffffu, top > m)) {
+            const float now = warp_max(fmaxf(top, m));
+            if (m != -INFINITY) {
+                const float dm = m - now;
                 const double f = expf(dm);
-                mine.t = f * (mine.t + (double)dm * mine.s);
-                mine.s = f * mine.s;
+                sum_t = f * (sum_t + (double)dm * sum_s);
+                sum_s = f * sum_s;
             }
-            mine.m = top;
+            m = now;
         }
-        if (mine.m != -INFINITY) {
-            float s = 0.0f, t = 0.0f;
+        if (m != -INFINITY) {
+            float2 s = make_float2(0.0f, 0.0f), t = s;
+            const float2 less = make_float2(-m, -m), log2e = make_float2(1.44269504088896f, 1.44269504088896f);
 #pragma unroll
-            for (int e = 0; e < kChunkElems; e++) {
-                const float d = fmaxf(x[e] - mine.m, -200.0f);  // e^-200 is 0 here; keeps 0 * -inf out
-                const float p = exp2_fast(d * 1.44269504088896f);
-                s += p;
-                t = fmaf(p, d, t);
+            for (int e = 0; e < kChunkElems; e += 2) {
+                float2 d = add2(make_float2(x[e], x[e + 1]), less);
+                d.x = fmaxf(d.x, -200.0f);  // e^-200 is 0 here; keeps 0 * -inf out
+                d.y = fmaxf(d.y, -200.0f);
+                const float2 y = mul2(d, log2e);
+                const float2 p = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                s = add2(s, p);
+                t = fma2(p, d, t);
             }
-            mine.s += (double)s;
-            mine.t += (double)t;
+            sum_s += (double)(s.x + s.y);
+            sum_t += (double)(t.x + t.y);
         }
         if (TOP) {
-            if (base == 0) {
-                // a first bound: the top-th largest of the lanes' maxima
-                uint32_t o = order_of(top);
-                int above = 0;
+            // after 1, 2, 4, ... steps the bound is the top-th largest of the maxima so far of groups of four lanes; a warp that is behind has smaller ones there
+            lane_top = fmaxf(lane_top, top);
+            if ((steps & (steps + 1)) == 0) {
+                uint32_t o = order_of(lane_top);
+                o = max(o, __shfl_xor_sync(0xffffffffu, o, 1));
+                o = max(o, __shfl_xor_sync(0xffffffffu, o, 2));
+                if ((lane & 3) == 0) s_top[threadIdx.x >> 2] = o;
+                if (steps == 0) __syncthreads();
+                else __syncwarp();
+                // at first every warp finds it, for itself; then one of them, for all
+                if (steps == 0 || warp == (__popc(steps) & (kWarps - 1))) {
+                    const uint32_t v0 = s_top[lane], v1 = s_top[32 + lane];
+                    int above0 = 0, above1 = 0;
 #pragma unroll
-                for (int k = 1; k < 32; k++) {
-                    const uint32_t other = __shfl_xor_sync(0xffffffffu, o, k);
-                    above += other > o || (other == o && (lane ^ k) < lane);
+                    for (int k = 0; k < kGroups; k += 4) {
+                        const uint4 u = *reinterpret_cast<const uint4*>(&s_top[k]);
+                        above0 += (u.x > v0) + (u.y > v0) + (u.z > v0) + (u.w > v0);
+                        above1 += (u.x > v1) + (u.y > v1) + (u.z > v1) + (u.w > v1);
+                    }
+                    // equal ones have equal counts
+                    const uint32_t kth = __reduce_min_sync(0xffffffffu, min(above0 < a.top ? v0 : 0xffffffffu, above1 < a.top ? v1 : 0xffffffffu));
+                    if (lane == 0) atomicMax(&s_bound, kth);
+                    __syncwarp();
                 }
-                if (above == a.top - 1) atomicMax(&s_bound, o);
-                __syncthreads();
             }
-            float bound = value_of(*(volatile uint32_t*)&s_bound);
+            steps++;
+            const float bound = value_of(*(volatile uint32_t*)&s_bound);
             if (__any_sync(0xffffffffu, top >= bound)) {
-                unsigned long long last = __shfl_sync(0xffffffffu, best, a.top - 1);
+                int mine = 0;
 #pragma unroll
-                for (int e = 0; e < kChunkElems; e++) {
-                    const int at = (piece0 + (e / E) * kThreads) * E + e % E;
-                    unsigned long long key = x[e] >= bound && at < n ? key_of(x[e], first + at) : 0ull;
-                    unsigned who = __ballot_sync(0xffffffffu, key > last);
-                    while (who) {
-                        const int src = __ffs(who) - 1;
-                        who &= who - 1;
-                        const unsigned long long in = __shfl_sync(0xffffffffu, key, src);
-                        if (in > last) {
-                            const unsigned long long up = __shfl_up_sync(0xffffffffu, best, 1);
-                            if (best < in) best = lane == 0 || up > in ? in : up;
-                            last = __shfl_sync(0xffffffffu, best, a.top - 1);
+                for (int e = 0; e < kChunkElems; e++) mine += x[e] >= bound && (piece0 + (e / E) * kThreads) * E + e % E < n;
+                int upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                const int more = __shfl_sync(0xffffffffu, upto, 31);
+                if (listed + more <= kList) {
+                    int to = listed + upto - mine;
+                    if (mine) {
+#pragma unroll
+                        for (int e = 0; e < kChunkElems; e++)
+                            if (x[e] >= bound && (piece0 + (e / E) * kThreads) * E + e % E < n) list[to++] = key_of(x[e], first + (piece0 + (e / E) * kThreads) * E + e % E);
+                    }
+                    listed += more;
+                } else {
+                    // more than the list has room for (many equal logits): one logit of every lane at a time, and only what beats the list's last
+#pragma unroll
+                    for (int e = 0; e < kChunkElems; e++) {
+                        const int at = (piece0 + (e / E) * kThreads) * E + e % E;
+                        const unsigned long long key = x[e] >= bound && at < n ? key_of(x[e], first + at) : 0ull;
+                        unsigned who = __ballot_sync(0xffffffffu, key > last);
+                        if (who) {
+                            if (listed > kList - 32) {
+                                last = cut_list(list, listed, a.top, &s_bound);
+                                listed = min(listed, a.top);
+                                who = __ballot_sync(0xffffffffu, key > last);
+                            }
+                            if (key > last) list[listed + __popc(who & ((1u << lane) - 1))] = key;
+                            listed += __popc(who);
                         }
                     }
                 }
-                if (last != 0 && lane == 0 && (uint32_t)(last >> 32) > *(volatile uint32_t*)&s_bound) atomicMax(&s_bound, (uint32_t)(last >> 32));
             }
         }
     }
@@ -185,80 +301,109 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(LogprobArgs
     // the block's part
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        Sums other;
-        other.m = __shfl_xor_sync(0xffffffffu, mine.m, o);
-        other.s = __shfl_xor_sync(0xffffffffu, mine.s, o);
-        other.t = __shfl_xor_sync(0xffffffffu, mine.t, o);
-        // the same order on both sides
-        mine = (lane & o) == 0 ? join(mine, other) : join(other, mine);
+        sum_s += __shfl_xor_sync(0xffffffffu, sum_s, o);
+        sum_t += __shfl_xor_sync(0xffffffffu, sum_t, o);
     }
+    const Sums mine{m, sum_s, sum_t};
     if (bad) s_bad = 1;
     if (lane == 0) warp_sums[warp] = mine;
-    if (TOP && lane < a.top) s_keys[warp * a.top + lane] = best;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        Sums all = warp_sums[0];
-        for (int w = 1; w < kWarps; w++) all = join(all, warp_sums[w]);
-        part.sums = all;
-        part.bad = s_bad;
-    }
     if (TOP) {
-        const int c = kWarps * a.top;
-        if (threadIdx.x < c) {  // 8 warps x 32 at most: as many as threads
+        __syncthreads();  // the bound is the block's last
+        const uint32_t bound = s_bound;
+        int kept = 0;
+#pragma unroll
+        for (int k = 0; k < kList; k += 32) {
+            const unsigned long long key = k + lane < listed ? list[k + lane] : 0ull;
+            const bool keep = key != 0ull && (uint32_t)(key >> 32) >= bound;
+            const unsigned who = __ballot_sync(0xffffffffu, keep);
+            if (keep) list[kept + __popc(who & ((1u << lane) - 1))] = key;
+            kept += __popc(who);
+            __syncwarp();
+        }
+        listed = kept;
+        if (lane == 0) s_count[warp] = listed;
+        __syncthreads();
+        int all = 0, before = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) all += s_count[w];
+        if (all > kThreads) {  // cut the lists first: `top` of each at most
+            if (listed > a.top) {
+                (void)cut_list(list, listed, a.top, &s_bound);
+                listed = a.top;
+            }
+            __syncthreads();
+            if (lane == 0) s_count[warp] = listed;
+            __syncthreads();
+            all = 0;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) all += s_count[w];
+        }
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) before += w < warp ? s_count[w] : 0;
+        __syncwarp();
+        for (int k = lane; k < listed; k += 32) s_keys[before + k] = list[k];
+        if (threadIdx.x < a.top) part.keys[threadIdx.x] = 0ull;
+        __syncthreads();
+        if ((int)threadIdx.x < all) {
             const unsigned long long key = s_keys[threadIdx.x];
             int above = 0;
-            for (int k = 0; k < c; k++) above += s_keys[k] > key || (s_keys[k] == key && k < (int)threadIdx.x);  // empty places are equal
+#pragma unroll 4
+            for (int k = 0; k < all; k++) above += s_keys[k] > key;
             if (above < a.top) part.keys[above] = key;
         }
-    }
-    cluster.sync();
-    if (rank == 0) {
-        if (TOP) {
-            for (int k = threadIdx.x; k < size * a.top; k += kThreads) s_keys[k] = cluster.map_shared_rank(&part, k / a.top)->keys[k % a.top];
-        }
-        Sums all = part.sums;
-        int any_bad = part.bad;
-        for (int b = 1; b < size; b++) {
-            const BlockPart* p = cluster.map_shared_rank(&part, b);
-            all = join(all, p->sums);
-            any_bad |= p->bad;
-        }
+    } else {
         __syncthreads();
+    }
+    if (warp == 0) {
+        const Sums sums = join_lanes(lane < kWarps ? warp_sums[lane] : Sums{-INFINITY, 0.0, 0.0});
+        if (lane == 0) {
+            part.sums = sums;
+            part.bad = s_bad;
+        }
+    }
+    // the cluster's first block joins the parts
+    cluster.sync();
+    if (rank == 0 && (TOP || warp == 0)) {
+        const BlockPart* p = cluster.map_shared_rank(&part, min(lane, size - 1));
+        const Sums all = join_lanes(lane < size ? p->sums : Sums{-INFINITY, 0.0, 0.0});
+        const bool any_bad = __any_sync(0xffffffffu, p->bad != 0);
         const float nan = __int_as_float(0x7fffffff);
         const bool empty = all.m == -INFINITY;
-        const double ls = empty ? 0.0 : log(all.s);
+        // log S to f32: near 1 by way of S - 1
+        const float ls = empty ? 0.0f : all.s < 1.5 ? log1pf((float)(all.s - 1.0)) : logf((float)all.s);
         if (threadIdx.x == 0) {
-            if (a.entropy) a.entropy[r] = any_bad ? nan : empty ? 0.0f : (float)(ls - all.t / all.s);
+            if (a.entropy) a.entropy[r] = any_bad ? nan : empty ? 0.0f : ls - (float)all.t / (float)all.s;
             if (a.logprob) {
-                const int64_t tok = a.tokens[r];
-                float y = nan;
-                if (!any_bad && tok >= 0 && tok < a.vocab) y = empty ? -INFINITY : (float)((double)elem_f(whole[tok]) - (double)all.m - ls);
-                a.logprob[r] = y;
+                a.logprob[r] = any_bad || isnan(asked) ? nan : empty ? -INFINITY : (asked - all.m) - ls;
             }
         }
         if (TOP) {
             const int c = size * a.top;
-            if (threadIdx.x < c) {
+            if ((int)threadIdx.x < c) s_keys[threadIdx.x] = cluster.map_shared_rank(&part, threadIdx.x / a.top)->keys[threadIdx.x % a.top];
+            __syncthreads();
+            if ((int)threadIdx.x < c) {
                 const unsigned long long key = s_keys[threadIdx.x];
                 int above = 0;
-                for (int k = 0; k < c; k++) above += s_keys[k] > key || (s_keys[k] == key && k < (int)threadIdx.x);
+#pragma unroll 4
+                for (int k = 0; k < c; k++) above += s_keys[k] > key || (s_keys[k] == key && k < (int)threadIdx.x);  // empty places are equal
                 if (above < a.top) {
-                    const float v = value_of((uint32_t)(key >> 32));
-                    a.top_logprob[r * a.top + above] = any_bad ? nan : empty ? -INFINITY : (float)((double)v - (double)all.m - ls);
+                    a.top_logprob[r * a.top + above] = any_bad ? nan : empty ? -INFINITY : (value_of((uint32_t)(key >> 32)) - all.m) - ls;
                     a.top_id[r * a.top + above] = any_bad ? -1 : (int64_t)(uint32_t)~(uint32_t)key;
                 }
             }
         }
     }
-    cluster.sync();  // no block leaves while another reads its part
+    if (size > 1) cluster.sync();  // no block leaves while another reads its part
 }
 
 template <typename T>
 int32_t logprobs_as(LogprobArgs a, int rows, cudaStream_t s) {
     a.vec = rows_aligned(a.x, rows > 1 ? a.stride : 0, sizeof(T), 16);
-    // a cluster is as large as leaves two blocks an SM, and its blocks a chunk each
+    // as few blocks to a row as give every SM one, since a block's beginning and end take about 5 us: 64 rows of 32,000, 20 alternatives: 17.3, 12.8, 11.9, 15.9 us with 1, 2, 4,
+    // 8; 2,048 of 128,256, four: 157 with 1, 188 with 2; one row of 32,000, five: 12.7 with 1, 6.9 with 8
     int size = 1;
-    while (size < kMaxCluster && (int64_t)rows * size < 2 * sm_count() && a.vocab >= 2 * size * kThreads * kChunkElems / 4) size *= 2;
+    while (size < kMaxCluster && (int64_t)rows * size < sm_count() && a.vocab >= size * kThreads * 8) size *= 2;
+    while ((1 << a.size_shift) < size) a.size_shift++;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * size);
     cfg.blockDim = dim3(kThreads);
@@ -291,7 +436,7 @@ int32_t check_logprobs(const char* call, int64_t rows, int64_t vocab, int64_t st
 int32_t launch_token_logprobs(uint32_t typ, const void* x, int32_t rows, int32_t vocab, int64_t stride, const int64_t* tokens, int32_t top,
                               float* logprob, float* entropy, float* top_logprob, int64_t* top_id, cudaStream_t s) {
     if (rows == 0) return LC_OK;
-    LogprobArgs a{x, tokens, logprob, entropy, top_logprob, top_id, stride, vocab, top, 0};
+    LogprobArgs a{x, tokens, logprob, entropy, top_logprob, top_id, stride, vocab, top, 0, 0};
     if (typ == LC_TYPE_F32) return logprobs_as<float>(a, rows, s);
     if (typ == LC_TYPE_F16) return logprobs_as<__half>(a, rows, s);
     return logprobs_as<__nv_bfloat16>(a, rows, s);
