@@ -160,7 +160,9 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(LogprobArgs
     __shared__ uint32_t s_bound;                       // order of a value that at least `top` logits reach
     __shared__ unsigned long long s_list[kWarps][kList];
     __shared__ int s_count[kWarps];
-    __shared__ __align__(16) uint32_t s_top[kGroups];                // maxima of four lanes each, in the order of whole numbers
+    __shared__ __align__(16) uint32_t s_seen[kWarps][kGroups];
+    static_assert(kGroups == 64, "two maxima a lane");
+    __shared__ uint32_t s_top[kGroups];                // maxima of four lanes each, in the order of whole numbers
     __shared__ unsigned long long s_keys[kThreads];
     static_assert(kMaxCluster * kMaxTop <= kThreads && kWarps * kMaxTop <= kThreads, "a thread for each of the keys that are joined");
     cg::cluster_group cluster = cg::this_cluster();
@@ -241,11 +243,16 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(LogprobArgs
                 else __syncwarp();
                 // at first every warp finds it, for itself; then one of them, for all
                 if (steps == 0 || warp == (__popc(steps) & (kWarps - 1))) {
-                    const uint32_t v0 = s_top[lane], v1 = s_top[32 + lane];
+                    // what the other warps go on writing is copied first: compared with later maxima, none of the earlier ones may be left
+                    const uint32_t v0 = *(volatile uint32_t*)&s_top[lane], v1 = *(volatile uint32_t*)&s_top[32 + lane];
+                    uint32_t* const seen = s_seen[warp];
+                    seen[lane] = v0;
+                    seen[32 + lane] = v1;
+                    __syncwarp();
                     int above0 = 0, above1 = 0;
 #pragma unroll
                     for (int k = 0; k < kGroups; k += 4) {
-                        const uint4 u = *reinterpret_cast<const uint4*>(&s_top[k]);
+                        const uint4 u = *reinterpret_cast<const uint4*>(&seen[k]);
                         above0 += (u.x > v0) + (u.y > v0) + (u.z > v0) + (u.w > v0);
                         above1 += (u.x > v1) + (u.y > v1) + (u.z > v1) + (u.w > v1);
                     }

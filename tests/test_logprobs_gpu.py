@@ -138,3 +138,11 @@ def test_many_rows_and_far_offsets(gpu):
     lp, ent, tl, ti = gpu.token_logprobs_dev(x, tokens, top=1)
     assert ti[-1].item() == 39999 and ti[-2].item() == 1 and ti[0].item() == 0
     assert abs(lp[-1].item() - (3 - math.log(39999 + math.exp(3)))) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_many_rows_whose_best_come_late(gpu, dtype):
+    """Rows that rise towards their end: bounds that are found while other warps go on must never pass the alternatives that are wanted."""
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(1500, 9001, generator=g) + torch.arange(9001)[None] * (torch.rand(1500, 1, generator=g) * 1e-3)
+    check(gpu, x.to(DT[dtype]).cuda(), torch.randint(9001, (1500,), generator=g).cuda(), 10)
