@@ -10,8 +10,10 @@
 // to 2^-64 of one, however far the position is (cos and sin of an f32 angle lose 2^-24 of the ANGLE: 0.06 at 10^6).
 //
 // Both kernels move bytes: an append reads its rows once from HBM (a page's second pass over them finds them in L1/L2) and writes a quarter or half of that.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 #include "lc_kv8.cuh"
 #include "lc_kernels.h"
 #include "lc_tma.cuh"
@@ -69,38 +71,384 @@ struct AppendArgs {
     int n_heads, half;            // half = rot_dim / 2
     const uint64_t* turns;
     int window, table_rows;       // rows of a block's window; rows that its table of rotations has room for
+    int kv_slices;                // blocks of a window for the keys and values; the others are the queries'
 };
 
 __device__ __forceinline__ double finite_abs(double x) { return isfinite(x) ? fabs(x) : 0.0; }
-// x / S as an integer of 8 bits; inv = 1 / S in 64 bits (0 where S is 0): one rounding more than the quotient, 2^-53 of it
-__device__ __forceinline__ int to_int8(double x, double inv) {
-    if (isnan(x) || inv == 0.0) return 0;
-    return (int)rint(fmin(fmax(x * inv, -127.0), 127.0));
+// x / S, correctly rounded: inv = 1 / S is, and the remainder of the first quotient brings it there (Markstein); ties of x / S are ties then
+__device__ __forceinline__ double quotient(double x, double scale, double inv) {
+    const double q = x * inv;
+    return fma(fma(-q, scale, x), inv, q);
+}
+// Added to 1.5 2^52, a number below 2^51 is rounded to a whole one, to the nearest even, which is then the sum's lower word.
+// For finite x no larger than 127.5 S: what is left after a page's largest magnitude has made its scale (S of 0: inv is 0 as well).
+__device__ __forceinline__ int near_int8(double x, double scale, double inv) {
+    return max(-127, min(127, __double2loint(quotient(x, scale, inv) + 0x1.8p52)));
+}
+__device__ __forceinline__ int to_int8(double x, double scale, double inv) {
+    if (!(fabs(x) < INFINITY)) return isnan(x) || inv == 0.0 ? 0 : x > 0.0 ? 127 : -127;
+    return near_int8(x, scale, inv);
 }
 
-// The rotations of rows pos0 .. pos0 + n - 1: (cosine, sine) of every pair.
-__device__ __forceinline__ void fill_table(double2* tab, const uint64_t* __restrict__ turns, int half, int pos0, int n) {
+// four elements in a row
+template <typename T> __device__ __forceinline__ void load4(const T* p, float (&v)[4]);
+template <> __device__ __forceinline__ void load4<float>(const float* p, float (&v)[4]) {
+    const float4 w = *reinterpret_cast<const float4*>(p);
+    v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+}
+template <> __device__ __forceinline__ void load4<__half>(const __half* p, float (&v)[4]) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+template <> __device__ __forceinline__ void load4<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[4]) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(w.x << 16); v[1] = __uint_as_float(w.x & 0xffff0000u); v[2] = __uint_as_float(w.y << 16); v[3] = __uint_as_float(w.y & 0xffff0000u);
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, const float (&v)[4]) {
+    __align__(16) T t[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) t[e] = to_elem<T>(v[e]);
+    if (sizeof(T) == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
+    else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(t);
+}
+// u c - w s in f32 with the cosine and sine as two f32 each: the difference of the products with what the second lost (Kahan), 1.5 2^-24 of the result off,
+// and what the high parts leave out
+__device__ __forceinline__ float turned(float u, float w, float ch, float cl, float sh, float sl) {
+    const float p = w * sh, lost = fmaf(-w, sh, p), d = fmaf(u, ch, -p);
+    const float y = d + (lost + fmaf(u, cl, -w * sl));
+    return fabsf(d) < INFINITY ? y : d;
+}
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
+}
+// four numbers' low bytes
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) { return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410); }
+
+// The rotations of rows pos0 .. pos0 + n - 1: (cosine, sine) of every pair.  Sine and cosine themselves for every eighth row and for the first
+// eight turns; the rest are products of the two, 2^-52 off.  SPREAD: pair d lies at place (d mod 4) half / 4 + d / 4, so that lanes with four pairs each read
+// neighbouring places.  They are kept as two f32 each, 2^-48 of them off.
+__device__ __forceinline__ double2 turn_of(uint64_t per_position, int64_t positions) {
+    const int64_t frac = (int64_t)((uint64_t)positions * per_position);
+    double2 r;
+    sincospi((double)frac * 0x1p-63, &r.y, &r.x);  // frac 2^-64 turns = frac 2^-63 pi
+    return r;
+}
+__device__ __forceinline__ void set_turn(float4& at, double2 t) {
+    at.x = (float)t.x; at.y = (float)(t.x - at.x);
+    at.z = (float)t.y; at.w = (float)(t.y - at.z);
+}
+// a pair's rotation in 64 bits
+__device__ __forceinline__ void turned64(float u, float w, const float4& t, double& y0, double& y1) {
+    const double c = (double)t.x + (double)t.y, s = (double)t.z + (double)t.w;
+    y0 = u * c - w * s;
+    y1 = u * s + w * c;
+}
+template <bool SPREAD>
+__device__ __forceinline__ void fill_table(float4* tab, double2* bases, const uint64_t* __restrict__ turns, int half, int pos0, int n) {
+    auto pair_at = [&](int at) {  // the pair at a place
+        if (!SPREAD) return at;
+        const int quarter = half >> 2, c = at / quarter;
+        return (at - c * quarter) * 4 + c;
+    };
+    if (n <= 8) {
+        for (int e = threadIdx.x; e < n * half; e += blockDim.x) {
+            const int j = e / half;
+            set_turn(tab[e], turn_of(turns[pair_at(e - j * half)], pos0 + j));
+        }
+        return;
+    }
+    const int n8 = (n + 7) >> 3;     // [n8 bases, then 8 first turns][half]
+    for (int e = threadIdx.x; e < (n8 + 8) * half; e += blockDim.x) {
+        const int j = e / half, at = e - j * half;
+        bases[e] = turn_of(turns[pair_at(at)], j < n8 ? pos0 + j * 8 : j - n8);
+    }
+    __syncthreads();
     for (int e = threadIdx.x; e < n * half; e += blockDim.x) {
-        const int j = e / half, d = e - j * half;
-        const int64_t frac = (int64_t)((uint64_t)(pos0 + j) * turns[d]);
-        double s, c;
-        sincospi((double)frac * 0x1p-63, &s, &c);  // frac 2^-64 turns = frac 2^-63 pi
-        tab[e] = make_double2(c, s);
+        const int j = e / half, at = e - j * half;
+        const double2 x = bases[(j >> 3) * half + at], y = bases[(n8 + (j & 7)) * half + at];
+        set_turn(tab[e], make_double2(x.x * y.x - x.y * y.y, x.x * y.y + x.y * y.x));
     }
 }
 
-// grid: (windows of rows, slices of heads).  A block serves the groups that begin in its window; a group is the rows of one sequence
-// in one page.  An item is a (keys or values, head) of the group and belongs to one warp, which passes over its rows twice: largest
-// magnitude, then integers.  The rotations are taken once for all heads of the slice.
-template <typename T>
-__global__ void __launch_bounds__(256) kv8_append_kernel(Kv8Pool pool, Kv8Seqs seqs, AppendArgs a) {
-    extern __shared__ double2 tab[];
-    if (blockIdx.x == 0 && blockIdx.y == 0) kv8_check_seqs(seqs, pool);
+// What of a group - the rows of one sequence in one page - a block serves.
+struct Group {
+    int row, cnt, pos, slot;
+    size_t page_head;             // page * kv heads
+    bool held;
+};
+
+// Keys and values of a group: an item is (keys or values, head) and belongs to one warp, which passes over its rows up to three times:
+//   kMost   the rows' largest magnitude, of keys after their rotation, in f32;
+//   kFine   of the rotated keys that may be the largest (a rotation is off by 2^-22 of the pair's length, at most 1.42 of the largest magnitude: those within 2^-19 of it), the
+//           largest in 64 bits;
+//   kInts   integers: x / S in f32 is within 2e-4 of the quotient (rotation 2^-22 of at most 180 S, product and inverse 2^-22 of 127.5), so that it gives the integer of
+//           the 64-bit quotient unless it lies so near a half; eight elements with such a one among them, one group in 300, are taken in 64 bits.
+// Rows with infinities or NaN, which the first maximum shows, and scales below 1e-30 go the long way, all in 64 bits.  5,000 rows of eight heads, bf16, 5 prompts: 171 us with
+// everything in 64 bits and an element per lane, 31 now (a table of rotations 2.3 of a block's 12, each pass 2 to 4: their instructions).
+//
+enum : int { kMost, kFine, kInts };
+struct Item {
+    double top, scale, inv;
+    float most, least, inv32;  // the largest magnitude in f32, what may be the largest in 64 bits, 1 / scale
+    bool slow;
+};
+// Rows row0 .. row0 + cn - 1 of an item by one warp: a lane has four pairs (d, d + hd / 2) of a row, a warp as many rows at a time as it has lanes for.
+template <typename T, int PASS, bool TURN>
+__device__ __forceinline__ void rows_pass(Item& it, const T* rows, int64_t stride, int cn, int8_t* dst, int hd, const float4* tab) {
+    const int lane = threadIdx.x & 31, lanes = hd >> 3, at_once = 32 / lanes, jl = lane / lanes, d = (lane - jl * lanes) * 4, other = hd >> 1, half = hd >> 1, quarter = hd >> 3;
+    if (jl >= at_once) return;
+    rows += d;
+    for (int j0 = jl; j0 < cn; j0 += 2 * at_once) {
+        float u[2][4], w[2][4];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const T* row = rows + (int64_t)min(j0 + b * at_once, cn - 1) * stride;
+            load4(row, u[b]);
+            load4(row + other, w[b]);
+        }
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int j = j0 + b * at_once;
+            if (j >= cn) break;
+            const float4* t = tab + j * half + (d >> 2);
+            float y0[4], y1[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                y0[e] = u[b][e];
+                y1[e] = w[b][e];
+                if (TURN) {
+                    const float4 cs = t[e * quarter];
+                    y0[e] = u[b][e] * cs.x - w[b][e] * cs.z;
+                    y1[e] = u[b][e] * cs.z + w[b][e] * cs.x;
+                }
+            }
+            if (PASS == kMost) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) it.most = max_abs_nan(max_abs_nan(it.most, y0[e]), y1[e]);
+            } else if (PASS == kFine) {
+                float here = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) here = fmaxf(here, fmaxf(fabsf(y0[e]), fabsf(y1[e])));
+                if (it.slow || here >= it.least) {
+#pragma unroll 1
+                    for (int e = 0; e < 4; e++) {
+                        double z0 = u[b][0], z1 = w[b][0];
+                        if (TURN) turned64(u[b][0], w[b][0], t[e * quarter], z0, z1);
+                        it.top = fmax(it.top, fmax(finite_abs(z0), finite_abs(z1)));
+#pragma unroll
+                        for (int k = 0; k < 3; k++) { u[b][k] = u[b][k + 1]; w[b][k] = w[b][k + 1]; }
+                    }
+                }
+            } else {
+                float r0[4], r1[4], off = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float q0 = y0[e] * it.inv32, q1 = y1[e] * it.inv32;
+                    r0[e] = q0 + 12582912.0f;  // 1.5 2^23: rounded to a whole number, in the low bits
+                    r1[e] = q1 + 12582912.0f;
+                    off = fmaxf(off, fmaxf(fabsf(q0 - (r0[e] - 12582912.0f)), fabsf(q1 - (r1[e] - 12582912.0f))));
+                }
+                uint32_t b0 = pack4(__float_as_int(r0[0]), __float_as_int(r0[1]), __float_as_int(r0[2]), __float_as_int(r0[3]));
+                uint32_t b1 = pack4(__float_as_int(r1[0]), __float_as_int(r1[1]), __float_as_int(r1[2]), __float_as_int(r1[3]));
+                if (it.slow || !(off < 0.4998f)) {
+                    b0 = b1 = 0;
+#pragma unroll 1
+                    for (int e = 0; e < 4; e++) {
+                        double z0 = u[b][0], z1 = w[b][0];
+                        if (TURN) turned64(u[b][0], w[b][0], t[e * quarter], z0, z1);
+                        b0 |= (uint32_t)(to_int8(z0, it.scale, it.inv) & 0xff) << (8 * e);
+                        b1 |= (uint32_t)(to_int8(z1, it.scale, it.inv) & 0xff) << (8 * e);
+#pragma unroll
+                        for (int k = 0; k < 3; k++) { u[b][k] = u[b][k + 1]; w[b][k] = w[b][k + 1]; }
+                    }
+                }
+                int8_t* o = dst + (size_t)j * hd + d;
+                *reinterpret_cast<uint32_t*>(o) = b0;
+                *reinterpret_cast<uint32_t*>(o + other) = b1;
+            }
+        }
+    }
+}
+// The same for any strides, alignment and rotated part of the dims, all in 64 bits.
+template <typename T, int PASS>
+__device__ __forceinline__ void rows_pass_plain(Item& it, const T* rows, int64_t stride, int cn, int8_t* dst, int hd, const float4* tab, int half) {
+    const int lane = threadIdx.x & 31;
+    for (int j = 0; j < cn; j++) {
+        const T* row = rows + (int64_t)j * stride;
+        int8_t* o = dst + (size_t)j * hd;
+        for (int d = lane; d < half; d += 32) {
+            double y0, y1;
+            turned64(elem_f(row[d]), elem_f(row[d + half]), tab[j * half + d], y0, y1);
+            if (PASS == kFine) {
+                it.top = fmax(it.top, fmax(finite_abs(y0), finite_abs(y1)));
+            } else {
+                o[d] = (int8_t)to_int8(y0, it.scale, it.inv);
+                o[d + half] = (int8_t)to_int8(y1, it.scale, it.inv);
+            }
+        }
+        for (int d = 2 * half + lane; d < hd; d += 32) {
+            const double y = elem_f(row[d]);
+            if (PASS == kFine) it.top = fmax(it.top, finite_abs(y));
+            else o[d] = (int8_t)to_int8(y, it.scale, it.inv);
+        }
+    }
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void append_kv(const Kv8Pool& pool, const AppendArgs& a, const Group& gr, float4* tab, double2* bases, int kv0, int kv1) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    const int page = 1 << pool.page_shift, hd = pool.hd, half = a.half, rot = 2 * half;
-    const int slices = gridDim.y, sl = blockIdx.y;
-    const int kv0 = (int)((long long)pool.n_kv * sl / slices), kv1 = (int)((long long)pool.n_kv * (sl + 1) / slices);
-    const int q0 = (int)((long long)a.n_heads * sl / slices), q1 = (int)((long long)a.n_heads * (sl + 1) / slices);
+    const int page = 1 << pool.page_shift, hd = pool.hd, half = a.half;
+    const bool one_table = gr.cnt <= a.table_rows;
+    const int items = gr.held ? 2 * (kv1 - kv0) : 0;
+    if (one_table) {
+        __syncthreads();  // the group before has done with the table
+        fill_table<VEC>(tab, bases, a.turns, half, gr.pos, gr.cnt);
+        __syncthreads();
+    }
+    // every warp takes as many turns as the one with most items: the table's refills are the block's
+    const int rounds = (items + nw - 1) / nw;
+    for (int round = 0; round < rounds; round++) {
+        const int n = round * nw + warp;
+        const bool mine = n < items;
+        const bool is_k = n < (kv1 - kv0), turn = is_k && half > 0;
+        const int h = kv0 + (is_k ? n : n - (kv1 - kv0));
+        const int64_t stride = is_k ? a.k_stride : a.v_stride;
+        const T* x = (const T*)(is_k ? a.k : a.v) + (int64_t)h * hd + (int64_t)gr.row * stride;
+        const size_t ph = gr.page_head + h;
+        int8_t* dst = (is_k ? pool.k : pool.v) + ph * page * hd;
+        Item it;
+        it.top = it.scale = it.inv = 0.0;
+        it.most = it.least = it.inv32 = 0.0f;
+        it.slow = !VEC;               // infinities or NaN among the rows, or a scale too small for f32
+        auto pass = [&](auto which) {
+            constexpr int PASS = decltype(which)::value;
+            for (int c0 = 0; c0 < gr.cnt; c0 += a.table_rows) {
+                const int cn = min(a.table_rows, gr.cnt - c0);
+                if (!one_table) {
+                    __syncthreads();
+                    fill_table<VEC>(tab, bases, a.turns, half, gr.pos + c0, cn);
+                    __syncthreads();
+                }
+                if (!mine || (PASS == kFine && !it.slow && !turn)) continue;
+                const T* rows = x + (int64_t)c0 * stride;
+                int8_t* to = dst + (size_t)(gr.slot + c0) * hd;
+                if constexpr (!VEC) {
+                    if (PASS != kMost) rows_pass_plain<T, PASS>(it, rows, stride, cn, to, hd, tab, turn ? half : 0);
+                } else if (turn) {
+                    rows_pass<T, PASS, true>(it, rows, stride, cn, to, hd, tab);
+                } else {
+                    rows_pass<T, PASS, false>(it, rows, stride, cn, to, hd, tab);
+                }
+            }
+        };
+        pass(std::integral_constant<int, kMost>());
+        if (VEC) {
+            it.slow = __any_sync(0xffffffffu, !(it.most < INFINITY));
+            it.most = warp_max(it.most);
+            it.least = it.most * (1.0f - 0x1p-19f);
+            it.top = it.slow || turn ? 0.0 : (double)it.most;
+        }
+        pass(std::integral_constant<int, kFine>());
+        if (mine) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) it.top = fmax(it.top, __shfl_xor_sync(0xffffffffu, it.top, o));
+            float* sp = (is_k ? pool.k_scale : pool.v_scale) + ph;
+            const float before = gr.slot > 0 ? *sp : 0.0f;
+            const float now = fmaxf(before, (float)(it.top / 127.0));
+            it.scale = (double)now;
+            it.inv = now > 0.0f ? 1.0 / it.scale : 0.0;
+            it.slow = it.slow || !(now > 1e-30f);
+            it.inv32 = (float)it.inv;
+            if (gr.slot > 0 && now != before) {
+                for (int e = lane * 4; e < gr.slot * hd; e += 128) {
+                    char4 b = *reinterpret_cast<char4*>(dst + e);
+                    b.x = (signed char)(int)rint((double)b.x * (double)before / (double)now);
+                    b.y = (signed char)(int)rint((double)b.y * (double)before / (double)now);
+                    b.z = (signed char)(int)rint((double)b.z * (double)before / (double)now);
+                    b.w = (signed char)(int)rint((double)b.w * (double)before / (double)now);
+                    *reinterpret_cast<char4*>(dst + e) = b;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) *sp = now;
+        }
+        pass(std::integral_constant<int, kInts>());
+    }
+}
+
+// The queries of a group, heads q0 .. q1 - 1.
+template <typename T, bool VEC>
+__device__ __forceinline__ void rotate_q(const Kv8Pool& pool, const AppendArgs& a, const Group& gr, float4* tab, double2* bases, int q0, int q1) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5, hd = pool.hd, half = a.half;
+    for (int c0 = 0; c0 < gr.cnt; c0 += a.table_rows) {
+        const int cn = min(a.table_rows, gr.cnt - c0);
+        __syncthreads();
+        fill_table<VEC>(tab, bases, a.turns, half, gr.pos + c0, cn);
+        __syncthreads();
+        if constexpr (VEC) {
+            // the lanes and pairs as above; a lane keeps its rotations for four heads, whose loads go out together
+            constexpr int B = 4;
+            const int lanes = hd >> 3, at_once = 32 / lanes, jl = lane / lanes, d = (lane - jl * lanes) * 4, other = hd >> 1;
+            const int quads = (q1 - q0 + B - 1) / B, rows = (cn + at_once - 1) / at_once;
+            for (int e = warp; e < rows * quads; e += nw) {
+                const int rj = e / quads, j = rj * at_once + jl, h = q0 + B * (e - rj * quads);
+                if (jl >= at_once || j >= cn) continue;
+                const int64_t row = gr.row + c0 + j;
+                const T* src = (const T*)a.q + row * a.q_stride + (int64_t)h * hd + d;
+                T* o = (T*)a.q_out + row * a.qo_stride + (int64_t)h * hd + d;
+                float u[B][4], w[B][4];
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    const int64_t at = (int64_t)min(b, q1 - 1 - h) * hd;
+                    load4(src + at, u[b]);
+                    load4(src + at + other, w[b]);
+                }
+                float4 t[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) t[k] = half ? tab[j * half + k * (half >> 2) + (d >> 2)] : make_float4(1.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int b = 0; b < B; b++) {
+                    if (h + b >= q1) break;
+                    float y0[4], y1[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        y0[k] = turned(u[b][k], w[b][k], t[k].x, t[k].y, t[k].z, t[k].w);
+                        y1[k] = turned(u[b][k], -w[b][k], t[k].z, t[k].w, t[k].x, t[k].y);
+                    }
+                    store4(o + (int64_t)b * hd, y0);
+                    store4(o + (int64_t)b * hd + other, y1);
+                }
+            }
+        } else {
+            for (int e = warp; e < cn * (q1 - q0); e += nw) {
+                const int j = e / (q1 - q0), h = q0 + e - j * (q1 - q0);
+                const T* src = (const T*)a.q + (int64_t)(gr.row + c0 + j) * a.q_stride + (int64_t)h * hd;
+                T* o = (T*)a.q_out + (int64_t)(gr.row + c0 + j) * a.qo_stride + (int64_t)h * hd;
+                for (int d = lane; d < half; d += 32) {
+                    const float u = elem_f(src[d]), w = elem_f(src[d + half]);
+                    const float4 t = tab[j * half + d];
+                    o[d] = to_elem<T>(turned(u, w, t.x, t.y, t.z, t.w));
+                    o[d + half] = to_elem<T>(turned(u, -w, t.z, t.w, t.x, t.y));
+                }
+                for (int d = 2 * half + lane; d < hd; d += 32) o[d] = src[d];
+            }
+        }
+    }
+}
+
+// grid: (windows of rows, slices of kv heads and then of query heads).  A block serves the groups that begin in its window.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256, 3) kv8_append_kernel(Kv8Pool pool, Kv8Seqs seqs, AppendArgs a) {
+    extern __shared__ float4 tab[];
+    double2* const bases = reinterpret_cast<double2*>(tab + a.table_rows * a.half);
+    if (blockIdx.x == 0 && blockIdx.y == 0) kv8_check_seqs(seqs, pool);
+    const int page = 1 << pool.page_shift;
+    const bool kv = (int)blockIdx.y < a.kv_slices;
+    const int slices = kv ? a.kv_slices : gridDim.y - a.kv_slices, sl = kv ? blockIdx.y : blockIdx.y - a.kv_slices, heads = kv ? pool.n_kv : a.n_heads;
+    const int h0 = heads * sl / slices, h1 = heads * (sl + 1) / slices;
     int r = blockIdx.x * a.window;
     const int r_end = min(r + a.window, seqs.n_rows);
     while (r < r_end) {
@@ -108,109 +456,28 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8Pool pool, Kv8Seqs s
         if (i < 0) { r++; continue; }
         int first, n;
         kv8_span(seqs, i, first, n);
-        const int ctx = seqs.ctx[i];
-        if (!kv8_in_table(seqs, pool, ctx, n)) { r = first + n; continue; }
-        const int pos = ctx + (r - first), slot = pos & (page - 1);
-        if (slot != 0 && r != first) { r += min(page - slot, first + n - r); continue; }  // inside a group that another window has
-        const int cnt = min(page - slot, first + n - r);
-        const int number = seqs.table[(size_t)i * seqs.width + (pos >> pool.page_shift)];
-        const bool held = number >= 0 && number < pool.n_pages;
-        if (!held && threadIdx.x == 0) kv8_raise(seqs, i);
-        const bool one_table = cnt <= a.table_rows;
-        const int items = held ? 2 * (kv1 - kv0) : 0;
-        if (one_table) {
-            __syncthreads();  // the group before has done with the table
-            fill_table(tab, a.turns, half, pos, cnt);
-            __syncthreads();
-        }
-        // every warp takes as many turns as the one with most items: the table's refills are the block's
-        const int rounds = (items + nw - 1) / nw;
-        for (int round = 0; round < rounds; round++) {
-            const int it = round * nw + warp;
-            const bool mine = it < items;
-            const bool is_k = it < (kv1 - kv0);
-            const int h = kv0 + (is_k ? it : it - (kv1 - kv0));
-            const T* x = (const T*)(is_k ? a.k : a.v) + (int64_t)h * hd;
-            const int64_t stride = is_k ? a.k_stride : a.v_stride;
-            const int hf = is_k ? half : 0, rt = is_k ? rot : 0;
-            const size_t ph = (size_t)number * pool.n_kv + h;
-            int8_t* dst = (is_k ? pool.k : pool.v) + ph * page * hd;
-            double top = 0.0, inv = 0.0;
-            for (int pass = 0; pass < 2; pass++) {
-                for (int c0 = 0; c0 < cnt; c0 += a.table_rows) {
-                    const int cn = min(a.table_rows, cnt - c0);
-                    if (!one_table) {
-                        __syncthreads();
-                        fill_table(tab, a.turns, half, pos + c0, cn);
-                        __syncthreads();
-                    }
-                    if (!mine) continue;
-                    for (int j = 0; j < cn; j++) {
-                        const T* row = x + (int64_t)(r + c0 + j) * stride;
-                        int8_t* o = dst + (size_t)(slot + c0 + j) * hd;
-                        for (int d = lane; d < hf; d += 32) {
-                            const double u = elem_f(row[d]), w = elem_f(row[d + hf]);
-                            const double2 cs = tab[j * hf + d];
-                            const double y0 = u * cs.x - w * cs.y, y1 = u * cs.y + w * cs.x;
-                            if (pass == 0) {
-                                top = fmax(top, fmax(finite_abs(y0), finite_abs(y1)));
-                            } else {
-                                o[d] = (int8_t)to_int8(y0, inv);
-                                o[d + hf] = (int8_t)to_int8(y1, inv);
-                            }
-                        }
-                        for (int d = rt + lane; d < hd; d += 32) {
-                            const double y = elem_f(row[d]);
-                            if (pass == 0) top = fmax(top, finite_abs(y));
-                            else o[d] = (int8_t)to_int8(y, inv);
-                        }
-                    }
-                }
-                if (pass == 0 && mine) {
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    float* sp = (is_k ? pool.k_scale : pool.v_scale) + ph;
-                    const float before = slot > 0 ? *sp : 0.0f;
-                    const float now = fmaxf(before, (float)(top / 127.0));
-                    inv = now > 0.0f ? 1.0 / (double)now : 0.0;
-                    if (slot > 0 && now != before) {
-                        for (int e = lane * 4; e < slot * hd; e += 128) {
-                            char4 b = *reinterpret_cast<char4*>(dst + e);
-                            b.x = (signed char)(int)rint((double)b.x * (double)before / (double)now);
-                            b.y = (signed char)(int)rint((double)b.y * (double)before / (double)now);
-                            b.z = (signed char)(int)rint((double)b.z * (double)before / (double)now);
-                            b.w = (signed char)(int)rint((double)b.w * (double)before / (double)now);
-                            *reinterpret_cast<char4*>(dst + e) = b;
-                        }
-                    }
-                    __syncwarp();
-                    if (lane == 0) *sp = now;
-                }
+        const int ctx = seqs.ctx[i], end = first + n;
+        if (!kv8_in_table(seqs, pool, ctx, n)) { r = end; continue; }
+        const int32_t* table = seqs.table + (size_t)i * seqs.width;
+        if (r != first) r += (-(ctx + r - first)) & (page - 1);  // inside a group that another window has: to the next page
+        while (r < min(r_end, end)) {
+            const int pos = ctx + (r - first), slot = pos & (page - 1);
+            const int number = table[pos >> pool.page_shift];
+            Group gr;
+            gr.row = r;
+            gr.cnt = min(page - slot, end - r);
+            gr.pos = pos;
+            gr.slot = slot;
+            gr.held = number >= 0 && number < pool.n_pages;
+            gr.page_head = (size_t)(gr.held ? number : 0) * pool.n_kv;
+            if (kv) {
+                if (!gr.held && threadIdx.x == 0) kv8_raise(seqs, i);
+                append_kv<T, VEC>(pool, a, gr, tab, bases, h0, h1);
+            } else {
+                rotate_q<T, VEC>(pool, a, gr, tab, bases, h0, h1);
             }
+            r += gr.cnt;
         }
-        if (a.q) {
-            for (int c0 = 0; c0 < cnt; c0 += a.table_rows) {
-                const int cn = min(a.table_rows, cnt - c0);
-                if (!one_table) {
-                    __syncthreads();
-                    fill_table(tab, a.turns, half, pos + c0, cn);
-                    __syncthreads();
-                }
-                for (int e = warp; e < cn * (q1 - q0); e += nw) {
-                    const int j = e / (q1 - q0), h = q0 + e - j * (q1 - q0);
-                    const T* src = (const T*)a.q + (int64_t)(r + c0 + j) * a.q_stride + (int64_t)h * hd;
-                    T* o = (T*)a.q_out + (int64_t)(r + c0 + j) * a.qo_stride + (int64_t)h * hd;
-                    for (int d = lane; d < half; d += 32) {
-                        const float u = elem_f(src[d]), w = elem_f(src[d + half]);
-                        const double2 cs = tab[j * half + d];
-                        o[d] = to_elem<T>((float)(u * cs.x - w * cs.y));
-                        o[d + half] = to_elem<T>((float)(u * cs.y + w * cs.x));
-                    }
-                    for (int d = rot + lane; d < hd; d += 32) o[d] = src[d];
-                }
-            }
-        }
-        r += cnt;
     }
 }
 
@@ -221,13 +488,15 @@ struct ReadArgs {
     int vec;  // whether 16 elements are stored in 16-byte pieces
 };
 
-// A warp per row: 16 integers of a head per lane.
+// A warp takes 32 pieces of 16 integers (of the keys', then the values' heads) of a row.
 template <typename T>
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Pool pool, Kv8Seqs seqs, ReadArgs a) {
     if (blockIdx.x == 0) kv8_check_seqs(seqs, pool);
     const int lane = threadIdx.x & 31, warps = gridDim.x * (blockDim.x >> 5);
-    const int pieces = pool.hd >> 4, all = pool.n_kv * pieces;
-    for (int r = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); r < seqs.n_rows; r += warps) {
+    const int pieces = pool.hd >> 4, all = pool.n_kv * pieces, parts = (2 * all + 31) >> 5;
+    const int64_t units = (int64_t)seqs.n_rows * parts;
+    for (int64_t unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); unit < units; unit += warps) {
+        const int r = (int)(unit / parts), e = (int)(unit - (int64_t)r * parts) * 32 + lane;
         const int i = kv8_seq_of_row(seqs, r);
         if (i < 0) continue;
         int first, n;
@@ -239,30 +508,28 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Pool pool, Kv8Seqs seq
         const bool held = number >= 0 && number < pool.n_pages;
         if (!held && lane == 0) kv8_raise(seqs, i);
         const int slot = pos & ((1 << pool.page_shift) - 1);
-        for (int e = lane; e < 2 * all; e += 32) {
-            const bool is_k = e < all;
-            T* out = (T*)(is_k ? a.k : a.v);
-            if (!out) continue;
-            const int f = is_k ? e : e - all, h = f / pieces, c = f - h * pieces;
-            float scale = __int_as_float(0x7fffffff);
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (held) {
-                const size_t ph = (size_t)number * pool.n_kv + h;
-                w = *reinterpret_cast<const uint4*>((is_k ? pool.k : pool.v) + ((ph << pool.page_shift) + slot) * pool.hd + c * 16);
-                scale = (is_k ? pool.k_scale : pool.v_scale)[ph];
-            }
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-            __align__(16) T t[16];
+        const bool is_k = e < all;
+        T* out = (T*)(is_k ? a.k : a.v);
+        if (e >= 2 * all || !out) continue;
+        const int f = is_k ? e : e - all, h = f / pieces, c = f - h * pieces;
+        float scale = __int_as_float(0x7fffffff);
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (held) {
+            const size_t ph = (size_t)number * pool.n_kv + h;
+            w = *reinterpret_cast<const uint4*>((is_k ? pool.k : pool.v) + ((ph << pool.page_shift) + slot) * pool.hd + c * 16);
+            scale = (is_k ? pool.k_scale : pool.v_scale)[ph];
+        }
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        __align__(16) T t[16];
 #pragma unroll
-            for (int b = 0; b < 16; b++) t[b] = to_elem<T>((float)(int8_t)(words[b >> 2] >> (8 * (b & 3))) * scale);
-            out += (int64_t)r * (is_k ? a.k_stride : a.v_stride) + (int64_t)h * pool.hd + c * 16;
-            if (a.vec) {
+        for (int b = 0; b < 16; b++) t[b] = to_elem<T>((float)(int8_t)(words[b >> 2] >> (8 * (b & 3))) * scale);
+        out += (int64_t)r * (is_k ? a.k_stride : a.v_stride) + (int64_t)h * pool.hd + c * 16;
+        if (a.vec) {
 #pragma unroll
-                for (int b = 0; b < (int)sizeof(T); b++) reinterpret_cast<uint4*>(out)[b] = reinterpret_cast<const uint4*>(t)[b];
-            } else {
+            for (int b = 0; b < (int)sizeof(T); b++) reinterpret_cast<uint4*>(out)[b] = reinterpret_cast<const uint4*>(t)[b];
+        } else {
 #pragma unroll
-                for (int b = 0; b < 16; b++) out[b] = t[b];
-            }
+            for (int b = 0; b < 16; b++) out[b] = t[b];
         }
     }
 }
@@ -277,20 +544,29 @@ int32_t append_as(const Kv8Pool& pool, const Kv8Seqs& seqs, AppendArgs a, int ma
     a.table_rows = 1;
     while (a.table_rows < 32 && a.table_rows < page && a.table_rows < max_rows) a.table_rows *= 2;
     const int windows = (seqs.n_rows + win - 1) / win;
-    int slices = (2 * sm_count() + windows - 1) / windows;
-    if (slices > pool.n_kv) slices = pool.n_kv;
-    if (slices < 1) slices = 1;
-    const size_t smem = (size_t)a.table_rows * a.half * sizeof(double2);
-    LC_CUDA(ensure_smem_limit((const void*)kv8_append_kernel<T>, smem));
-    kv8_append_kernel<T><<<dim3((unsigned)windows, (unsigned)slices), 256, smem, s>>>(pool, seqs, a);
+    auto slices_of = [&](int heads, int least) {
+        int n = (2 * sm_count() + windows - 1) / windows;
+        n = std::min(n, (heads + least - 1) / least);
+        return std::max(n, 1);
+    };
+    const bool vec = pool.hd % 8 == 0 && pool.hd <= 256 && (a.half == 0 || 2 * a.half == pool.hd) && rows_aligned(a.k, a.k_stride, sizeof(T), 4 * sizeof(T)) &&
+                     rows_aligned(a.v, a.v_stride, sizeof(T), 4 * sizeof(T)) &&
+                     (!a.q || (rows_aligned(a.q, a.q_stride, sizeof(T), 4 * sizeof(T)) && rows_aligned(a.q_out, a.qo_stride, sizeof(T), 4 * sizeof(T))));
+    // rows of the table, and behind it every eighth and the eight first turns of more than eight rows
+    const size_t smem = (size_t)(a.table_rows + (a.table_rows > 8 ? a.table_rows / 8 + 8 : 0)) * a.half * sizeof(float4);
+    a.kv_slices = slices_of(pool.n_kv, 4);  // a block's eight warps have an item each
+    const int slices = a.kv_slices + (a.q ? slices_of(a.n_heads, 4) : 0);
+    const auto kern = vec ? kv8_append_kernel<T, true> : kv8_append_kernel<T, false>;
+    LC_CUDA(ensure_smem_limit((const void*)kern, smem));
+    kern<<<dim3((unsigned)windows, (unsigned)slices), 256, smem, s>>>(pool, seqs, a);
     LC_CUDA(cudaGetLastError());
     return LC_OK;
 }
 template <typename T>
 int32_t read_as(const Kv8Pool& pool, const Kv8Seqs& seqs, ReadArgs a, cudaStream_t s) {
     a.vec = (!a.k || rows_aligned(a.k, a.k_stride, sizeof(T), 16)) && (!a.v || rows_aligned(a.v, a.v_stride, sizeof(T), 16));
-    int blocks = (seqs.n_rows + 7) / 8;
-    if (blocks > 8 * sm_count()) blocks = 8 * sm_count();
+    const int64_t units = (int64_t)seqs.n_rows * ((2 * pool.n_kv * (pool.hd >> 4) + 31) >> 5);
+    const int blocks = (int)std::min<int64_t>((units + 7) / 8, (int64_t)8 * sm_count());
     kv8_read_kernel<T><<<blocks, 256, 0, s>>>(pool, seqs, a);
     LC_CUDA(cudaGetLastError());
     return LC_OK;
@@ -335,7 +611,7 @@ int32_t lc_kv8_append_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows, ui
     }
     DeviceScope dev;
     LC_TRY(dev.enter(cache->k_dev, "lc_kv8_append_dev: cache"));
-    AppendArgs a{k_dev, v_dev, q_dev, q_out_dev, k_stride, v_stride, q_stride, q_out_stride, q_dev ? n_heads : 0, rot_dim / 2, turns_dev, 0, 0};
+    AppendArgs a{k_dev, v_dev, q_dev, q_out_dev, k_stride, v_stride, q_stride, q_out_stride, q_dev ? n_heads : 0, rot_dim / 2, turns_dev, 0, 0, 0};
     cudaStream_t s = stream_or_own(stream_);
     if (typ == LC_TYPE_F32) return append_as<float>(pool, seqs, a, rows->max_rows, s);
     if (typ == LC_TYPE_F16) return append_as<__half>(pool, seqs, a, rows->max_rows, s);
