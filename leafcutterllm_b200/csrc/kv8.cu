@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(256, 3) kv8_append_kernel(Kv8Pool pool, Kv8Seq
         const int ctx = seqs.ctx[i], end = first + n;
         if (!kv8_in_table(seqs, pool, ctx, n)) { r = end; continue; }
         const int32_t* table = seqs.table + (size_t)i * seqs.width;
-        if (r != first) r += (-(ctx + r - first)) & (page - 1);  // inside a group that another window has: to the next page
+        if (r != first) r = min(end, r + ((-(ctx + r - first)) & (page - 1)));  // inside a group that another window has: to the next page or sequence
         while (r < min(r_end, end)) {
             const int pos = ctx + (r - first), slot = pos & (page - 1);
             const int number = table[pos >> pool.page_shift];
