@@ -31,7 +31,7 @@ constexpr int kRunWarps = 4;
 // ------------------------------------------------------------------------------------------------------------------------------------
 
 // The line of `total` steps in equal runs, none of them empty, and none shorter than kLeast where that leaves warps without one.
-constexpr uint32_t kLeast = 4;
+constexpr uint32_t kLeast = 2;
 struct Runs {
     uint32_t n, per, more;  // the first `more` runs have a step more than `per`
     __device__ __forceinline__ Runs(uint32_t total, uint32_t warps) {
@@ -69,12 +69,12 @@ __device__ __forceinline__ void place_at(Place& at, const Kv8Seqs& s, const Kv8P
 // MT tiles of 16 rows: 8 MT rows in the split form, 16 MT in the plain one
 template <int HD, int MT, bool SPLIT> struct RunShape {
     static constexpr int kRows = MT * (SPLIT ? 8 : 16);
-    static constexpr int kStageBytes = 2 * kStep * HD + 16;   // keys, values, their two scales
-    static constexpr int kStages = HD == 64 ? 4 : 3;
+    static constexpr int kStageBytes = 2 * kStep * HD + 16;   // keys, values; scales of the first 16 keys, of the others, of the values likewise
+    static constexpr int kStages = HD == 64 ? 3 : 2;
     static constexpr bool kQueriesShared = HD == 256 || MT > 1;  // operand fragments of the queries in shared memory, not in registers
     static constexpr int kQueries = kQueriesShared ? MT * (HD / 16) * 512 : 0;
     static constexpr int kWarp = kStages * kStageBytes + kQueries;
-    static constexpr int kBlocks = HD == 256 || MT > 1 ? 2 : SPLIT ? 4 : 3;
+    static constexpr int kBlocks = HD == 256 ? 1 : MT > 1 ? 2 : 3;
 };
 
 template <int HD, int MT, bool SPLIT, bool FULL>
@@ -115,36 +115,43 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
         const SeqWork& w = at.w;
         const int s0 = at.step, s1 = min(w.steps, s0 + (int)(t_end - t));
         const int32_t* table = seqs.table + (size_t)at.seq * seqs.width;
-        const int row_lo = at.rb * RB, row_n = min(RB, w.n * a.group - row_lo);
+        const int row_lo = at.rb * RB, row_n = min(RB, w.n * a.group - row_lo), key_end = w.ctx + w.n;
 
-        // pages of 32 steps on, one per lane
+        // pages of 16 steps on, one per lane and 16 keys
         int pages_at = s0, pages = -1;
         auto look_up = [&]() {
-            const int st = pages_at + lane;
-            pages = w.inside && st < s1 ? table[((w.step0 + st) * kStep) >> pool.page_shift] : -1;
+            const int st = pages_at + (lane >> 1), key = (w.step0 + st) * kStep + (lane & 1) * 16;
+            pages = w.inside && st < s1 && key < key_end ? table[key >> pool.page_shift] : -1;
         };
         look_up();
         bool poisoned = !w.inside;
         auto fetch = [&](int st) {
-            if (st - pages_at == 32) { pages_at += 32; look_up(); }
+            if (st - pages_at == 16) { pages_at += 16; look_up(); }
             if (st < s1 && w.inside) {
-                const int number = __shfl_sync(0xffffffffu, pages, st - pages_at);
-                if (number < 0 || number >= pool.n_pages) {
-                    poisoned = true;
-                    if (lane == 0) kv8_raise(seqs, at.seq);
-                } else {
-                    const uint32_t dst = ring + (uint32_t)(st % S) * Shape::kStageBytes;
+                const uint32_t dst = ring + (uint32_t)(st % S) * Shape::kStageBytes;
+                float* const scales = reinterpret_cast<float*>(mine + (st % S) * Shape::kStageBytes + 2 * kStep * HD);
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int number = __shfl_sync(0xffffffffu, pages, 2 * (st - pages_at) + x), key = (w.step0 + st) * kStep + 16 * x;
+                    if (key >= key_end || number < 0 || number >= pool.n_pages) {
+                        if (key < key_end) {
+                            poisoned = true;
+                            if (lane == 0) kv8_raise(seqs, at.seq);
+                        }
+                        if (lane < 2) scales[2 * lane + x] = 0.0f;  // nothing of what lies there has a weight
+                        continue;
+                    }
                     const size_t ph = (size_t)number * pool.n_kv + at.kvh;
-                    const size_t off = ((ph << pool.page_shift) + (((w.step0 + st) * kStep) & page_mask)) * hd + lsrc;
+                    const size_t off = ((ph << pool.page_shift) + (key & page_mask)) * hd + lsrc;
                     const int8_t* ks = pool.k + off;
                     const int8_t* vs = pool.v + off;
 #pragma unroll
-                    for (int i = 0; i < kStep / kRowsPer; i++) {
+                    for (int i = 0; i < 16 / kRowsPer; i++) {
                         const int row = lrow + i * kRowsPer;
-                        cp_async16(dst + row * HD + ((lch ^ ((row & 1) << 2)) & (kChunks - 1)) * 16, ks + i * kRowsPer * hd);
-                        cp_async16(dst + kStep * HD + row * HD + ((lch ^ (row & 6)) & (kChunks - 1)) * 16, vs + i * kRowsPer * hd);
+                        cp_async16(dst + (16 * x + row) * HD + ((lch ^ ((row & 1) << 2)) & (kChunks - 1)) * 16, ks + i * kRowsPer * hd);
+                        cp_async16(dst + (kStep + 16 * x + row) * HD + ((lch ^ (row & 6)) & (kChunks - 1)) * 16, vs + i * kRowsPer * hd);
                     }
-                    if (lane < 2) cp_async4(dst + 2 * kStep * HD + lane * 4, (lane ? pool.v_scale : pool.k_scale) + ph);
+                    if (lane < 2) cp_async4(dst + 2 * kStep * HD + (2 * lane + x) * 4, (lane ? pool.v_scale : pool.k_scale) + ph);
                 }
             }
             cp_async_commit();
@@ -215,24 +222,26 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
             for (int hf = 0; hf < HF; hf++) { m[mt][hf] = kNegInf; l[mt][hf] = 0.0f; }
         }
 
+        // rows see all keys up to the first row's position (with a window, from the last row's on)
+        const int sees = w.ctx + row_lo / a.group, from = a.window > 0 ? w.ctx + (row_lo + row_n - 1) / a.group - a.window : -1;
         for (int st = s0; st < s1; st++) {
             cp_async_wait<S - 2>();
             __syncwarp();
+            fetch(st + S - 1);  // into the place of the step before
             const int key0 = (w.step0 + st) * kStep;
+            const bool plain = key0 + kStep - 1 <= sees && key0 > from;
             const unsigned char* kp = mine + (st % S) * Shape::kStageBytes;
-            const float ksc = *reinterpret_cast<const float*>(kp + 2 * kStep * HD), vsc = *reinterpret_cast<const float*>(kp + 2 * kStep * HD + 4);
-            float s[MT][2][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int tl = 0; tl < 2; tl++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[mt][tl][e] = 0.0f;
+            const float4 scales = *reinterpret_cast<const float4*>(kp + 2 * kStep * HD);
+            const float ksc[2] = {scales.x, scales.y};
+            // the values' scales over the larger of them go to the weights, that one to their sums
+            const float vmax = fmaxf(fabsf(scales.z), fabsf(scales.w)), vinv = vmax > 0.0f ? 1.0f / vmax : 0.0f;
+            const float vr[2] = {scales.z * vinv, scales.w * vinv};
+            float s[MT][4][4];
 #pragma unroll
             for (int j = 0; j < HD / 64; j++) {
-                uint32_t kw[2][4];
+                uint32_t kw[4][4];
 #pragma unroll
-                for (int tl = 0; tl < 2; tl++) {
+                for (int tl = 0; tl < 4; tl++) {
                     const int row = 8 * tl + g, ch = 4 * j + c;
                     const uint4 u = *reinterpret_cast<const uint4*>(kp + row * HD + ((ch ^ ((row & 1) << 2)) & (kChunks - 1)) * 16);
                     kw[tl][0] = u.x ^ 0x80808080u; kw[tl][1] = u.y ^ 0x80808080u; kw[tl][2] = u.z ^ 0x80808080u; kw[tl][3] = u.w ^ 0x80808080u;
@@ -240,36 +249,48 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
 #pragma unroll
                 for (int wd = 0; wd < 4; wd++) {
                     const int ks = 4 * j + wd;
-                    const uint32_t b00 = ints01(kw[0][wd]), b01 = ints23(kw[0][wd]), b10 = ints01(kw[1][wd]), b11 = ints23(kw[1][wd]);
+                    uint32_t f[MT][4];
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
-                        uint32_t f[4];
                         if (Shape::kQueriesShared) {
                             const uint4 u = qs[(mt * KS + ks) * 32 + lane];
-                            f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+                            f[mt][0] = u.x; f[mt][1] = u.y; f[mt][2] = u.z; f[mt][3] = u.w;
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 4; e++) f[e] = qf[Shape::kQueriesShared ? 0 : ks][e];
+                            for (int e = 0; e < 4; e++) f[mt][e] = qf[Shape::kQueriesShared ? 0 : ks][e];
                         }
-                        mma_f16(s[mt][0], f, b00, b01);
-                        mma_f16(s[mt][1], f, b10, b11);
+                    }
+#pragma unroll
+                    for (int tl = 0; tl < 4; tl++) {
+                        const uint32_t b0 = ints01(kw[tl][wd]), b1 = ints23(kw[tl][wd]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            if (ks == 0) mma_f16_first(s[mt][tl], f[mt], b0, b1);
+                            else mma_f16(s[mt][tl], f[mt], b0, b1);
+                        }
                     }
                 }
             }
-            uint32_t pf[MT][4];
+            uint32_t pf[MT][2][4];           // weights of the first 16 keys, of the others
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int hf = 0; hf < HF; hf++) {
-                    float v[4];
-                    const float f = rf[mt][hf] * ksc;
+                    float v[8];
+                    const float f[2] = {rf[mt][hf] * ksc[0], rf[mt][hf] * ksc[1]};
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int tl = e >> 1, k = e & 1, key = key0 + 8 * tl + 2 * c + k;
-                        v[e] = (SPLIT ? s[mt][tl][k] + s[mt][tl][2 + k] : s[mt][tl][2 * hf + k]) * f;
-                        if (key > limit[mt][hf] || (a.window > 0 && key <= limit[mt][hf] - a.window)) v[e] = kNegInf;
+                    for (int e = 0; e < 8; e++) {
+                        const int tl = e >> 1, k = e & 1;
+                        v[e] = (SPLIT ? s[mt][tl][k] + s[mt][tl][2 + k] : s[mt][tl][2 * hf + k]) * f[tl >> 1];
                     }
-                    float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+                    if (!plain) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const int key = key0 + 8 * (e >> 1) + 2 * c + (e & 1);
+                            if (key > limit[mt][hf] || (a.window > 0 && key <= limit[mt][hf] - a.window)) v[e] = kNegInf;
+                        }
+                    }
+                    float mx = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                     mx = fmaxf(mx, m[mt][hf]);
@@ -281,64 +302,79 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                         for (int n = 0; n < NT; n++) { o[mt][n][2 * hf] *= corr; o[mt][n][2 * hf + 1] *= corr; }
                         m[mt][hf] = mx;
                     }
-                    float p[4];
+                    const float less = 8.0f - ref;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) p[e] = exp2_fast(v[e] - ref + 8.0f);
-                    l[mt][hf] += (p[0] + p[1]) + (p[2] + p[3]);
-                    if (SPLIT) {
-                        h2_split(p[0], p[1], pf[mt][0], pf[mt][1]);
-                        h2_split(p[2], p[3], pf[mt][2], pf[mt][3]);
-                    } else {
-                        pf[mt][hf] = h2_pack(p[0], p[1]);
-                        pf[mt][2 + hf] = h2_pack(p[2], p[3]);
+                    for (int e = 0; e < 8; e++) v[e] = exp2_fast(v[e] + less);
+                    l[mt][hf] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const float p0 = v[4 * x] * vr[x], p1 = v[4 * x + 1] * vr[x], p2 = v[4 * x + 2] * vr[x], p3 = v[4 * x + 3] * vr[x];
+                        if (SPLIT) {
+                            h2_split(p0, p1, pf[mt][x][0], pf[mt][x][1]);
+                            h2_split(p2, p3, pf[mt][x][2], pf[mt][x][3]);
+                        } else {
+                            pf[mt][x][hf] = h2_pack(p0, p1);
+                            pf[mt][x][2 + hf] = h2_pack(p2, p3);
+                        }
                     }
                 }
-            // values: a thread's keys are 2c, 2c + 1, 8 + 2c, 9 + 2c; its dims NT in a row (HD 256: 16 and 16 more 128 further)
+            // values: of each 16 keys a thread's are 2c, 2c + 1, 8 + 2c, 9 + 2c; its dims NT in a row (HD 256: 16 and 16 more 128 further)
             const unsigned char* vp = kp + kStep * HD;
             constexpr int WORDS = HD == 64 ? 2 : 4;
 #pragma unroll
             for (int gr = 0; gr < (HD == 256 ? 2 : 1); gr++) {
                 const int ch = HD == 64 ? g >> 1 : 8 * gr + g;
-                uint32_t kv[4][WORDS];
+                uint32_t kv[2][4][WORDS];
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const int row = (x >> 1) * 8 + 2 * c + (x & 1);
+                for (int x = 0; x < 8; x++) {
+                    const int row = (x >> 2) * 16 + ((x >> 1) & 1) * 8 + 2 * c + (x & 1);
                     const unsigned char* at16 = vp + row * HD + ((ch ^ (row & 6)) & (kChunks - 1)) * 16;
+                    uint32_t(&k4)[WORDS] = kv[x >> 2][x & 3];
                     if (HD == 64) {
                         const uint2 u = *reinterpret_cast<const uint2*>(at16 + (g & 1) * 8);
-                        kv[x][0] = u.x ^ 0x80808080u; kv[x][1] = u.y ^ 0x80808080u;
+                        k4[0] = u.x ^ 0x80808080u; k4[1] = u.y ^ 0x80808080u;
                     } else {
                         const uint4 u = *reinterpret_cast<const uint4*>(at16);
-                        kv[x][0] = u.x ^ 0x80808080u; kv[x][1] = u.y ^ 0x80808080u;
-                        kv[x][WORDS - 2] = u.z ^ 0x80808080u; kv[x][WORDS - 1] = u.w ^ 0x80808080u;
+                        k4[0] = u.x ^ 0x80808080u; k4[1] = u.y ^ 0x80808080u;
+                        k4[WORDS - 2] = u.z ^ 0x80808080u; k4[WORDS - 1] = u.w ^ 0x80808080u;
                     }
                 }
 #pragma unroll
                 for (int wd = 0; wd < WORDS; wd++) {
-                    const uint32_t a01 = __byte_perm(kv[0][wd], kv[1][wd], 0x5140), a23 = __byte_perm(kv[0][wd], kv[1][wd], 0x7362);
-                    const uint32_t b01 = __byte_perm(kv[2][wd], kv[3][wd], 0x5140), b23 = __byte_perm(kv[2][wd], kv[3][wd], 0x7362);
+                    uint32_t a01[2], a23[2], b01[2], b23[2];
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        a01[x] = __byte_perm(kv[x][0][wd], kv[x][1][wd], 0x5140);
+                        a23[x] = __byte_perm(kv[x][0][wd], kv[x][1][wd], 0x7362);
+                        b01[x] = __byte_perm(kv[x][2][wd], kv[x][3][wd], 0x5140);
+                        b23[x] = __byte_perm(kv[x][2][wd], kv[x][3][wd], 0x7362);
+                    }
 #pragma unroll
                     for (int b = 0; b < 4; b++) {
-                        const uint32_t va = b < 2 ? a01 : a23, vb = b < 2 ? b01 : b23;
-                        const uint32_t v0 = b & 1 ? ints23(va) : ints01(va), v1 = b & 1 ? ints23(vb) : ints01(vb);
+                        uint32_t v0[2], v1[2];
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            const uint32_t va = b < 2 ? a01[x] : a23[x], vb = b < 2 ? b01[x] : b23[x];
+                            v0[x] = b & 1 ? ints23(va) : ints01(va);
+                            v1[x] = b & 1 ? ints23(vb) : ints01(vb);
+                        }
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
-                            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma_f16(acc, pf[mt], v0, v1);
+                            float acc[4];
+                            mma_f16_first(acc, pf[mt][0], v0[0], v1[0]);
+                            mma_f16(acc, pf[mt][1], v0[1], v1[1]);
                             float(&oo)[OC] = o[mt][16 * gr + 4 * wd + b];
                             if (SPLIT) {
-                                oo[0] = fmaf(acc[0] + acc[2], vsc, oo[0]);
-                                oo[1] = fmaf(acc[1] + acc[3], vsc, oo[1]);
+                                oo[0] = fmaf(acc[0] + acc[2], vmax, oo[0]);
+                                oo[1] = fmaf(acc[1] + acc[3], vmax, oo[1]);
                             } else {
 #pragma unroll
-                                for (int e = 0; e < OC; e++) oo[e] = fmaf(acc[e], vsc, oo[e]);
+                                for (int e = 0; e < OC; e++) oo[e] = fmaf(acc[e], vmax, oo[e]);
                             }
                         }
                     }
                 }
             }
-            __syncwarp();
-            fetch(st + S - 1);
         }
         cp_async_wait<0>();
 
@@ -466,7 +502,7 @@ RunPlan plan_runs(const Kv8Pool& pool, uint32_t typ, int group, int max_rows) {
     const int64_t rows = (int64_t)group * (max_rows < 1 ? 1 : max_rows);
     p.split = typ == LC_TYPE_F32 || rows <= 8;
     p.mt = rows > (p.split ? 8 : 16) && p.hd < 256 ? 2 : 1;
-    p.blocks = sm_count() * (p.hd == 256 || p.mt > 1 ? 2 : p.split ? 4 : 3);
+    p.blocks = sm_count() * (p.hd == 256 ? 1 : p.mt > 1 ? 2 : 3);
     p.bytes = (size_t)2 * p.blocks * kRunWarps * p.rows() * (p.hd + 2) * sizeof(float);
     return p;
 }
