@@ -1,13 +1,13 @@
 // Attention over the key/value cache in 8 bits: out = sum_j p_j v_j, p = softmax_j(scale q . k_j) over the positions j up to the row's own.
 //
-// A cached element is q8 * S with one scale S per page and head, and an integer of 8 bits is exact in f16: scores and weighted sums are
-// products on the matrix unit (mma.sync m16n8k16, f16 in, f32 out) of f16 integers with the queries and the weights, and the scales are
-// applied outside, S_k to the scores and S_v to a block's sums.
-//
-// Queries are scaled by a power of two per row, so that their largest element is in [2^14, 2^15) whatever its size.  The weights are
-// 2^(s - max + 8).  In the split form (RB = 8 rows to a tile of 16) rows 0 .. 7 of the tile hold the f16 value and rows 8 .. 15 what its
-// rounding lost, 22 bits together: the two halves of a sum lie in the same thread.  In the plain form (RB = 16) a tile holds 16 rows, weights
-// rounded to f16 (2^-12 of each).
+// A cached element is an integer times the scale of its page and head, so both products are taken of the integers as they are, and the scales are applied outside.
+//   Scores  on the matrix unit's integers (mma.sync m16n8k32, exact): a row of queries is whole numbers in units of its largest / 32,512 (f32: / 8,323,072), and
+//           these are digits of 8 bits, in rows of their own of the operand, so that keys go in as they lie in the cache.  16 bits are as good as f16 or bf16
+//           queries ask for: a score of size 1 is off by 3e-5; 24 bits for f32.
+//   Values  an integer of 8 bits is exact in f16 (m16n8k16, f32 out); the weights are 2^(s - max + 8).  A step's sums are multiplied by its page's scale and added in
+//           f32, so that what the matrix unit cuts off when it adds stays within 16 keys.  Split form (8 rows to a tile of 16): rows 0 .. 7 of the tile hold
+//           the weight in f16 and rows 8 .. 15 what its rounding lost, 22 bits together, and the two halves of a sum lie in the same thread.  Plain form: 16
+//           rows, weights rounded to f16 (2^-11 of each).
 #include <algorithm>
 #include "lc_kv8.cuh"
 #include "lc_kernels.h"
@@ -21,8 +21,8 @@ constexpr int kRunWarps = 4;
 
 // ------------------------------------------------------------------------------------------------------------------------------------
 // Runs: few rows per sequence.  A unit is (sequence, kv head, row block of RB rows = tokens x heads of the group); its keys are cut into
-// steps of 16.  All steps of all units stand in one line, which is cut into equal runs, one per WARP, so that contexts of any lengths
-// keep all warps equally long at work and none waits for another.  A unit that lies in several runs leaves partial results, which the next kernel
+// steps of 16.  All steps of all units, and some places for what a unit costs besides, stand in one line, which is cut into equal runs, one per WARP, so that
+// contexts of any lengths keep all warps equally long at work and none waits for another.  A unit that lies in several runs leaves partial results, which the next kernel
 // joins.  Keys and values come through a ring of the warp's own in shared memory (cp.async).
 //
 // Operand layouts, so that nothing is transposed: the dims of a score and the keys of a weighted sum are sums' indexes and may stand in any
@@ -31,7 +31,7 @@ constexpr int kRunWarps = 4;
 // ------------------------------------------------------------------------------------------------------------------------------------
 
 // The line of `total` steps in equal runs, none of them empty, and none shorter than kLeast where that leaves warps without one.
-constexpr uint32_t kLeast = 2;
+constexpr uint32_t kLeast = 4;
 struct Runs {
     uint32_t n, per, more;  // the first `more` runs have a step more than `per`
     __device__ __forceinline__ Runs(uint32_t total, uint32_t warps) {
@@ -49,41 +49,42 @@ struct Runs {
 // floats of one partial result: maxima, sums and rows of HD
 template <int HD, int RB> __host__ __device__ constexpr int part_floats() { return RB * (HD + 2); }
 
-// Where a place of the line lies.
+// Where a place of the line lies: `in` of its unit, whose first kUnitCost places are no steps.
 struct Place {
-    int seq, kvh, rb, step;        // step: index within the unit
+    int seq, kvh, rb, in;
     SeqWork w;
-    uint32_t unit_start;           // place of the unit's first step
 };
 template <int RB>
 __device__ __forceinline__ void place_at(Place& at, const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, const uint32_t* cum, uint32_t t) {
     at.seq = seq_at(cum, s.n_seqs, t);
     at.w = seq_work<RB>(s, p, a, at.seq);
-    const uint32_t in = t - cum[at.seq], unit = in / at.w.steps;
-    at.step = in - unit * at.w.steps;
-    at.unit_start = t - at.step;
+    const uint32_t cost = at.w.steps + kUnitCost, in = t - cum[at.seq], unit = in / cost;
+    at.in = in - unit * cost;
     at.kvh = unit / at.w.blocks;
     at.rb = unit - at.kvh * at.w.blocks;
 }
 
 // MT tiles of 16 rows: 8 MT rows in the split form, 16 MT in the plain one
-template <int HD, int MT, bool SPLIT> struct RunShape {
+// F32: queries of 24 bits (and split weights)
+template <int HD, int MT, bool SPLIT, bool F32> struct RunShape {
     static constexpr int kRows = MT * (SPLIT ? 8 : 16);
-    static constexpr int kStageBytes = 2 * kStep * HD + 16;   // keys, values; scales of the first 16 keys, of the others, of the values likewise
-    static constexpr int kStages = HD == 64 ? 3 : 2;
+    static constexpr int kStageBytes = 2 * kStep * HD + 16;   // keys, values, their two scales
+    static constexpr int kStages = HD == 64 ? 4 : 3;
+    static constexpr int kGroups = MT * (SPLIT ? 1 : 2);         // of 8 rows
     static constexpr bool kQueriesShared = HD == 256 || MT > 1;  // operand fragments of the queries in shared memory, not in registers
-    static constexpr int kQueries = kQueriesShared ? MT * (HD / 16) * 512 : 0;
+    static constexpr int kQueries = kQueriesShared ? kGroups * (F32 ? 2 : 1) * (HD / 32) * 512 : 0;
     static constexpr int kWarp = kStages * kStageBytes + kQueries;
-    static constexpr int kBlocks = HD == 256 ? 1 : MT > 1 ? 2 : 3;
+    static constexpr int kBlocks = HD == 256 || MT > 1 ? 2 : SPLIT ? 4 : 3;
 };
 
-template <int HD, int MT, bool SPLIT, bool FULL>
-__global__ void __launch_bounds__(kRunWarps * 32, RunShape<HD, MT, SPLIT>::kBlocks)
+template <int HD, int MT, bool SPLIT, bool F32, bool FULL>
+__global__ void __launch_bounds__(kRunWarps * 32, RunShape<HD, MT, SPLIT, F32>::kBlocks)
 kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
-    using Shape = RunShape<HD, MT, SPLIT>;
+    using Shape = RunShape<HD, MT, SPLIT, F32>;
+    constexpr int NG = Shape::kGroups, ND = F32 ? 2 : 1;  // groups of 8 rows, tiles of digits of each
     constexpr int RB = Shape::kRows;
     constexpr int NT = HD / 8;              // tiles of 8 dims of the output; a thread's values of a key are NT in a row
-    constexpr int KS = HD / 16;             // k steps of the scores
+    constexpr int KS = HD / 32;             // k steps of the scores
     constexpr int HF = SPLIT ? 1 : 2;       // rows of a tile that a thread has a part in
     constexpr int OC = 2 * HF;
     constexpr int S = Shape::kStages;
@@ -113,45 +114,40 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
         Place at;
         place_at<RB>(at, seqs, pool, a, cum, t);
         const SeqWork& w = at.w;
-        const int s0 = at.step, s1 = min(w.steps, s0 + (int)(t_end - t));
+        const int end = min(w.steps + kUnitCost, at.in + (int)(t_end - t)), s0 = max(0, at.in - kUnitCost), s1 = end - kUnitCost;
+        t += (uint32_t)(end - at.in);
+        if (s1 <= s0) continue;  // the unit's steps are the next run's
         const int32_t* table = seqs.table + (size_t)at.seq * seqs.width;
-        const int row_lo = at.rb * RB, row_n = min(RB, w.n * a.group - row_lo), key_end = w.ctx + w.n;
+        const int row_lo = at.rb * RB, row_n = min(RB, w.n * a.group - row_lo);
 
-        // pages of 16 steps on, one per lane and 16 keys
+        // pages of 32 steps on, one per lane
         int pages_at = s0, pages = -1;
         auto look_up = [&]() {
-            const int st = pages_at + (lane >> 1), key = (w.step0 + st) * kStep + (lane & 1) * 16;
-            pages = w.inside && st < s1 && key < key_end ? table[key >> pool.page_shift] : -1;
+            const int st = pages_at + lane;
+            pages = w.inside && st < s1 ? table[((w.step0 + st) * kStep) >> pool.page_shift] : -1;
         };
         look_up();
         bool poisoned = !w.inside;
         auto fetch = [&](int st) {
-            if (st - pages_at == 16) { pages_at += 16; look_up(); }
+            if (st - pages_at == 32) { pages_at += 32; look_up(); }
             if (st < s1 && w.inside) {
-                const uint32_t dst = ring + (uint32_t)(st % S) * Shape::kStageBytes;
-                float* const scales = reinterpret_cast<float*>(mine + (st % S) * Shape::kStageBytes + 2 * kStep * HD);
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int number = __shfl_sync(0xffffffffu, pages, 2 * (st - pages_at) + x), key = (w.step0 + st) * kStep + 16 * x;
-                    if (key >= key_end || number < 0 || number >= pool.n_pages) {
-                        if (key < key_end) {
-                            poisoned = true;
-                            if (lane == 0) kv8_raise(seqs, at.seq);
-                        }
-                        if (lane < 2) scales[2 * lane + x] = 0.0f;  // nothing of what lies there has a weight
-                        continue;
-                    }
+                const int number = __shfl_sync(0xffffffffu, pages, st - pages_at);
+                if (number < 0 || number >= pool.n_pages) {
+                    poisoned = true;
+                    if (lane == 0) kv8_raise(seqs, at.seq);
+                } else {
+                    const uint32_t dst = ring + (uint32_t)(st % S) * Shape::kStageBytes;
                     const size_t ph = (size_t)number * pool.n_kv + at.kvh;
-                    const size_t off = ((ph << pool.page_shift) + (key & page_mask)) * hd + lsrc;
+                    const size_t off = ((ph << pool.page_shift) + (((w.step0 + st) * kStep) & page_mask)) * hd + lsrc;
                     const int8_t* ks = pool.k + off;
                     const int8_t* vs = pool.v + off;
 #pragma unroll
-                    for (int i = 0; i < 16 / kRowsPer; i++) {
+                    for (int i = 0; i < kStep / kRowsPer; i++) {
                         const int row = lrow + i * kRowsPer;
-                        cp_async16(dst + (16 * x + row) * HD + ((lch ^ ((row & 1) << 2)) & (kChunks - 1)) * 16, ks + i * kRowsPer * hd);
-                        cp_async16(dst + (kStep + 16 * x + row) * HD + ((lch ^ (row & 6)) & (kChunks - 1)) * 16, vs + i * kRowsPer * hd);
+                        cp_async16(dst + row * HD + ((lch ^ ((row & 1) << 2)) & (kChunks - 1)) * 16, ks + i * kRowsPer * hd);
+                        cp_async16(dst + (kStep + row) * HD + ((lch ^ (row & 6)) & (kChunks - 1)) * 16, vs + i * kRowsPer * hd);
                     }
-                    if (lane < 2) cp_async4(dst + 2 * kStep * HD + (2 * lane + x) * 4, (lane ? pool.v_scale : pool.k_scale) + ph);
+                    if (lane < 2) cp_async4(dst + 2 * kStep * HD + lane * 4, (lane ? pool.v_scale : pool.k_scale) + ph);
                 }
             }
             cp_async_commit();
@@ -159,57 +155,66 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < S - 1; k++) fetch(s0 + k);
 
-        // the queries as operand fragments: step ks = 4 j + wd of the scores takes dims 64 j + 16 c + 4 wd .. + 3
-        uint32_t qf[Shape::kQueriesShared ? 1 : KS][4];
+        // the queries as operand fragments: step ks = 2 j + x of the scores takes dims 64 j + 16 c + 8 x .. + 7.  A group's first tile has the highest digit in rows
+        // 0 .. 7 and the next in rows 8 .. 15, its second tile the lowest in rows 0 .. 7.
+        uint32_t qf[Shape::kQueriesShared ? 1 : NG * ND * KS][4];
         float rf[MT][HF];
         int limit[MT][HF];                   // last position that the row sees (-1: no row)
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            uint32_t f[KS][4];
+        for (int mt = 0; mt < MT; mt++)
 #pragma unroll
             for (int hf = 0; hf < HF; hf++) {
-                const int r = (SPLIT ? 8 : 16) * mt + g + 8 * hf;
+                const int group = mt * HF + hf, r = 8 * group + g;
                 const bool has = r < row_n;
                 const int tok = has ? (row_lo + r) / a.group : 0, hq = has ? (row_lo + r) - tok * a.group : 0;
                 const int64_t src = (int64_t)(w.first + tok) * a.q_stride + (int64_t)(at.kvh * a.group + hq) * hd;
                 limit[mt][hf] = has ? w.ctx + tok : -1;
-                float v[KS][4], top = 0.0f;
+                float v[HD / 64][16], top = 0.0f;
 #pragma unroll
-                for (int j = 0; j < KS / 4; j++) {
+                for (int j = 0; j < HD / 64; j++) {
                     const int d = 64 * j + 16 * c;
-                    if (has && (FULL || d < hd)) load16(a.q, src + d, a.typ, a.q_vec, &v[4 * j][0]);
+                    if (has && (FULL || d < hd)) load16(a.q, src + d, a.typ, a.q_vec, v[j]);
                     else
 #pragma unroll
-                        for (int e = 0; e < 16; e++) v[4 * j + (e >> 2)][e & 3] = 0.0f;
+                        for (int e = 0; e < 16; e++) v[j][e] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) top = max_nan(top, fabsf(v[j][e]));
                 }
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(v[ks][e]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 float up, down;
                 row_scale(top, up, down);
-                rf[mt][hf] = a.scale_log2 * down;
+                const float unit = top > 0.0f ? top * up * (F32 ? 1.0f / 8323072.0f : 1.0f / 32512.0f) : 1.0f, per = 1.0f / unit;
+                rf[mt][hf] = top < INFINITY ? a.scale_log2 * down * unit : __int_as_float(0x7fffffff);  // not finite: the row is NaN
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
-                    if (SPLIT) {
-                        h2_split(v[ks][0] * up, v[ks][1] * up, f[ks][0], f[ks][1]);
-                        h2_split(v[ks][2] * up, v[ks][3] * up, f[ks][2], f[ks][3]);
-                    } else {
-                        f[ks][hf] = h2_pack(v[ks][0] * up, v[ks][1] * up);
-                        f[ks][2 + hf] = h2_pack(v[ks][2] * up, v[ks][3] * up);
+                    uint32_t digit[3][2];    // [highest first][four dims]
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        int n[4], lo[4], mid[4], hi[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            n[e] = __float2int_rn(v[ks >> 1][8 * (ks & 1) + 4 * x + e] * up * per);
+                            lo[e] = (int)(int8_t)n[e];
+                            mid[e] = (n[e] - lo[e]) >> 8;
+                            hi[e] = (mid[e] - (int)(int8_t)mid[e]) >> 8;
+                        }
+                        digit[0][x] = F32 ? pack4(hi[0], hi[1], hi[2], hi[3]) : pack4(mid[0], mid[1], mid[2], mid[3]);
+                        digit[1][x] = F32 ? pack4(mid[0], mid[1], mid[2], mid[3]) : pack4(lo[0], lo[1], lo[2], lo[3]);
+                        digit[2][x] = pack4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+#pragma unroll
+                    for (int nd = 0; nd < ND; nd++) {
+                        const uint32_t f0 = digit[2 * nd][0], f1 = nd ? 0u : digit[1][0], f2 = digit[2 * nd][1], f3 = nd ? 0u : digit[1][1];
+                        const int at_f = (group * ND + nd) * KS + ks;
+                        if (Shape::kQueriesShared) qs[at_f * 32 + lane] = make_uint4(f0, f1, f2, f3);
+                        else {
+                            uint32_t(&f)[4] = qf[Shape::kQueriesShared ? 0 : at_f];
+                            f[0] = f0; f[1] = f1; f[2] = f2; f[3] = f3;
+                        }
                     }
                 }
             }
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                if (Shape::kQueriesShared) qs[(mt * KS + ks) * 32 + lane] = make_uint4(f[ks][0], f[ks][1], f[ks][2], f[ks][3]);
-                else
-#pragma unroll
-                    for (int e = 0; e < 4; e++) qf[Shape::kQueriesShared ? 0 : ks][e] = f[ks][e];
-            }
-        }
 
         float o[MT][NT][OC], m[MT][HF], l[MT][HF];
 #pragma unroll
@@ -231,66 +236,67 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
             const int key0 = (w.step0 + st) * kStep;
             const bool plain = key0 + kStep - 1 <= sees && key0 > from;
             const unsigned char* kp = mine + (st % S) * Shape::kStageBytes;
-            const float4 scales = *reinterpret_cast<const float4*>(kp + 2 * kStep * HD);
-            const float ksc[2] = {scales.x, scales.y};
-            // the values' scales over the larger of them go to the weights, that one to their sums
-            const float vmax = fmaxf(fabsf(scales.z), fabsf(scales.w)), vinv = vmax > 0.0f ? 1.0f / vmax : 0.0f;
-            const float vr[2] = {scales.z * vinv, scales.w * vinv};
-            float s[MT][4][4];
+            const float2 scales = *reinterpret_cast<const float2*>(kp + 2 * kStep * HD);
+            const float ksc = scales.x, vsc = scales.y;
+            constexpr int TL = kStep / 8;    // tiles of 8 keys
+            float s[NG][TL][2];              // [group][tile][two keys]
+            {
+                int dot[NG * ND][TL][4];
 #pragma unroll
-            for (int j = 0; j < HD / 64; j++) {
-                uint32_t kw[4][4];
+                for (int j = 0; j < HD / 64; j++) {
+                    uint4 kw[TL];
 #pragma unroll
-                for (int tl = 0; tl < 4; tl++) {
-                    const int row = 8 * tl + g, ch = 4 * j + c;
-                    const uint4 u = *reinterpret_cast<const uint4*>(kp + row * HD + ((ch ^ ((row & 1) << 2)) & (kChunks - 1)) * 16);
-                    kw[tl][0] = u.x ^ 0x80808080u; kw[tl][1] = u.y ^ 0x80808080u; kw[tl][2] = u.z ^ 0x80808080u; kw[tl][3] = u.w ^ 0x80808080u;
-                }
-#pragma unroll
-                for (int wd = 0; wd < 4; wd++) {
-                    const int ks = 4 * j + wd;
-                    uint32_t f[MT][4];
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        if (Shape::kQueriesShared) {
-                            const uint4 u = qs[(mt * KS + ks) * 32 + lane];
-                            f[mt][0] = u.x; f[mt][1] = u.y; f[mt][2] = u.z; f[mt][3] = u.w;
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; e++) f[mt][e] = qf[Shape::kQueriesShared ? 0 : ks][e];
-                        }
+                    for (int tl = 0; tl < TL; tl++) {
+                        const int row = 8 * tl + g, ch = 4 * j + c;
+                        kw[tl] = *reinterpret_cast<const uint4*>(kp + row * HD + ((ch ^ ((row & 1) << 2)) & (kChunks - 1)) * 16);
                     }
 #pragma unroll
-                    for (int tl = 0; tl < 4; tl++) {
-                        const uint32_t b0 = ints01(kw[tl][wd]), b1 = ints23(kw[tl][wd]);
+                    for (int x = 0; x < 2; x++) {
+                        const int ks = 2 * j + x;
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            if (ks == 0) mma_f16_first(s[mt][tl], f[mt], b0, b1);
-                            else mma_f16(s[mt][tl], f[mt], b0, b1);
+                        for (int gd = 0; gd < NG * ND; gd++) {
+                            uint4 f;
+                            if (Shape::kQueriesShared) f = qs[(gd * KS + ks) * 32 + lane];
+                            else {
+                                const uint32_t(&q4)[4] = qf[Shape::kQueriesShared ? 0 : gd * KS + ks];
+                                f = make_uint4(q4[0], q4[1], q4[2], q4[3]);
+                            }
+#pragma unroll
+                            for (int tl = 0; tl < TL; tl++) {
+                                const uint32_t b0 = x ? kw[tl].z : kw[tl].x, b1 = x ? kw[tl].w : kw[tl].y;
+                                if (ks == 0) mma_s8_first(dot[gd][tl], f.x, f.y, f.z, f.w, b0, b1);
+                                else mma_s8(dot[gd][tl], f.x, f.y, f.z, f.w, b0, b1);
+                            }
                         }
                     }
                 }
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                    for (int tl = 0; tl < TL; tl++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            const float high = (float)(256 * dot[gr * ND][tl][k] + dot[gr * ND][tl][2 + k]);
+                            s[gr][tl][k] = F32 ? fmaf(high, 256.0f, (float)dot[gr * ND + ND - 1][tl][k]) : high;
+                        }
             }
-            uint32_t pf[MT][2][4];           // weights of the first 16 keys, of the others
+            uint32_t pf[MT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int hf = 0; hf < HF; hf++) {
-                    float v[8];
-                    const float f[2] = {rf[mt][hf] * ksc[0], rf[mt][hf] * ksc[1]};
+                    float v[4];
+                    const float f = rf[mt][hf] * ksc;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const int tl = e >> 1, k = e & 1;
-                        v[e] = (SPLIT ? s[mt][tl][k] + s[mt][tl][2 + k] : s[mt][tl][2 * hf + k]) * f[tl >> 1];
-                    }
+                    for (int e = 0; e < 4; e++) v[e] = s[mt * HF + hf][e >> 1][e & 1] * f;
                     if (!plain) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
+                        for (int e = 0; e < 4; e++) {
                             const int key = key0 + 8 * (e >> 1) + 2 * c + (e & 1);
                             if (key > limit[mt][hf] || (a.window > 0 && key <= limit[mt][hf] - a.window)) v[e] = kNegInf;
                         }
                     }
-                    float mx = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+                    float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                     mx = fmaxf(mx, m[mt][hf]);
@@ -304,72 +310,55 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                     }
                     const float less = 8.0f - ref;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = exp2_fast(v[e] + less);
-                    l[mt][hf] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const float p0 = v[4 * x] * vr[x], p1 = v[4 * x + 1] * vr[x], p2 = v[4 * x + 2] * vr[x], p3 = v[4 * x + 3] * vr[x];
-                        if (SPLIT) {
-                            h2_split(p0, p1, pf[mt][x][0], pf[mt][x][1]);
-                            h2_split(p2, p3, pf[mt][x][2], pf[mt][x][3]);
-                        } else {
-                            pf[mt][x][hf] = h2_pack(p0, p1);
-                            pf[mt][x][2 + hf] = h2_pack(p2, p3);
-                        }
+                    for (int e = 0; e < 4; e++) v[e] = exp2_fast(v[e] + less);
+                    l[mt][hf] += (v[0] + v[1]) + (v[2] + v[3]);
+                    if (SPLIT) {
+                        h2_split(v[0], v[1], pf[mt][0], pf[mt][1]);
+                        h2_split(v[2], v[3], pf[mt][2], pf[mt][3]);
+                    } else {
+                        pf[mt][hf] = h2_pack(v[0], v[1]);
+                        pf[mt][2 + hf] = h2_pack(v[2], v[3]);
                     }
                 }
-            // values: of each 16 keys a thread's are 2c, 2c + 1, 8 + 2c, 9 + 2c; its dims NT in a row (HD 256: 16 and 16 more 128 further)
+            // values: a thread's keys are 2c, 2c + 1, 8 + 2c, 9 + 2c; its dims NT in a row (HD 256: 16 and 16 more 128 further)
             const unsigned char* vp = kp + kStep * HD;
             constexpr int WORDS = HD == 64 ? 2 : 4;
 #pragma unroll
             for (int gr = 0; gr < (HD == 256 ? 2 : 1); gr++) {
                 const int ch = HD == 64 ? g >> 1 : 8 * gr + g;
-                uint32_t kv[2][4][WORDS];
+                uint32_t kv[4][WORDS];
 #pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    const int row = (x >> 2) * 16 + ((x >> 1) & 1) * 8 + 2 * c + (x & 1);
+                for (int x = 0; x < 4; x++) {
+                    const int row = (x >> 1) * 8 + 2 * c + (x & 1);
                     const unsigned char* at16 = vp + row * HD + ((ch ^ (row & 6)) & (kChunks - 1)) * 16;
-                    uint32_t(&k4)[WORDS] = kv[x >> 2][x & 3];
                     if (HD == 64) {
                         const uint2 u = *reinterpret_cast<const uint2*>(at16 + (g & 1) * 8);
-                        k4[0] = u.x ^ 0x80808080u; k4[1] = u.y ^ 0x80808080u;
+                        kv[x][0] = u.x ^ 0x80808080u; kv[x][1] = u.y ^ 0x80808080u;
                     } else {
                         const uint4 u = *reinterpret_cast<const uint4*>(at16);
-                        k4[0] = u.x ^ 0x80808080u; k4[1] = u.y ^ 0x80808080u;
-                        k4[WORDS - 2] = u.z ^ 0x80808080u; k4[WORDS - 1] = u.w ^ 0x80808080u;
+                        kv[x][0] = u.x ^ 0x80808080u; kv[x][1] = u.y ^ 0x80808080u;
+                        kv[x][WORDS - 2] = u.z ^ 0x80808080u; kv[x][WORDS - 1] = u.w ^ 0x80808080u;
                     }
                 }
 #pragma unroll
                 for (int wd = 0; wd < WORDS; wd++) {
-                    uint32_t a01[2], a23[2], b01[2], b23[2];
-#pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        a01[x] = __byte_perm(kv[x][0][wd], kv[x][1][wd], 0x5140);
-                        a23[x] = __byte_perm(kv[x][0][wd], kv[x][1][wd], 0x7362);
-                        b01[x] = __byte_perm(kv[x][2][wd], kv[x][3][wd], 0x5140);
-                        b23[x] = __byte_perm(kv[x][2][wd], kv[x][3][wd], 0x7362);
-                    }
+                    const uint32_t a01 = __byte_perm(kv[0][wd], kv[1][wd], 0x5140), a23 = __byte_perm(kv[0][wd], kv[1][wd], 0x7362);
+                    const uint32_t b01 = __byte_perm(kv[2][wd], kv[3][wd], 0x5140), b23 = __byte_perm(kv[2][wd], kv[3][wd], 0x7362);
 #pragma unroll
                     for (int b = 0; b < 4; b++) {
-                        uint32_t v0[2], v1[2];
-#pragma unroll
-                        for (int x = 0; x < 2; x++) {
-                            const uint32_t va = b < 2 ? a01[x] : a23[x], vb = b < 2 ? b01[x] : b23[x];
-                            v0[x] = b & 1 ? ints23(va) : ints01(va);
-                            v1[x] = b & 1 ? ints23(vb) : ints01(vb);
-                        }
+                        const uint32_t va = b < 2 ? a01 : a23, vb = b < 2 ? b01 : b23;
+                        const uint32_t v0 = b & 1 ? ints23(va) : ints01(va), v1 = b & 1 ? ints23(vb) : ints01(vb);
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
                             float acc[4];
-                            mma_f16_first(acc, pf[mt][0], v0[0], v1[0]);
-                            mma_f16(acc, pf[mt][1], v0[1], v1[1]);
+                            mma_f16_first(acc, pf[mt], v0, v1);
                             float(&oo)[OC] = o[mt][16 * gr + 4 * wd + b];
                             if (SPLIT) {
-                                oo[0] = fmaf(acc[0] + acc[2], vmax, oo[0]);
-                                oo[1] = fmaf(acc[1] + acc[3], vmax, oo[1]);
+                                oo[0] = fmaf(acc[0] + acc[2], vsc, oo[0]);
+                                oo[1] = fmaf(acc[1] + acc[3], vsc, oo[1]);
                             } else {
 #pragma unroll
-                                for (int e = 0; e < OC; e++) oo[e] = fmaf(acc[e], vmax, oo[e]);
+                                for (int e = 0; e < OC; e++) oo[e] = fmaf(acc[e], vsc, oo[e]);
                             }
                         }
                     }
@@ -388,7 +377,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 if (poisoned) sum = __int_as_float(0x7fffffff);
-                const int r = (SPLIT ? 8 : 16) * mt + g + 8 * hf;
+                const int r = 8 * (mt * HF + hf) + g;
                 if (r >= row_n) continue;
                 const bool whole = starts && ends;
                 // a NaN sum makes all of the row NaN
@@ -414,7 +403,6 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                     }
             }
         __syncwarp();
-        t += (uint32_t)(s1 - s0);
     }
 }
 
@@ -438,7 +426,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(Kv8Pool pool, Kv
     for (uint32_t u = blockIdx.x; u < units[seqs.n_seqs]; u += gridDim.x) {
         const int i = seq_at(units, seqs.n_seqs, u);
         const SeqWork w = seq_work<RB>(seqs, pool, a, i);
-        const uint32_t in = u - units[i], u0 = cum[i] + in * w.steps;
+        const uint32_t in = u - units[i], u0 = cum[i] + in * (w.steps + kUnitCost) + kUnitCost;  // its first step
         const uint32_t b = runs.run_of(u0), last = runs.run_of(u0 + w.steps - 1);
         if (b == last) continue;                         // that run has written the rows
         const int kvh = in / w.blocks, row_lo = (in - kvh * w.blocks) * RB, row_n = min(RB, w.n * a.group - row_lo);
@@ -502,17 +490,17 @@ RunPlan plan_runs(const Kv8Pool& pool, uint32_t typ, int group, int max_rows) {
     const int64_t rows = (int64_t)group * (max_rows < 1 ? 1 : max_rows);
     p.split = typ == LC_TYPE_F32 || rows <= 8;
     p.mt = rows > (p.split ? 8 : 16) && p.hd < 256 ? 2 : 1;
-    p.blocks = sm_count() * (p.hd == 256 ? 1 : p.mt > 1 ? 2 : 3);
+    p.blocks = sm_count() * (p.hd == 256 || p.mt > 1 ? 2 : p.split ? 4 : 3);
     p.bytes = (size_t)2 * p.blocks * kRunWarps * p.rows() * (p.hd + 2) * sizeof(float);
     return p;
 }
 
-template <int HD, int MT, bool SPLIT, bool FULL>
+template <int HD, int MT, bool SPLIT, bool F32, bool FULL>
 int32_t runs_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, int blocks, cudaStream_t s) {
-    using Shape = RunShape<HD, MT, SPLIT>;
+    using Shape = RunShape<HD, MT, SPLIT, F32>;
     const size_t cum = (size_t)(seqs.n_seqs + 1) * 4, smem = kRunWarps * Shape::kWarp + cum;
-    LC_CUDA(ensure_smem_limit((const void*)kv8_runs_kernel<HD, MT, SPLIT, FULL>, smem));
-    kv8_runs_kernel<HD, MT, SPLIT, FULL><<<blocks, kRunWarps * 32, smem, s>>>(pool, seqs, a);
+    LC_CUDA(ensure_smem_limit((const void*)kv8_runs_kernel<HD, MT, SPLIT, F32, FULL>, smem));
+    kv8_runs_kernel<HD, MT, SPLIT, F32, FULL><<<blocks, kRunWarps * 32, smem, s>>>(pool, seqs, a);
     LC_CUDA(cudaGetLastError());
     // units by what max_rows says (the kernel goes on to more); few of them are cut into thinner slices, with more shares
     const int64_t rows = std::min<int64_t>(Shape::kRows, (int64_t)a.group * std::max(1, max_rows));
@@ -523,15 +511,17 @@ int32_t runs_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int
     LC_CUDA(launch_pdl(kv8_join_kernel<HD, Shape::kRows>, dim3((unsigned)units, slices), dim3(kJoinThreads), 2 * cum, s, pool, seqs, a, blocks * kRunWarps, per));
     return LC_OK;
 }
-template <int HD, int MT, bool SPLIT>
+template <int HD, int MT, bool SPLIT, bool F32>
 int32_t runs_full(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, int blocks, cudaStream_t s) {
-    return pool.hd == HD ? runs_as<HD, MT, SPLIT, true>(pool, seqs, a, max_rows, blocks, s) : runs_as<HD, MT, SPLIT, false>(pool, seqs, a, max_rows, blocks, s);
+    return pool.hd == HD ? runs_as<HD, MT, SPLIT, F32, true>(pool, seqs, a, max_rows, blocks, s) : runs_as<HD, MT, SPLIT, F32, false>(pool, seqs, a, max_rows, blocks, s);
 }
 template <int HD>
 int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, const RunPlan& p, cudaStream_t s) {
+    const bool f32 = a.typ == LC_TYPE_F32;
     if constexpr (HD < 256)
-        if (p.mt == 2) return p.split ? runs_full<HD, 2, true>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 2, false>(pool, seqs, a, max_rows, p.blocks, s);
-    return p.split ? runs_full<HD, 1, true>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 1, false>(pool, seqs, a, max_rows, p.blocks, s);
+        if (p.mt == 2) return f32 ? runs_full<HD, 2, true, true>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 2, false, false>(pool, seqs, a, max_rows, p.blocks, s);
+    if (f32) return runs_full<HD, 1, true, true>(pool, seqs, a, max_rows, p.blocks, s);
+    return p.split ? runs_full<HD, 1, true, false>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 1, false, false>(pool, seqs, a, max_rows, p.blocks, s);
 }
 
 int32_t check_heads(const char* call, const Kv8Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {

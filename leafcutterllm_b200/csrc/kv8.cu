@@ -119,14 +119,6 @@ __device__ __forceinline__ float turned(float u, float w, float ch, float cl, fl
     const float y = d + (lost + fmaf(u, cl, -w * sl));
     return fabsf(d) < INFINITY ? y : d;
 }
-__device__ __forceinline__ float max_abs_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
-    return r;
-}
-// four numbers' low bytes
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) { return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410); }
-
 // The rotations of rows pos0 .. pos0 + n - 1: (cosine, sine) of every pair.  Sine and cosine themselves for every eighth row and for the first
 // eight turns; the rest are products of the two, 2^-52 off.  SPREAD: pair d lies at place (d mod 4) half / 4 + d / 4, so that lanes with four pairs each read
 // neighbouring places.  They are kept as two f32 each, 2^-48 of them off.
@@ -227,7 +219,7 @@ __device__ __forceinline__ void rows_pass(Item& it, const T* rows, int64_t strid
             }
             if (PASS == kMost) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) it.most = max_abs_nan(max_abs_nan(it.most, y0[e]), y1[e]);
+                for (int e = 0; e < 4; e++) it.most = max_nan(max_nan(it.most, fabsf(y0[e])), fabsf(y1[e]));
             } else if (PASS == kFine) {
                 float here = 0.0f;
 #pragma unroll

@@ -50,6 +50,15 @@ template <> __device__ __forceinline__ float to_elem<float>(float v) { return v;
 template <> __device__ __forceinline__ __half to_elem<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 to_elem<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// the larger one, NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// four numbers' low bytes
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) { return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410); }
+
 // Rows [first, first + n) of sequence i; false where row_start is not ascending within the call's rows.
 __device__ __forceinline__ bool kv8_span(const Kv8Seqs& s, int i, int& first, int& n) {
     const int a = s.row_start[i], b = s.row_start[i + 1];

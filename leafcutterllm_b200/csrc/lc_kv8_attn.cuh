@@ -24,6 +24,15 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
+// 16 x 8 sums of 32 products of integers of 8 bits, exact in 32
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8_first(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
 __device__ __forceinline__ uint32_t h2_pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -34,13 +43,15 @@ __device__ __forceinline__ void h2_split(float a, float b, uint32_t& hi, uint32_
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = h2_pack(a - __low2float(h), b - __high2float(h));
 }
-// Bytes 0, 1 (or 2, 3) of x = integers + 128 as f16 integers: 0x64 is the high byte of 1024.0, and 1152 = 1024 + 128.
+// Bytes 0, 1 (or 2, 3) of x = integers + 128 as f16 integers + 1152: 0x64 is the high byte of 1024.0, and 1152 = 1024 + 128; then without the 1152.
+__device__ __forceinline__ uint32_t biased01(uint32_t x) { return __byte_perm(x, 0x64646464u, 0x4140u); }
+__device__ __forceinline__ uint32_t biased23(uint32_t x) { return __byte_perm(x, 0x64646464u, 0x4342u); }
 __device__ __forceinline__ uint32_t minus_1152(uint32_t v) {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(1152.0f));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t ints01(uint32_t x) { return minus_1152(__byte_perm(x, 0x64646464u, 0x4140u)); }
-__device__ __forceinline__ uint32_t ints23(uint32_t x) { return minus_1152(__byte_perm(x, 0x64646464u, 0x4342u)); }
+__device__ __forceinline__ uint32_t ints01(uint32_t x) { return minus_1152(biased01(x)); }
+__device__ __forceinline__ uint32_t ints23(uint32_t x) { return minus_1152(biased23(x)); }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -111,7 +122,8 @@ __device__ __forceinline__ void row_scale(float top, float& up, float& down) {
 }
 
 constexpr float kNegInf = -INFINITY;
-constexpr int kStep = 32;            // keys of a step of the line: two pages', one page's or a part of one page's
+constexpr int kStep = 16;            // keys of a step of the line: one page's, or a part of one page's
+constexpr int kUnitCost = 4;         // steps that a unit's beginning and end take as long as
 
 // A unit is (sequence, kv head, row block of RB rows = tokens x heads of the group).
 struct SeqWork {
@@ -136,7 +148,7 @@ __device__ __forceinline__ SeqWork seq_work(const Kv8Seqs& s, const Kv8Pool& p, 
     }
     return w;
 }
-// cum[i] = steps of the sequences before i, cum[n_seqs] = all; units[i] (if wanted) the units before i; by one block, returns the total
+// cum[i] = the line's places before sequence i (kUnitCost and its steps for every unit), cum[n_seqs] = all; units[i] (if wanted) the units before i; by one block, returns the total
 template <int RB>
 __device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, uint32_t* cum, uint32_t* units, uint2* warp_sums) {
     const int per = (s.n_seqs + blockDim.x - 1) / blockDim.x, i0 = min((int)threadIdx.x * per, s.n_seqs), i1 = min(i0 + per, s.n_seqs);
@@ -145,7 +157,7 @@ __device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, 
         const SeqWork w = seq_work<RB>(s, p, a, i);
         cum[i] = sum;
         if (units) units[i] = usum;
-        sum += (uint32_t)w.blocks * (uint32_t)p.n_kv * (uint32_t)w.steps;
+        sum += (uint32_t)w.blocks * (uint32_t)p.n_kv * (uint32_t)(w.steps + kUnitCost);
         usum += (uint32_t)w.blocks * (uint32_t)p.n_kv;
     }
     uint32_t incl = sum, uincl = usum;
@@ -174,7 +186,7 @@ __device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, 
     __syncthreads();
     return total;
 }
-__device__ __forceinline__ int seq_at(const uint32_t* cum, int n_seqs, uint32_t t) {  // the sequence whose steps t is one of
+__device__ __forceinline__ int seq_at(const uint32_t* cum, int n_seqs, uint32_t t) {  // the sequence that has place t
     int lo = 0, hi = n_seqs;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
