@@ -4,10 +4,10 @@
 //   Scores  on the matrix unit's integers (mma.sync m16n8k32, exact): a row of queries is whole numbers in units of its largest / 32,512 (f32: / 8,323,072), and
 //           these are digits of 8 bits, in rows of their own of the operand, so that keys go in as they lie in the cache.  16 bits are as good as f16 or bf16
 //           queries ask for: a score of size 1 is off by 3e-5; 24 bits for f32.
-//   Values  an integer of 8 bits is exact in f16 (m16n8k16, f32 out); the weights are 2^(s - max + 8).  A step's sums are multiplied by its page's scale and added in
-//           f32, so that what the matrix unit cuts off when it adds stays within 16 keys.  Split form (8 rows to a tile of 16): rows 0 .. 7 of the tile hold
-//           the weight in f16 and rows 8 .. 15 what its rounding lost, 22 bits together, and the two halves of a sum lie in the same thread.  Plain form: 16
-//           rows, weights rounded to f16 (2^-11 of each).
+//   Values  an integer of 8 bits is exact in f16 (m16n8k16, f32 out): values are the operand of 16 rows (dims) and weights that of 8 columns (rows of queries), which the
+//           scores' layout already is.  The weights are 2^(s - max + 6) in f16, 2^-11 of each off, times their page's scale over a reference that follows the scales, so that sums stay
+//           in the matrix unit's accumulators.  For f32 they are the f16 value and what its rounding lost, 22 bits together, in two products; a step's sums are multiplied by the page's
+//           scale and added in f32, so that what the matrix unit cuts off when it adds stays within 16 keys.
 #include <algorithm>
 #include "lc_kv8.cuh"
 #include "lc_kernels.h"
@@ -64,29 +64,26 @@ __device__ __forceinline__ void place_at(Place& at, const Kv8Seqs& s, const Kv8P
     at.rb = unit - at.kvh * at.w.blocks;
 }
 
-// MT tiles of 16 rows: 8 MT rows in the split form, 16 MT in the plain one
-// F32: queries of 24 bits (and split weights)
-template <int HD, int MT, bool SPLIT, bool F32> struct RunShape {
-    static constexpr int kRows = MT * (SPLIT ? 8 : 16);
+// NG groups of 8 rows; F32: queries of 24 bits and weights of 22
+template <int HD, int NG, bool F32> struct RunShape {
+    static constexpr int kRows = 8 * NG;
     static constexpr int kStageBytes = 2 * kStep * HD + 16;   // keys, values, their two scales
-    static constexpr int kStages = HD == 64 ? 4 : 3;
-    static constexpr int kGroups = MT * (SPLIT ? 1 : 2);         // of 8 rows
-    static constexpr bool kQueriesShared = HD == 256 || MT > 1;  // operand fragments of the queries in shared memory, not in registers
-    static constexpr int kQueries = kQueriesShared ? kGroups * (F32 ? 2 : 1) * (HD / 32) * 512 : 0;
+    static constexpr int kStages = HD == 64 ? 4 : HD == 128 && !(F32 && NG == 4) ? 3 : 2;
+    static constexpr bool kQueriesShared = HD == 256 || NG > 1;  // operand fragments of the queries in shared memory, not in registers
+    static constexpr int kQueries = kQueriesShared ? NG * (F32 ? 2 : 1) * (HD / 32) * 512 : 0;
     static constexpr int kWarp = kStages * kStageBytes + kQueries;
-    static constexpr int kBlocks = HD == 256 || MT > 1 ? 2 : SPLIT ? 4 : 3;
+    static constexpr int kByRegisters = HD == 256 ? (NG == 1 ? 3 : 2) : NG == 1 ? 4 : NG == 2 ? 3 : 2;
+    static constexpr int kByMemory = (220 << 10) / (kRunWarps * kWarp + 2048);
+    static constexpr int kBlocks = kByRegisters < kByMemory ? kByRegisters : kByMemory;
 };
-
-template <int HD, int MT, bool SPLIT, bool F32, bool FULL>
-__global__ void __launch_bounds__(kRunWarps * 32, RunShape<HD, MT, SPLIT, F32>::kBlocks)
+template <int HD, int NG, bool F32, bool FULL>
+__global__ void __launch_bounds__(kRunWarps * 32, RunShape<HD, NG, F32>::kBlocks)
 kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
-    using Shape = RunShape<HD, MT, SPLIT, F32>;
-    constexpr int NG = Shape::kGroups, ND = F32 ? 2 : 1;  // groups of 8 rows, tiles of digits of each
+    using Shape = RunShape<HD, NG, F32>;
+    constexpr int ND = F32 ? 2 : 1;         // tiles of a group's digits
     constexpr int RB = Shape::kRows;
-    constexpr int NT = HD / 8;              // tiles of 8 dims of the output; a thread's values of a key are NT in a row
+    constexpr int NT = HD / 16;             // tiles of 16 dims of the output: a thread has two neighbouring ones of each, NT pairs in a row
     constexpr int KS = HD / 32;             // k steps of the scores
-    constexpr int HF = SPLIT ? 1 : 2;       // rows of a tile that a thread has a part in
-    constexpr int OC = 2 * HF;
     constexpr int S = Shape::kStages;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint2 warp_sums[kRunWarps];
@@ -158,17 +155,15 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
         // the queries as operand fragments: step ks = 2 j + x of the scores takes dims 64 j + 16 c + 8 x .. + 7.  A group's first tile has the highest digit in rows
         // 0 .. 7 and the next in rows 8 .. 15, its second tile the lowest in rows 0 .. 7.
         uint32_t qf[Shape::kQueriesShared ? 1 : NG * ND * KS][4];
-        float rf[MT][HF];
-        int limit[MT][HF];                   // last position that the row sees (-1: no row)
+        float rf[NG];
+        int limit[NG];                       // last position that the row sees (-1: no row)
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int hf = 0; hf < HF; hf++) {
-                const int group = mt * HF + hf, r = 8 * group + g;
+        for (int group = 0; group < NG; group++) {
+                const int r = 8 * group + g;
                 const bool has = r < row_n;
                 const int tok = has ? (row_lo + r) / a.group : 0, hq = has ? (row_lo + r) - tok * a.group : 0;
                 const int64_t src = (int64_t)(w.first + tok) * a.q_stride + (int64_t)(at.kvh * a.group + hq) * hd;
-                limit[mt][hf] = has ? w.ctx + tok : -1;
+                limit[group] = has ? w.ctx + tok : -1;
                 float v[HD / 64][16], top = 0.0f;
 #pragma unroll
                 for (int j = 0; j < HD / 64; j++) {
@@ -185,7 +180,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 float up, down;
                 row_scale(top, up, down);
                 const float unit = top > 0.0f ? top * up * (F32 ? 1.0f / 8323072.0f : 1.0f / 32512.0f) : 1.0f, per = 1.0f / unit;
-                rf[mt][hf] = top < INFINITY ? a.scale_log2 * down * unit : __int_as_float(0x7fffffff);  // not finite: the row is NaN
+                rf[group] = top < INFINITY ? a.scale_log2 * down * unit : __int_as_float(0x7fffffff);  // not finite: the row is NaN
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     uint32_t digit[3][2];    // [highest first][four dims]
@@ -216,16 +211,18 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 }
             }
 
-        float o[MT][NT][OC], m[MT][HF], l[MT][HF];
+        // o: dims (a thread's 2 t, 2 t + 1 of tile t) x rows 2c, 2c + 1 of the group; m, l: of row g
+        float o[NG][NT][4], m[NG], l[NG];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
+        for (int gr = 0; gr < NG; gr++) {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int e = 0; e < OC; e++) o[mt][n][e] = 0.0f;
-#pragma unroll
-            for (int hf = 0; hf < HF; hf++) { m[mt][hf] = kNegInf; l[mt][hf] = 0.0f; }
+                for (int e = 0; e < 4; e++) o[gr][t][e] = 0.0f;
+            m[gr] = kNegInf;
+            l[gr] = 0.0f;
         }
+        float vref = 0.0f;                   // 16-bit types: what the sums' scales are relative to
 
         // rows see all keys up to the first row's position (with a window, from the last row's on)
         const int sees = w.ctx + row_lo / a.group, from = a.window > 0 ? w.ctx + (row_lo + row_n - 1) / a.group - a.window : -1;
@@ -280,52 +277,68 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                             s[gr][tl][k] = F32 ? fmaf(high, 256.0f, (float)dot[gr * ND + ND - 1][tl][k]) : high;
                         }
             }
-            uint32_t pf[MT][4];
+            float to_weight = 1.0f;
+            if (!F32) {
+                // within 2^-8 and 2^4 of the reference a scale goes to the weights; others make a reference of themselves (of 0 nothing is added)
+                const float ratio = fabsf(vsc) / vref;
+                if (vsc != 0.0f && !(ratio >= 0x1p-8f && ratio <= 0x1p4f)) {
+                    const float by = vref > 0.0f ? vref / fabsf(vsc) : 0.0f;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+                    for (int gr = 0; gr < NG; gr++)
 #pragma unroll
-                for (int hf = 0; hf < HF; hf++) {
-                    float v[4];
-                    const float f = rf[mt][hf] * ksc;
+                        for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = s[mt * HF + hf][e >> 1][e & 1] * f;
-                    if (!plain) {
+                            for (int e = 0; e < 4; e++) o[gr][t][e] *= by;
+                    vref = fabsf(vsc);
+                }
+                to_weight = vref > 0.0f ? vsc / vref : 0.0f;
+                if (isnan(vsc)) to_weight = vsc;
+            }
+            uint32_t ph[NG][2], pl[NG][2];   // weights, and what their rounding lost: keys 2c, 2c + 1 and 8 + 2c, 9 + 2c of row g
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int key = key0 + 8 * (e >> 1) + 2 * c + (e & 1);
-                            if (key > limit[mt][hf] || (a.window > 0 && key <= limit[mt][hf] - a.window)) v[e] = kNegInf;
-                        }
-                    }
-                    float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    mx = fmaxf(mx, m[mt][hf]);
-                    const float ref = mx == kNegInf ? 0.0f : mx;
-                    if (__any_sync(0xffffffffu, mx > m[mt][hf])) {
-                        const float corr = exp2_fast(m[mt][hf] - ref);
-                        l[mt][hf] *= corr;
+            for (int gr = 0; gr < NG; gr++) {
+                float v[4];
+                const float f = rf[gr] * ksc;
 #pragma unroll
-                        for (int n = 0; n < NT; n++) { o[mt][n][2 * hf] *= corr; o[mt][n][2 * hf + 1] *= corr; }
-                        m[mt][hf] = mx;
-                    }
-                    const float less = 8.0f - ref;
+                for (int e = 0; e < 4; e++) v[e] = s[gr][e >> 1][e & 1] * f;
+                if (!plain) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = exp2_fast(v[e] + less);
-                    l[mt][hf] += (v[0] + v[1]) + (v[2] + v[3]);
-                    if (SPLIT) {
-                        h2_split(v[0], v[1], pf[mt][0], pf[mt][1]);
-                        h2_split(v[2], v[3], pf[mt][2], pf[mt][3]);
-                    } else {
-                        pf[mt][hf] = h2_pack(v[0], v[1]);
-                        pf[mt][2 + hf] = h2_pack(v[2], v[3]);
+                    for (int e = 0; e < 4; e++) {
+                        const int key = key0 + 8 * (e >> 1) + 2 * c + (e & 1);
+                        if (key > limit[gr] || (a.window > 0 && key <= limit[gr] - a.window)) v[e] = kNegInf;
                     }
                 }
-            // values: a thread's keys are 2c, 2c + 1, 8 + 2c, 9 + 2c; its dims NT in a row (HD 256: 16 and 16 more 128 further)
+                float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                // the reference is raised when a row's maximum has grown by more than 2^4, so that a weight is 2^10 at most (with its scale 2^14)
+                if (__any_sync(0xffffffffu, mx > m[gr] + 4.0f)) {
+                    mx = fmaxf(mx, m[gr]);
+                    const float corr = mx == kNegInf ? 1.0f : exp2_fast(m[gr] - mx);
+                    l[gr] *= corr;
+                    m[gr] = mx;
+                    const float c0 = __shfl_sync(0xffffffffu, corr, 8 * c), c1 = __shfl_sync(0xffffffffu, corr, 8 * c + 4);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) { o[gr][t][0] *= c0; o[gr][t][1] *= c1; o[gr][t][2] *= c0; o[gr][t][3] *= c1; }
+                }
+                const float less = m[gr] == kNegInf ? 6.0f : 6.0f - m[gr];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = exp2_fast(v[e] + less);
+                l[gr] += (v[0] + v[1]) + (v[2] + v[3]);
+                if (F32) {
+                    h2_split(v[0], v[1], ph[gr][0], pl[gr][0]);
+                    h2_split(v[2], v[3], ph[gr][1], pl[gr][1]);
+                } else {
+                    ph[gr][0] = h2_pack(v[0] * to_weight, v[1] * to_weight);
+                    ph[gr][1] = h2_pack(v[2] * to_weight, v[3] * to_weight);
+                }
+            }
+            // values: a thread's keys are 2c, 2c + 1, 8 + 2c, 9 + 2c; its dims 2 NT in a row (HD 256: 16 and 16 more 128 further)
             const unsigned char* vp = kp + kStep * HD;
             constexpr int WORDS = HD == 64 ? 2 : 4;
 #pragma unroll
-            for (int gr = 0; gr < (HD == 256 ? 2 : 1); gr++) {
-                const int ch = HD == 64 ? g >> 1 : 8 * gr + g;
+            for (int half = 0; half < (HD == 256 ? 2 : 1); half++) {
+                const int ch = HD == 64 ? g >> 1 : 8 * half + g;
                 uint32_t kv[4][WORDS];
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
@@ -341,28 +354,25 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                     }
                 }
 #pragma unroll
-                for (int wd = 0; wd < WORDS; wd++) {
-                    const uint32_t a01 = __byte_perm(kv[0][wd], kv[1][wd], 0x5140), a23 = __byte_perm(kv[0][wd], kv[1][wd], 0x7362);
-                    const uint32_t b01 = __byte_perm(kv[2][wd], kv[3][wd], 0x5140), b23 = __byte_perm(kv[2][wd], kv[3][wd], 0x7362);
+                for (int wd = 0; wd < WORDS; wd++)
 #pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        const uint32_t va = b < 2 ? a01 : a23, vb = b < 2 ? b01 : b23;
-                        const uint32_t v0 = b & 1 ? ints23(va) : ints01(va), v1 = b & 1 ? ints23(vb) : ints01(vb);
+                    for (int b = 0; b < 2; b++) {  // bytes 2b, 2b + 1: dims of a tile's rows g, g + 8
+                        const uint32_t va = __byte_perm(kv[0][wd], kv[1][wd], b ? 0x7362 : 0x5140), vb = __byte_perm(kv[2][wd], kv[3][wd], b ? 0x7362 : 0x5140);
+                        const uint32_t vf[4] = {ints01(va), ints23(va), ints01(vb), ints23(vb)};
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            float acc[4];
-                            mma_f16_first(acc, pf[mt], v0, v1);
-                            float(&oo)[OC] = o[mt][16 * gr + 4 * wd + b];
-                            if (SPLIT) {
-                                oo[0] = fmaf(acc[0] + acc[2], vsc, oo[0]);
-                                oo[1] = fmaf(acc[1] + acc[3], vsc, oo[1]);
+                        for (int gr = 0; gr < NG; gr++) {
+                            float(&oo)[4] = o[gr][8 * half + 2 * wd + b];
+                            if (F32) {
+                                float acc[4];
+                                mma_f16_first(acc, vf, pl[gr][0], pl[gr][1]);
+                                mma_f16(acc, vf, ph[gr][0], ph[gr][1]);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) oo[e] = fmaf(acc[e], vsc, oo[e]);
                             } else {
-#pragma unroll
-                                for (int e = 0; e < OC; e++) oo[e] = fmaf(acc[e], vsc, oo[e]);
+                                mma_f16(oo, vf, ph[gr][0], ph[gr][1]);
                             }
                         }
                     }
-                }
             }
         }
         cp_async_wait<0>();
@@ -370,38 +380,34 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
         const bool starts = s0 == 0, ends = s1 == w.steps;
         float* part = a.part + (size_t)(2 * run + (starts ? 1 : 0)) * part_floats<HD, RB>();
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int gr = 0; gr < NG; gr++) {
+            float sum = l[gr];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (poisoned) sum = __int_as_float(0x7fffffff);
+            const bool whole = starts && ends;
+            if (!whole && c == 0 && 8 * gr + g < row_n) { part[8 * gr + g] = m[gr]; part[RB + 8 * gr + g] = sum; }
 #pragma unroll
-            for (int hf = 0; hf < HF; hf++) {
-                float sum = l[mt][hf];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (poisoned) sum = __int_as_float(0x7fffffff);
-                const int r = 8 * (mt * HF + hf) + g;
+            for (int x = 0; x < 2; x++) {
+                const int r = 8 * gr + 2 * c + x;
+                const float total = __shfl_sync(0xffffffffu, sum, 8 * c + 4 * x);
                 if (r >= row_n) continue;
-                const bool whole = starts && ends;
                 // a NaN sum makes all of the row NaN
-                const float inv = whole ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+                const float inv = (whole ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f) * (F32 ? 1.0f : vref);
                 const int tok = (row_lo + r) / a.group, hq = (row_lo + r) - tok * a.group;
                 const int64_t dst = (int64_t)(w.first + tok) * a.out_stride + (int64_t)(at.kvh * a.group + hq) * hd;
-                if (!whole && c == 0) { part[r] = m[mt][hf]; part[RB + r] = sum; }
-                constexpr int GR = HD == 256 ? 2 : 1, W = HD == 64 ? 1 : 2;  // W runs of 16 dims
+                constexpr int N = HD == 64 ? 8 : 16;  // dims in a row
 #pragma unroll
-                for (int gr = 0; gr < GR; gr++)
+                for (int half = 0; half < (HD == 256 ? 2 : 1); half++) {
+                    float v[N];
 #pragma unroll
-                    for (int x = 0; x < W; x++) {
-                        float v[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            // HD 64: dims 8 (2c) + e of the first column, then of the second
-                            const int tile = HD == 64 ? e & 7 : 16 * gr + e, col = HD == 64 ? e >> 3 : x;
-                            v[e] = o[mt][tile][2 * hf + col] * inv;
-                        }
-                        const int d = HD == 64 ? 16 * c : 128 * gr + 32 * c + 16 * x;
-                        if (!whole) store16(part + 2 * RB + r * HD + d, true, v);
-                        else if (FULL || d < hd) store16(a.out, dst + d, a.typ, a.out_vec, v);
-                    }
+                    for (int e = 0; e < N; e++) v[e] = o[gr][8 * half + (e >> 1)][2 * (e & 1) + x] * inv;
+                    const int d = HD == 64 ? 8 * g : 128 * half + 16 * g;
+                    if (!whole) store_run<N>(part + 2 * RB + r * HD + d, true, v);
+                    else if (FULL || d < hd) store_run<N>(a.out, dst + d, a.typ, a.out_vec, v);
+                }
             }
+        }
         __syncwarp();
     }
 }
@@ -477,30 +483,33 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(Kv8Pool pool, Kv
 }
 
 struct RunPlan {
-    int hd, mt, blocks;
-    bool split;
+    int hd, groups, blocks;
     size_t bytes;
-    int rows() const { return mt * (split ? 8 : 16); }
 };
-// f32 is always in the split form, for its 22 bits; 16-bit types where a unit has 8 rows at most, since it costs no more products there.  Two
-// tiles share a step's keys and values where a unit has rows for them (heads of 256: their sums have no room in registers).
+template <int HD, bool F32> int run_blocks(int groups) {
+    if (HD < 256 && groups == 4) return RunShape<HD, HD < 256 ? 4 : 1, F32>::kBlocks;
+    return groups == 2 ? RunShape<HD, 2, F32>::kBlocks : RunShape<HD, 1, F32>::kBlocks;
+}
+// As many groups of 8 rows share a step's keys and values as a unit has rows for: four at most, whose sums are 128 registers (two for heads of 256).
 RunPlan plan_runs(const Kv8Pool& pool, uint32_t typ, int group, int max_rows) {
     RunPlan p;
     p.hd = pool.hd <= 64 ? 64 : pool.hd <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)group * (max_rows < 1 ? 1 : max_rows);
-    p.split = typ == LC_TYPE_F32 || rows <= 8;
-    p.mt = rows > (p.split ? 8 : 16) && p.hd < 256 ? 2 : 1;
-    p.blocks = sm_count() * (p.hd == 256 || p.mt > 1 ? 2 : p.split ? 4 : 3);
-    p.bytes = (size_t)2 * p.blocks * kRunWarps * p.rows() * (p.hd + 2) * sizeof(float);
+    p.groups = rows <= 8 ? 1 : rows <= 16 || p.hd == 256 ? 2 : 4;
+    const bool f32 = typ == LC_TYPE_F32;
+    p.blocks = sm_count() * (p.hd == 64    ? (f32 ? run_blocks<64, true>(p.groups) : run_blocks<64, false>(p.groups))
+                             : p.hd == 128 ? (f32 ? run_blocks<128, true>(p.groups) : run_blocks<128, false>(p.groups))
+                                           : (f32 ? run_blocks<256, true>(p.groups) : run_blocks<256, false>(p.groups)));
+    p.bytes = (size_t)2 * p.blocks * kRunWarps * 8 * p.groups * (p.hd + 2) * sizeof(float);
     return p;
 }
 
-template <int HD, int MT, bool SPLIT, bool F32, bool FULL>
+template <int HD, int NG, bool F32, bool FULL>
 int32_t runs_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, int blocks, cudaStream_t s) {
-    using Shape = RunShape<HD, MT, SPLIT, F32>;
+    using Shape = RunShape<HD, NG, F32>;
     const size_t cum = (size_t)(seqs.n_seqs + 1) * 4, smem = kRunWarps * Shape::kWarp + cum;
-    LC_CUDA(ensure_smem_limit((const void*)kv8_runs_kernel<HD, MT, SPLIT, F32, FULL>, smem));
-    kv8_runs_kernel<HD, MT, SPLIT, F32, FULL><<<blocks, kRunWarps * 32, smem, s>>>(pool, seqs, a);
+    LC_CUDA(ensure_smem_limit((const void*)kv8_runs_kernel<HD, NG, F32, FULL>, smem));
+    kv8_runs_kernel<HD, NG, F32, FULL><<<blocks, kRunWarps * 32, smem, s>>>(pool, seqs, a);
     LC_CUDA(cudaGetLastError());
     // units by what max_rows says (the kernel goes on to more); few of them are cut into thinner slices, with more shares
     const int64_t rows = std::min<int64_t>(Shape::kRows, (int64_t)a.group * std::max(1, max_rows));
@@ -511,17 +520,16 @@ int32_t runs_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int
     LC_CUDA(launch_pdl(kv8_join_kernel<HD, Shape::kRows>, dim3((unsigned)units, slices), dim3(kJoinThreads), 2 * cum, s, pool, seqs, a, blocks * kRunWarps, per));
     return LC_OK;
 }
-template <int HD, int MT, bool SPLIT, bool F32>
+template <int HD, int NG>
 int32_t runs_full(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, int blocks, cudaStream_t s) {
-    return pool.hd == HD ? runs_as<HD, MT, SPLIT, F32, true>(pool, seqs, a, max_rows, blocks, s) : runs_as<HD, MT, SPLIT, F32, false>(pool, seqs, a, max_rows, blocks, s);
+    if (a.typ == LC_TYPE_F32) return pool.hd == HD ? runs_as<HD, NG, true, true>(pool, seqs, a, max_rows, blocks, s) : runs_as<HD, NG, true, false>(pool, seqs, a, max_rows, blocks, s);
+    return pool.hd == HD ? runs_as<HD, NG, false, true>(pool, seqs, a, max_rows, blocks, s) : runs_as<HD, NG, false, false>(pool, seqs, a, max_rows, blocks, s);
 }
 template <int HD>
 int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, const RunPlan& p, cudaStream_t s) {
-    const bool f32 = a.typ == LC_TYPE_F32;
     if constexpr (HD < 256)
-        if (p.mt == 2) return f32 ? runs_full<HD, 2, true, true>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 2, false, false>(pool, seqs, a, max_rows, p.blocks, s);
-    if (f32) return runs_full<HD, 1, true, true>(pool, seqs, a, max_rows, p.blocks, s);
-    return p.split ? runs_full<HD, 1, true, false>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 1, false, false>(pool, seqs, a, max_rows, p.blocks, s);
+        if (p.groups == 4) return runs_full<HD, 4>(pool, seqs, a, max_rows, p.blocks, s);
+    return p.groups == 2 ? runs_full<HD, 2>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 1>(pool, seqs, a, max_rows, p.blocks, s);
 }
 
 int32_t check_heads(const char* call, const Kv8Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {

@@ -86,11 +86,11 @@ __device__ __forceinline__ void load16(const void* p, int64_t at, int typ, bool 
     else if (typ == LC_TYPE_F16) load16((const __half*)p + at, vec, v);
     else load16((const __nv_bfloat16*)p + at, vec, v);
 }
-template <typename T> __device__ __forceinline__ void store16(T* p, bool vec, const float* v) {
+template <int N, typename T> __device__ __forceinline__ void store_run(T* p, bool vec, const float* v) {
     constexpr int E = 16 / sizeof(T);
     if (vec) {
 #pragma unroll
-        for (int u = 0; u < 16 / E; u++) {
+        for (int u = 0; u < N / E; u++) {
             __align__(16) T t[E];
 #pragma unroll
             for (int e = 0; e < E; e++) t[e] = to_elem<T>(v[u * E + e]);
@@ -98,14 +98,16 @@ template <typename T> __device__ __forceinline__ void store16(T* p, bool vec, co
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 16; e++) p[e] = to_elem<T>(v[e]);
+        for (int e = 0; e < N; e++) p[e] = to_elem<T>(v[e]);
     }
 }
-__device__ __forceinline__ void store16(void* p, int64_t at, int typ, bool vec, const float* v) {
-    if (typ == LC_TYPE_F32) store16((float*)p + at, vec, v);
-    else if (typ == LC_TYPE_F16) store16((__half*)p + at, vec, v);
-    else store16((__nv_bfloat16*)p + at, vec, v);
+template <int N> __device__ __forceinline__ void store_run(void* p, int64_t at, int typ, bool vec, const float* v) {
+    if (typ == LC_TYPE_F32) store_run<N>((float*)p + at, vec, v);
+    else if (typ == LC_TYPE_F16) store_run<N>((__half*)p + at, vec, v);
+    else store_run<N>((__nv_bfloat16*)p + at, vec, v);
 }
+__device__ __forceinline__ void store16(float* p, bool vec, const float* v) { store_run<16>(p, vec, v); }
+__device__ __forceinline__ void store16(void* p, int64_t at, int typ, bool vec, const float* v) { store_run<16>(p, at, typ, vec, v); }
 __device__ __forceinline__ void store1(void* p, int64_t at, int typ, float v) {
     if (typ == LC_TYPE_F32) ((float*)p)[at] = v;
     else if (typ == LC_TYPE_F16) ((__half*)p)[at] = to_elem<__half>(v);
