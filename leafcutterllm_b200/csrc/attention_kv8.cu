@@ -94,6 +94,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
     const uint32_t total = line_up<RB>(seqs, pool, a, cum, nullptr, warp_sums);
     const Runs runs(total, gridDim.x * kRunWarps);
     const uint32_t run = blockIdx.x * kRunWarps + warp;
+    if (lane == 0) a.records[run].row_n = 0;
     if (run >= runs.n) return;
     uint32_t t = runs.start(run);
     const uint32_t t_end = runs.start(run + 1);
@@ -114,6 +115,10 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
         const int end = min(w.steps + kUnitCost, at.in + (int)(t_end - t)), s0 = max(0, at.in - kUnitCost), s1 = end - kUnitCost;
         t += (uint32_t)(end - at.in);
         if (s1 <= s0) continue;  // the unit's steps are the next run's
+        if (s0 == 0 && s1 < w.steps && lane == 0) {
+            a.records[run].last = (int)runs.run_of(t + (uint32_t)(w.steps - s1) - 1);
+            *reinterpret_cast<int4*>(&a.records[run]) = make_int4(w.first, at.kvh, at.rb * RB, min(RB, w.n * a.group - at.rb * RB));
+        }
         const int32_t* table = seqs.table + (size_t)at.seq * seqs.width;
         const int row_lo = at.rb * RB, row_n = min(RB, w.n * a.group - row_lo);
 
@@ -294,36 +299,49 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 to_weight = vref > 0.0f ? vsc / vref : 0.0f;
                 if (isnan(vsc)) to_weight = vsc;
             }
-            uint32_t ph[NG][2], pl[NG][2];   // weights, and what their rounding lost: keys 2c, 2c + 1 and 8 + 2c, 9 + 2c of row g
+            float mx[NG];
+            bool raise = false;
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) {
-                float v[4];
                 const float f = rf[gr] * ksc;
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = s[gr][e >> 1][e & 1] * f;
+                for (int e = 0; e < 4; e++) s[gr][e >> 1][e & 1] *= f;
                 if (!plain) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int key = key0 + 8 * (e >> 1) + 2 * c + (e & 1);
-                        if (key > limit[gr] || (a.window > 0 && key <= limit[gr] - a.window)) v[e] = kNegInf;
+                        if (key > limit[gr] || (a.window > 0 && key <= limit[gr] - a.window)) s[gr][e >> 1][e & 1] = kNegInf;
                     }
                 }
-                float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                // the reference is raised when a row's maximum has grown by more than 2^4, so that a weight is 2^10 at most (with its scale 2^14)
-                if (__any_sync(0xffffffffu, mx > m[gr] + 4.0f)) {
-                    mx = fmaxf(mx, m[gr]);
-                    const float corr = mx == kNegInf ? 1.0f : exp2_fast(m[gr] - mx);
+                mx[gr] = fmaxf(fmaxf(s[gr][0][0], s[gr][0][1]), fmaxf(s[gr][1][0], s[gr][1][1]));
+            }
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) mx[gr] = fmaxf(mx[gr], __shfl_xor_sync(0xffffffffu, mx[gr], 1));
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+                mx[gr] = fmaxf(mx[gr], __shfl_xor_sync(0xffffffffu, mx[gr], 2));
+                raise = raise || mx[gr] > m[gr] + 4.0f;
+            }
+            // the references are raised when a row's maximum has grown by more than 2^4, so that a weight is 2^10 at most (with its scale 2^14); one vote for all
+            // groups, whose chains of instructions then run side by side
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) {
+                    const float top = fmaxf(mx[gr], m[gr]), corr = top == kNegInf ? 1.0f : exp2_fast(m[gr] - top);
                     l[gr] *= corr;
-                    m[gr] = mx;
+                    m[gr] = top;
                     const float c0 = __shfl_sync(0xffffffffu, corr, 8 * c), c1 = __shfl_sync(0xffffffffu, corr, 8 * c + 4);
 #pragma unroll
                     for (int t = 0; t < NT; t++) { o[gr][t][0] *= c0; o[gr][t][1] *= c1; o[gr][t][2] *= c0; o[gr][t][3] *= c1; }
                 }
-                const float less = m[gr] == kNegInf ? 6.0f : 6.0f - m[gr];
+            }
+            uint32_t ph[NG][2], pl[NG][2];   // weights, and what their rounding lost: keys 2c, 2c + 1 and 8 + 2c, 9 + 2c of row g
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = exp2_fast(v[e] + less);
+            for (int gr = 0; gr < NG; gr++) {
+                const float less = m[gr] == kNegInf ? 6.0f : 6.0f - m[gr];
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = exp2_fast(s[gr][e >> 1][e & 1] + less);
                 l[gr] += (v[0] + v[1]) + (v[2] + v[3]);
                 if (F32) {
                     h2_split(v[0], v[1], ph[gr][0], pl[gr][0]);
@@ -412,39 +430,32 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
     }
 }
 
-// Joins the partial results of units that lie in several runs.  grid: (units, slices of `per` groups of four dims of a unit's rows); what threads are
-// left over take shares of the partial results.
-constexpr int kJoinThreads = 128;
+// Joins the partial results of units that lie in several runs.  grid: (runs, slices of kJoinRows rows); a run's record says which unit begins in it.  Threads
+// take four dims of a row each, and what threads are left over shares of the partial results.
+constexpr int kJoinThreads = 128, kJoinRows = 4;
 template <int HD, int RB>
-__global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a, int warps, int per) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint2 warp_sums[kJoinThreads / 32];
+__global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(AttnArgs a, int hd) {
     __shared__ float4 s_val[kJoinThreads];
     __shared__ float s_m[kJoinThreads], s_sum[kJoinThreads];
-    uint32_t* cum = reinterpret_cast<uint32_t*>(smem);
-    uint32_t* units = cum + seqs.n_seqs + 1;
-    const uint32_t total = line_up<RB>(seqs, pool, a, cum, units, warp_sums);
-    pdl_wait();  // every block: this kernel's end then means that of the one before
-    const Runs runs(total, warps);
     constexpr int P = part_floats<HD, RB>(), Q = HD / 4;
-    const int shares = kJoinThreads / per, share = threadIdx.x / per, e = blockIdx.y * per + threadIdx.x - share * per;
-    const int r = e / Q, d = (e - r * Q) * 4;
-    for (uint32_t u = blockIdx.x; u < units[seqs.n_seqs]; u += gridDim.x) {
-        const int i = seq_at(units, seqs.n_seqs, u);
-        const SeqWork w = seq_work<RB>(seqs, pool, a, i);
-        const uint32_t in = u - units[i], u0 = cum[i] + in * (w.steps + kUnitCost) + kUnitCost;  // its first step
-        const uint32_t b = runs.run_of(u0), last = runs.run_of(u0 + w.steps - 1);
-        if (b == last) continue;                         // that run has written the rows
-        const int kvh = in / w.blocks, row_lo = (in - kvh * w.blocks) * RB, row_n = min(RB, w.n * a.group - row_lo);
-        const bool here = r < row_n;
+    pdl_wait();  // every block: this kernel's end then means that of the one before
+    const int b = blockIdx.x;
+    const int4 at = *reinterpret_cast<const int4*>(&a.records[b]);
+    const int last = a.records[b].last, row0 = blockIdx.y * kJoinRows, rows = min(kJoinRows, at.w - row0);
+    if (rows <= 0) return;
+    const int cells = rows * Q, per = min(cells, kJoinThreads), shares = kJoinThreads / per, share = threadIdx.x / per;
+    for (int e0 = 0; e0 < cells; e0 += per) {
+        const int e = e0 + threadIdx.x - share * per, r = row0 + e / Q, d = (e % Q) * 4;
+        const bool here = share < shares && e < cells;
         float mx = kNegInf, sum = 0.0f;
         float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (here) {
-#pragma unroll 4
-            for (uint32_t x = b + share; x <= last; x += shares) {
-                const float* p = a.part + (size_t)(2 * x + (x == b ? 1 : 0)) * P;
-                const float pm = p[r], ps = p[RB + r];
-                const float4 v = *reinterpret_cast<const float4*>(p + 2 * RB + r * HD + d);
+            const float* p = a.part + (size_t)(2 * b + 1) * P;  // of the run itself the second place, of the later ones the first
+#pragma unroll 8
+            for (int x = b + share; x <= last; x += shares) {
+                const float* q = x == b ? p : a.part + (size_t)(2 * x) * P;
+                const float pm = q[r], ps = q[RB + r];
+                const float4 v = *reinterpret_cast<const float4*>(q + 2 * RB + r * HD + d);
                 const float m2 = fmaxf(mx, pm), ref = m2 == kNegInf ? 0.0f : m2;
                 const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(pm - ref);
                 sum = f0 * sum + (isnan(ps) ? ps : f1 * ps);
@@ -470,9 +481,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(Kv8Pool pool, Kv
                 }
             }
         }
-        if (share == 0 && here && d < pool.hd) {
-            const int tok = (row_lo + r) / a.group, hq = (row_lo + r) - tok * a.group;
-            const int64_t dst = (int64_t)(w.first + tok) * a.out_stride + (int64_t)(kvh * a.group + hq) * pool.hd + d;
+        if (share == 0 && here && d < hd) {
+            const int tok = (at.z + r) / a.group, hq = (at.z + r) - tok * a.group;
+            const int64_t dst = (int64_t)(at.x + tok) * a.out_stride + (int64_t)(at.y * a.group + hq) * hd + d;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             store1(a.out, dst, a.typ, val.x * inv);
             store1(a.out, dst + 1, a.typ, val.y * inv);
@@ -500,36 +511,30 @@ RunPlan plan_runs(const Kv8Pool& pool, uint32_t typ, int group, int max_rows) {
     p.blocks = sm_count() * (p.hd == 64    ? (f32 ? run_blocks<64, true>(p.groups) : run_blocks<64, false>(p.groups))
                              : p.hd == 128 ? (f32 ? run_blocks<128, true>(p.groups) : run_blocks<128, false>(p.groups))
                                            : (f32 ? run_blocks<256, true>(p.groups) : run_blocks<256, false>(p.groups)));
-    p.bytes = (size_t)2 * p.blocks * kRunWarps * 8 * p.groups * (p.hd + 2) * sizeof(float);
+    p.bytes = (size_t)p.blocks * kRunWarps * (sizeof(UnitRecord) + (size_t)2 * 8 * p.groups * (p.hd + 2) * sizeof(float));
     return p;
 }
 
 template <int HD, int NG, bool F32, bool FULL>
-int32_t runs_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, int blocks, cudaStream_t s) {
+int32_t runs_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int blocks, cudaStream_t s) {
     using Shape = RunShape<HD, NG, F32>;
     const size_t cum = (size_t)(seqs.n_seqs + 1) * 4, smem = kRunWarps * Shape::kWarp + cum;
     LC_CUDA(ensure_smem_limit((const void*)kv8_runs_kernel<HD, NG, F32, FULL>, smem));
     kv8_runs_kernel<HD, NG, F32, FULL><<<blocks, kRunWarps * 32, smem, s>>>(pool, seqs, a);
     LC_CUDA(cudaGetLastError());
-    // units by what max_rows says (the kernel goes on to more); few of them are cut into thinner slices, with more shares
-    const int64_t rows = std::min<int64_t>(Shape::kRows, (int64_t)a.group * std::max(1, max_rows));
-    const int64_t units = std::min<int64_t>(4096, ((int64_t)seqs.n_rows * a.group / Shape::kRows + seqs.n_seqs) * pool.n_kv);
-    int per = kJoinThreads;
-    while (per > 32 && units * ((rows * HD / 4 + per - 1) / per) < 2 * sm_count()) per /= 2;
-    const unsigned slices = (unsigned)((Shape::kRows * HD / 4 + per - 1) / per);
-    LC_CUDA(launch_pdl(kv8_join_kernel<HD, Shape::kRows>, dim3((unsigned)units, slices), dim3(kJoinThreads), 2 * cum, s, pool, seqs, a, blocks * kRunWarps, per));
+    LC_CUDA(launch_pdl(kv8_join_kernel<HD, Shape::kRows>, dim3((unsigned)blocks * kRunWarps, (Shape::kRows + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads), 0, s, a, pool.hd));
     return LC_OK;
 }
 template <int HD, int NG>
-int32_t runs_full(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, int blocks, cudaStream_t s) {
-    if (a.typ == LC_TYPE_F32) return pool.hd == HD ? runs_as<HD, NG, true, true>(pool, seqs, a, max_rows, blocks, s) : runs_as<HD, NG, true, false>(pool, seqs, a, max_rows, blocks, s);
-    return pool.hd == HD ? runs_as<HD, NG, false, true>(pool, seqs, a, max_rows, blocks, s) : runs_as<HD, NG, false, false>(pool, seqs, a, max_rows, blocks, s);
+int32_t runs_full(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int blocks, cudaStream_t s) {
+    if (a.typ == LC_TYPE_F32) return pool.hd == HD ? runs_as<HD, NG, true, true>(pool, seqs, a, blocks, s) : runs_as<HD, NG, true, false>(pool, seqs, a, blocks, s);
+    return pool.hd == HD ? runs_as<HD, NG, false, true>(pool, seqs, a, blocks, s) : runs_as<HD, NG, false, false>(pool, seqs, a, blocks, s);
 }
 template <int HD>
-int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int max_rows, const RunPlan& p, cudaStream_t s) {
+int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const RunPlan& p, cudaStream_t s) {
     if constexpr (HD < 256)
-        if (p.groups == 4) return runs_full<HD, 4>(pool, seqs, a, max_rows, p.blocks, s);
-    return p.groups == 2 ? runs_full<HD, 2>(pool, seqs, a, max_rows, p.blocks, s) : runs_full<HD, 1>(pool, seqs, a, max_rows, p.blocks, s);
+        if (p.groups == 4) return runs_full<HD, 4>(pool, seqs, a, p.blocks, s);
+    return p.groups == 2 ? runs_full<HD, 2>(pool, seqs, a, p.blocks, s) : runs_full<HD, 1>(pool, seqs, a, p.blocks, s);
 }
 
 int32_t check_heads(const char* call, const Kv8Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {
@@ -587,12 +592,13 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
     window = std::min(window, 1 << 30);  // the kernels' differences of positions stay in 32 bits
     const size_t elem = typ == LC_TYPE_F32 ? 4 : 2;
     AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, n_heads, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16),
-               scale * 1.44269504088896f, (float*)workspace_dev};
+               scale * 1.44269504088896f, nullptr, (UnitRecord*)workspace_dev};
+    a.part = by_tiles ? (float*)workspace_dev : (float*)((char*)workspace_dev + (size_t)plan.blocks * kRunWarps * sizeof(UnitRecord));
     cudaStream_t s = stream_or_own(stream_);
     if (by_tiles) return launch_kv8_tiles(pool, seqs, a, tiles, s);
-    if (plan.hd == 64) return runs_of<64>(pool, seqs, a, rows->max_rows, plan, s);
-    if (plan.hd == 128) return runs_of<128>(pool, seqs, a, rows->max_rows, plan, s);
-    return runs_of<256>(pool, seqs, a, rows->max_rows, plan, s);
+    if (plan.hd == 64) return runs_of<64>(pool, seqs, a, plan, s);
+    if (plan.hd == 128) return runs_of<128>(pool, seqs, a, plan, s);
+    return runs_of<256>(pool, seqs, a, plan, s);
 }
 
 }  // extern "C"

@@ -13,6 +13,11 @@ struct AttnArgs {
     bool q_vec, out_vec;             // 16-byte accesses
     float scale_log2;                // scale * log2(e)
     float* part;                     // partial results of runs that end inside a unit
+    struct UnitRecord* records;      // one per run: the unit that begins in it and goes on behind it
+};
+struct __align__(16) UnitRecord {
+    int first, kvh, row_lo, row_n;   // the sequence's first row, kv head, rows; row_n 0: none
+    int last, pad0, pad1, pad2;      // the run with the unit's end
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
