@@ -4,7 +4,7 @@
 // take turns on the matrix unit while the other's softmax runs.  It walks the keys in tiles of 128.
 //   warps 0-3, 4-7   the softmax of row tile 0, 1: a row per thread, scores and sums in tensor memory;
 //   warp 13          copies the next keys and values from the cache into shared memory (bulk copies of 16 keys);
-//   warps 8-11       unpack them to f16 (K as [key][dim], V as [dim][key], 128-byte swizzle);
+//   warps 8-11, 14, 15   unpack them to f16 (K as [key][dim], V as [dim][key], 128-byte swizzle);
 //   warp 12          one thread issues the products.  With the unpacking in the same warp an iteration took 9,500 cycles instead of 4,000: the issue waits
 //                    for the matrix unit's queue.
 // Scores: S = Q K^T, the queries times one power of two for the whole unit; f32 queries as f16 high and low parts, two products.
@@ -27,7 +27,9 @@ namespace lc {
 
 namespace {
 
-constexpr int kTileRows2 = 256, kKeys = 128, kTileThreads = 512, kSlots = 4;
+constexpr int kTileRows2 = 256, kKeys = 128, kTileThreads = 512, kConvWarps = 6, kSlots = 4;
+// registers a thread at the launch
+constexpr int kLaunchRegs = 128;
 constexpr int kGroups = kKeys / 16;
 
 // what the softmax needs to know of 16 keys: score factor, log2 of the values' scale, its inverse; and what the unpacking does
@@ -40,7 +42,8 @@ struct TileShared {
     uint64_t s_full[2], p_full[2], o_full[2];  // scores, weights, sums of a row tile
     uint64_t c_full[kSlots];                   // consts of a key tile
     uint64_t raw_full[2], raw_free[2];         // copied keys, values
-    uint64_t f16_full[2];                      // unpacked keys, values; their places are free when the last row tile's products are done
+    uint64_t f16_full[2];                      // unpacked keys, values; the keys' place is free when the last row tile's scores are done,
+    uint64_t v_free[2];                        // the values' when its sums are
     GroupConst consts[kSlots][kGroups];
     uint2 sums[kTileThreads / 32];
     uint32_t tmem;
@@ -52,8 +55,11 @@ template <int HD, bool SPLIT> struct TileShape {
     static constexpr int kPart = HD * 256;                    // 128 rows of HD f16
     static constexpr int kQ = 2 * (SPLIT ? 2 : 1) * kPart;    // [row tile][high, low]
     static constexpr int kK = HD * 256, kV = HD * 256;
+    static constexpr int kSoftRegs = SPLIT ? 176 : 184, kOtherRegs = 256 - kSoftRegs;  // of the softmax's 256 threads, of the other 256
+    static_assert(256 * (kSoftRegs + kOtherRegs) <= kLaunchRegs * kTileThreads, "setmaxnreg waits for registers that the launch does not have");
+    static constexpr int kVs = SPLIT ? 1 : 2;                 // places for unpacked values: f32 queries leave room for one
     static constexpr int kRaw = kKeys * HD;                   // keys, values as they are in the cache
-    static constexpr int kBytes = kQ + kK + kV + 2 * kRaw + 1024;
+    static constexpr int kBytes = kQ + kK + kVs * kV + 2 * kRaw + 1024;
 };
 
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -79,7 +85,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
     unsigned char* const sq = smem;
     unsigned char* const sk = sq + Shape::kQ;
     unsigned char* const sv = sk + Shape::kK;
-    unsigned char* const raw[2] = {sv + Shape::kV, sv + Shape::kV + Shape::kRaw};
+    unsigned char* const raw[2] = {sv + Shape::kVs * Shape::kV, sv + Shape::kVs * Shape::kV + Shape::kRaw};
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (blockIdx.x == 0 && blockIdx.y == 0) kv8_check_seqs(seqs, pool);
 
@@ -127,10 +133,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         for (int t = 0; t < 2; t++) {
             mbar_init(&sh.s_full[t], 1);
             mbar_init(&sh.o_full[t], 1);
+            mbar_init(&sh.v_free[t], 1);
             mbar_init(&sh.p_full[t], 128);
             mbar_init(&sh.raw_full[t], 1);
-            mbar_init(&sh.raw_free[t], 4);
-            mbar_init(&sh.f16_full[t], 4);
+            mbar_init(&sh.raw_free[t], kConvWarps);
+            mbar_init(&sh.f16_full[t], kConvWarps);
         }
         for (int t = 0; t < kSlots; t++) mbar_init(&sh.c_full[t], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -194,8 +201,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
     __syncthreads();
 
     const int last = n_tiles - 1;
-    if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp >= 8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Shape::kOtherRegs));
+      if (warp == 12 || warp == 13) {
         if (warp == 12) {
             // ------------------------------------------------------------------------------------------------ products
             if (lane == 0) {
@@ -212,14 +220,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                     }
                     umma_commit(&sh.s_full[t]);
                 };
-                auto sums = [&](int t, bool on) {
-                    const uint64_t dv = umma_desc_sw128(v_at);
+                auto sums = [&](int t, int i) {
+                    const bool on = !SPLIT && i > 0;
+                    const uint64_t dv = umma_desc_sw128(v_at + (i % Shape::kVs) * Shape::kV);
 #pragma unroll
                     for (int term = 0; term < TERMS; term++)
 #pragma unroll
                         for (int ks = 0; ks < kKeys / 16; ks++)
                             umma_f16_ts(col_o[t], col_s[t] + 16 * ks + 8 * term, dv + (((ks >> 2) * (HD * 128) + (ks & 3) * 32) >> 4), idesc_f16(HD), (uint32_t)(on || term + ks > 0));
                     umma_commit(&sh.o_full[t]);
+                    if (t == last) umma_commit(&sh.v_free[i % Shape::kVs]);
                 };
                 bool ok = mbar_wait(&sh.f16_full[0], 0);
                 tc_fence_after();
@@ -231,7 +241,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         ok = mbar_wait(&sh.p_full[t], i & 1);
                         tc_fence_after();
                         if (!ok) break;
-                        sums(t, !SPLIT && i > 0);
+                        sums(t, i);
                         if (more) {
                             if (t == 0) ok = mbar_wait(&sh.f16_full[0], (i + 1) & 1);
                             if (!ok) break;
@@ -297,12 +307,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                 for (int x = 0; x < 2; x++) (void)mbar_wait(&sh.raw_full[x], 0), (void)mbar_wait(&sh.raw_full[x], 1);
             }
         }
-    } else if (warp >= 8) {
+      } else {
         // ---------------------------------------------------------------------------------------------------- unpacking
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        const int ct = tid - 256, cw = warp - 8;
-        constexpr int KC = HD / 16, KP = 128 / KC, KN = kKeys / KP;   // K: chunks of a key, keys of a pass, passes
-        constexpr int LPK = HD / 4, VU = 4 * LPK / 32;                // V: lanes of a key, octets of keys per lane
+        const int cw = warp < 12 ? warp - 8 : warp - 10, ct = cw * 32 + lane;
+        constexpr int KC = HD / 16, LPK = HD / 4, OPW = 32 / LPK;     // K: pieces of a key; V: lanes of a key, octets of keys that a warp has at a time
         bool ok = true;
         for (int i = 0; i < n && ok; i++) {
             const GroupConst* gc = sh.consts[i % kSlots];
@@ -310,9 +318,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             if (i > 0) ok = ok && mbar_wait(&sh.s_full[last], (i - 1) & 1);  // the keys' place is free
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-#pragma unroll 4
-            for (int u = 0; u < KN; u++) {
-                const int key = ct / KC + u * KP, ch = ct % KC, state = gc[key >> 4].state;
+#pragma unroll 2
+            for (int e = ct; e < kKeys * KC; e += 32 * kConvWarps) {
+                const int key = e / KC, ch = e % KC, state = gc[key >> 4].state;
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (!(state & (kAbsent | kOutside)) && ch * 16 < hd) x = *reinterpret_cast<const uint4*>(raw[0] + key * hd + ch * 16);
                 x.x ^= 0x80808080u; x.y ^= 0x80808080u; x.z ^= 0x80808080u; x.w ^= 0x80808080u;
@@ -330,12 +338,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             if (lane == 0) { mbar_arrive(&sh.f16_full[0]); mbar_arrive(&sh.raw_free[0]); }
 
             ok = mbar_wait(&sh.raw_full[1], i & 1);
-            if (i > 0) ok = ok && mbar_wait(&sh.o_full[last], (i - 1) & 1);  // the values' place is free
+            if (i >= Shape::kVs) ok = ok && mbar_wait(&sh.v_free[i % Shape::kVs], (i / Shape::kVs - 1) & 1);  // the values' place is free
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-#pragma unroll
-            for (int u = 0; u < VU; u++) {
-                const int octet = 4 * cw + u * (32 / LPK) + lane / LPK, d = (lane % LPK) * 4;
+            unsigned char* const to = sv + (i % Shape::kVs) * Shape::kV;
+#pragma unroll 1
+            for (int u = cw; u < 16 / OPW; u += kConvWarps) {
+                const int octet = u * OPW + lane / LPK, d = (lane % LPK) * 4;
                 const bool none = gc[octet >> 1].state != kHere || d >= hd;
                 uint32_t x[8];
 #pragma unroll
@@ -358,7 +367,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                     out.z = b & 1 ? ints23(p[2]) : ints01(p[2]);
                     out.w = b & 1 ? ints23(p[3]) : ints01(p[3]);
                     // row b LPK + l holds dim 4 l + b: eight lanes write eight rows
-                    *reinterpret_cast<uint4*>(sv + (octet >> 3) * (HD * 128) + sw128(b * LPK + lane % LPK, octet & 7)) = out;
+                    *reinterpret_cast<uint4*>(to + (octet >> 3) * (HD * 128) + sw128(b * LPK + lane % LPK, octet & 7)) = out;
                 }
             }
             fence_async();
@@ -366,9 +375,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             if (lane == 0) { mbar_arrive(&sh.f16_full[1]); mbar_arrive(&sh.raw_free[1]); }
         }
         if (!ok) sh.dead = 1;
+      }
     } else {
         // ------------------------------------------------------------------------------------------------------ softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Shape::kSoftRegs));
         const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t my_s = col_s[t] + lanes, my_o = col_o[t] + lanes;
@@ -594,6 +604,11 @@ int32_t tiles_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, co
     const void* kern = (const void*)kv8_tiles_kernel<HD, SPLIT>;
     const size_t smem = std::max<size_t>(Shape::kBytes, (size_t)2 * (seqs.n_seqs + 1) * 4 + 1024);
     LC_CUDA(ensure_smem_limit(kern, smem));
+    static const int regs = [&] {  // setmaxnreg counts on the launch's registers: a build that has fewer must not start it
+        cudaFuncAttributes at;
+        return cudaFuncGetAttributes(&at, kern) == cudaSuccess ? at.numRegs : 0;
+    }();
+    LC_CHECK(regs == kLaunchRegs, LC_ERR_UNSUPPORTED, "attention in tiles was built with %d registers a thread instead of %d", regs, kLaunchRegs);
     kv8_tiles_kernel<HD, SPLIT><<<dim3((unsigned)plan.units, (unsigned)plan.splits), kTileThreads, smem, s>>>(pool, seqs, a, plan.splits);
     LC_CUDA(cudaGetLastError());
     if (plan.splits > 1) {
