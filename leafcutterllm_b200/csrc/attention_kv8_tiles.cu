@@ -72,6 +72,17 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// products issued by the lane whose `by` is set, in a warp that goes through this together
+__device__ __forceinline__ void mma_ss_by(uint32_t by, uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(da), "l"(db),
+                 "r"(idesc), "r"(accumulate), "r"(by)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts_by(uint32_t by, uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(db),
+                 "r"(idesc), "r"(accumulate), "r"(by)
+                 : "memory");
+}
 // 16-byte chunk `ch` (of 8) of a row of 128 bytes
 __device__ __forceinline__ int sw128(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
 
@@ -206,53 +217,58 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
       if (warp == 12 || warp == 13) {
         if (warp == 12) {
             // ------------------------------------------------------------------------------------------------ products
-            if (lane == 0) {
-                const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv);
-                auto scores = [&](int t) {
+            // All lanes go the same way and one of them issues: descriptors then are the warp's and not a thread's (2,048-token prompt in f32 127 -> 119 us).
+            const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv), base = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t one = lane == 0;
+            auto scores = [&](int t) {
+                const uint32_t d = base + 128 * t;
 #pragma unroll
-                    for (int term = 0; term < TERMS; term++) {
-                        const uint64_t dq = umma_desc_sw128(q_at + (t * TERMS + term) * Shape::kPart), dk = umma_desc_sw128(k_at);
+                for (int term = TERMS - 1; term >= 0; term--) {  // the low parts first: what is cut off then is small
+                    const uint64_t dq = umma_desc_sw128(q_at + (t * TERMS + term) * Shape::kPart), dk = umma_desc_sw128(k_at);
 #pragma unroll
-                        for (int ks = 0; ks < HD / 16; ks++) {
-                            const uint64_t off = ((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4;
-                            umma_f16_ss(col_s[t], dq + off, dk + off, idesc_f16(kKeys), term + ks > 0);
-                        }
-                    }
-                    umma_commit(&sh.s_full[t]);
-                };
-                auto sums = [&](int t, int i) {
-                    const bool on = !SPLIT && i > 0;
-                    const uint64_t dv = umma_desc_sw128(v_at + (i % Shape::kVs) * Shape::kV);
-#pragma unroll
-                    for (int term = 0; term < TERMS; term++)
-#pragma unroll
-                        for (int ks = 0; ks < kKeys / 16; ks++)
-                            umma_f16_ts(col_o[t], col_s[t] + 16 * ks + 8 * term, dv + (((ks >> 2) * (HD * 128) + (ks & 3) * 32) >> 4), idesc_f16(HD), (uint32_t)(on || term + ks > 0));
-                    umma_commit(&sh.o_full[t]);
-                    if (t == last) umma_commit(&sh.v_free[i % Shape::kVs]);
-                };
-                bool ok = mbar_wait(&sh.f16_full[0], 0);
-                tc_fence_after();
-                for (int t = 0; t < n_tiles && ok; t++) scores(t);
-                for (int i = 0; i < n && ok; i++) {
-                    const bool more = i + 1 < n;
-                    ok = mbar_wait(&sh.f16_full[1], i & 1);
-                    for (int t = 0; t < n_tiles && ok; t++) {
-                        ok = mbar_wait(&sh.p_full[t], i & 1);
-                        tc_fence_after();
-                        if (!ok) break;
-                        sums(t, i);
-                        if (more) {
-                            if (t == 0) ok = mbar_wait(&sh.f16_full[0], (i + 1) & 1);
-                            if (!ok) break;
-                            tc_fence_after();
-                            scores(t);
-                        }
+                    for (int ks = 0; ks < HD / 16; ks++) {
+                        const uint64_t off = ((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4;
+                        mma_ss_by(one, d, dq + off, dk + off, idesc_f16(kKeys), term < TERMS - 1 || ks > 0);
                     }
                 }
-                if (!ok) sh.dead = 1;
+                if (one) umma_commit(&sh.s_full[t]);
+                __syncwarp();
+            };
+            auto sums = [&](int t, int i) {
+                const uint32_t d = base + 256 + 128 * t, p = base + 128 * t;
+                const uint64_t dv = umma_desc_sw128(v_at + (i % Shape::kVs) * Shape::kV);
+                const uint32_t on = !SPLIT && i > 0;
+#pragma unroll
+                for (int term = TERMS - 1; term >= 0; term--)
+#pragma unroll
+                    for (int ks = 0; ks < kKeys / 16; ks++)
+                        mma_ts_by(one, d, p + 16 * ks + 8 * term, dv + (((ks >> 2) * (HD * 128) + (ks & 3) * 32) >> 4), idesc_f16(HD), term < TERMS - 1 || ks > 0 ? 1u : on);
+                if (one) {
+                    umma_commit(&sh.o_full[t]);
+                    if (t == last) umma_commit(&sh.v_free[i % Shape::kVs]);
+                }
+                __syncwarp();
+            };
+            bool ok = __all_sync(0xffffffffu, mbar_wait(&sh.f16_full[0], 0));
+            tc_fence_after();
+            for (int t = 0; t < n_tiles && ok; t++) scores(t);
+            for (int i = 0; i < n && ok; i++) {
+                const bool more = i + 1 < n;
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.f16_full[1], i & 1));
+                for (int t = 0; t < n_tiles && ok; t++) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[t], i & 1));
+                    tc_fence_after();
+                    if (!ok) break;
+                    sums(t, i);
+                    if (more) {
+                        if (t == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.f16_full[0], (i + 1) & 1));
+                        if (!ok) break;
+                        tc_fence_after();
+                        scores(t);
+                    }
+                }
             }
-            __syncwarp();
+            if (!ok) sh.dead = 1;
         } else if (warp == 13) {
             // -------------------------------------------------------------------------------------------------- copies
             const int32_t* table = seqs.table + (size_t)seq * seqs.width;
@@ -622,12 +638,21 @@ int32_t tiles_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, co
 
 bool kv8_tiles_apply(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, TilePlan* plan) {
     const int64_t rows = (int64_t)group * max_rows;
-    if (pool.hd > 128 || rows < 64) return false;
     const int64_t units = ((int64_t)seqs.n_rows * group / kTileRows2 + seqs.n_seqs) * pool.n_kv;
-    if (units > 1 << 20) return false;
+    const int64_t tiles = (((int64_t)seqs.width << pool.page_shift) + kKeys - 1) / kKeys;  // of a sequence's keys, at most
+    if (pool.hd > 128 || units > 1 << 20) return false;
+    // Runs or tiles, us in runs / in tiles (32 heads over 8 kv heads of 128 unless said).  16-bit types: one sequence behind 4,000 tokens with 8 rows (tokens x heads of a
+    // group) 22.7 / 24.1, 32 rows 35 / 25, 256 rows 44 / 36; 16 sequences of 32 rows behind 2,000 43.6 / 47.7, 64 of 64 rows behind 1,000 116.5 / 119, of 128 rows (4 kv heads of
+    // 64) 86 / 50.  f32: one of 64 rows 39.5 / 34, of 512 78 / 58, with one kv head of 512 rows 39 / 47; 64 sequences of 64 rows 154 / 176, of 128 rows 94 / 73.
+    if (typ == LC_TYPE_F32) {
+        if (units < 16 || rows < (units > sm_count() ? 128 : 64)) return false;
+    } else if (rows < (seqs.n_seqs * pool.n_kv * tiles <= 4 * sm_count() ? 32 : 64)) {  // fewer rows waste a tile: they only may where there is little to do
+        return false;
+    }
+    // fewer units than SMs: their keys are cut, into parts of at least four tiles where contexts are as long as the table
     plan->units = (int)units;
-    plan->splits = 1;
-    plan->bytes = 16;
+    plan->splits = (int)std::max<int64_t>(1, std::min<int64_t>({sm_count() / units, (tiles + 3) / 4, 64}));
+    plan->bytes = plan->splits > 1 ? (size_t)units * plan->splits * kTileRows2 * ((pool.hd <= 64 ? 64 : 128) + 2) * sizeof(float) : 16;
     return true;
 }
 
