@@ -3,12 +3,13 @@
 // A cached element is an integer times the scale of its page and head, so both products are taken of the integers as they are, and the scales are applied outside.
 //   Scores  on the matrix unit's integers (mma.sync m16n8k32, exact): a row of queries is whole numbers in units of its largest / 32,512 (f32: / 8,323,072), and
 //           these are digits of 8 bits, in rows of their own of the operand, so that keys go in as they lie in the cache.  16 bits are as good as f16 or bf16
-//           queries ask for: a score of size 1 is off by 3e-5; 24 bits for f32.
+//           queries ask for: a score of size 1 is off by 3e-5; 24 bits for f32.  Rows whose largest element is above 32 times the mean get a digit more.
 //   Values  an integer of 8 bits is exact in f16 (m16n8k16, f32 out): values are the operand of 16 rows (dims) and weights that of 8 columns (rows of queries), which the
 //           scores' layout already is.  The weights are 2^(s - max + 6) in f16, 2^-11 of each off, times their page's scale over a reference that follows the scales, so that sums stay
 //           in the matrix unit's accumulators.  For f32 they are the f16 value and what its rounding lost, 22 bits together, in two products; a step's sums are multiplied by the page's
 //           scale and added in f32, so that what the matrix unit cuts off when it adds stays within 16 keys.
 #include <algorithm>
+#include <type_traits>
 #include "lc_kv8.cuh"
 #include "lc_kernels.h"
 #include "lc_kv8_attn.cuh"
@@ -76,6 +77,56 @@ template <int HD, int NG, bool F32> struct RunShape {
     static constexpr int kByMemory = (220 << 10) / (kRunWarps * kWarp + 2048);
     static constexpr int kBlocks = kByRegisters < kByMemory ? kByRegisters : kByMemory;
 };
+
+// The unit of a row's numbers, of its scaled largest element.
+template <bool F32> __device__ __forceinline__ float query_unit(float top) { return top > 0.0f ? top * (F32 ? 1.0f / 8323072.0f : 1.0f / 32512.0f) : 1.0f; }
+
+// What the scores of 16 keys gain by the digit behind the units, in units: keys 2c, 2c + 1 and 8 + 2c, 9 + 2c of row g.  hd: 0 for no row.  Few rows need it, so it is taken
+// from the queries again.
+template <int HD, bool F32>
+__device__ __forceinline__ float4 next_digit(const void* q, int64_t src, int typ, bool vec, int hd, const unsigned char* kp) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    float v[HD / 64][16], top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < HD / 64; j++) {
+        const int d = 64 * j + 16 * c;
+        if (d < hd) load16(q, src + d, typ, vec, v[j]);
+        else
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[j][e] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = max_nan(top, fabsf(v[j][e]));
+    }
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float up, down;
+    row_scale(top, up, down);
+    const float per = 1.0f / query_unit<F32>(top * up);
+    int dot[2][4] = {};
+#pragma unroll
+    for (int j = 0; j < HD / 64; j++) {
+        uint32_t f[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            int n[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float u = v[j][4 * x + e] * up * per;  // as above
+                n[e] = min(127, __float2int_rn((u - rintf(u)) * 256.0f));
+            }
+            f[x] = pack4(n[0], n[1], n[2], n[3]);
+        }
+#pragma unroll
+        for (int tl = 0; tl < 2; tl++) {
+            const int row = 8 * tl + g, ch = 4 * j + c;
+            const uint4 kw = *reinterpret_cast<const uint4*>(kp + row * HD + ((ch ^ ((row & 1) << 2)) & (HD / 16 - 1)) * 16);
+            mma_s8(dot[tl], f[0], 0u, f[1], 0u, kw.x, kw.y);
+            mma_s8(dot[tl], f[2], 0u, f[3], 0u, kw.z, kw.w);
+        }
+    }
+    return make_float4((float)dot[0][0] / 256.0f, (float)dot[0][1] / 256.0f, (float)dot[1][0] / 256.0f, (float)dot[1][1] / 256.0f);
+}
+
 template <int HD, int NG, bool F32, bool FULL>
 __global__ void __launch_bounds__(kRunWarps * 32, RunShape<HD, NG, F32>::kBlocks)
 kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
@@ -160,8 +211,9 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
         // the queries as operand fragments: step ks = 2 j + x of the scores takes dims 64 j + 16 c + 8 x .. + 7.  A group's first tile has the highest digit in rows
         // 0 .. 7 and the next in rows 8 .. 15, its second tile the lowest in rows 0 .. 7.
         uint32_t qf[Shape::kQueriesShared ? 1 : NG * ND * KS][4];
-        float rf[NG];
+        float rf[NG];                        // exponent of a unit of the queries' numbers
         int limit[NG];                       // last position that the row sees (-1: no row)
+        bool fine = false;                   // some row's numbers get a digit more
 #pragma unroll
         for (int group = 0; group < NG; group++) {
                 const int r = 8 * group + g;
@@ -169,7 +221,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 const int tok = has ? (row_lo + r) / a.group : 0, hq = has ? (row_lo + r) - tok * a.group : 0;
                 const int64_t src = (int64_t)(w.first + tok) * a.q_stride + (int64_t)(at.kvh * a.group + hq) * hd;
                 limit[group] = has ? w.ctx + tok : -1;
-                float v[HD / 64][16], top = 0.0f;
+                float v[HD / 64][16], top = 0.0f, all = 0.0f;
 #pragma unroll
                 for (int j = 0; j < HD / 64; j++) {
                     const int d = 64 * j + 16 * c;
@@ -178,13 +230,16 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
 #pragma unroll
                         for (int e = 0; e < 16; e++) v[j][e] = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) top = max_nan(top, fabsf(v[j][e]));
+                    for (int e = 0; e < 16; e++) { top = max_nan(top, fabsf(v[j][e])); all += fabsf(v[j][e]); }
                 }
+                all += __shfl_xor_sync(0xffffffffu, all, 1);
+                all += __shfl_xor_sync(0xffffffffu, all, 2);
                 top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 float up, down;
                 row_scale(top, up, down);
-                const float unit = top > 0.0f ? top * up * (F32 ? 1.0f / 8323072.0f : 1.0f / 32512.0f) : 1.0f, per = 1.0f / unit;
+                const float unit = query_unit<F32>(top * up), per = 1.0f / unit;
+                fine = fine || top * (float)hd > 32.0f * all;
                 rf[group] = top < INFINITY ? a.scale_log2 * down * unit : __int_as_float(0x7fffffff);  // not finite: the row is NaN
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
@@ -231,6 +286,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
 
         // rows see all keys up to the first row's position (with a window, from the last row's on)
         const int sees = w.ctx + row_lo / a.group, from = a.window > 0 ? w.ctx + (row_lo + row_n - 1) / a.group - a.window : -1;
+        auto steps = [&](auto finer) {
         for (int st = s0; st < s1; st++) {
             cp_async_wait<S - 2>();
             __syncwarp();
@@ -281,6 +337,15 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                             const float high = (float)(256 * dot[gr * ND][tl][k] + dot[gr * ND][tl][2 + k]);
                             s[gr][tl][k] = F32 ? fmaf(high, 256.0f, (float)dot[gr * ND + ND - 1][tl][k]) : high;
                         }
+            }
+            if (decltype(finer)::value) {
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) {
+                    const int r = 8 * gr + g, rr = r < row_n ? r : 0, tok = (row_lo + rr) / a.group;
+                    const int64_t src = (int64_t)(w.first + tok) * a.q_stride + (int64_t)(at.kvh * a.group + row_lo + rr - tok * a.group) * hd;
+                    const float4 more = next_digit<HD, F32>(a.q, src, a.typ, a.q_vec, r < row_n ? hd : 0, kp);
+                    s[gr][0][0] += more.x; s[gr][0][1] += more.y; s[gr][1][0] += more.z; s[gr][1][1] += more.w;
+                }
             }
             float to_weight = 1.0f;
             if (!F32) {
@@ -393,6 +458,10 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                     }
             }
         }
+        };
+        // the loop twice, as the digit's values took other calls' registers in one (64 tokens on 32 sequences: 161 us instead of 152)
+        if (__any_sync(0xffffffffu, fine)) steps(std::true_type{});
+        else steps(std::false_type{});
         cp_async_wait<0>();
 
         const bool starts = s0 == 0, ends = s1 == w.steps;
@@ -540,7 +609,7 @@ int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, con
 int32_t check_heads(const char* call, const Kv8Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {
     LC_CHECK(n_heads > 0 && n_heads <= 65536 && n_heads % pool.n_kv == 0, LC_ERR_INVALID, "%s: %d heads over %d kv heads", call, n_heads, pool.n_kv);
     // places of the line, row blocks of 8 at worst, in 31 bits
-    const double chunks = (double)((int64_t)seqs.width << pool.page_shift) / kStep + 2, blocks = (double)seqs.n_rows * (n_heads / pool.n_kv) / 8 + seqs.n_seqs;
+    const double chunks = (double)((int64_t)seqs.width << pool.page_shift) / kStep + 2 + kUnitCost, blocks = (double)seqs.n_rows * (n_heads / pool.n_kv) / 8 + seqs.n_seqs;
     LC_CHECK(chunks * blocks * pool.n_kv < 2147483648.0, LC_ERR_INVALID, "%s: %d rows of %d heads over tables of %d pages are too many for one call", call, seqs.n_rows, n_heads, seqs.width);
     return LC_OK;
 }

@@ -230,6 +230,18 @@ def test_attention_queries_of_any_size(gpu, q_scale):
     check_attention(s, 4, "bfloat16", q_scale=q_scale, scale=0.125 / q_scale)
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("heads,kv,dim,new", [(4, 4, 128, 1), (8, 1, 64, 3), (4, 1, 256, 2), (4, 2, 96, 70)])
+def test_attention_queries_with_an_outlier(gpu, dtype, heads, kv, dim, new):
+    """One element of the queries a thousand times the others, where the keys are zero: the others' part of the scores keeps its bits."""
+    s = Setup(gpu, [(200, new), (31, new)], kv, dim, 16, seed=16)
+    s.plain.k[..., 5] = 0
+    s.pools[0].copy_(torch.from_numpy(s.plain.k))
+    q, q64 = s.normal(heads, dtype)
+    q[..., 5], q64[..., 5] = 1000.0, 1000.0
+    check_attention(s, heads, dtype, q=(q, q64))
+
+
 def test_attention_of_zero_queries_and_zero_pages(gpu):
     s = Setup(gpu, [(60, 3)], 2, 64, 16, seed=6)
     for pool, scale in ((s.plain.k, s.plain.k_scale), (s.plain.v, s.plain.v_scale)):
@@ -339,6 +351,49 @@ def test_bad_pages_and_rows_are_kept_out(gpu, dtype, new):
     b = gpu.Kv8Rows(cuda(table), cuda(ctx), cuda(good.start), new)
     good.cache.attention(b, q)
     torch.cuda.synchronize()
+
+
+def test_first_calls_of_a_process_inside_a_capture(gpu):
+    """No call needs a run outside the capture first."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, leafcutterllm_b200 as lc
+i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+k, v = (torch.zeros(8, 2, 16, 128, dtype=torch.int8, device="cuda") for _ in range(2))
+cache = lc.Kv8Cache(k, v, torch.zeros(8, 2, device="cuda"), torch.zeros(8, 2, device="cuda"))
+table = torch.arange(8, dtype=torch.int32, device="cuda").reshape(1, 8)
+turns = torch.from_numpy(lc.rope_turns(10000.0, 128).view("int64")).cuda()
+q, x = torch.randn(80, 4, 128, device="cuda").bfloat16(), torch.randn(80, 2, 128, device="cuda").bfloat16()
+tokens = torch.zeros(80, dtype=torch.int64, device="cuda")
+one, many = lc.Kv8Rows(table, i32(80), i32(0, 1), 1), lc.Kv8Rows(table, i32(0), i32(0, 80), 80)
+ws = [torch.empty(cache.attention_workspace(r, y), dtype=torch.uint8, device="cuda") for r, y in ((many, q), (one, q[:1]))]
+out, out1, ro, kx = torch.empty_like(q), torch.empty_like(q[:1]), torch.empty_like(q), torch.empty_like(x)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    cache.append(many, x, x, turns=turns, q=q, q_out=ro)
+    cache.attention(many, ro, out, workspace=ws[0])
+    cache.append(one, x[:1], x[:1], turns=turns)
+    cache.attention(one, ro[:1], out1, workspace=ws[1])
+    cache.read(many, kx)
+    lp = lc.token_logprobs_dev(out.reshape(80, -1), tokens, top=2)
+g.replay()
+torch.cuda.synchronize()
+first = [t.clone() for t in (out, out1, kx, *lp)]
+cache.append(many, x, x, turns=turns, q=q, q_out=ro)
+cache.attention(many, ro, out, workspace=ws[0])
+cache.append(one, x[:1], x[:1], turns=turns)
+cache.attention(one, ro[:1], out1, workspace=ws[1])
+cache.read(many, kx)
+lp = lc.token_logprobs_dev(out.reshape(80, -1), tokens, top=2)
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) and bool(torch.isfinite(a.float()).all()) for a, b in zip(first, (out, out1, kx, *lp)))
+print("same")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr
 
 
 def test_streams_and_graphs(gpu):
