@@ -140,7 +140,7 @@ int32_t lc_attention_decode_static(const float* q_dev, const void* k_pool_dev, c
 /* ---- A key/value cache in 8 bits (no counterpart in the reference, whose cache is f16: rust/src/cache/mod.rs:33-61) ----
  * The pools hold integers of 8 bits, [page][kv head][page_tokens][head_dim], 16-byte aligned; the scales are f32, [page][kv head],
  * one for the keys and one for the values.  A cached element is its integer times the scale of its page and head.
- * page_tokens: 16, 32, 64, 128 or 256; head_dim: a multiple of 16, 256 at most; the pools may pass 2^32 bytes. */
+ * The scales are 0 or more.  page_tokens: 16, 32, 64, 128 or 256; head_dim: a multiple of 16, 256 at most; the pools may pass 2^32 bytes. */
 typedef struct lc_kv8_cache {
     void* k_dev;
     void* v_dev;
@@ -156,7 +156,9 @@ typedef struct lc_kv8_cache {
  * sequences have more is slower, not wrong.
  * status_dev (may be NULL): a word that a call raises to i + 1, for the highest such i, where sequence i cannot be served: its row_start is
  * not ascending within the call's rows (its rows are left alone), or its positions leave the table or a page that it needs is not
- * in 0 .. n_pages - 1 (appends skip that page, reads and attention give NaN in those rows).  No call clears it.
+ * in 0 .. n_pages - 1.  Appends skip that page (a sequence that leaves the table: all of its rows, queries too), reads and attention give NaN in those
+ * rows.  Where a row_start that goes back and forth gives rows to several sequences, those rows may hold any of their results; what the rows of
+ * others hold, and memory outside the call's tensors, is as it would be.  No call clears the word.
  * n_seqs: 4096 at most. */
 typedef struct lc_kv8_rows {
     const int32_t* page_table_dev; /* [n_seqs][table_width] */
@@ -175,7 +177,7 @@ typedef struct lc_kv8_rows {
  * own fills such a table itself.  Positions times entries wrap around, so far positions lose nothing. */
 int32_t lc_rope_turns(double theta, int32_t rot_dim, uint64_t* out);
 /* Appends rows of keys and values, each [n_rows][n_kv_heads][head_dim], at their positions, the keys rotated by turns_dev (rot_dim / 2
- * entries; rot_dim 0: no rotation).  Rotations and quotients are taken in 64 bits.  Per page and head that receives rows: the scale becomes the largest finite
+ * entries; rot_dim 0: no rotation).  Integers and scales are those of rotations and quotients in 64 bits; rotated queries are within 2^-23 of theirs, and rounded to typ.  Per page and head that receives rows: the scale becomes the largest finite
  * magnitude among the new rows / 127 (rounded to f32) or, where the page already holds rows of the sequence, the larger of that and the scale before; if it grows,
  * the integers of the earlier rows are rounded once more, to the new scale.  New integers are round(x / scale) to the nearest even, infinities
  * become +-127 and NaN 0 (all 0 where the scale is 0).  Slots behind the last row keep what they hold.
@@ -189,7 +191,8 @@ int32_t lc_kv8_read_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows, uint
                         int64_t k_stride, void* v_out_dev, int64_t v_stride, void* stream);
 /* Attention of the rows over the cache (the core of rust/src/inference/attention.rs:69-113, as lc_attention_decode_dev): each row of q_dev
  * [n_rows][n_heads][head_dim], already rotated, attends to the positions up to its own, which the cache already holds (append first), and
- * with window > 0 only to the last `window` of them.  Scores are q . k * scale (0: 1 / sqrt(head_dim)).  Queries of any finite size are taken.
+ * with window > 0 only to the last `window` of them.  Scores are q . k * scale (0: 1 / sqrt(head_dim); 2e38 at most).  Queries of any finite size are taken; a
+ * row with one that is not finite gives NaN.  Softmax and sums are in f32, its weights in 11 bits (f32: 22).  The values' scales of a sequence and head may differ by factors up to 2^100.
  * The workspace is the caller's: lc_attention_kv8_workspace says how many bytes, for any contexts and any rows of at most
  * these arguments' sizes; it needs no initial value and keeps nothing between calls.  Calls that may run at the same time (graphs that may be replayed at the
  * same time among them) need a workspace each. */

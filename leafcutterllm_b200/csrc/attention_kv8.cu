@@ -167,7 +167,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
         t += (uint32_t)(end - at.in);
         if (s1 <= s0) continue;  // the unit's steps are the next run's
         if (s0 == 0 && s1 < w.steps && lane == 0) {
-            a.records[run].last = (int)runs.run_of(t + (uint32_t)(w.steps - s1) - 1);
+            a.records[run].last = (int)min(runs.run_of(t + (uint32_t)(w.steps - s1) - 1), runs.n - 1);
             *reinterpret_cast<int4*>(&a.records[run]) = make_int4(w.first, at.kvh, at.rb * RB, min(RB, w.n * a.group - at.rb * RB));
         }
         const int32_t* table = seqs.table + (size_t)at.seq * seqs.width;
@@ -644,7 +644,7 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
     LC_TRY(kv8_check("lc_attention_kv8_dev", cache, rows, typ, n_rows, &pool, &seqs));
     LC_TRY(check_heads("lc_attention_kv8_dev", pool, seqs, n_heads));
     LC_CHECK(window >= 0, LC_ERR_INVALID, "lc_attention_kv8_dev: window=%d", window);
-    LC_CHECK(scale >= 0.0f && scale <= 3.0e38f, LC_ERR_INVALID, "lc_attention_kv8_dev: scale=%g", scale);
+    LC_CHECK(scale >= 0.0f && scale <= 2.0e38f, LC_ERR_INVALID, "lc_attention_kv8_dev: scale=%g", scale);
     if (n_rows == 0 || seqs.n_seqs == 0) return LC_OK;
     LC_CHECK(q_dev && out_dev, LC_ERR_INVALID, "lc_attention_kv8_dev: null queries or output");
     LC_CHECK(q_stride >= (int64_t)n_heads * pool.hd && out_stride >= (int64_t)n_heads * pool.hd, LC_ERR_INVALID, "lc_attention_kv8_dev: rows overlap");
@@ -660,7 +660,7 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
     if (scale == 0.0f) scale = 1.0f / sqrtf((float)pool.hd);
     window = std::min(window, 1 << 30);  // the kernels' differences of positions stay in 32 bits
     const size_t elem = typ == LC_TYPE_F32 ? 4 : 2;
-    AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, n_heads, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16),
+    AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16),
                scale * 1.44269504088896f, nullptr, (UnitRecord*)workspace_dev};
     a.part = by_tiles ? (float*)workspace_dev : (float*)((char*)workspace_dev + (size_t)plan.blocks * kRunWarps * sizeof(UnitRecord));
     cudaStream_t s = stream_or_own(stream_);

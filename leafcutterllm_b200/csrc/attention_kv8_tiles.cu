@@ -5,7 +5,7 @@
 //   warps 0-3, 4-7   the softmax of row tile 0, 1: a row per thread, scores and sums in tensor memory;
 //   warp 13          copies the next keys and values from the cache into shared memory (bulk copies of 16 keys);
 //   warps 8-11, 14, 15   unpack them to f16 (K as [key][dim], V as [dim][key], 128-byte swizzle);
-//   warp 12          one thread issues the products.  With the unpacking in the same warp an iteration took 9,500 cycles instead of 4,000: the issue waits
+//   warp 12          one thread issues the products.  With the unpacking in the same warps an iteration took 9,500 cycles instead of 4,000: the issue waits
 //                    for the matrix unit's queue.
 // Scores: S = Q K^T, the queries times one power of two for the whole unit; f32 queries as f16 high and low parts, two products.
 // Weights: with f the key's scale factor (scale log2 e S_k) and S_v of the key's page, P_j = 2^(s_j f_j + log2 S_v,j - M + 6), M the row's largest exponent so far: the
@@ -47,7 +47,6 @@ struct TileShared {
     GroupConst consts[kSlots][kGroups];
     uint2 sums[kTileThreads / 32];
     uint32_t tmem;
-    int dead;
     float top;
 };
 
@@ -153,7 +152,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         for (int t = 0; t < kSlots; t++) mbar_init(&sh.c_full[t], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
-        sh.dead = 0;
         sh.top = 0.0f;
     }
     if (warp == 0) tmem_alloc(&sh.tmem, 512);
@@ -268,8 +266,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                     }
                 }
             }
-            if (!ok) sh.dead = 1;
-        } else if (warp == 13) {
+        } else {
             // -------------------------------------------------------------------------------------------------- copies
             const int32_t* table = seqs.table + (size_t)seq * seqs.width;
             const int page_mask = (1 << pool.page_shift) - 1;
@@ -318,10 +315,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                 }
                 page = next;
             }
-            if (!ok) {  // whatever is under way lands before the block ends
-                sh.dead = 1;
+            if (!ok)  // whatever is under way lands before the block ends
                 for (int x = 0; x < 2; x++) (void)mbar_wait(&sh.raw_full[x], 0), (void)mbar_wait(&sh.raw_full[x], 1);
-            }
         }
       } else {
         // ---------------------------------------------------------------------------------------------------- unpacking
@@ -390,7 +385,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             __syncwarp();
             if (lane == 0) { mbar_arrive(&sh.f16_full[1]); mbar_arrive(&sh.raw_free[1]); }
         }
-        if (!ok) sh.dead = 1;
       }
     } else {
         // ------------------------------------------------------------------------------------------------------ softmax
@@ -542,7 +536,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                 for (int d = 0; d < HD; d++) o[d] = 0.0f;
             }
             if (ok) add_up(n - 1);
-            if (!ok) sh.dead = 1;
             if (!ok || isnan(l)) l = __int_as_float(0x7fffffff);
             if (!ok && lane == 0) kv8_raise(seqs, seq);
             if (r < row_n) {

@@ -4,8 +4,8 @@
 // An append gives a page and head the scale S = max(S_before, f32(A / 127)), A the largest finite magnitude of its new rows, S_before that of
 // the rows that the page already holds (none: 0).  Those are rounded again where S grew: q <- rint(q S_before / S); new rows: q = rint(x / S).
 //
-// The keys' rotation, the quotients and their rounding are done in 64 bits: an integer then depends on the definition alone and not on how
-// a kernel orders its arithmetic, so that every implementation holds the same cache.  The angle comes from a table of turns per
+// The keys' rotation, the quotients and their rounding are defined in 64 bits: an integer then depends on the definition alone and not on how
+// a kernel orders its arithmetic, so that every implementation holds the same cache.  (f32 stands in for them where its bounds decide an integer.)  The angle comes from a table of turns per
 // position, as 64-bit fractions of a turn: position * entry wraps around by itself, and what is left is the angle's fraction of a turn
 // to 2^-64 of one, however far the position is (cos and sin of an f32 angle lose 2^-24 of the ANGLE: 0.06 at 10^6).
 //
@@ -178,7 +178,7 @@ struct Group {
 //           largest in 64 bits;
 //   kInts   integers: x / S in f32 is within 2e-4 of the quotient (rotation 2^-22 of at most 180 S, product and inverse 2^-22 of 127.5), so that it gives the integer of
 //           the 64-bit quotient unless it lies so near a half; eight elements with such a one among them, one group in 300, are taken in 64 bits.
-// Rows with infinities or NaN, which the first maximum shows, and scales below 1e-30 go the long way, all in 64 bits.  5,000 rows of eight heads, bf16, 5 prompts: 171 us with
+// Rows with infinities or NaN, which the first maximum shows, and maxima and scales below 1e-30 go the long way, all in 64 bits.  5,000 rows of eight heads, bf16, 5 prompts: 171 us with
 // everything in 64 bits and an element per lane, 31 now (a table of rotations 2.3 of a block's 12, each pass 2 to 4: their instructions).
 //
 enum : int { kMost, kFine, kInts };
@@ -340,6 +340,7 @@ __device__ __forceinline__ void append_kv(const Kv8Pool& pool, const AppendArgs&
         if (VEC) {
             it.slow = __any_sync(0xffffffffu, !(it.most < INFINITY));
             it.most = warp_max(it.most);
+            it.slow = it.slow || it.most < 1e-30f;  // what follows of f32's relative errors does not hold next to its smallest numbers
             it.least = it.most * (1.0f - 0x1p-19f);
             it.top = it.slow || turn ? 0.0 : (double)it.most;
         }

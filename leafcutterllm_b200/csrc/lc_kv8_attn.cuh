@@ -9,7 +9,7 @@ struct AttnArgs {
     const void* q;
     void* out;
     int64_t q_stride, out_stride;
-    int typ, n_heads, group, window;
+    int typ, group, window;
     bool q_vec, out_vec;             // 16-byte accesses
     float scale_log2;                // scale * log2(e)
     float* part;                     // partial results of runs that end inside a unit
@@ -155,6 +155,8 @@ __device__ __forceinline__ SeqWork seq_work(const Kv8Seqs& s, const Kv8Pool& p, 
     }
     return w;
 }
+// Sums that stop at 2^31 - 1: the calls' checks keep those of ascending rows below it, and rows given to several sequences must not make a place of the line another's.
+__device__ __forceinline__ uint32_t add_places(uint32_t a, uint32_t b) { return min(a + b, 0x7fffffffu); }
 // cum[i] = the line's places before sequence i (kUnitCost and its steps for every unit), cum[n_seqs] = all; units[i] (if wanted) the units before i; by one block, returns the total
 template <int RB>
 __device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, const AttnArgs& a, uint32_t* cum, uint32_t* units, uint2* warp_sums) {
@@ -164,27 +166,28 @@ __device__ __forceinline__ uint32_t line_up(const Kv8Seqs& s, const Kv8Pool& p, 
         const SeqWork w = seq_work<RB>(s, p, a, i);
         cum[i] = sum;
         if (units) units[i] = usum;
-        sum += (uint32_t)w.blocks * (uint32_t)p.n_kv * (uint32_t)(w.steps + kUnitCost);
-        usum += (uint32_t)w.blocks * (uint32_t)p.n_kv;
+        sum = add_places(sum, (uint32_t)w.blocks * (uint32_t)p.n_kv * (uint32_t)(w.steps + kUnitCost));
+        usum = add_places(usum, (uint32_t)w.blocks * (uint32_t)p.n_kv);
     }
     uint32_t incl = sum, uincl = usum;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, uincl, o);
-        if (lane >= o) { incl += v; uincl += u; }
+        if (lane >= o) { incl = add_places(incl, v); uincl = add_places(uincl, u); }
     }
     if (lane == 31) warp_sums[warp] = make_uint2(incl, uincl);
     __syncthreads();
-    uint32_t before = incl - sum, ubefore = uincl - usum, total = 0, utotal = 0;
+    uint32_t before = __shfl_up_sync(0xffffffffu, incl, 1), ubefore = __shfl_up_sync(0xffffffffu, uincl, 1), total = 0, utotal = 0;
+    if (lane == 0) before = ubefore = 0;
     for (int w = 0; w < (int)(blockDim.x >> 5); w++) {
         const uint2 v = warp_sums[w];
-        if (w < warp) { before += v.x; ubefore += v.y; }
-        total += v.x;
-        utotal += v.y;
+        if (w < warp) { before = add_places(before, v.x); ubefore = add_places(ubefore, v.y); }
+        total = add_places(total, v.x);
+        utotal = add_places(utotal, v.y);
     }
     for (int i = i0; i < i1; i++) {
-        cum[i] += before;
-        if (units) units[i] += ubefore;
+        cum[i] = add_places(cum[i], before);
+        if (units) units[i] = add_places(units[i], ubefore);
     }
     if (threadIdx.x == 0) {
         cum[s.n_seqs] = total;

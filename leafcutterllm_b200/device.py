@@ -2,7 +2,7 @@
 
 The counterparts of the `_dev` calls of include/leafcutter_b200.h for torch tensors.  A call queues its kernels on torch's current
 stream of the tensors' device (or on `stream`: a torch stream or a cudaStream_t as an integer) and returns without waiting; it allocates nothing but
-what it is not given, from torch's allocator, so it can be captured into a graph.  Shapes, types and devices are checked
+what it is not given, from torch's allocator and as that stream's memory (a stream given as a number: nothing), so it can be captured into a graph.  Shapes, types and devices are checked
 here, everything else by the library (LeafcutterError).  Nothing of the reference's corresponds to them.
 """
 from __future__ import annotations
@@ -32,6 +32,17 @@ def _stream(index, stream):
     """A cudaStream_t: the current stream of device `index` where none is given.  Handle 0 is the legacy stream there; the library takes 0 for its own."""
     handle = _raw_stream(index) if stream is None else getattr(stream, "cuda_stream", stream)
     return handle or 1  # cudaStreamLegacy
+
+
+def _empty(call, like, shape, dtype, stream):
+    """A tensor on the device of `like`, from the memory of the stream that will write it: the current stream's may still be at work on what it frees."""
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if not hasattr(stream, "cuda_stream"):
+        raise ValueError(f"{call}: a stream given as a number needs outputs and workspaces of the caller's")
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=like.device)
 
 
 def _typ(t):
@@ -127,7 +138,7 @@ class Kv8Cache:
         qp = qs = op = os = heads = tp = rot = 0
         if q is not None:
             if q_out is None:
-                q_out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+                q_out = _empty("append", q, q.shape, q.dtype, stream)
             heads = q.shape[1]
             if q.dtype != k.dtype or q_out.dtype != k.dtype or q.shape[0] != n or q_out.shape[0] != n:
                 raise ValueError("append: queries of the keys' type and as many rows expected, q_out like q")
@@ -177,16 +188,12 @@ class Kv8Cache:
         qs = _rows(q, None, self.head_dim, "q")
         n, heads = q.shape[:2]
         if out is None:
-            out = _torch().empty(q.shape, dtype=q.dtype, device=q.device)
+            out = _empty("attention", q, q.shape, q.dtype, stream)
         if out.dtype != q.dtype or out.shape[0] != n:
             raise ValueError("attention: out like q expected")
         os = _rows(out, heads, self.head_dim, "out")
         if workspace is None:
-            torch = _torch()
-            if stream is not None and not hasattr(stream, "cuda_stream"):
-                raise ValueError("attention: a stream given as a number needs a workspace of the caller's")
-            with torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.device):
-                workspace = torch.empty(self.attention_workspace(rows, q), dtype=torch.uint8, device=self.device)
+            workspace = _empty("attention", q, self.attention_workspace(rows, q), _torch().uint8, stream)
         if rows.index != index or q.get_device() != index or out.get_device() != index or workspace.get_device() != index:
             _elsewhere(index, q, out, workspace)
         check(load().lc_attention_kv8_dev(self._ref, rows._ref, typ, n, q.data_ptr(), qs, heads, 0.0 if scale is None else scale, window, out.data_ptr(), os,
@@ -210,12 +217,12 @@ def token_logprobs_dev(logits, tokens, logprob=None, entropy=None, top_logprob=N
         raise ValueError("token_logprobs_dev: top_id is not `top` wide")
     top = top_id.shape[-1] if top_id is not None else top or 0
     if logprob is None:
-        logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        logprob = _empty("token_logprobs_dev", logits, rows, torch.float32, stream)
     if entropy is None:
-        entropy = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        entropy = _empty("token_logprobs_dev", logits, rows, torch.float32, stream)
     if top_id is None:
-        top_logprob = torch.empty(rows, max(top, 0), dtype=torch.float32, device=logits.device)
-        top_id = torch.empty(rows, max(top, 0), dtype=torch.int64, device=logits.device)
+        top_logprob = _empty("token_logprobs_dev", logits, (rows, max(top, 0)), torch.float32, stream)
+        top_id = _empty("token_logprobs_dev", logits, (rows, max(top, 0)), torch.int64, stream)
     _contiguous("token_logprobs_dev", torch.int64, tokens, top_id)
     _contiguous("token_logprobs_dev", torch.float32, logprob, entropy, top_logprob)
     one, wide = (rows,), (rows, top)

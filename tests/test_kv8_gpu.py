@@ -158,6 +158,52 @@ def test_append_of_zeros_infinities_and_nan(gpu):
     assert (host(s.pools[2])[s.table[1, 0]] == 0).all()
 
 
+@pytest.mark.parametrize("size", [1e-30, 1e-37, 3e-41, 2e-44])
+def test_append_next_to_the_smallest_numbers(gpu, size):
+    """Magnitudes where a relative error of f32 is not one: the integers and scales are still those of the definition."""
+    s = Setup(gpu, [(4, 30), (0, 2)], 2, 64, 16, seed=9)
+    turns = gpu.rope_turns(10000.0, 64)
+    (k, k64), (v, v64) = s.normal(2, "float32", size), s.normal(2, "float32", size)
+    s.cache.append(s.batch, k, v, turns=cuda(turns.view("int64")))
+    s.plain.append(s.table, s.ctx, s.start, k64, v64, turns)
+    s.same_cache()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new", [3, 40])
+def test_rows_given_to_several_sequences(gpu, dtype, new):
+    """A row_start that goes back and forth: the sequence that shares no rows has its results, and nothing else is written."""
+    s = Setup(gpu, [(20, new), (50, new), (9, new)], 2, 64, 16, tail=2)
+    start = np.array([0, new, 0, 0], np.int32)      # the second goes back, the third has no rows: all rows are the first's
+    q, q64 = s.normal(4, dtype)
+    out = torch.full_like(q, 7.0)
+    s.cache.attention(s.rows_of(new, start=start), q, out)
+    want, mass, big, keys = s.plain.attention(s.table, s.ctx[:1], start[:2], q64)
+    bound = plain.attention_bound(want, mass, big, keys, 64, dtype, dtype == "float32")
+    assert (np.abs(host(out).astype(np.float64) - want)[:new] <= bound[:new]).all() and (host(out)[new:] == 7.0).all()
+    assert s.status.item() == 2
+    start = np.array([0, new, 2 * new, 0], np.int32)    # the last goes back: left alone
+    s.status.zero_()
+    s.cache.attention(s.rows_of(new, start=start), q, out.fill_(7.0))
+    assert (host(out)[:2 * new] != 7.0).all() and (host(out)[2 * new:] == 7.0).all() and s.status.item() == 3
+
+
+def test_results_made_for_another_stream(gpu):
+    """Outputs and workspaces that a call makes for another stream are that stream's memory; a number for a stream makes none."""
+    s = Setup(gpu, [(30, 2)], 2, 64, 16)
+    (k, k64), (v, v64), (q, q64) = s.normal(2, "bfloat16"), s.normal(2, "bfloat16"), s.normal(4, "bfloat16")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    same = s.cache.append(s.batch, k, v, q=q, stream=side)
+    out = s.cache.attention(s.batch, q, stream=side)
+    side.synchronize()
+    assert torch.equal(same, q) and torch.equal(out, s.cache.attention(s.batch, q))
+    for call in (lambda: s.cache.append(s.batch, k, v, q=q, stream=side.cuda_stream), lambda: s.cache.attention(s.batch, q, torch.empty_like(q), stream=side.cuda_stream),
+                 lambda: s.cache.attention(s.batch, q, workspace=torch.empty(1 << 20, dtype=torch.uint8, device="cuda"), stream=side.cuda_stream)):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_rows_outside_the_sequences_are_left_alone(gpu):
     s = Setup(gpu, [(3, 2), (18, 1)], 2, 64, 16, lead=2, tail=3)
     turns = gpu.rope_turns(10000.0, 64)
