@@ -459,14 +459,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
 #pragma unroll
                             for (int e = 0; e < 16; e++)
                                 if (c + e > to || c + e < from) x[e] = __float_as_uint(kNegInf);
-                        float gs = 0.0f;
+                        const float2 f2 = make_float2(k.f, k.f), off2 = make_float2(off, off);
+                        float2 gs = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            const float p0 = exp2_fast(fmaf(__uint_as_float(x[e]), k.f, off)), p1 = exp2_fast(fmaf(__uint_as_float(x[e + 1]), k.f, off));
-                            gs += p0 + p1;
-                            h2_split(p0, p1, p[e / 2], q[e / 2]);
+                            const float2 y = fma2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, off2), v = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                            gs = add2(gs, v);
+                            h2_split(v.x, v.y, p[e / 2], q[e / 2]);
                         }
-                        sum = fmaf(gs, k.inv, sum);
+                        sum = fmaf(gs.x + gs.y, k.inv, sum);
                         tmem_st8(my_s + c, p);
                         tmem_st8(my_s + c + 8, q);
                     }
@@ -514,15 +515,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         uint32_t p[8];
                         const GroupConst k = gc[c / 16];
                         const float off = k.lv - ref + 6.0f;
-                        float g0 = 0.0f, g1 = 0.0f;
+                        const float2 f2 = make_float2(k.f, k.f), off2 = make_float2(off, off);
+                        float2 gs = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            const float p0 = exp2_fast(fmaf(__uint_as_float(x[c + e]), k.f, off)), p1 = exp2_fast(fmaf(__uint_as_float(x[c + e + 1]), k.f, off));
-                            g0 += p0;
-                            g1 += p1;
-                            p[e / 2] = h2_pack(p0, p1);
+                            const float2 y = fma2(make_float2(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])), f2, off2), v = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                            gs = add2(gs, v);
+                            p[e / 2] = h2_pack(v.x, v.y);
                         }
-                        sum = fmaf(g0 + g1, k.inv, sum);
+                        sum = fmaf(gs.x + gs.y, k.inv, sum);
                         tmem_st8(my_s + c, p);
                     }
                     l += sum;
