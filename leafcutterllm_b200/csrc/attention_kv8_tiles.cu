@@ -16,8 +16,10 @@
 //   16-bit types    O stays in tensor memory for all keys (the same error is a hundredth of the outputs' rounding), and so that it rarely
 //                   has to be scaled again, M is raised only when a row's largest exponent has grown by more than 8.
 //
-// What bounds it (a pair of row tiles x 128 keys, head dim 128): products 2,048 cycles (f32: 4,096), exponentials 2,048 on the special-function unit, and about
-// 2,500 issue cycles of softmax, sums and unpacking per scheduler.
+// What bounds it (a pair of row tiles x 128 keys, head dim 128): products 2,048 cycles (f32: 4,096), exponentials 2,048 on the special-function unit, and 320 KB through
+// shared memory, 2,500 cycles (128 of queries and keys, 64 of values for the products, 128 of copies and unpacking); about 3,900 pass, as a row tile's softmax, its sums
+// and its next scores wait for one another.  Steps of 64 keys, whose scores are under way while the 64 before are weighted, took 571 us instead of 412 (8 chunks): products half
+// as wide read the queries twice.
 #include <algorithm>
 #include "lc_kernels.h"
 #include "lc_kv8_attn.cuh"
@@ -42,8 +44,8 @@ struct TileShared {
     uint64_t s_full[2], p_full[2], o_full[2];  // scores, weights, sums of a row tile
     uint64_t c_full[kSlots];                   // consts of a key tile
     uint64_t raw_full[2], raw_free[2];         // copied keys, values
-    uint64_t f16_full[2];                      // unpacked keys, values; the keys' place is free when the last row tile's scores are done,
-    uint64_t v_free[2];                        // the values' when its sums are
+    uint64_t k_full, v_full[2];                // unpacked keys, values (a barrier for each place: the next tile's values may be there before this one's are waited for);
+    uint64_t v_free[2];                        // the keys' place is free when the last row tile's scores are done, the values' when its sums are
     GroupConst consts[kSlots][kGroups];
     uint2 sums[kTileThreads / 32];
     uint32_t tmem;
@@ -147,8 +149,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             mbar_init(&sh.p_full[t], 128);
             mbar_init(&sh.raw_full[t], 1);
             mbar_init(&sh.raw_free[t], kConvWarps);
-            mbar_init(&sh.f16_full[t], kConvWarps);
+            mbar_init(&sh.v_full[t], kConvWarps);
         }
+        mbar_init(&sh.k_full, kConvWarps);
         for (int t = 0; t < kSlots; t++) mbar_init(&sh.c_full[t], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
@@ -247,19 +250,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                 }
                 __syncwarp();
             };
-            bool ok = __all_sync(0xffffffffu, mbar_wait(&sh.f16_full[0], 0));
+            bool ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_full, 0));
             tc_fence_after();
             for (int t = 0; t < n_tiles && ok; t++) scores(t);
             for (int i = 0; i < n && ok; i++) {
                 const bool more = i + 1 < n;
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.f16_full[1], i & 1));
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_full[i % Shape::kVs], (i / Shape::kVs) & 1));
                 for (int t = 0; t < n_tiles && ok; t++) {
                     ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[t], i & 1));
                     tc_fence_after();
                     if (!ok) break;
                     sums(t, i);
                     if (more) {
-                        if (t == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.f16_full[0], (i + 1) & 1));
+                        if (t == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_full, (i + 1) & 1));
                         if (!ok) break;
                         tc_fence_after();
                         scores(t);
@@ -346,7 +349,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             }
             fence_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(&sh.f16_full[0]); mbar_arrive(&sh.raw_free[0]); }
+            if (lane == 0) { mbar_arrive(&sh.k_full); mbar_arrive(&sh.raw_free[0]); }
 
             ok = mbar_wait(&sh.raw_full[1], i & 1);
             if (i >= Shape::kVs) ok = ok && mbar_wait(&sh.v_free[i % Shape::kVs], (i / Shape::kVs - 1) & 1);  // the values' place is free
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             }
             fence_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(&sh.f16_full[1]); mbar_arrive(&sh.raw_free[1]); }
+            if (lane == 0) { mbar_arrive(&sh.v_full[i % Shape::kVs]); mbar_arrive(&sh.raw_free[1]); }
         }
       }
     } else {
