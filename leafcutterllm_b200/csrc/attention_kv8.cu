@@ -8,6 +8,8 @@
 //           scores' layout already is.  The weights are 2^(s - max + 6) in f16, 2^-11 of each off, times their page's scale over a reference that follows the scales, so that sums stay
 //           in the matrix unit's accumulators.  For f32 they are the f16 value and what its rounding lost, 22 bits together, in two products; a step's sums are multiplied by the page's
 //           scale and added in f32, so that what the matrix unit cuts off when it adds stays within 16 keys.
+// What bounds it: single tokens, the instructions' waits for one another at 16 warps an SM (64 sequences of 128 - 4,096 tokens, 32 heads over 8, bf16: 43 us, 154 MB at 4.1 TB/s, half of the issue slots);
+// more rows, the same with 8 warps of 255 registers (32 rows behind 60,000 - 131,000: 152 us, 392 MB at 2.7 TB/s, 39 % of the slots); one sequence, the two launches' beginnings and ends (700 tokens 10 us).
 #include <algorithm>
 #include <type_traits>
 #include "lc_kv8.cuh"
@@ -459,7 +461,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
             }
         }
         };
-        // the loop twice, as the digit's values took other calls' registers in one (64 tokens on 32 sequences: 161 us instead of 152)
+        // the loop twice, as the digit's values took other calls' registers in one (4 tokens x 8 heads of a group, two sequences behind 60,000 and more: 161 us instead of 152)
         if (__any_sync(0xffffffffu, fine)) steps(std::true_type{});
         else steps(std::false_type{});
         cp_async_wait<0>();

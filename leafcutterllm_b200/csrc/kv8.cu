@@ -9,7 +9,8 @@
 // position, as 64-bit fractions of a turn: position * entry wraps around by itself, and what is left is the angle's fraction of a turn
 // to 2^-64 of one, however far the position is (cos and sin of an f32 angle lose 2^-24 of the ANGLE: 0.06 at 10^6).
 //
-// Both kernels move bytes: an append reads its rows once from HBM (a page's second pass over them finds them in L1/L2) and writes a quarter or half of that.
+// Both kernels move bytes: an append reads its rows once from HBM (a page's second pass over them finds them in L1/L2) and writes a quarter or half of that.  Prompts
+// are bound by the passes' instructions (57 % of the issue slots; 61 MB read at 1.2 TB/s), single tokens by the launch and a chain of loads: row_start, context, table, scale, rows.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -178,9 +179,8 @@ struct Group {
 //           largest in 64 bits;
 //   kInts   integers: x / S in f32 is within 2e-4 of the quotient (rotation 2^-22 of at most 180 S, product and inverse 2^-22 of 127.5), so that it gives the integer of
 //           the 64-bit quotient unless it lies so near a half; eight elements with such a one among them, one group in 300, are taken in 64 bits.
-// Rows with infinities or NaN, which the first maximum shows, and maxima and scales below 1e-30 go the long way, all in 64 bits.  5,000 rows of eight heads, bf16, 5 prompts: 171 us with
-// everything in 64 bits and an element per lane, 31 now (a table of rotations 2.3 of a block's 12, each pass 2 to 4: their instructions).
-//
+// Rows with infinities or NaN, which the first maximum shows, and maxima and scales below 1e-30 go the long way, all in 64 bits.  Five prompts of 300 - 2,100 tokens, 8 kv heads and 32 of queries
+// of 128, bf16: 171 us with everything in 64 bits and an element per lane, 44 now (a table of rotations 2.3 of a block's 12, each pass 2 to 4: their instructions).
 enum : int { kMost, kFine, kInts };
 struct Item {
     double top, scale, inv;

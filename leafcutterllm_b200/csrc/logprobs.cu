@@ -3,7 +3,7 @@
 // With m the row's maximum, d = x - m, S = sum e^d and T = sum e^d d:   log p(x) = d - log S,   entropy = log S - T / S.
 // Every thread keeps a running S and T against its warp's m, sixteen logits at a time, whose f32 sums are added in 64 bits.  A later maximum m' turns
 // (S, T) into (f S, f (T + (m - m') S)), f = e^(m - m').  m is the warp's and not the lane's: some lane finds a new maximum of its own in most steps, a warp in
-// one of six (128,256 logits: 255 -> 130 us with the change, 2,048 rows).
+// one of six (2,048 rows of 128,256, bf16: 255 us with maxima of lanes, 157 now: 3.3 TB/s, three quarters of the issue slots).
 //
 // The best `top`: a logit below the block's bound cannot be among them.  The bound is the top-th largest of the maxima of groups of
 // four threads after 1, 2, 4, ... steps, and every logit that reaches it goes to a list of its warp's; a full list is cut to its best `top` by counting,
