@@ -1,7 +1,7 @@
 // Attention over the key/value cache in 8 bits: out = sum_j p_j v_j, p = softmax_j(scale q . k_j) over the positions j up to the row's own.
 //
 // A cached element is an integer times the scale of its page and head, so both products are taken of the integers as they are, and the scales are applied outside.
-//   Scores  on the matrix unit's integers (mma.sync m16n8k32, exact): a row of queries is whole numbers in units of its largest / 32,512 (f32: / 8,323,072), and
+//   Scores  on the matrix unit's integers (mma.sync m16n8k32, exact): a row of queries is whole numbers in units of its largest / (127 x 256), f32: / (127 x 65,536), and
 //           these are digits of 8 bits, in rows of their own of the operand, so that keys go in as they lie in the cache.  16 bits are as good as f16 or bf16
 //           queries ask for: a score of size 1 is off by 3e-5; 24 bits for f32.  Rows whose largest element is above 32 times the mean get a digit more.
 //   Values  an integer of 8 bits is exact in f16 (m16n8k16, f32 out): values are the operand of 16 rows (dims) and weights that of 8 columns (rows of queries), which the
@@ -81,7 +81,7 @@ template <int HD, int NG, bool F32> struct RunShape {
 };
 
 // The unit of a row's numbers, of its scaled largest element.
-template <bool F32> __device__ __forceinline__ float query_unit(float top) { return top > 0.0f ? top * (F32 ? 1.0f / 8323072.0f : 1.0f / 32512.0f) : 1.0f; }
+template <bool F32> __device__ __forceinline__ float query_unit(float top) { return top > 0.0f ? top * (F32 ? 1.0f / (127.0f * 65536.0f) : 1.0f / (127.0f * 256.0f)) : 1.0f; }
 
 // What the scores of 16 keys gain by the digit behind the units, in units: keys 2c, 2c + 1 and 8 + 2c, 9 + 2c of row g.  hd: 0 for no row.  Few rows need it, so it is taken
 // from the queries again.
