@@ -630,6 +630,10 @@ int32_t lc_attention_kv8_workspace(const lc_kv8_cache* cache, const lc_kv8_rows*
     LC_CHECK(out_bytes, LC_ERR_INVALID, "lc_attention_kv8_workspace: null output");
     LC_TRY(kv8_check("lc_attention_kv8_workspace", cache, rows, typ, n_rows, &pool, &seqs));
     LC_TRY(check_heads("lc_attention_kv8_workspace", pool, seqs, n_heads));
+    if (n_rows == 0 || seqs.n_seqs == 0) {  // nothing to do, as for the call itself
+        *out_bytes = 16;
+        return LC_OK;
+    }
     DeviceScope dev;
     LC_TRY(dev.enter(cache->k_dev, "lc_attention_kv8_workspace: cache"));
     TilePlan tiles;

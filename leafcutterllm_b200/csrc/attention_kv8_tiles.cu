@@ -637,7 +637,7 @@ bool kv8_tiles_apply(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int
     const int64_t rows = (int64_t)group * max_rows;
     const int64_t units = ((int64_t)seqs.n_rows * group / kTileRows2 + seqs.n_seqs) * pool.n_kv;
     const int64_t tiles = (((int64_t)seqs.width << pool.page_shift) + kKeys - 1) / kKeys;  // of a sequence's keys, at most
-    if (pool.hd > 128 || units > 1 << 20) return false;
+    if (pool.hd > 128 || units < 1 || units > 1 << 20) return false;
     // Runs or tiles, us in runs / in tiles (32 heads over 8 kv heads of 128 unless said).  16-bit types: one sequence behind 4,000 tokens with 8 rows (tokens x heads of a
     // group) 22.7 / 24.1, 32 rows 35 / 25, 256 rows 44 / 36; 16 sequences of 32 rows behind 2,000 43.6 / 47.7, 64 of 64 rows behind 1,000 116.5 / 119, of 128 rows (4 kv heads of
     // 64) 86 / 50.  f32: one of 64 rows 39.5 / 34, of 512 78 / 58, with one kv head of 512 rows 39 / 47; 64 sequences of 64 rows 154 / 176, of 128 rows 94 / 73.

@@ -1,0 +1,28 @@
+"""The workspace of attention over the 8-bit cache: what the host says without a device."""
+import ctypes as C
+
+import pytest
+
+from test_kv8 import cache, rows
+
+
+def workspace(lc, typ, n, heads, **over):
+    out = C.c_size_t(1 << 60)
+    rc = lc.load().lc_attention_kv8_workspace(C.byref(cache(lc)), C.byref(rows(lc, **over)), typ, n, heads, C.byref(out))
+    return rc, out.value
+
+
+@pytest.mark.parametrize("typ", [0, 1, 30])
+@pytest.mark.parametrize("max_rows", [0, 1, 8, 16, 32, 100, 4000])
+@pytest.mark.parametrize("heads", [2, 8, 64])
+def test_of_calls_that_have_nothing_to_do(lc, typ, max_rows, heads):
+    """A step without sequences or rows asks for no more than an allocator's smallest piece, and the call itself takes it, with or without a device."""
+    for n_seqs, n in ((0, 0), (0, 5), (0, 4000), (2, 0), (4096, 0)):
+        rc, size = workspace(lc, typ, n, heads, n_seqs=n_seqs, max_rows=max_rows)
+        assert rc == lc._capi.LC_OK and size <= 512
+
+
+def test_arguments_are_checked_all_the_same(lc):
+    assert workspace(lc, 0, 0, 3)[0] == lc._capi.LC_ERR_INVALID
+    assert workspace(lc, 8, 0, 2)[0] == lc._capi.LC_ERR_UNSUPPORTED
+    assert workspace(lc, 0, 0, 2, max_rows=-1)[0] == lc._capi.LC_ERR_INVALID
