@@ -573,17 +573,27 @@ template <int HD, bool F32> int run_blocks(int groups) {
     return groups == 2 ? RunShape<HD, 2, F32>::kBlocks : RunShape<HD, 1, F32>::kBlocks;
 }
 // As many groups of 8 rows share a step's keys and values as a unit has rows for: four at most, whose sums are 128 registers (two for heads of 256).
-RunPlan plan_runs(const Kv8Pool& pool, uint32_t typ, int group, int max_rows) {
+int run_groups(const Kv8Pool& pool, int group, int max_rows) {
+    const int64_t rows = (int64_t)group * (max_rows < 1 ? 1 : max_rows);
+    return rows <= 8 ? 1 : rows <= 16 || pool.hd > 128 ? 2 : 4;
+}
+RunPlan plan_runs(const Kv8Pool& pool, uint32_t typ, int groups) {
     RunPlan p;
     p.hd = pool.hd <= 64 ? 64 : pool.hd <= 128 ? 128 : 256;
-    const int64_t rows = (int64_t)group * (max_rows < 1 ? 1 : max_rows);
-    p.groups = rows <= 8 ? 1 : rows <= 16 || p.hd == 256 ? 2 : 4;
+    p.groups = groups;
     const bool f32 = typ == LC_TYPE_F32;
     p.blocks = sm_count() * (p.hd == 64    ? (f32 ? run_blocks<64, true>(p.groups) : run_blocks<64, false>(p.groups))
                              : p.hd == 128 ? (f32 ? run_blocks<128, true>(p.groups) : run_blocks<128, false>(p.groups))
                                            : (f32 ? run_blocks<256, true>(p.groups) : run_blocks<256, false>(p.groups)));
     p.bytes = (size_t)p.blocks * kRunWarps * (sizeof(UnitRecord) + (size_t)2 * 8 * p.groups * (p.hd + 2) * sizeof(float));
     return p;
+}
+// The most that a call with at most these rows per sequence needs: fewer rows, sequences or pages may go by runs instead of tiles, take fewer groups (whose
+// runs are more), or have their keys cut where larger ones are not, so the answer goes by none of them.
+size_t most_bytes(const Kv8Pool& pool, uint32_t typ, int group, int max_rows) {
+    size_t most = kv8_tiles_most_bytes(pool, group, max_rows);
+    for (int groups = run_groups(pool, group, max_rows); groups >= 1; groups /= 2) most = std::max(most, plan_runs(pool, typ, groups).bytes);
+    return most;
 }
 
 template <int HD, int NG, bool F32, bool FULL>
@@ -636,9 +646,7 @@ int32_t lc_attention_kv8_workspace(const lc_kv8_cache* cache, const lc_kv8_rows*
     }
     DeviceScope dev;
     LC_TRY(dev.enter(cache->k_dev, "lc_attention_kv8_workspace: cache"));
-    TilePlan tiles;
-    const int group = n_heads / pool.n_kv;
-    *out_bytes = kv8_tiles_apply(pool, seqs, typ, group, rows->max_rows, &tiles) ? tiles.bytes : plan_runs(pool, typ, group, rows->max_rows).bytes;
+    *out_bytes = most_bytes(pool, typ, n_heads / pool.n_kv, rows->max_rows);
     return LC_OK;
 }
 
@@ -657,7 +665,7 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
     DeviceScope dev;
     LC_TRY(dev.enter(cache->k_dev, "lc_attention_kv8_dev: cache"));
     const int group = n_heads / pool.n_kv;
-    const RunPlan plan = plan_runs(pool, typ, group, rows->max_rows);
+    const RunPlan plan = plan_runs(pool, typ, run_groups(pool, group, rows->max_rows));
     TilePlan tiles;
     const bool by_tiles = kv8_tiles_apply(pool, seqs, typ, group, rows->max_rows, &tiles);
     const size_t need = by_tiles ? tiles.bytes : plan.bytes;

@@ -631,6 +631,9 @@ int32_t tiles_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, co
     return LC_OK;
 }
 
+constexpr int kLeastRows = 32;  // of a sequence and kv head, below which no call goes by tiles
+size_t part_bytes(const Kv8Pool& pool) { return (size_t)kTileRows2 * ((pool.hd <= 64 ? 64 : 128) + 2) * sizeof(float); }
+
 }  // namespace
 
 bool kv8_tiles_apply(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, TilePlan* plan) {
@@ -643,14 +646,18 @@ bool kv8_tiles_apply(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int
     // 64) 86 / 50.  f32: one of 64 rows 39.5 / 34, of 512 78 / 58, with one kv head of 512 rows 39 / 47; 64 sequences of 64 rows 154 / 176, of 128 rows 94 / 73.
     if (typ == LC_TYPE_F32) {
         if (units < 16 || rows < (units > sm_count() ? 128 : 64)) return false;
-    } else if (rows < (seqs.n_seqs * pool.n_kv * tiles <= 4 * sm_count() ? 32 : 64)) {  // fewer rows waste a tile: they only may where there is little to do
+    } else if (rows < (seqs.n_seqs * pool.n_kv * tiles <= 4 * sm_count() ? kLeastRows : 64)) {  // fewer rows waste a tile: they only may where there is little to do
         return false;
     }
     // fewer units than SMs: their keys are cut, into parts of at least four tiles where contexts are as long as the table
     plan->units = (int)units;
     plan->splits = (int)std::max<int64_t>(1, std::min<int64_t>({sm_count() / units, (tiles + 3) / 4, 64}));
-    plan->bytes = plan->splits > 1 ? (size_t)units * plan->splits * kTileRows2 * ((pool.hd <= 64 ? 64 : 128) + 2) * sizeof(float) : 16;
+    plan->bytes = plan->splits > 1 ? (size_t)units * plan->splits * part_bytes(pool) : 16;
     return true;
+}
+size_t kv8_tiles_most_bytes(const Kv8Pool& pool, int group, int max_rows) {
+    // parts are no more than SMs
+    return pool.hd <= 128 && (int64_t)group * max_rows >= kLeastRows ? sm_count() * part_bytes(pool) : 16;
 }
 
 int32_t launch_kv8_tiles(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const TilePlan& plan, cudaStream_t s) {

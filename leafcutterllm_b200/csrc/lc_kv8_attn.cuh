@@ -210,6 +210,7 @@ struct TilePlan {
     size_t bytes;
 };
 bool kv8_tiles_apply(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, TilePlan* plan);
+size_t kv8_tiles_most_bytes(const Kv8Pool& pool, int group, int max_rows);  // of any call with at most so many rows per sequence
 int32_t launch_kv8_tiles(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const TilePlan& plan, cudaStream_t s);
 
 }  // namespace lc

@@ -174,7 +174,7 @@ class Kv8Cache:
         return k_out, v_out
 
     def attention_workspace(self, rows: Kv8Rows, q) -> int:
-        """Bytes of workspace of attention over such rows."""
+        """Bytes of workspace of attention over such rows, or over fewer: no more rows, sequences, pages and max_rows than these."""
         typ = _typ(q)
         out = C.c_size_t()
         check(load().lc_attention_kv8_workspace(self._ref, rows._ref, typ, q.shape[0], q.shape[1], C.byref(out)))

@@ -1,0 +1,60 @@
+"""The 8-bit key/value cache on the GPU at the edges of what its calls allow: workspaces that serve smaller calls, tables far wider than contexts, windows whose
+pages are gone, rows of very different size, numbers that are not finite, values next to zero, bad pages in the middle of a draft."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import plain_kv8 as plain
+from test_kv8_gpu import DT, Setup, check_attention, cuda, host
+
+pytestmark = pytest.mark.gpu
+
+
+def want_of(s, heads, q64, dtype, window=0):
+    want, mass, big, keys = s.plain.attention(s.table, s.ctx, s.start, q64, None, window)
+    return want, plain.attention_bound(want, mass, big, keys, s.dim, dtype, dtype == "float32")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("heads,kv,dim", [(32, 8, 128), (8, 2, 64), (4, 1, 256)])
+def test_a_workspace_serves_smaller_calls(gpu, dtype, heads, kv, dim):
+    """One workspace, asked for with the largest chunk, for shorter chunks and single tokens after it."""
+    pages = 2
+    pools = [torch.randint(-127, 128, (pages, kv, 16, dim), dtype=torch.int8, device="cuda") for _ in range(2)] + [torch.full((pages, kv), 0.01, device="cuda") for _ in range(2)]
+    cache = gpu.Kv8Cache(*pools)
+    table = torch.zeros(4, 512, dtype=torch.int32, device="cuda")       # 8,192 positions, all on one page
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    largest = 4096
+    q = torch.randn(largest, heads, dim, device="cuda").to(DT[dtype])
+    ws = torch.empty(cache.attention_workspace(gpu.Kv8Rows(table, i32([0] * 4), i32([0] * 5), largest), q), dtype=torch.uint8, device="cuda")
+    for n in (4096, 2048, 1024, 512, 256, 64, 33, 8, 1):
+        for seqs in (1, 4):
+            for max_rows in sorted({n, 1, -(-n // seqs)}):
+                start = [n * i // seqs for i in range(seqs + 1)]
+                rows = gpu.Kv8Rows(table[:seqs], i32([5] * seqs), i32(start), max_rows)
+                assert cache.attention_workspace(rows, q[:n]) <= ws.numel()
+                out = cache.attention(rows, q[:n], workspace=ws)
+                if n <= 64:
+                    assert torch.equal(out, cache.attention(rows, q[:n]))
+    torch.cuda.synchronize()
+
+
+def test_workspaces_grow_with_their_calls(gpu):
+    """Whatever a call has less of than another, its workspace is no larger."""
+    rng = np.random.default_rng(21)
+    pools = [torch.zeros(1, 8, 16, 128, dtype=torch.int8, device="cuda") for _ in range(2)] + [torch.zeros(1, 8, device="cuda") for _ in range(2)]
+    cache = gpu.Kv8Cache(*pools)
+    z = torch.zeros(1, dtype=torch.int32, device="cuda").data_ptr()
+    import ctypes as C
+
+    def size(typ, n_seqs, width, max_rows, n_rows, heads):
+        rows, out = gpu._capi.Kv8RowsStruct(z, z, z, None, n_seqs, width, max_rows, 0), C.c_size_t()
+        gpu._capi.check(gpu.load().lc_attention_kv8_workspace(cache._ref, C.byref(rows), typ, n_rows, heads, C.byref(out)))
+        return out.value
+    for _ in range(300):
+        typ, heads = int(rng.choice([0, 1, 30])), int(rng.choice([8, 16, 32, 64]))
+        big = [int(np.exp(rng.uniform(0, math.log(m)))) for m in (256, 4096, 4096, 8192)]
+        small = [int(rng.integers(0, b + 1)) for b in big]
+        assert size(typ, *small, heads) <= size(typ, *big, heads), (typ, heads, small, big)
