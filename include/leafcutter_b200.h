@@ -193,6 +193,8 @@ int32_t lc_kv8_read_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows, uint
  * [n_rows][n_heads][head_dim], already rotated, attends to the positions up to its own, which the cache already holds (append first), and
  * with window > 0 only to the last `window` of them.  Scores are q . k * scale (0: 1 / sqrt(head_dim); 2e38 at most).  Queries of any finite size are taken; a
  * row with one that is not finite gives NaN.  Softmax and sums are in f32, its weights in 11 bits (f32: 22).  The values' scales of a sequence and head may differ by factors up to 2^100.
+ * A call is refused where its work, with every context as long as its table, could not be counted in 31 bits.  Taken for sure: (n_rows * heads per kv head / 256 + n_seqs) * n_kv_heads * (positions
+ * of a table / 16 + 6) below 2^31 and n_rows * n_heads up to 2^27; with heads above 128 the first factor is n_rows * heads per kv head / 16 + n_seqs.
  * The workspace is the caller's: lc_attention_kv8_workspace says how many bytes, for any contexts and any calls of this typ over this cache and these heads
  * with at most these arguments' n_rows, n_seqs, table_width and max_rows: asked once with the largest chunk, it serves shorter ones and single tokens too.  It needs no initial value and keeps nothing between calls.  Calls that may run at the same time (graphs that may be replayed at the
  * same time among them) need a workspace each. */

@@ -588,11 +588,39 @@ RunPlan plan_runs(const Kv8Pool& pool, uint32_t typ, int groups) {
     p.bytes = (size_t)p.blocks * kRunWarps * (sizeof(UnitRecord) + (size_t)2 * 8 * p.groups * (p.hd + 2) * sizeof(float));
     return p;
 }
-// The most that a call with at most these rows per sequence needs: fewer rows, sequences or pages may go by runs instead of tiles, take fewer groups (whose
+// Whether the places of the line, with row blocks of so many rows, are sure to stay in 31 bits: every context as long as its table.
+bool line_fits(const Kv8Pool& pool, const Kv8Seqs& seqs, int group, int block_rows) {
+    const double steps = (double)((int64_t)seqs.width << pool.page_shift) / kStep + 2 + kUnitCost;
+    const double blocks = (double)seqs.n_rows * group / block_rows + std::min(seqs.n_seqs, seqs.n_rows);
+    return steps * blocks * pool.n_kv < 2147483648.0;
+}
+int most_groups(const Kv8Pool& pool) { return pool.hd > 128 ? 2 : 4; }
+bool tiles_fit(const Kv8Pool& pool, const Kv8Seqs& seqs, int group) {
+    TilePlan tiles;
+    return line_fits(pool, seqs, group, kTileRows2) && kv8_tiles_plan(pool, seqs, group, &tiles);
+}
+struct Plan {
+    bool by_tiles;
+    TilePlan tiles;
+    RunPlan runs;
+    size_t bytes() const { return by_tiles ? tiles.bytes : runs.bytes; }
+};
+// The faster kernel, unless its line does not fit: a call with many more rows than its max_rows says goes by tiles then, or by as many groups as it takes.
+Plan plan_call(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows) {
+    Plan p;
+    int groups = run_groups(pool, group, max_rows);
+    p.by_tiles = kv8_tiles_plan(pool, seqs, group, &p.tiles) && line_fits(pool, seqs, group, kTileRows2) &&
+                 (kv8_tiles_pay(pool, seqs, typ, group, max_rows, p.tiles) || !line_fits(pool, seqs, group, 8 * groups));
+    while (!p.by_tiles && groups < most_groups(pool) && !line_fits(pool, seqs, group, 8 * groups)) groups *= 2;
+    p.runs = plan_runs(pool, typ, groups);
+    return p;
+}
+// The most that a call with at most these arguments needs: fewer rows, sequences or pages may go by runs instead of tiles, take fewer groups (whose
 // runs are more), or have their keys cut where larger ones are not, so the answer goes by none of them.
-size_t most_bytes(const Kv8Pool& pool, uint32_t typ, int group, int max_rows) {
-    size_t most = kv8_tiles_most_bytes(pool, group, max_rows);
-    for (int groups = run_groups(pool, group, max_rows); groups >= 1; groups /= 2) most = std::max(most, plan_runs(pool, typ, groups).bytes);
+size_t most_bytes(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows) {
+    const bool any = !line_fits(pool, seqs, group, 8);  // then a smaller max_rows may lead to every kernel
+    size_t most = kv8_tiles_most_bytes(pool, any ? 1 << 30 : (int64_t)group * max_rows);
+    for (int groups = any ? most_groups(pool) : run_groups(pool, group, max_rows); groups >= 1; groups /= 2) most = std::max(most, plan_runs(pool, typ, groups).bytes);
     return most;
 }
 
@@ -620,9 +648,9 @@ int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, con
 
 int32_t check_heads(const char* call, const Kv8Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {
     LC_CHECK(n_heads > 0 && n_heads <= 65536 && n_heads % pool.n_kv == 0, LC_ERR_INVALID, "%s: %d heads over %d kv heads", call, n_heads, pool.n_kv);
-    // places of the line, row blocks of 8 at worst, in 31 bits
-    const double chunks = (double)((int64_t)seqs.width << pool.page_shift) / kStep + 2 + kUnitCost, blocks = (double)seqs.n_rows * (n_heads / pool.n_kv) / 8 + seqs.n_seqs;
-    LC_CHECK(chunks * blocks * pool.n_kv < 2147483648.0, LC_ERR_INVALID, "%s: %d rows of %d heads over tables of %d pages are too many for one call", call, seqs.n_rows, n_heads, seqs.width);
+    const int group = n_heads / pool.n_kv;
+    LC_CHECK(line_fits(pool, seqs, group, 8 * most_groups(pool)) || tiles_fit(pool, seqs, group), LC_ERR_INVALID, "%s: %d rows of %d heads over tables of %d pages are too many for one call",
+             call, seqs.n_rows, n_heads, seqs.width);
     return LC_OK;
 }
 
@@ -646,7 +674,7 @@ int32_t lc_attention_kv8_workspace(const lc_kv8_cache* cache, const lc_kv8_rows*
     }
     DeviceScope dev;
     LC_TRY(dev.enter(cache->k_dev, "lc_attention_kv8_workspace: cache"));
-    *out_bytes = most_bytes(pool, typ, n_heads / pool.n_kv, rows->max_rows);
+    *out_bytes = most_bytes(pool, seqs, typ, n_heads / pool.n_kv, rows->max_rows);
     return LC_OK;
 }
 
@@ -665,10 +693,8 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
     DeviceScope dev;
     LC_TRY(dev.enter(cache->k_dev, "lc_attention_kv8_dev: cache"));
     const int group = n_heads / pool.n_kv;
-    const RunPlan plan = plan_runs(pool, typ, run_groups(pool, group, rows->max_rows));
-    TilePlan tiles;
-    const bool by_tiles = kv8_tiles_apply(pool, seqs, typ, group, rows->max_rows, &tiles);
-    const size_t need = by_tiles ? tiles.bytes : plan.bytes;
+    const Plan plan = plan_call(pool, seqs, typ, group, rows->max_rows);
+    const size_t need = plan.bytes();
     LC_CHECK(workspace_dev && workspace_bytes >= need && (uintptr_t)workspace_dev % 16 == 0, LC_ERR_INVALID,
              "lc_attention_kv8_dev: needs a workspace of %zu bytes, 16-byte aligned (got %zu)", need, workspace_bytes);
     if (scale == 0.0f) scale = 1.0f / sqrtf((float)pool.hd);
@@ -676,12 +702,12 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
     const size_t elem = typ == LC_TYPE_F32 ? 4 : 2;
     AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16),
                scale * 1.44269504088896f, nullptr, (UnitRecord*)workspace_dev};
-    a.part = by_tiles ? (float*)workspace_dev : (float*)((char*)workspace_dev + (size_t)plan.blocks * kRunWarps * sizeof(UnitRecord));
+    a.part = plan.by_tiles ? (float*)workspace_dev : (float*)((char*)workspace_dev + (size_t)plan.runs.blocks * kRunWarps * sizeof(UnitRecord));
     cudaStream_t s = stream_or_own(stream_);
-    if (by_tiles) return launch_kv8_tiles(pool, seqs, a, tiles, s);
-    if (plan.hd == 64) return runs_of<64>(pool, seqs, a, plan, s);
-    if (plan.hd == 128) return runs_of<128>(pool, seqs, a, plan, s);
-    return runs_of<256>(pool, seqs, a, plan, s);
+    if (plan.by_tiles) return launch_kv8_tiles(pool, seqs, a, plan.tiles, s);
+    if (plan.runs.hd == 64) return runs_of<64>(pool, seqs, a, plan.runs, s);
+    if (plan.runs.hd == 128) return runs_of<128>(pool, seqs, a, plan.runs, s);
+    return runs_of<256>(pool, seqs, a, plan.runs, s);
 }
 
 }  // extern "C"

@@ -29,7 +29,7 @@ namespace lc {
 
 namespace {
 
-constexpr int kTileRows2 = 256, kKeys = 128, kTileThreads = 512, kConvWarps = 6, kSlots = 4;
+constexpr int kKeys = 128, kTileThreads = 512, kConvWarps = 6, kSlots = 4;
 // registers a thread at the launch
 constexpr int kLaunchRegs = 128;
 constexpr int kGroups = kKeys / 16;
@@ -632,32 +632,31 @@ int32_t tiles_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, co
 }
 
 constexpr int kLeastRows = 32;  // of a sequence and kv head, below which no call goes by tiles
+int64_t table_tiles(const Kv8Pool& pool, const Kv8Seqs& seqs) { return (((int64_t)seqs.width << pool.page_shift) + kKeys - 1) / kKeys; }  // of a sequence's keys, at most
 size_t part_bytes(const Kv8Pool& pool) { return (size_t)kTileRows2 * ((pool.hd <= 64 ? 64 : 128) + 2) * sizeof(float); }
 
 }  // namespace
 
-bool kv8_tiles_apply(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, TilePlan* plan) {
-    const int64_t rows = (int64_t)group * max_rows;
+bool kv8_tiles_plan(const Kv8Pool& pool, const Kv8Seqs& seqs, int group, TilePlan* plan) {
     const int64_t units = ((int64_t)seqs.n_rows * group / kTileRows2 + seqs.n_seqs) * pool.n_kv;
-    const int64_t tiles = (((int64_t)seqs.width << pool.page_shift) + kKeys - 1) / kKeys;  // of a sequence's keys, at most
     if (pool.hd > 128 || units < 1 || units > 1 << 20) return false;
-    // Runs or tiles, us in runs / in tiles (32 heads over 8 kv heads of 128 unless said).  16-bit types: one sequence behind 4,000 tokens with 8 rows (tokens x heads of a
-    // group) 22.7 / 24.1, 32 rows 35 / 25, 256 rows 44 / 36; 16 sequences of 32 rows behind 2,000 43.6 / 47.7, 64 of 64 rows behind 1,000 116.5 / 119, of 128 rows (4 kv heads of
-    // 64) 86 / 50.  f32: one of 64 rows 39.5 / 34, of 512 78 / 58, with one kv head of 512 rows 39 / 47; 64 sequences of 64 rows 154 / 176, of 128 rows 94 / 73.
-    if (typ == LC_TYPE_F32) {
-        if (units < 16 || rows < (units > sm_count() ? 128 : 64)) return false;
-    } else if (rows < (seqs.n_seqs * pool.n_kv * tiles <= 4 * sm_count() ? kLeastRows : 64)) {  // fewer rows waste a tile: they only may where there is little to do
-        return false;
-    }
     // fewer units than SMs: their keys are cut, into parts of at least four tiles where contexts are as long as the table
     plan->units = (int)units;
-    plan->splits = (int)std::max<int64_t>(1, std::min<int64_t>({sm_count() / units, (tiles + 3) / 4, 64}));
+    plan->splits = (int)std::max<int64_t>(1, std::min<int64_t>({sm_count() / units, (table_tiles(pool, seqs) + 3) / 4, 64}));
     plan->bytes = plan->splits > 1 ? (size_t)units * plan->splits * part_bytes(pool) : 16;
     return true;
 }
-size_t kv8_tiles_most_bytes(const Kv8Pool& pool, int group, int max_rows) {
+bool kv8_tiles_pay(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, const TilePlan& plan) {
+    const int64_t rows = (int64_t)group * max_rows;
+    // Runs or tiles, us in runs / in tiles (32 heads over 8 kv heads of 128 unless said).  16-bit types: one sequence behind 4,000 tokens with 8 rows (tokens x heads of a
+    // group) 22.7 / 24.1, 32 rows 35 / 25, 256 rows 44 / 36; 16 sequences of 32 rows behind 2,000 43.6 / 47.7, 64 of 64 rows behind 1,000 116.5 / 119, of 128 rows (4 kv heads of
+    // 64) 86 / 50.  f32: one of 64 rows 39.5 / 34, of 512 78 / 58, with one kv head of 512 rows 39 / 47; 64 sequences of 64 rows 154 / 176, of 128 rows 94 / 73.
+    if (typ == LC_TYPE_F32) return plan.units >= 16 && rows >= (plan.units > sm_count() ? 128 : 64);
+    return rows >= (seqs.n_seqs * pool.n_kv * table_tiles(pool, seqs) <= 4 * sm_count() ? kLeastRows : 64);  // fewer rows waste a tile: they only may where there is little to do
+}
+size_t kv8_tiles_most_bytes(const Kv8Pool& pool, int64_t rows) {
     // parts are no more than SMs
-    return pool.hd <= 128 && (int64_t)group * max_rows >= kLeastRows ? sm_count() * part_bytes(pool) : 16;
+    return pool.hd <= 128 && rows >= kLeastRows ? sm_count() * part_bytes(pool) : 16;
 }
 
 int32_t launch_kv8_tiles(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const TilePlan& plan, cudaStream_t s) {

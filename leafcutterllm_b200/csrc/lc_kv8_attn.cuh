@@ -205,12 +205,14 @@ __device__ __forceinline__ int seq_at(const uint32_t* cum, int n_seqs, uint32_t 
     return lo;
 }
 // attention_kv8_tiles.cu: many rows per sequence, in tiles of 256 rows on tcgen05; heads of up to 128
+constexpr int kTileRows2 = 256;       // of a unit
 struct TilePlan {
     int units, splits;               // blocks: at most so many units; every unit's keys in so many parts
     size_t bytes;
 };
-bool kv8_tiles_apply(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, TilePlan* plan);
-size_t kv8_tiles_most_bytes(const Kv8Pool& pool, int group, int max_rows);  // of any call with at most so many rows per sequence
+bool kv8_tiles_plan(const Kv8Pool& pool, const Kv8Seqs& seqs, int group, TilePlan* plan);                                                          // whether they can
+bool kv8_tiles_pay(const Kv8Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, const TilePlan& plan);                          // whether they are faster
+size_t kv8_tiles_most_bytes(const Kv8Pool& pool, int64_t rows);                                                                                     // of any call with at most so many rows (tokens x heads of a group) per sequence
 int32_t launch_kv8_tiles(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const TilePlan& plan, cudaStream_t s);
 
 }  // namespace lc

@@ -58,3 +58,24 @@ def test_workspaces_grow_with_their_calls(gpu):
         big = [int(np.exp(rng.uniform(0, math.log(m)))) for m in (256, 4096, 4096, 8192)]
         small = [int(rng.integers(0, b + 1)) for b in big]
         assert size(typ, *small, heads) <= size(typ, *big, heads), (typ, heads, small, big)
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,new,max_rows", [("bfloat16", 64, 8, 128, 4096, 4096), ("float32", 64, 8, 128, 4096, 4096), ("bfloat16", 64, 8, 128, 4096, 1), ("bfloat16", 16, 8, 64, 3, 3),
+                                                             ("bfloat16", 64, 8, 256, 6000, 6000)])
+def test_tables_for_a_million_positions(gpu, dtype, heads, kv, dim, new, max_rows):
+    """A table far wider than the contexts: the same results as with a narrow one."""
+    pages = -(-(new + 20) // 16)
+    pools = [torch.randint(-127, 128, (pages, kv, 16, dim), dtype=torch.int8, device="cuda") for _ in range(2)] + [torch.rand(pages, kv, device="cuda") * 0.02 for _ in range(2)]
+    cache = gpu.Kv8Cache(*pools)
+    wide = torch.full((1, 2 ** 16), -1, dtype=torch.int32, device="cuda")
+    wide[0, :pages] = torch.randperm(pages, device="cuda").to(torch.int32)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = torch.randn(new, heads, dim, device="cuda").to(DT[dtype])
+    outs = []
+    for table in (wide, wide[:, :pages].contiguous()):
+        status = i32([0])
+        rows = gpu.Kv8Rows(table, i32([20]), i32([0, new]), max_rows, status)
+        outs.append(cache.attention(rows, q).double())
+        assert status.item() == 0
+    # both are sums of the same terms, in f32 and in another order at most; then one rounding each
+    assert (outs[0] - outs[1]).abs().max() <= outs[1].abs().max() * (plain.EPS[dtype] + 2.0 ** -10 * (dtype != "float32") + 2.0 ** -18)
