@@ -35,7 +35,7 @@ constexpr int kLaunchRegs = 128;
 constexpr int kGroups = kKeys / 16;
 
 // what the softmax needs to know of 16 keys: score factor, log2 of the values' scale, its inverse; and what the unpacking does
-enum : int { kHere = 0, kAbsent = 1, kOutside = 2, kZeroValues = 4 };  // behind the end: zeros; outside the pool: keys of NaN
+enum : int { kHere = 0, kAbsent = 1, kOutside = 2, kZeroValues = 4 };  // not among the unit's keys: zeros; outside the pool: keys of NaN
 struct GroupConst {
     float f, lv, inv;
     int state;
@@ -275,9 +275,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             const int page_mask = (1 << pool.page_shift) - 1;
             const float k_factor = a.scale_log2 * down;
             const uint32_t bytes = 16 * hd;
-            auto look_up = [&](int i) {  // lane g < 8: the page of group g: -1 behind the end, -2 outside the pool
+            auto look_up = [&](int i) {  // lane g < 8: the page of group g: -1 in front of every row's window and behind the end, -2 outside the pool
                 const int key = (tile0 + i) * kKeys + lane * 16;
-                if (lane >= kGroups || i >= n || key >= key_end) return -1;
+                if (lane >= kGroups || i >= n || key + 15 < key_lo || key >= key_end) return -1;
                 const int p = table[key >> pool.page_shift];
                 return p >= 0 && p < pool.n_pages ? p : -2;
             };

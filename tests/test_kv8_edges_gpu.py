@@ -79,3 +79,25 @@ def test_tables_for_a_million_positions(gpu, dtype, heads, kv, dim, new, max_row
         assert status.item() == 0
     # both are sums of the same terms, in f32 and in another order at most; then one rounding each
     assert (outs[0] - outs[1]).abs().max() <= outs[1].abs().max() * (plain.EPS[dtype] + 2.0 ** -10 * (dtype != "float32") + 2.0 ** -18)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("seqs,window", [([(1000, 40), (700, 64), (333, 33), (1001, 150)], 100), ([(300, 70), (129, 130), (200, 64), (77, 40)], 37), ([(1000, 3), (500, 1), (777, 2)], 100)])
+def test_pages_in_front_of_a_window_are_gone(gpu, dtype, page, seqs, window):
+    """A serving loop drops the pages that no row sees any more, and their numbers, or what stands there, mean nothing."""
+    s = Setup(gpu, seqs, 4, 64, page, seed=31)
+    q = s.normal(16, dtype)
+    first = check_attention(s, 16, dtype, window=window, q=q).clone()
+    gone = [(i, p) for i, (c, _) in enumerate(seqs) for p in range(s.table.shape[1]) if (p + 1) * page <= c - window + 1]
+    assert gone
+    for scale, bad in zip(s.pools[2:], (math.nan, math.inf)):
+        for i, p in gone:
+            scale[int(s.table[i, p])] = bad
+    assert torch.equal(first, check_attention(s, 16, dtype, window=window, q=q))
+    table = s.table.copy()
+    for number in (-1, 2 ** 31 - 1):
+        for i, p in gone:
+            table[i, p] = number
+        s.batch = s.rows_of(max(n for _, n in seqs), table=table)
+        assert torch.equal(first, check_attention(s, 16, dtype, window=window, q=q))
