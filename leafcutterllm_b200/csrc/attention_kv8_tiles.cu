@@ -398,7 +398,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         const int limit = w.ctx + (row_lo + min(r, row_n - 1)) / a.group;      // last position that the row sees
         const int least = __shfl_sync(0xffffffffu, limit, 0), most = __shfl_sync(0xffffffffu, limit, 31);
         float o[HD], m = kNegInf, l = 0.0f, corr = 1.0f;
-        bool ok = true;
+        bool ok = true, far = false;
+        // Rounded as the scores of a far reference are (below), so that the largest of these is no more than a rounding of S_v from it.
+        auto exponent = [](float x, float f, float lv) { return __fadd_rn(__fmul_rn(x, f), lv); };
+        // Far from 0 a reference has no bits left for what is added to it, and a product that is rounded with it may be off by more than f16's range
+        // (scores of 1e8: 2^4).  There a score is rounded by itself, as the reference was, and what remains over it goes on; without loss in a neighbourhood of the reference.
+        auto is_far = [](float mx) { return __any_sync(0xffffffffu, fabsf(mx) > 65536.0f && mx != kNegInf); };
+        auto over = [](float x, float f, float ref, float lv) {
+            const float y = __fsub_rn(__fmul_rn(x, f), ref);
+            return y > 9.0f - lv ? 9.0f - lv : y;  // 2^15 at most; NaN stays
+        };
         auto add_up = [&](int i) {  // o = o corr + the key tile's sums
             ok = mbar_wait(&sh.o_full[t], i & 1) && ok;
             ok = __all_sync(0xffffffffu, ok);
@@ -444,10 +453,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
 #pragma unroll
                             for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(x[16 * h + e]));
                             const GroupConst k = gc[c / 16 + h];
-                            mx = fmaxf(mx, fmaf(g, k.f, k.lv));
+                            mx = fmaxf(mx, exponent(g, k.f, k.lv));
                         }
                     }
                     const float ref = mx == kNegInf ? 0.0f : mx;
+                    far = is_far(mx);
+                    const float less = far ? 6.0f : 6.0f - ref;
                     corr = exp2_fast(m - ref);
                     m = mx;
                     // 16 keys' weights take the first 8 columns of their scores' 16, their low parts the other 8
@@ -457,12 +468,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         tmem_ld16(my_s + c, x);
                         tmem_wait_ld();
                         const GroupConst k = gc[c / 16];
-                        const float off = k.lv - ref + 6.0f;
+                        const float off = k.lv + less, f = far ? 1.0f : k.f;
                         if (!plain)
 #pragma unroll
                             for (int e = 0; e < 16; e++)
                                 if (c + e > to || c + e < from) x[e] = __float_as_uint(kNegInf);
-                        const float2 f2 = make_float2(k.f, k.f), off2 = make_float2(off, off);
+                        if (far)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) x[e] = __float_as_uint(over(__uint_as_float(x[e]), k.f, ref, k.lv));
+                        const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
                         float2 gs = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
@@ -490,12 +504,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
 #pragma unroll
                         for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(x[c + e]));
                         const GroupConst k = gc[c / 16];
-                        mx = fmaxf(mx, fmaf(g, k.f, k.lv));
+                        mx = fmaxf(mx, exponent(g, k.f, k.lv));
                     }
                     const bool raise = mx > m + 8.0f;  // also from minus infinity
                     if (__any_sync(0xffffffffu, raise)) {
                         const float f = raise ? exp2_fast(m - mx) : 1.0f;
                         if (raise) m = mx;
+                        far = is_far(m);
                         l *= f;
                         if (i > 0) {
                             ok = mbar_wait(&sh.o_full[t], (i - 1) & 1);
@@ -513,12 +528,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         }
                     }
                     const float ref = m == kNegInf ? 0.0f : m;
+                    const float less = far ? 6.0f : 6.0f - ref;
+                    if (far)
+#pragma unroll
+                        for (int c = 0; c < kKeys; c += 16) {
+                            const GroupConst k = gc[c / 16];
+#pragma unroll
+                            for (int e = 0; e < 16; e++) x[c + e] = __float_as_uint(over(__uint_as_float(x[c + e]), k.f, ref, k.lv));
+                        }
 #pragma unroll
                     for (int c = 0; c < kKeys; c += 16) {
                         uint32_t p[8];
                         const GroupConst k = gc[c / 16];
-                        const float off = k.lv - ref + 6.0f;
-                        const float2 f2 = make_float2(k.f, k.f), off2 = make_float2(off, off);
+                        const float off = k.lv + less, f = far ? 1.0f : k.f;
+                        const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
                         float2 gs = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {

@@ -12,6 +12,27 @@ from test_kv8_gpu import DT, Setup, check_attention, cuda, host
 pytestmark = pytest.mark.gpu
 
 
+def check_relative(s, heads, dtype, q):
+    """As check_attention, for weights and values of any size: what a weight loses below f16's normal range counts against the row's largest weight and the
+    largest value scale, not against 1 or the output."""
+    q, q64 = q
+    out = torch.full_like(q, math.nan)
+    s.cache.attention(s.batch, q, out)
+    want, mass, big, keys = s.plain.attention(s.table, s.ctx, s.start, q64)
+    split = dtype == "float32"
+    d = big * (2.0 ** -22 + (s.dim / 16 + 4) * 2.0 ** -23) + 2.0 ** -21
+    eps = 2 * (d[..., None] + (2.0 ** -22 if split else 2.0 ** -11)) + 2.0 ** -20
+    # a weight below 2^-14 (f32: its low part) is off by 2^-25 at most, values are 127 of their scale, and the sum of weights is 2^6 or more;
+    # the last term is the rounding of numbers below the types' normal range
+    low = 2.0 ** -31 * keys[:, None, None] * 127 * s.plain.v_scale.max()
+    bound = mass * eps + low + np.abs(want) * (plain.EPS[dtype] / 2 + 2.0 ** -23) + (2.0 ** -149 if split else max(plain.TINY[dtype], 2.0 ** -134))
+    err = np.abs(host(out).astype(np.float64) - want)
+    assert (err <= bound).all(), f"{np.nanmax(err / np.maximum(bound, 1e-300)):.2f} of the bound"
+    assert s.status.item() == 0
+    assert np.abs(want).max() > 100 * low.max() or not split
+    return out
+
+
 def want_of(s, heads, q64, dtype, window=0):
     want, mass, big, keys = s.plain.attention(s.table, s.ctx, s.start, q64, None, window)
     return want, plain.attention_bound(want, mass, big, keys, s.dim, dtype, dtype == "float32")
@@ -101,3 +122,29 @@ def test_pages_in_front_of_a_window_are_gone(gpu, dtype, page, seqs, window):
             table[i, p] = number
         s.batch = s.rows_of(max(n for _, n in seqs), table=table)
         assert torch.equal(first, check_attention(s, 16, dtype, window=window, q=q))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("q_scale", [1e4, 1e8, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("seqs,heads", [([(300, 100), (0, 130), (64, 70)], 8), ([(300, 2), (5000, 1)], 8), ([(3000, 90)], 16)])
+def test_scores_far_beyond_softmaxs_range(gpu, dtype, q_scale, seqs, heads):
+    """One key has all of the weight: where the best two scores differ by more than their errors, the output is its value."""
+    s = Setup(gpu, seqs, 4, 64, 16, seed=35)
+    q, q64 = s.normal(heads, dtype, q_scale)
+    out = host(check_relative(s, heads, dtype, (q, q64))).astype(np.float64)
+    n_clear = 0
+    for i, (c, n) in enumerate(s.seqs):
+        k, v = s.plain.values("k", s.table[i], c + n), s.plain.values("v", s.table[i], c + n)
+        for j in range(n):
+            r = int(s.start[i]) + j
+            for h in range(heads):
+                g = h // (heads // 4)
+                score = k[:c + j + 1, g] @ q64[r, h] / 8
+                best = int(score.argmax())
+                # a score is off by 2^-17 of the sum of its terms' magnitudes at most (queries in 22 bits, 8 additions cut off, roundings); 40: weights below e^-40
+                if (score[best] - np.delete(score, best)).min(initial=np.inf) < 2.0 ** -16 * (np.abs(k[:c + j + 1, g]) @ np.abs(q64[r, h]) / 8).max() + 40:
+                    continue
+                n_clear += 1
+                # the value is an integer times two roundings' scale, its weight over itself rounded to 11 bits, then the output's rounding
+                assert (np.abs(out[r, h] - v[best, g]) <= np.abs(v[best, g]) * (plain.EPS[dtype] / 2 + 2.0 ** -20 + (dtype != "float32") * 2.0 ** -10) + 1e-12).all(), (r, h)
+    assert n_clear > s.rows * heads / 2
