@@ -7,8 +7,8 @@
 //   warps 8-11, 14, 15   unpack them to f16 (K as [key][dim], V as [dim][key], 128-byte swizzle);
 //   warp 12          one thread issues the products.  With the unpacking in the same warps an iteration took 9,500 cycles instead of 4,000: the issue waits
 //                    for the matrix unit's queue.
-// Scores: S = Q K^T, the queries times one power of two for the whole unit; f32 queries as f16 high and low parts, two products.
-// Weights: with f the key's scale factor (scale log2 e S_k) and S_v of the key's page, P_j = 2^(s_j f_j + log2 S_v,j - M + 6), M the row's largest exponent so far: the
+// Scores: S = Q K^T, each row of queries times a power of two of its own; f32 queries as f16 high and low parts, two products.
+// Weights: with f the score's factor (scale log2 e S_k over the row's power of two) and S_v of the key's page, P_j = 2^(s_j f_j + log2 S_v,j - M + 6), M the row's largest exponent so far: the
 // value's scale is in the weight, so a page's scale costs an addition per 16 keys; the denominator is sum P_j / S_v,j.  P goes back into the place of S, as f16
 // (f32: high and low parts).  O = P V:
 //   f32             a key tile's sums are added to the row's in registers: what the matrix unit cuts off when it adds stays within a tile of keys (2,048 keys in
@@ -34,7 +34,7 @@ constexpr int kKeys = 128, kTileThreads = 512, kConvWarps = 6, kSlots = 4;
 constexpr int kLaunchRegs = 128;
 constexpr int kGroups = kKeys / 16;
 
-// what the softmax needs to know of 16 keys: score factor, log2 of the values' scale, its inverse; and what the unpacking does
+// what the softmax needs to know of 16 keys: their scale, log2 of the values' scale, its inverse; and what the unpacking does
 enum : int { kHere = 0, kAbsent = 1, kOutside = 2, kZeroValues = 4 };  // not among the unit's keys: zeros; outside the pool: keys of NaN
 struct GroupConst {
     float f, lv, inv;
@@ -49,7 +49,7 @@ struct TileShared {
     GroupConst consts[kSlots][kGroups];
     uint2 sums[kTileThreads / 32];
     uint32_t tmem;
-    float top;
+    uint8_t down[kTileRows2];                  // exponents of the factors that undo the rows' powers of two
 };
 
 template <int HD, bool SPLIT> struct TileShape {
@@ -155,7 +155,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         for (int t = 0; t < kSlots; t++) mbar_init(&sh.c_full[t], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
-        sh.top = 0.0f;
     }
     if (warp == 0) tmem_alloc(&sh.tmem, 512);
     tc_fence_before();
@@ -164,36 +163,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
     const uint32_t tmem = sh.tmem;
     const uint32_t col_s[2] = {tmem, tmem + 128}, col_o[2] = {tmem + 256, tmem + 384};
 
-    // the queries: their largest magnitude, then f16 in place
+    // the queries as f16, each row times a power of two of its own: what a row gives does not depend on the others
     {
-        constexpr int C = HD / 16;
-        const int chunks = n_tiles * 128 * C;
-        float top = 0.0f;
-        for (int e = tid; e < chunks; e += kTileThreads) {
-            const int r = e / C, ch = e % C;
-            if (r < row_n && ch * 16 < hd) {
-                float v[16];
-                load16(a.q, row_at(r, a.q_stride) + ch * 16, a.typ, a.q_vec, v);
-#pragma unroll
-                for (int x = 0; x < 16; x++) top = fabsf(v[x]) < INFINITY ? fmaxf(top, fabsf(v[x])) : top;
-            }
-        }
-        top = warp_max(top);
-        if (lane == 0) atomicMax(reinterpret_cast<int*>(&sh.top), __float_as_int(top));  // not negative: ordered as integers
-    }
-    __syncthreads();
-    float up, down;
-    row_scale(sh.top, up, down);
-    {
-        constexpr int C = HD / 16;
+        constexpr int C = HD / 16;  // lanes of a row, neighbours in a warp
         const int chunks = n_tiles * 128 * C;
         for (int e = tid; e < chunks; e += kTileThreads) {
             const int r = e / C, ch = e % C;
-            float v[16];
+            float v[16], top = 0.0f;
             if (r < row_n && ch * 16 < hd) load16(a.q, row_at(r, a.q_stride) + ch * 16, a.typ, a.q_vec, v);
             else
 #pragma unroll
                 for (int x = 0; x < 16; x++) v[x] = 0.0f;
+#pragma unroll
+            for (int x = 0; x < 16; x++) top = fmaxf(top, fabsf(v[x]));
+#pragma unroll
+            for (int o = C / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            float up, down;
+            row_scale(top, up, down);
+            if (ch == 0) sh.down[r] = (uint8_t)(__float_as_uint(down) >> 23);
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int x = 0; x < 8; x++) {
@@ -273,7 +260,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             // -------------------------------------------------------------------------------------------------- copies
             const int32_t* table = seqs.table + (size_t)seq * seqs.width;
             const int page_mask = (1 << pool.page_shift) - 1;
-            const float k_factor = a.scale_log2 * down;
             const uint32_t bytes = 16 * hd;
             auto look_up = [&](int i) {  // lane g < 8: the page of group g: -1 in front of every row's window and behind the end, -2 outside the pool
                 const int key = (tile0 + i) * kKeys + lane * 16;
@@ -299,10 +285,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         // a page of zeros counts in the denominator alone: its weights take the scale of its neighbours, its values are zeros
                         if (lv == kNegInf) lv = most == kNegInf ? 0.0f : most;
                         if (lane < kGroups) {
-                            // a score factor of 0 as 2^-100, so that a masked score of minus infinity stays one
-                            const float f = page < 0 ? 1.0f : ksc * k_factor;
                             GroupConst g;
-                            g.f = f == 0.0f ? 0x1p-100f : f;
+                            g.f = page < 0 ? 1.0f : ksc;
                             g.lv = lv;
                             g.inv = exp2f(-lv);
                             g.state = page == -1 ? kAbsent : page == -2 ? kOutside : vsc == 0.0f ? kZeroValues : kHere;
@@ -397,13 +381,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         const uint32_t my_s = col_s[t] + lanes, my_o = col_o[t] + lanes;
         const int limit = w.ctx + (row_lo + min(r, row_n - 1)) / a.group;      // last position that the row sees
         const int least = __shfl_sync(0xffffffffu, limit, 0), most = __shfl_sync(0xffffffffu, limit, 31);
+        // The row's part of a score's factor; the page's is its keys' scale.  A factor of 0 as 2^-100, so that a masked score of minus infinity stays one (what it
+        // stands for is below 2^-69: a sum of products is below 2^31)
+        const float row_f = a.scale_log2 * __uint_as_float((uint32_t)sh.down[r] << 23);
+        auto factor = [&](float f) { return max_nan(f * row_f, 0x1p-100f); };
         float o[HD], m = kNegInf, l = 0.0f, corr = 1.0f;
         bool ok = true, far = false;
         // Rounded as the scores of a far reference are (below), so that the largest of these is no more than a rounding of S_v from it.
         auto exponent = [](float x, float f, float lv) { return __fadd_rn(__fmul_rn(x, f), lv); };
         // Far from 0 a reference has no bits left for what is added to it, and a product that is rounded with it may be off by more than f16's range
         // (scores of 1e8: 2^4).  There a score is rounded by itself, as the reference was, and what remains over it goes on; without loss in a neighbourhood of the reference.
-        auto is_far = [](float mx) { return __any_sync(0xffffffffu, fabsf(mx) > 65536.0f && mx != kNegInf); };
+        auto is_far = [](float mx) { return fabsf(mx) > 65536.0f && mx != kNegInf; };
         auto over = [](float x, float f, float ref, float lv) {
             const float y = __fsub_rn(__fmul_rn(x, f), ref);
             return y > 9.0f - lv ? 9.0f - lv : y;  // 2^15 at most; NaN stays
@@ -453,11 +441,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
 #pragma unroll
                             for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(x[16 * h + e]));
                             const GroupConst k = gc[c / 16 + h];
-                            mx = fmaxf(mx, exponent(g, k.f, k.lv));
+                            mx = fmaxf(mx, exponent(g, factor(k.f), k.lv));
                         }
                     }
                     const float ref = mx == kNegInf ? 0.0f : mx;
                     far = is_far(mx);
+                    const bool any_far = __any_sync(0xffffffffu, far);
                     const float less = far ? 6.0f : 6.0f - ref;
                     corr = exp2_fast(m - ref);
                     m = mx;
@@ -468,14 +457,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         tmem_ld16(my_s + c, x);
                         tmem_wait_ld();
                         const GroupConst k = gc[c / 16];
-                        const float off = k.lv + less, f = far ? 1.0f : k.f;
+                        const float off = k.lv + less, f = far ? 1.0f : factor(k.f);
                         if (!plain)
 #pragma unroll
                             for (int e = 0; e < 16; e++)
                                 if (c + e > to || c + e < from) x[e] = __float_as_uint(kNegInf);
-                        if (far)
+                        if (any_far)
 #pragma unroll
-                            for (int e = 0; e < 16; e++) x[e] = __float_as_uint(over(__uint_as_float(x[e]), k.f, ref, k.lv));
+                            for (int e = 0; e < 16; e++) x[e] = far ? __float_as_uint(over(__uint_as_float(x[e]), factor(k.f), ref, k.lv)) : x[e];
                         const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
                         float2 gs = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -504,7 +493,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
 #pragma unroll
                         for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(x[c + e]));
                         const GroupConst k = gc[c / 16];
-                        mx = fmaxf(mx, exponent(g, k.f, k.lv));
+                        mx = fmaxf(mx, exponent(g, factor(k.f), k.lv));
                     }
                     const bool raise = mx > m + 8.0f;  // also from minus infinity
                     if (__any_sync(0xffffffffu, raise)) {
@@ -529,18 +518,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                     }
                     const float ref = m == kNegInf ? 0.0f : m;
                     const float less = far ? 6.0f : 6.0f - ref;
-                    if (far)
+                    if (__any_sync(0xffffffffu, far))
 #pragma unroll
                         for (int c = 0; c < kKeys; c += 16) {
                             const GroupConst k = gc[c / 16];
 #pragma unroll
-                            for (int e = 0; e < 16; e++) x[c + e] = __float_as_uint(over(__uint_as_float(x[c + e]), k.f, ref, k.lv));
+                            for (int e = 0; e < 16; e++) x[c + e] = far ? __float_as_uint(over(__uint_as_float(x[c + e]), factor(k.f), ref, k.lv)) : x[c + e];
                         }
 #pragma unroll
                     for (int c = 0; c < kKeys; c += 16) {
                         uint32_t p[8];
                         const GroupConst k = gc[c / 16];
-                        const float off = k.lv + less, f = far ? 1.0f : k.f;
+                        const float off = k.lv + less, f = far ? 1.0f : factor(k.f);
                         const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
                         float2 gs = make_float2(0.0f, 0.0f);
 #pragma unroll

@@ -148,3 +148,28 @@ def test_scores_far_beyond_softmaxs_range(gpu, dtype, q_scale, seqs, heads):
                 # the value is an integer times two roundings' scale, its weight over itself rounded to 11 bits, then the output's rounding
                 assert (np.abs(out[r, h] - v[best, g]) <= np.abs(v[best, g]) * (plain.EPS[dtype] / 2 + 2.0 ** -20 + (dtype != "float32") * 2.0 ** -10) + 1e-12).all(), (r, h)
     assert n_clear > s.rows * heads / 2
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("heads,kv,dim,seqs", [(8, 4, 128, [(300, 100), (0, 130), (64, 70)]), (8, 8, 64, [(600, 200), (33, 129)]), (12, 4, 96, [(40, 90)] * 3)])
+def test_rows_of_very_different_size_side_by_side(gpu, dtype, heads, kv, dim, seqs):
+    """What a row gives does not depend on how large the others of its call are."""
+    s = Setup(gpu, seqs, kv, dim, 16, seed=41)
+    q, q64 = s.normal(heads, dtype)
+    alone = check_attention(s, heads, dtype, q=(q, q64)).clone()
+    large = s.rng.random(s.rows) < 0.5
+    up = 2.0 ** 12 if dtype == "float16" else 2.0 ** 40                 # exact in every type
+    q64 = q64 * np.where(large, up, 1.0)[:, None, None]
+    q = torch.from_numpy(q64).to(DT[dtype]).cuda()
+    assert np.array_equal(q.double().cpu().numpy(), q64)
+    both = check_relative(s, heads, dtype, (q, q64))
+    assert torch.equal(both[~large], alone[~large])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("sizes", [(-12, 12), (-25, -5)])
+def test_rows_of_all_sizes(gpu, dtype, sizes):
+    s = Setup(gpu, [(200, 128), (70, 80)], 4, 64, 16, seed=42)
+    q64 = s.rng.normal(0, 1, (s.rows, 16, 64)) * 10.0 ** s.rng.uniform(*sizes, (s.rows, 16, 1))
+    q = torch.from_numpy(q64).to(DT[dtype])
+    check_relative(s, 16, dtype, (q.cuda(), q.double().numpy()))
