@@ -49,7 +49,7 @@ struct TileShared {
     GroupConst consts[kSlots][kGroups];
     uint2 sums[kTileThreads / 32];
     uint32_t tmem;
-    uint8_t down[kTileRows2];                  // exponents of the factors that undo the rows' powers of two
+    uint8_t down[kTileRows2];                  // exponents of the factors that undo the rows' powers of two; 255: a row that is not finite
 };
 
 template <int HD, bool SPLIT> struct TileShape {
@@ -175,12 +175,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
 #pragma unroll
                 for (int x = 0; x < 16; x++) v[x] = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 16; x++) top = fmaxf(top, fabsf(v[x]));
+            for (int x = 0; x < 16; x++) top = max_nan(top, fabsf(v[x]));
 #pragma unroll
-            for (int o = C / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int o = C / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
             float up, down;
             row_scale(top, up, down);
-            if (ch == 0) sh.down[r] = (uint8_t)(__float_as_uint(down) >> 23);
+            if (ch == 0) sh.down[r] = top < INFINITY ? (uint8_t)(__float_as_uint(down) >> 23) : 255;
             uint32_t hi[8], lo[8];
 #pragma unroll
             for (int x = 0; x < 8; x++) {
@@ -382,8 +382,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         const int limit = w.ctx + (row_lo + min(r, row_n - 1)) / a.group;      // last position that the row sees
         const int least = __shfl_sync(0xffffffffu, limit, 0), most = __shfl_sync(0xffffffffu, limit, 31);
         // The row's part of a score's factor; the page's is its keys' scale.  A factor of 0 as 2^-100, so that a masked score of minus infinity stays one (what it
-        // stands for is below 2^-69: a sum of products is below 2^31)
-        const float row_f = a.scale_log2 * __uint_as_float((uint32_t)sh.down[r] << 23);
+        // stands for is below 2^-69: a sum of products is below 2^31).  NaN for a row that is not finite, whose scores may all be minus infinity, as masked ones are.
+        const float row_f = sh.down[r] == 255 ? __int_as_float(0x7fffffff) : a.scale_log2 * __uint_as_float((uint32_t)sh.down[r] << 23);
         auto factor = [&](float f) { return max_nan(f * row_f, 0x1p-100f); };
         float o[HD], m = kNegInf, l = 0.0f, corr = 1.0f;
         bool ok = true, far = false;

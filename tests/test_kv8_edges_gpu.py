@@ -173,3 +173,31 @@ def test_rows_of_all_sizes(gpu, dtype, sizes):
     q64 = s.rng.normal(0, 1, (s.rows, 16, 64)) * 10.0 ** s.rng.uniform(*sizes, (s.rows, 16, 1))
     q = torch.from_numpy(q64).to(DT[dtype])
     check_relative(s, 16, dtype, (q.cuda(), q.double().numpy()))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("heads,kv,seqs", [(16, 4, [(0, 130), (5, 70), (300, 64)]), (4, 4, [(0, 3), (40, 1), (700, 4)])])
+def test_rows_that_are_not_finite(gpu, dtype, heads, kv, seqs):
+    """A row with an infinity or NaN is NaN, the first one of a prompt, which sees one key, among them; the others are as ever."""
+    s = Setup(gpu, seqs, kv, 64, 16, seed=51)
+    s.plain.k[..., 3] = np.where(s.plain.k[..., 3] == 0, -5, -np.abs(s.plain.k[..., 3]))   # one sign: an infinity alone gives scores of minus infinity
+    s.pools[0].copy_(torch.from_numpy(s.plain.k))
+    q, q64 = s.normal(heads, dtype)
+    bad = {}
+    for i, (at, n) in enumerate(zip(s.start, np.diff(s.start))):
+        for j, x in enumerate((math.inf, -math.inf, math.nan)):
+            if j < n:
+                bad[int(at) + (j if i != 1 else n - 1 - j)] = (x, (i + j) % heads)
+    for r, (x, h) in bad.items():
+        q[r, h, 3] = x
+        q64[r, h] = 0.0
+    out = torch.zeros_like(q)
+    s.cache.attention(s.batch, q, out)
+    want, bound = want_of(s, heads, q64, dtype)
+    out = host(out).astype(np.float64)
+    nan = np.zeros(out.shape[:2], bool)
+    for r, (x, h) in bad.items():
+        nan[r, h] = True
+    assert np.isnan(out[nan]).all()
+    assert (np.abs(out - want)[~nan] <= bound[~nan]).all()
+    assert s.status.item() == 0
