@@ -192,7 +192,8 @@ int32_t lc_kv8_read_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows, uint
 /* Attention of the rows over the cache (the core of rust/src/inference/attention.rs:69-113, as lc_attention_decode_dev): each row of q_dev
  * [n_rows][n_heads][head_dim], already rotated, attends to the positions up to its own, which the cache already holds (append first), and
  * with window > 0 only to the last `window` of them: pages that lie wholly in front of the first row's window are not looked at.  Scores are q . k * scale (0: 1 / sqrt(head_dim); 2e38 at most).  Queries of any finite size are taken as long as scores stay below 2^126; a
- * row with one that is not finite gives NaN.  Softmax and sums are in f32, its weights in 11 bits (f32: 22).  The values' scales of a sequence and head may differ by factors up to 2^100.
+ * row with one that is not finite gives NaN.  Softmax and sums are in f32, its weights in 11 bits (f32: 22).  The values' scales are
+ * 2^64 at most, and those below 2^-64 of the largest of their sequence and head, or below 2^-140, may count as 0.
  * A call is refused where its work, with every context as long as its table, could not be counted in 31 bits.  Taken for sure: (n_rows * heads per kv head / 256 + n_seqs) * n_kv_heads * (positions
  * of a table / 16 + 6) below 2^31 and n_rows * n_heads up to 2^27; with heads above 128 the first factor is n_rows * heads per kv head / 16 + n_seqs.
  * The workspace is the caller's: lc_attention_kv8_workspace says how many bytes, for any contexts and any calls of this typ over this cache and these heads

@@ -8,8 +8,8 @@
 //   warp 12          one thread issues the products.  With the unpacking in the same warps an iteration took 9,500 cycles instead of 4,000: the issue waits
 //                    for the matrix unit's queue.
 // Scores: S = Q K^T, each row of queries times a power of two of its own; f32 queries as f16 high and low parts, two products.
-// Weights: with f the score's factor (scale log2 e S_k over the row's power of two) and S_v of the key's page, P_j = 2^(s_j f_j + log2 S_v,j - M + 6), M the row's largest exponent so far: the
-// value's scale is in the weight, so a page's scale costs an addition per 16 keys; the denominator is sum P_j / S_v,j.  P goes back into the place of S, as f16
+// Weights: with f the score's factor (scale log2 e S_k over the row's power of two) and S_v of the key's page over a power of two (the first page's), P_j = 2^(s_j f_j + log2 S_v,j - M + 6), M the row's largest exponent so far: the
+// value's scale is in the weight, so a page's scale costs an addition per 16 keys; the denominator is sum P_j / S_v,j, and the power of two multiplies what is written.  P goes back into the place of S, as f16
 // (f32: high and low parts).  O = P V:
 //   f32             a key tile's sums are added to the row's in registers: what the matrix unit cuts off when it adds stays within a tile of keys (2,048 keys in
 //                   its own sums were off by 1e-5);
@@ -49,6 +49,7 @@ struct TileShared {
     GroupConst consts[kSlots][kGroups];
     uint2 sums[kTileThreads / 32];
     uint32_t tmem;
+    float base;                                // what the values' scales of the unit are relative to
     uint8_t down[kTileRows2];                  // exponents of the factors that undo the rows' powers of two; 255: a row that is not finite
 };
 
@@ -155,6 +156,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         for (int t = 0; t < kSlots; t++) mbar_init(&sh.c_full[t], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
+        sh.base = 1.0f;
     }
     if (warp == 0) tmem_alloc(&sh.tmem, 512);
     tc_fence_before();
@@ -261,11 +263,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             const int32_t* table = seqs.table + (size_t)seq * seqs.width;
             const int page_mask = (1 << pool.page_shift) - 1;
             const uint32_t bytes = 16 * hd;
-            auto look_up = [&](int i) {  // lane g < 8: the page of group g: -1 in front of every row's window and behind the end, -2 outside the pool
-                const int key = (tile0 + i) * kKeys + lane * 16;
-                if (lane >= kGroups || i >= n || key + 15 < key_lo || key >= key_end) return -1;
+            auto page_of = [&](int i, int group) {  // -1 in front of every row's window and behind the end, -2 outside the pool
+                const int key = (tile0 + i) * kKeys + group * 16;
+                if (i >= n || key + 15 < key_lo || key >= key_end) return -1;
                 const int p = table[key >> pool.page_shift];
                 return p >= 0 && p < pool.n_pages ? p : -2;
+            };
+            auto look_up = [&](int i) { return lane < kGroups ? page_of(i, lane) : -1; };  // lane g < 8: the page of group g
+            // log2 of a scale of values over `base`, which is the first that is not 0, as a power of two between 2^-56 and 2^56; minus infinity for pages that count as zeros: 2^-90 of it
+            // and less.  All lanes take part; `low` is the smallest so far.
+            float base = 0.0f, to_base = 1.0f, low = INFINITY;
+            auto log_scale = [&](float vsc) {
+                const uint32_t which = __ballot_sync(0xffffffffu, vsc != 0.0f);
+                if (base == 0.0f && which) {
+                    const uint32_t e = (__float_as_uint(__shfl_sync(0xffffffffu, vsc, __ffs(which) - 1)) >> 23) & 0xff;
+                    const uint32_t at = min(max(e, 127u - 56u), 127u + 56u);
+                    base = __uint_as_float(at << 23);
+                    to_base = __uint_as_float((254u - at) << 23);
+                    if (lane == 0) sh.base = base;
+                }
+                float lv = vsc != 0.0f ? log2f(vsc * to_base) : kNegInf;
+                if (lv < -90.0f) lv = kNegInf;
+                float least = lv == kNegInf ? INFINITY : lv;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+                low = fminf(low, least);
+                return lv;
             };
             int page = look_up(0);
             bool ok = true;
@@ -279,17 +302,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                     if (i > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.raw_free[x], (i - 1) & 1));
                     if (!ok) break;
                     if (x == 0) {
-                        float lv = page >= 0 && vsc != 0.0f ? log2f(vsc) : kNegInf, most = lv;
-#pragma unroll
-                        for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                        // a page of zeros counts in the denominator alone: its weights take the scale of its neighbours, its values are zeros
-                        if (lv == kNegInf) lv = most == kNegInf ? 0.0f : most;
+                        float lv = log_scale(vsc);
+                        const bool counts = lv != kNegInf;
+                        // A page of zeros counts in the denominator alone: its weights take the smallest scale so far (where there is none, that of the first pages that have one), so that
+                        // they do not lift the reference above what the other pages' weights need, and its values are zeros.
+                        if (i == 0 && low == INFINITY)
+                            for (int k = 1; k < n && low == INFINITY; k += 4) {
+                                const int p = page_of(k + (lane >> 3), lane & 7);
+                                (void)log_scale(p >= 0 ? pool.v_scale[(size_t)p * pool.n_kv + kvh] : 0.0f);
+                            }
+                        if (!counts) lv = low == INFINITY ? 0.0f : low;
                         if (lane < kGroups) {
                             GroupConst g;
                             g.f = page < 0 ? 1.0f : ksc;
                             g.lv = lv;
                             g.inv = exp2f(-lv);
-                            g.state = page == -1 ? kAbsent : page == -2 ? kOutside : vsc == 0.0f ? kZeroValues : kHere;
+                            g.state = page == -1 ? kAbsent : page == -2 ? kOutside : counts ? kHere : kZeroValues;
                             sh.consts[i % kSlots][lane] = g;
                             if (page == -2) kv8_raise(seqs, seq);
                         }
@@ -554,6 +582,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
             if (ok) add_up(n - 1);
             if (!ok || isnan(l)) l = __int_as_float(0x7fffffff);
             if (!ok && lane == 0) kv8_raise(seqs, seq);
+            const float base = sh.base;  // behind the last tile's consts
             if (r < row_n) {
                 if (splits == 1) {
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -562,7 +591,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                     for (int d = 0; d < HD; d += 16) {
                         float v[16];
 #pragma unroll
-                        for (int e = 0; e < 16; e++) v[e] = o[((d + e) >> 2) + ((d + e) & 3) * (HD / 4)] * inv;
+                        for (int e = 0; e < 16; e++) v[e] = o[((d + e) >> 2) + ((d + e) & 3) * (HD / 4)] * inv * base;
                         if (d < hd) store16(a.out, dst + d, a.typ, a.out_vec, v);
                     }
                 } else {
@@ -572,7 +601,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                     for (int d = 0; d < HD; d += 16) {
                         float v[16];
 #pragma unroll
-                        for (int e = 0; e < 16; e++) v[e] = o[((d + e) >> 2) + ((d + e) & 3) * (HD / 4)];
+                        for (int e = 0; e < 16; e++) v[e] = o[((d + e) >> 2) + ((d + e) & 3) * (HD / 4)] * base;
                         store16(part + 2 * kTileRows2 + (size_t)r * HD + d, true, v);
                     }
                 }

@@ -201,3 +201,35 @@ def test_rows_that_are_not_finite(gpu, dtype, heads, kv, seqs):
     assert np.isnan(out[nan]).all()
     assert (np.abs(out - want)[~nan] <= bound[~nan]).all()
     assert s.status.item() == 0
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("where", ["first", "middle", "last", "all but one"])
+@pytest.mark.parametrize("exponent", [0, -16, -40, -110, -130])
+@pytest.mark.parametrize("page", [16, 128])
+def test_tiles_of_values_that_are_zero(gpu, dtype, where, exponent, page):
+    """128 keys whose values have scale 0 count in the denominator alone, however small the scales of the others are."""
+    s = Setup(gpu, [(520, 70), (384, 128), (700, 64)], 4, 64, page, seed=61)
+    s.plain.v_scale *= np.float32(2.0) ** np.float32(exponent / 2)      # in two steps: the power itself may be below the smallest number
+    s.plain.v_scale *= np.float32(2.0) ** np.float32(exponent / 2)
+    per = 128 // page
+    for i, (c, n) in enumerate(s.seqs):
+        tiles = -(-(c + n) // 128)
+        zero = {"first": [0], "middle": [tiles // 2], "last": [tiles - 1], "all but one": [t for t in range(tiles) if t != 2]}[where]
+        for t in zero:
+            for p in s.table[i, t * per:(t + 1) * per]:
+                if p >= 0:
+                    s.plain.v_scale[p] = 0.0
+    s.pools[3].copy_(torch.from_numpy(s.plain.v_scale))
+    check_relative(s, 16, dtype, s.normal(16, dtype))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("small", [2.0 ** -50, 1e-39, 1e-44])
+def test_a_page_of_values_next_to_nothing(gpu, dtype, small):
+    """One page whose values are all but zero, among others: as good as zeros, for every row."""
+    s = Setup(gpu, [(520, 70), (384, 128), (700, 64), (5, 1)], 4, 64, 16, seed=62)
+    for i, p in ((0, 3), (1, 0), (2, 40)):
+        s.plain.v_scale[s.table[i, p]] = small
+    s.pools[3].copy_(torch.from_numpy(s.plain.v_scale))
+    check_relative(s, 16, dtype, s.normal(16, dtype))
