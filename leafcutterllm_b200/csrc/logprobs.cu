@@ -23,13 +23,16 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32, kChunkElems = 16, kMaxCluster = 8, kMaxTop = 32, kList = 128, kGroups = kThreads / 4;
 
+// e^-200 is 0 in f32; a difference of logits may be minus infinity, and 0 times that is not 0
+constexpr float kLeastExponent = -200.0f;
+
 struct Sums {
     float m;
     double s, t;
 };
 // Of the sums in the lanes of a warp (m minus infinity: none), in all lanes.
 __device__ __forceinline__ Sums join_lanes(Sums a) {
-    const float m = warp_max(a.m), d = a.m - m;
+    const float m = warp_max(a.m), d = fmaxf(a.m - m, kLeastExponent);
     const double f = a.m == -INFINITY ? 0.0 : (double)expf(d);
     double s = f * a.s, t = a.m == -INFINITY ? 0.0 : f * (a.t + (double)d * a.s);
 #pragma unroll
@@ -185,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(LogprobArgs
         if (__any_sync(0xffffffffu, top > m)) {
             const float now = warp_max(fmaxf(top, m));
             if (m != -INFINITY) {
-                const float dm = m - now;
+                const float dm = fmaxf(m - now, kLeastExponent);
                 const double f = expf(dm);
                 sum_t = f * (sum_t + (double)dm * sum_s);
                 sum_s = f * sum_s;
@@ -198,8 +201,8 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(LogprobArgs
 #pragma unroll
             for (int e = 0; e < kChunkElems; e += 2) {
                 float2 d = add2(make_float2(x[e], x[e + 1]), less);
-                d.x = fmaxf(d.x, -200.0f);  // e^-200 is 0 here; keeps 0 * -inf out
-                d.y = fmaxf(d.y, -200.0f);
+                d.x = fmaxf(d.x, kLeastExponent);
+                d.y = fmaxf(d.y, kLeastExponent);
                 const float2 y = mul2(d, log2e);
                 const float2 p = make_float2(exp2_fast(y.x), exp2_fast(y.y));
                 s = add2(s, p);
