@@ -182,13 +182,13 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
             pages = w.inside && st < s1 ? table[((w.step0 + st) * kStep) >> pool.page_shift] : -1;
         };
         look_up();
-        bool poisoned = !w.inside;
         auto fetch = [&](int st) {
             if (st - pages_at == 32) { pages_at += 32; look_up(); }
             if (st < s1 && w.inside) {
                 const int number = __shfl_sync(0xffffffffu, pages, st - pages_at);
                 if (number < 0 || number >= pool.n_pages) {
-                    poisoned = true;
+                    // a page outside the pool: with a scale of NaN the scores of rows that see it are, those of others are masked; its values, whatever is in their place, count nothing
+                    if (lane < 2) *reinterpret_cast<float*>(mine + (st % S) * Shape::kStageBytes + 2 * kStep * HD + lane * 4) = lane ? 0.0f : __int_as_float(0x7fffffff);
                     if (lane == 0) kv8_raise(seqs, at.seq);
                 } else {
                     const uint32_t dst = ring + (uint32_t)(st % S) * Shape::kStageBytes;
@@ -473,7 +473,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
             float sum = l[gr];
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (poisoned) sum = __int_as_float(0x7fffffff);
+            if (!w.inside) sum = __int_as_float(0x7fffffff);
             const bool whole = starts && ends;
             if (!whole && c == 0 && 8 * gr + g < row_n) { part[8 * gr + g] = m[gr]; part[RB + 8 * gr + g] = sum; }
 #pragma unroll

@@ -233,3 +233,27 @@ def test_a_page_of_values_next_to_nothing(gpu, dtype, small):
         s.plain.v_scale[s.table[i, p]] = small
     s.pools[3].copy_(torch.from_numpy(s.plain.v_scale))
     check_relative(s, 16, dtype, s.normal(16, dtype))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("heads,kv,new", [(4, 2, 5), (4, 4, 20), (1, 1, 2), (16, 4, 80)])
+@pytest.mark.parametrize("window", [0, 9])
+def test_rows_that_do_not_need_a_bad_page(gpu, dtype, heads, kv, new, window):
+    """A page outside the pool makes NaN of the rows that see a position of it; rows in front of it, and those whose window has left it, are as ever."""
+    seqs = [(46, new), (300, new), (17, new)]
+    for i, page in ((0, 3), (1, 300 // 16), (1, (300 + new - 1) // 16), (2, 1)):
+        s = Setup(gpu, seqs, kv, 64, 16, seed=71)
+        q, q64 = s.normal(heads, dtype)
+        want, bound = want_of(s, heads, q64, dtype, window)
+        table = s.table.copy()
+        table[i, page] = (-1, 10 ** 6)[page % 2]
+        out = torch.full_like(q, 7.0)
+        s.cache.attention(s.rows_of(new, table=table), q, out, window=window)
+        out = host(out).astype(np.float64)
+        bad = np.zeros(s.rows, bool)
+        for j in range(new):
+            pos = seqs[i][0] + j
+            bad[s.start[i] + j] = page * 16 <= pos and (not window or page * 16 + 15 > pos - window)
+        assert np.isnan(out[bad]).all()
+        assert (np.abs(out - want)[~bad] <= bound[~bad]).all()
+        assert s.status.item() == (i + 1 if bad.any() else 0)
