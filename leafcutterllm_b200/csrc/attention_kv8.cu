@@ -284,7 +284,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
             m[gr] = kNegInf;
             l[gr] = 0.0f;
         }
-        float vref = 0.0f;                   // 16-bit types: what the sums' scales are relative to
+        float vref = 0.0f, vtop = 0.0f;      // 16-bit types: what the sums' scales are relative to; the largest that was
 
         // rows see all keys up to the first row's position (with a window, from the last row's on)
         const int sees = w.ctx + row_lo / a.group, from = a.window > 0 ? w.ctx + (row_lo + row_n - 1) / a.group - a.window : -1;
@@ -351,17 +351,19 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
             }
             float to_weight = 1.0f;
             if (!F32) {
-                // within 2^-8 and 2^4 of the reference a scale goes to the weights; others make a reference of themselves (of 0 nothing is added)
+                // within 2^-8 and 2^4 of the reference a scale goes to the weights; others make a reference of themselves (of 0 nothing is added), but none below 2^-64 of the
+                // largest: the sums, 2^10 x 2^4 x 127 a key, would pass f32's range there
                 const float ratio = fabsf(vsc) / vref;
                 if (vsc != 0.0f && !(ratio >= 0x1p-8f && ratio <= 0x1p4f)) {
-                    const float by = vref > 0.0f ? vref / fabsf(vsc) : 0.0f;
+                    vtop = fmaxf(vtop, fabsf(vsc));
+                    const float now = fmaxf(fabsf(vsc), vtop * 0x1p-64f), by = vref > 0.0f ? vref / now : 0.0f;
 #pragma unroll
                     for (int gr = 0; gr < NG; gr++)
 #pragma unroll
                         for (int t = 0; t < NT; t++)
 #pragma unroll
                             for (int e = 0; e < 4; e++) o[gr][t][e] *= by;
-                    vref = fabsf(vsc);
+                    vref = now;
                 }
                 to_weight = vref > 0.0f ? vsc / vref : 0.0f;
                 if (isnan(vsc)) to_weight = vsc;
@@ -482,7 +484,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 const float total = __shfl_sync(0xffffffffu, sum, 8 * c + 4 * x);
                 if (r >= row_n) continue;
                 // a NaN sum makes all of the row NaN
-                const float inv = (whole ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f) * (F32 ? 1.0f : vref);
+                const float inv = whole ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f, unit = F32 ? 1.0f : vref;  // their product may be below the smallest number
                 const int tok = (row_lo + r) / a.group, hq = (row_lo + r) - tok * a.group;
                 const int64_t dst = (int64_t)(w.first + tok) * a.out_stride + (int64_t)(at.kvh * a.group + hq) * hd;
                 constexpr int N = HD == 64 ? 8 : 16;  // dims in a row
@@ -490,7 +492,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 for (int half = 0; half < (HD == 256 ? 2 : 1); half++) {
                     float v[N];
 #pragma unroll
-                    for (int e = 0; e < N; e++) v[e] = o[gr][8 * half + (e >> 1)][2 * (e & 1) + x] * inv;
+                    for (int e = 0; e < N; e++) v[e] = o[gr][8 * half + (e >> 1)][2 * (e & 1) + x] * inv * unit;
                     const int d = HD == 64 ? 8 * g : 128 * half + 16 * g;
                     if (!whole) store_run<N>(part + 2 * RB + r * HD + d, true, v);
                     else if (FULL || d < hd) store_run<N>(a.out, dst + d, a.typ, a.out_vec, v);

@@ -257,3 +257,47 @@ def test_rows_that_do_not_need_a_bad_page(gpu, dtype, heads, kv, new, window):
         assert np.isnan(out[bad]).all()
         assert (np.abs(out - want)[~bad] <= bound[~bad]).all()
         assert s.status.item() == (i + 1 if bad.any() else 0)
+
+
+@pytest.mark.parametrize("small", [1e-12, 2.0 ** -100, 1e-38])
+def test_long_sums_in_front_of_far_smaller_values(gpu, small):
+    """Many heavy keys, then pages whose values are far smaller: the sums so far stay what they are."""
+    seqs, kv, dim, steps = 64, 8, 64, 7500
+    # page 0: scores of 0; page 1: scores 3.9 higher in powers of two; page 2: small values.  A run that begins in page 0 holds weights of almost 2^10.
+    k = torch.zeros(3, kv, 16, dim, dtype=torch.int8, device="cuda")
+    k[1, :, :, 0] = 127
+    v = torch.full_like(k, 127)
+    k_scale, v_scale = torch.full((3, kv), 1 / 127, device="cuda"), torch.tensor([1.0, 1.0, small], device="cuda")[:, None].repeat(1, kv)
+    cache = gpu.Kv8Cache(k, v, k_scale, v_scale)
+    number = torch.arange(steps, dtype=torch.int32, device="cuda") % 2
+    number[6000:] = 2
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    rows = gpu.Kv8Rows(number[None].repeat(seqs, 1).contiguous(), i32([steps * 16 - 1] * seqs), torch.arange(seqs + 1, dtype=torch.int32, device="cuda"), 1)
+    q = torch.zeros(seqs, kv, dim, device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 2.6875                                                   # 3.877 log 2
+    out = cache.attention(rows, q, scale=1.0).double().cpu().numpy()
+    e = math.exp(2.6875)
+    want = 127 * (3000 + 3000 * e + 1500 * small) / (4500 + 3000 * e)
+    # the weights' rounding and the matrix unit's additions (2^-23 of the sum each, 26,000 in a run at most, cut off), then bf16
+    assert np.abs(out - want).max() <= want * (2.0 ** -10 + 26000 * 2.0 ** -23 + 2.0 ** -8)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("exponent", [-60, -110, -130])
+def test_values_next_to_the_smallest_numbers(gpu, dtype, exponent):
+    s = Setup(gpu, [(20, 2), (130, 1), (4000, 3)], 2, 64, 16, seed=82)
+    for _ in range(2):
+        s.plain.v_scale *= np.float32(2.0) ** np.float32(exponent / 2)
+    s.pools[3].copy_(torch.from_numpy(s.plain.v_scale))
+    check_relative(s, 4, dtype, s.normal(4, dtype))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("small", [2.0 ** -50, 1e-39, 1e-44])
+def test_a_page_of_values_next_to_nothing_in_runs(gpu, dtype, small):
+    s = Setup(gpu, [(520, 7), (384, 1), (700, 64), (5, 1)], 4, 64, 16, seed=62)
+    for i, p in ((0, 3), (1, 0), (2, 40)):
+        s.plain.v_scale[s.table[i, p]] = small
+    s.pools[3].copy_(torch.from_numpy(s.plain.v_scale))
+    s.batch = s.rows_of(1)
+    check_relative(s, 16, dtype, s.normal(16, dtype))
