@@ -157,8 +157,8 @@ typedef struct lc_kv8_cache {
  * status_dev (may be NULL): a word that a call raises to i + 1, for the highest such i, where sequence i cannot be served: its row_start is
  * not ascending within the call's rows (its rows are left alone), or its positions leave the table or a page that it needs is not
  * in 0 .. n_pages - 1.  Appends skip that page, reads give NaN in the rows on it and attention in the rows that
- * see a position of it; of a sequence that leaves the table appends skip all rows, queries too, and the others give NaN in all of them.  Where a row_start that goes back and forth gives rows to several sequences, those rows may hold any of their results; what the rows of
- * others hold, and memory outside the call's tensors, is as it would be.  No call clears the word.
+ * see a position of it; of a sequence that leaves the table appends skip all rows, queries too, and the others give NaN in all of them.  Sequences that share no rows may stand in any order (the one between two whose row_start goes
+ * back is then raised).  Where sequences share rows, their rows and those of later sequences hold any of their results or stay as they were; memory outside the call's tensors is not touched. No call clears the word.
  * n_seqs: 4096 at most. */
 typedef struct lc_kv8_rows {
     const int32_t* page_table_dev; /* [n_seqs][table_width] */

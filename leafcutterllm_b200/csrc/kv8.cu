@@ -445,8 +445,9 @@ __global__ void __launch_bounds__(256, 3) kv8_append_kernel(Kv8Pool pool, Kv8Seq
     int r = blockIdx.x * a.window;
     const int r_end = min(r + a.window, seqs.n_rows);
     while (r < r_end) {
-        const int i = kv8_seq_of_row(seqs, r);
-        if (i < 0) { r++; continue; }
+        int next;
+        const int i = kv8_seq_of_row(seqs, r, next);
+        if (i < 0) { r = next; continue; }
         int first, n;
         kv8_span(seqs, i, first, n);
         const int ctx = seqs.ctx[i], end = first + n;
@@ -490,7 +491,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8Pool pool, Kv8Seqs seq
     const int64_t units = (int64_t)seqs.n_rows * parts;
     for (int64_t unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); unit < units; unit += warps) {
         const int r = (int)(unit / parts), e = (int)(unit - (int64_t)r * parts) * 32 + lane;
-        const int i = kv8_seq_of_row(seqs, r);
+        int next;
+        const int i = kv8_seq_of_row(seqs, r, next);
         if (i < 0) continue;
         int first, n;
         kv8_span(seqs, i, first, n);

@@ -98,22 +98,38 @@ __device__ __forceinline__ void kv8_check_seqs(const Kv8Seqs& s, const Kv8Pool& 
         if (!kv8_span(s, i, first, n) || (n > 0 && !kv8_in_table(s, p, s.ctx[i], n))) kv8_raise(s, i);
     }
 }
-// By one whole warp: the sequence whose rows row `r` is one of (-1: none), 32 probes a step.
-__device__ __forceinline__ int kv8_seq_of_row(const Kv8Seqs& s, int r) {
+// By one whole warp: the first of all sequences that has row `r` (-1: none), and where there is none the next row that one of them begins with.  For rows that the
+// search below does not find: in front of, between and behind the sequences, or where row_start goes back and forth.
+[[maybe_unused]] static __device__ __noinline__ int2 kv8_seq_among(const int32_t* row_start, int n_seqs, int n_rows, int r) {
+    const int lane = threadIdx.x & 31;
+    int next = 0x7fffffff;
+    for (int i0 = 0; i0 < n_seqs; i0 += 32) {
+        const int i = i0 + lane, a = i < n_seqs ? row_start[i] : 0, b = i < n_seqs ? row_start[i + 1] : 0;
+        const bool rows = a >= 0 && b > a && b <= n_rows;
+        const unsigned has = __ballot_sync(0xffffffffu, rows && r >= a && r < b);
+        if (has) return make_int2(i0 + __ffs(has) - 1, r);
+        if (rows && a > r) next = min(next, a);
+    }
+    return make_int2(-1, __reduce_min_sync(0xffffffffu, next));
+}
+// By one whole warp: the sequence whose rows row `r` is one of (-1: none; `next` is then the next row that has one), 32 probes a step.
+__device__ __forceinline__ int kv8_seq_of_row(const Kv8Seqs& s, int r, int& next) {
     const int lane = threadIdx.x & 31;
     int lo = 0, len = s.n_seqs + 1;
     for (;;) {
         const int step = (len + 31) >> 5, at = lane * step;
         const bool le = at < len && s.row_start[lo + at] <= r;
         const int cnt = __popc(__ballot_sync(0xffffffffu, le));
-        if (cnt == 0) return -1;
+        if (cnt == 0) { lo = s.n_seqs; break; }
         lo += (cnt - 1) * step;
         len = min(step, len - (cnt - 1) * step);
         if (step == 1) break;
     }
-    if (lo >= s.n_seqs) return -1;
     int first, n;
-    return kv8_span(s, lo, first, n) && r - first < n && r >= first ? lo : -1;
+    if (lo < s.n_seqs && kv8_span(s, lo, first, n) && r - first < n && r >= first) return lo;
+    const int2 found = kv8_seq_among(s.row_start, s.n_seqs, s.n_rows, r);
+    next = found.y;
+    return found.x;
 }
 #endif
 

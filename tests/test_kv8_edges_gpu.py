@@ -301,3 +301,35 @@ def test_a_page_of_values_next_to_nothing_in_runs(gpu, dtype, small):
     s.pools[3].copy_(torch.from_numpy(s.plain.v_scale))
     s.batch = s.rows_of(1)
     check_relative(s, 16, dtype, s.normal(16, dtype))
+
+
+@pytest.mark.parametrize("many", [0, 60])
+def test_sequences_that_share_no_rows_in_any_order(gpu, many):
+    """row_start that goes back between sequences which share no rows: the one that goes back is named, the others are served by every call."""
+    seqs = [(20, 8), (0, 0), (50, 12)] + [(5, 0)] * many
+    s = Setup(gpu, seqs, 2, 64, 16, seed=91, tail=20)
+    start = np.array([30, 38, 4, 16] + [16] * many, np.int32)           # rows 30 .. 37, a step back, rows 4 .. 15
+    (k, k64), (v, v64), (q, q64) = s.normal(2, "float32"), s.normal(2, "float32"), s.normal(4, "float32")
+    batch = s.rows_of(12, start=start)
+    turned = torch.full_like(q, 7.0)
+    turns = gpu.rope_turns(10000.0, 64)
+    s.cache.append(batch, k, v, turns=cuda(turns.view("int64")), q=q, q_out=turned)
+    for i, (a, b) in ((0, (30, 38)), (2, (4, 16))):
+        s.plain.append(s.table[i:i + 1], s.ctx[i:i + 1], [a, b], k64, v64, turns)
+    s.same_cache()
+    inside = np.zeros(s.rows, bool)
+    inside[30:38] = inside[4:16] = True
+    assert (host(turned)[~inside] == 7.0).all() and (host(turned)[inside] != 7.0).any(axis=(1, 2)).all()
+    assert s.status.item() == 2
+    out = torch.full_like(k, 7.0)
+    s.cache.read(batch, k_out=out)
+    assert (host(out)[~inside] == 7.0).all()
+    for i, (a, b), c in ((0, (30, 38), 20), (2, (4, 16), 50)):
+        want = s.plain.values("k", s.table[i], c + b - a)[c:]
+        assert (np.abs(host(out)[a:b] - want) <= np.abs(want) * 2.0 ** -23).all()
+    att = s.cache.attention(batch, q, torch.full_like(q, 7.0))
+    assert (host(att)[~inside] == 7.0).all()
+    for i, (a, b) in ((0, (30, 38)), (2, (4, 16))):
+        want, mass, big, keys = s.plain.attention(s.table[i:i + 1], s.ctx[i:i + 1], [a, b], q64)
+        bound = plain.attention_bound(want, mass, big, keys, 64, "float32", True)
+        assert (np.abs(host(att) - want)[a:b] <= bound[a:b]).all()
