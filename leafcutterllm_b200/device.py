@@ -194,6 +194,8 @@ class Kv8Cache:
         os = _rows(out, heads, self.head_dim, "out")
         if workspace is None:
             workspace = _empty("attention", q, self.attention_workspace(rows, q), _torch().uint8, stream)
+        elif not workspace.is_contiguous():
+            raise ValueError("attention: a contiguous workspace expected")
         if rows.index != index or q.get_device() != index or out.get_device() != index or workspace.get_device() != index:
             _elsewhere(index, q, out, workspace)
         check(load().lc_attention_kv8_dev(self._ref, rows._ref, typ, n, q.data_ptr(), qs, heads, 0.0 if scale is None else scale, window, out.data_ptr(), os,

@@ -26,3 +26,17 @@ def test_arguments_are_checked_all_the_same(lc):
     assert workspace(lc, 0, 0, 3)[0] == lc._capi.LC_ERR_INVALID
     assert workspace(lc, 8, 0, 2)[0] == lc._capi.LC_ERR_UNSUPPORTED
     assert workspace(lc, 0, 0, 2, max_rows=-1)[0] == lc._capi.LC_ERR_INVALID
+
+
+def tensors():
+    import torch
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    return torch, torch.zeros(4, 2, 16, 64, dtype=torch.int8), torch.zeros(4, 2), torch.zeros(2, 3, dtype=torch.int32), i32(0, 0), i32(0, 1, 2)
+
+
+def test_workspaces_with_gaps_are_refused(lc):
+    """Bytes between a view's are not the call's."""
+    torch, k, s, table, ctx, start = tensors()
+    c, r = lc.Kv8Cache(k, k, s, s), lc.Kv8Rows(table, ctx, start, 1)
+    with pytest.raises(ValueError, match="workspace"):
+        c.attention(r, torch.zeros(2, 4, 64), workspace=torch.zeros(1 << 20, dtype=torch.uint8)[::2])
