@@ -147,7 +147,7 @@ class Kv8Cache:
             if q.get_device() != index or q_out.get_device() != index:
                 _elsewhere(index, q, q_out)
         if turns is not None:
-            if turns.element_size() != 8 or turns.is_floating_point() or not turns.is_contiguous() or turns.dim() != 1:
+            if turns.element_size() != 8 or turns.is_floating_point() or turns.is_complex() or not turns.is_contiguous() or turns.dim() != 1:
                 raise ValueError("append: turns are contiguous 64-bit integers")
             if turns.get_device() != index:
                 _elsewhere(index, turns)

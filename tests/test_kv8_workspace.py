@@ -40,3 +40,12 @@ def test_workspaces_with_gaps_are_refused(lc):
     c, r = lc.Kv8Cache(k, k, s, s), lc.Kv8Rows(table, ctx, start, 1)
     with pytest.raises(ValueError, match="workspace"):
         c.attention(r, torch.zeros(2, 4, 64), workspace=torch.zeros(1 << 20, dtype=torch.uint8)[::2])
+
+
+def test_rotation_tables_of_other_types_are_refused(lc):
+    torch, k, s, table, ctx, start = tensors()
+    c, r = lc.Kv8Cache(k, k, s, s), lc.Kv8Rows(table, ctx, start, 1)
+    x = torch.zeros(2, 2, 64)
+    for dtype in (torch.complex64, torch.float64, torch.int32):
+        with pytest.raises(ValueError, match="turns"):
+            c.append(r, x, x, turns=torch.zeros(32, dtype=dtype))
