@@ -198,7 +198,7 @@ class Kv8Cache:
             raise ValueError("attention: a contiguous workspace expected")
         if rows.index != index or q.get_device() != index or out.get_device() != index or workspace.get_device() != index:
             _elsewhere(index, q, out, workspace)
-        check(load().lc_attention_kv8_dev(self._ref, rows._ref, typ, n, q.data_ptr(), qs, heads, 0.0 if scale is None else scale, window, out.data_ptr(), os,
+        check(load().lc_attention_kv8_dev(self._ref, rows._ref, typ, n, q.data_ptr(), qs, heads, 0.0 if scale is None else scale, min(window, 2 ** 31 - 1), out.data_ptr(), os,
                                           workspace.data_ptr(), workspace.nbytes, _stream(index, stream)))
         return out
 

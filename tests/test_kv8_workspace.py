@@ -49,3 +49,25 @@ def test_rotation_tables_of_other_types_are_refused(lc):
     for dtype in (torch.complex64, torch.float64, torch.int32):
         with pytest.raises(ValueError, match="turns"):
             c.append(r, x, x, turns=torch.zeros(32, dtype=dtype))
+
+
+def test_windows_beyond_32_bits(lc, monkeypatch):
+    """As wide as a table can be, not what is left of them in 32 bits."""
+    torch, k, s, table, ctx, start = tensors()
+    c, r = lc.Kv8Cache(k, k, s, s), lc.Kv8Rows(table, ctx, start, 1)
+    seen = []
+
+    class Library:
+        def lc_attention_kv8_dev(self, *a):
+            seen.append(a[8])
+            return lc._capi.LC_OK
+    import leafcutterllm_b200.device as device
+    monkeypatch.setattr(device, "load", lambda: Library())
+    device._torch()
+    monkeypatch.setattr(device, "_raw_stream", lambda index: 0)
+    q, ws = torch.zeros(2, 4, 64), torch.zeros(64, dtype=torch.uint8)
+    for window in (0, 5, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 63 - 1):
+        c.attention(r, q, torch.empty_like(q), window=window, workspace=ws)
+        assert seen[-1] == min(window, 2 ** 31 - 1)
+    c.attention(r, q, torch.empty_like(q), window=-1, workspace=ws)
+    assert seen[-1] == -1                                 # the library refuses it
