@@ -651,6 +651,8 @@ int32_t runs_of(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, con
 int32_t check_heads(const char* call, const Kv8Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {
     LC_CHECK(n_heads > 0 && n_heads <= 65536 && n_heads % pool.n_kv == 0, LC_ERR_INVALID, "%s: %d heads over %d kv heads", call, n_heads, pool.n_kv);
     const int group = n_heads / pool.n_kv;
+    // a sequence outside its table may have all rows: what a call's rows are in the kernels' 32 bits
+    LC_CHECK((int64_t)seqs.n_rows * group < (int64_t)0x7fffffff - kTileRows2, LC_ERR_INVALID, "%s: %d rows of %d heads are too many for one call", call, seqs.n_rows, n_heads);
     LC_CHECK(line_fits(pool, seqs, group, 8 * most_groups(pool)) || tiles_fit(pool, seqs, group), LC_ERR_INVALID, "%s: %d rows of %d heads over tables of %d pages are too many for one call",
              call, seqs.n_rows, n_heads, seqs.width);
     return LC_OK;

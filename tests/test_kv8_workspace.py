@@ -71,3 +71,16 @@ def test_windows_beyond_32_bits(lc, monkeypatch):
         assert seen[-1] == min(window, 2 ** 31 - 1)
     c.attention(r, q, torch.empty_like(q), window=-1, workspace=ws)
     assert seen[-1] == -1                                 # the library refuses it
+
+
+def test_rows_times_heads_beyond_31_bits_are_refused(lc):
+    """The kernels count a sequence's rows times the heads of a group in 32 bits: a sequence outside its table may have all rows, however few pages there are."""
+    from test_kv8 import attend
+    one = cache(lc, n_kv_heads=1, head_dim=16)
+    few = rows(lc, n_seqs=1, table_width=1, max_rows=1)
+    for heads, n in ((256, 1 << 24), (128, 1 << 24), (65536, 1 << 15)):
+        args = dict(c=one, r=few, n=n, heads=heads, qs=heads * 16, os=heads * 16)
+        assert attend(lc, **args) == lc._capi.LC_ERR_INVALID and b"too many" in lc.load().lc_last_error()
+        out = C.c_size_t()
+        assert lc.load().lc_attention_kv8_workspace(C.byref(one), C.byref(few), 30, n, heads, C.byref(out)) == lc._capi.LC_ERR_INVALID
+        assert b"too many" in lc.load().lc_last_error()
