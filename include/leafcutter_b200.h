@@ -192,7 +192,8 @@ int32_t lc_kv8_read_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows, uint
 /* Attention of the rows over the cache (the core of rust/src/inference/attention.rs:69-113, as lc_attention_decode_dev): each row of q_dev
  * [n_rows][n_heads][head_dim], already rotated, attends to the positions up to its own, which the cache already holds (append first), and
  * with window > 0 only to the last `window` of them: pages that lie wholly in front of the first row's window are not looked at.  Scores are q . k * scale (0: 1 / sqrt(head_dim); 2e38 at most).  Queries of any finite size are taken as long as scores stay below 2^126; a
- * row with one that is not finite gives NaN.  Softmax and sums are in f32, its weights in 11 bits (f32: 22).  The values' scales are
+ * row with one that is not finite gives NaN.  Softmax and sums are in f32.  Weights have 11 bits (f32: 22) or are off by 2^-31 of their
+ * row's largest weight times scale of values, whichever is more; queries of 16-bit types have 16 bits of their row's largest element or more, f32 22 or more.  The values' scales are
  * 2^64 at most, and those below 2^-64 of the largest of their sequence and head, or below 2^-140, may count as 0.
  * A call is refused where its work, with every context as long as its table, could not be counted in 31 bits.  Taken for sure: (n_rows * heads per kv head / 256 + n_seqs) * n_kv_heads * (positions
  * of a table / 16 + 6) below 2^31 and n_rows * n_heads up to 2^27; with heads above 128 the first factor is n_rows * heads per kv head / 16 + n_seqs.
@@ -209,7 +210,7 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
  * (NaN where tokens[r] is outside 0 .. vocab - 1), entropy[r] in nats, and the `top` (0 .. 32, vocab at most) likeliest tokens with their log probabilities,
  * the larger logit first, equal logits by the lower index (-0 equals 0).  logprob, entropy, top_logprob / top_id may be NULL (tokens with logprob, and the last
  * two together).  Logits of minus infinity have probability 0; a row of nothing else has logprob and top_logprob of minus infinity and entropy 0.  A row
- * with a NaN or plus infinity has NaN everywhere and top_id -1.  Sums are in 64 bits.
+ * with a NaN or plus infinity has NaN everywhere and top_id -1.  Terms and sums of sixteen are in f32, all others in 64 bits.
  * The _dev form: streams and types as above. */
 int32_t lc_token_logprobs(const float* logits, size_t rows, size_t vocab, const int64_t* tokens, int32_t top, float* logprob,
                           float* entropy, float* top_logprob, int64_t* top_id);
