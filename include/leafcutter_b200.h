@@ -206,6 +206,69 @@ int32_t lc_attention_kv8_dev(const lc_kv8_cache* cache, const lc_kv8_rows* rows,
                              int64_t q_stride, int32_t n_heads, float scale, int32_t window, void* out_dev, int64_t out_stride,
                              void* workspace_dev, size_t workspace_bytes, void* stream);
 
+/* A key/value cache in 4 bits (no counterpart in the reference): pages as above, of integers from -7 to 7 with a scale for every 16 dims of a row and one for every
+ * kv head.  An integer n is stored as n + 8 in 4 bits, two neighbouring dims in a byte, the even one in its low half.  A block scale is e4m3 (4 bits of exponent, 3 of mantissa) without a sign:
+ * the top bit is not looked at and 0x7f counts as 480, so that every byte is a finite number.  A value is n * block scale * head scale.  The heads' scales are the caller's, positive
+ * numbers between 2^-60 and 2^60 (which no call checks): values up to 3136 times the head's scale are held, and blocks whose largest is 0.11 times it or more with 4 bits of scale.  A row
+ * depends on nothing but itself, so rows can be moved between pages. */
+typedef struct lc_kv4_cache {
+    void* k_dev;                 /* [n_pages][n_kv_heads][page_tokens][head_dim / 2], 16-byte aligned */
+    void* v_dev;
+    uint8_t* k_block_dev;        /* [n_pages][n_kv_heads][page_tokens][head_dim / 16], 16-byte aligned */
+    uint8_t* v_block_dev;
+    const float* k_scale_dev;    /* [n_kv_heads] */
+    const float* v_scale_dev;
+    int32_t n_pages, n_kv_heads, page_tokens, head_dim;  /* page_tokens 16, 32, 64, 128 or 256; head_dim a multiple of 16, at most 256 */
+} lc_kv4_cache;
+/* The calls over it take rows, types, strides, streams and workspaces as those over the 8-bit cache do, and treat bad pages and sequences as they do, unless said. */
+
+/* How a head's rotated dims pair up: (d, d + rot_dim / 2), or neighbours (2 d, 2 d + 1). */
+enum { LC_ROPE_HALF = 0, LC_ROPE_INTERLEAVED = 1 };
+/* How frequencies change for contexts `factor` times as long as the `original` one: not; all divided by factor; the base raised by
+ * factor^(rot_dim / (rot_dim - 2)); those of pairs below `slow` turns per original length divided by factor, those above `fast` as they are, the ones between mixed by their index (YARN, which
+ * also asks for values multiplied by 0.1 ln(factor) + 1) or by their turns (LLAMA3). */
+enum { LC_ROPE_PLAIN = 0, LC_ROPE_LINEAR = 1, LC_ROPE_NTK = 2, LC_ROPE_YARN = 3, LC_ROPE_LLAMA3 = 4 };
+/* A table as lc_rope_turns makes it, scaled; *magnitude is what turned values are to be multiplied by.  fast, slow: 0 for the usual 32 and 1 (YARN), 4 and 1 (LLAMA3). */
+int32_t lc_rope_turns_scaled(double theta, int32_t rot_dim, int32_t kind, double factor, int32_t original, double fast, double slow, uint64_t* out,
+                             double* magnitude);
+/* Rows turned by their positions: of each head the first rot_dim dims, pair p by positions_dev[row] * turns_dev[p] (which wraps around), times magnitude; the other dims are copied.
+ * inverse != 0: the other way round, which is also the gradient's way.  x is [n_rows][x_heads][head_dim], y (NULL: none) [n_rows][y_heads][head_dim] with the same positions; the outputs may be the
+ * inputs themselves (with their strides) and must not overlap them otherwise.  head_dim: 1 to 1024.  Results are within 2^-23 of the turned value (before typ's rounding).  n_rows: 2^24 at most. */
+int32_t lc_rope_dev(uint32_t typ, int32_t n_rows, const int64_t* positions_dev, const uint64_t* turns_dev, int32_t rot_dim, int32_t head_dim,
+                    int32_t layout, int32_t inverse, double magnitude, const void* x_dev, int64_t x_stride, void* x_out_dev, int64_t x_out_stride,
+                    int32_t x_heads, const void* y_dev, int64_t y_stride, void* y_out_dev, int64_t y_out_stride, int32_t y_heads, void* stream);
+/* Appends rows as lc_kv8_append_dev does, into slots ctx[i] + (r - row_start[i]).  positions_dev (NULL: the slots) has for each sequence the position of its first row, for caches that
+ * have lost rows.  A block's scale is its largest finite magnitude / (7 * head scale) rounded to e4m3 to the nearest even, 448 at most; an integer is value / (block scale * head scale),
+ * to the nearest even, -7 .. 7; infinities become +-7, NaN 0, and all are 0 where the scales' product is.  All of that as if in 64 bits. */
+int32_t lc_kv4_append_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, const int64_t* positions_dev,
+                          const void* k_dev, int64_t k_stride, const void* v_dev, int64_t v_stride, const void* q_dev, int64_t q_stride,
+                          void* q_out_dev, int64_t q_out_stride, int32_t n_heads, const uint64_t* turns_dev, int32_t rot_dim, int32_t layout,
+                          double magnitude, void* stream);
+/* The cached rows as values, as lc_kv8_read_dev. */
+int32_t lc_kv4_read_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, void* k_out_dev, int64_t k_stride,
+                        void* v_out_dev, int64_t v_stride, void* stream);
+/* Attention as lc_attention_kv8_dev, each row over the slots up to its own.  lse_dev (may be NULL), f32 [n_rows][n_heads], lse_stride between rows, receives
+ * ln sum exp of a row's scores.  Queries of 16-bit types are exact down to 2^-24 of their row's largest element, f32 ones have 22 bits; weights 11 bits (f32: 22) or 2^-35 of the row's largest; sums in f32. */
+int32_t lc_attention_kv4_workspace(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, int32_t n_heads, size_t* out_bytes);
+int32_t lc_attention_kv4_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, const void* q_dev, int64_t q_stride,
+                             int32_t n_heads, float scale, int32_t window, void* out_dev, int64_t out_stride, float* lse_dev, int64_t lse_stride,
+                             void* workspace_dev, size_t workspace_bytes, void* stream);
+/* Adds to mass_dev[i * mass_stride + h * mass_head_stride + slot] what weight the rows of sequence i gave the cached key of kv head h in `slot`: the sum over the rows and the heads of the
+ * group of exp(q . k * scale - lse), with the lse that attention over the same rows gave (rows whose lse is not finite add nothing).  A sequence with more slots than `capacity`, which
+ * is no more than either stride, is left out and raises the status, and so do sequences that leave their table; keys on bad pages are left out.  Sums are in f32, in an order that depends on the arguments and lengths
+ * alone.  Sequences never share sums, whatever pages they share; sequences that share rows all count them. */
+int32_t lc_kv4_weights_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, const void* q_dev, int64_t q_stride,
+                           int32_t n_heads, float scale, int32_t window, const float* lse_dev, int64_t lse_stride, float* mass_dev,
+                           int64_t mass_stride, int64_t mass_head_stride, int32_t capacity, void* stream);
+/* Cuts sequences whose length (context and rows) is above `limit` to `keep` rows: for each kv head by itself the `first` first and `recent` last rows and, of those between, the ones with the
+ * largest mass (equal ones by the lower slot; NaN counts as the smallest).  They move to the front of the sequence's pages in their order, their sums in mass_dev with them; sums behind them become 0.  kept_dev
+ * [n_seqs][n_kv_heads][limit] receives the slots that they came from, -1 behind them, and ctx_out_dev [n_seqs] the new lengths (shorter sequences: as they are).
+ * first + recent <= keep <= limit <= capacity, keep > 0.  Pages of a sequence that is cut must be its own.  A sequence that leaves its table, has a bad page among those of its length or
+ * is longer than `capacity` raises the status and stays as it is, -1 in kept_dev. */
+int32_t lc_kv4_evict_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, float* mass_dev, int64_t mass_stride, int64_t mass_head_stride,
+                         int32_t capacity, int32_t keep, int32_t limit, int32_t recent, int32_t first, int32_t* kept_dev, int32_t* ctx_out_dev,
+                         void* stream);
+
 /* Log probabilities (no counterpart in the reference).  For each row of logits [rows][vocab] (stride elements apart): logprob[r] = log softmax of the row at tokens[r]
  * (NaN where tokens[r] is outside 0 .. vocab - 1), entropy[r] in nats, and the `top` (0 .. 32, vocab at most) likeliest tokens with their log probabilities,
  * the larger logit first, equal logits by the lower index (-0 equals 0).  logprob, entropy, top_logprob / top_id may be NULL (tokens with logprob, and the last

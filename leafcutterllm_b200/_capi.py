@@ -53,6 +53,11 @@ class Kv8CacheStruct(C.Structure):
                 ("n_pages", C.c_int32), ("n_kv_heads", C.c_int32), ("page_tokens", C.c_int32), ("head_dim", C.c_int32)]
 
 
+class Kv4CacheStruct(C.Structure):
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("k_block_dev", C.c_void_p), ("v_block_dev", C.c_void_p), ("k_scale_dev", C.c_void_p),
+                ("v_scale_dev", C.c_void_p), ("n_pages", C.c_int32), ("n_kv_heads", C.c_int32), ("page_tokens", C.c_int32), ("head_dim", C.c_int32)]
+
+
 class Kv8RowsStruct(C.Structure):
     _fields_ = [("page_table_dev", C.c_void_p), ("ctx_dev", C.c_void_p), ("row_start_dev", C.c_void_p), ("status_dev", C.c_void_p),
                 ("n_seqs", C.c_int32), ("table_width", C.c_int32), ("max_rows", C.c_int32), ("reserved", C.c_int32)]
@@ -104,6 +109,14 @@ SIGNATURES = {
     "lc_kv8_read_dev": (_i32, [_vp, _vp, _u32, _i32, _vp, _i64, _vp, _i64, _vp]),
     "lc_attention_kv8_workspace": (_i32, [_vp, _vp, _u32, _i32, _i32, C.POINTER(_sz)]),
     "lc_attention_kv8_dev": (_i32, [_vp, _vp, _u32, _i32, _vp, _i64, _i32, C.c_float, _i32, _vp, _i64, _vp, _sz, _vp]),
+    "lc_rope_turns_scaled": (_i32, [C.c_double, _i32, _i32, C.c_double, _i32, C.c_double, C.c_double, _vp, C.POINTER(C.c_double)]),
+    "lc_rope_dev": (_i32, [_u32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, C.c_double, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _vp]),
+    "lc_kv4_append_dev": (_i32, [_vp, _vp, _u32, _i32, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i32, _i32, C.c_double, _vp]),
+    "lc_kv4_read_dev": (_i32, [_vp, _vp, _u32, _i32, _vp, _i64, _vp, _i64, _vp]),
+    "lc_attention_kv4_workspace": (_i32, [_vp, _vp, _u32, _i32, _i32, C.POINTER(_sz)]),
+    "lc_attention_kv4_dev": (_i32, [_vp, _vp, _u32, _i32, _vp, _i64, _i32, C.c_float, _i32, _vp, _i64, _vp, _i64, _vp, _sz, _vp]),
+    "lc_kv4_weights_dev": (_i32, [_vp, _vp, _u32, _i32, _vp, _i64, _i32, C.c_float, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _vp]),
+    "lc_kv4_evict_dev": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
     "lc_token_logprobs": (_i32, [_vp, _sz, _sz, _vp, _i32, _vp, _vp, _vp, _vp]),
     "lc_token_logprobs_dev": (_i32, [_u32, _vp, _i32, _i32, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
     "lc_timer_begin": (_i32, []),

@@ -17,6 +17,7 @@
 #include <type_traits>
 #include "lc_kv8.cuh"
 #include "lc_kernels.h"
+#include "lc_rope.cuh"
 #include "lc_tma.cuh"
 
 namespace lc {
@@ -113,26 +114,9 @@ template <typename T> __device__ __forceinline__ void store4(T* p, const float (
     if (sizeof(T) == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
     else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(t);
 }
-// u c - w s in f32 with the cosine and sine as two f32 each: the difference of the products with what the second lost (Kahan), 1.5 2^-24 of the result off,
-// and what the high parts leave out
-__device__ __forceinline__ float turned(float u, float w, float ch, float cl, float sh, float sl) {
-    const float p = w * sh, lost = fmaf(-w, sh, p), d = fmaf(u, ch, -p);
-    const float y = d + (lost + fmaf(u, cl, -w * sl));
-    return fabsf(d) < INFINITY ? y : d;
-}
 // The rotations of rows pos0 .. pos0 + n - 1: (cosine, sine) of every pair.  Sine and cosine themselves for every eighth row and for the first
 // eight turns; the rest are products of the two, 2^-52 off.  SPREAD: pair d lies at place (d mod 4) half / 4 + d / 4, so that lanes with four pairs each read
 // neighbouring places.  They are kept as two f32 each, 2^-48 of them off.
-__device__ __forceinline__ double2 turn_of(uint64_t per_position, int64_t positions) {
-    const int64_t frac = (int64_t)((uint64_t)positions * per_position);
-    double2 r;
-    sincospi((double)frac * 0x1p-63, &r.y, &r.x);  // frac 2^-64 turns = frac 2^-63 pi
-    return r;
-}
-__device__ __forceinline__ void set_turn(float4& at, double2 t) {
-    at.x = (float)t.x; at.y = (float)(t.x - at.x);
-    at.z = (float)t.y; at.w = (float)(t.y - at.z);
-}
 // a pair's rotation in 64 bits
 __device__ __forceinline__ void turned64(float u, float w, const float4& t, double& y0, double& y1) {
     const double c = (double)t.x + (double)t.y, s = (double)t.z + (double)t.w;
