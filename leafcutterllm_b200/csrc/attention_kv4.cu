@@ -1,6 +1,13 @@
 // Attention over the key/value cache in 4 bits: out = sum_j p_j v_j, p = softmax_j(scale q . k_j) over the slots j up to the row's own.
 //
-// A warp per row and head: a lane scores a key of 32 at a time, then all lanes add up the values' dims.
+// Here: few rows per sequence, by runs.  A unit is (sequence, kv head, row block of 8 NG rows = tokens x heads of the group); the units' steps of 16 keys stand in one line, which is cut into equal
+// runs, one per warp, so that contexts of any lengths keep all warps equally long at work; what lies in several runs is joined by the next kernel.  Bytes come through a ring of the warp's
+// own in shared memory (cp.async) and become f16 values, exact, in registers, on the way into the matrix unit (mma.sync m16n8k16, f32 sums):
+//   Scores  queries are the operand of 16 rows, keys that of 8 columns.  Queries are f16 after a power of two for each row (16-bit types: exact down to 2^-24 of the row's largest element), f32 ones a
+//           high and a low part, 22 bits; where a unit has 8 rows the low parts are the operand's other 8 rows and cost nothing.
+//   Values  are the operand of 16 rows (dims), weights that of 8 columns (rows of queries), which the scores' layout already is.  Weights are 2^(s - max + 10) in f16; f32: and what that rounding lost, in a second
+//           product, a step's sums added in f32, so that what the matrix unit cuts off when it adds stays within 16 keys.
+// Dims of a score and keys of a sum may stand in any order, so a thread takes neighbouring dims of its key, whose scale they share, and two keys' dims become pairs by one byte permutation for eight of them.
 #include <algorithm>
 #include "lc_kernels.h"
 #include "lc_kv4.cuh"
@@ -10,94 +17,492 @@ namespace lc {
 
 namespace {
 
-struct Attn4Args {
-    const void* q;
-    void* out;
-    float* lse;
-    int64_t q_stride, out_stride, lse_stride;
-    int typ, heads, group, window;
-    float scale;
-};
-constexpr int kWarps = 4;
+constexpr float kWeightUp = 10.0f;   // weights are 2^this too large, and up to 2^4 more before the reference is raised: 2^14 at most, and f16's smallest is 2^-34 of the largest
 
-__global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Kv4Pool pool, Kv8Seqs seqs, Attn4Args a) {
-    __shared__ float qs[kWarps][256];
-    if (blockIdx.x == 0) kv8_check_seqs(seqs, pool);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hd = pool.hd, blocks = hd >> 4;
-    const int64_t unit = (int64_t)blockIdx.x * kWarps + warp;
-    const int r = (int)(unit / a.heads), h = (int)(unit % a.heads), kvh = h / a.group;
-    if (r >= seqs.n_rows) return;
-    const RowPlace at = row_place(seqs, pool, r);
-    if (at.seq < 0) return;
-    const int64_t dst = (int64_t)r * a.out_stride + (int64_t)h * hd;
-    float l = 0.0f, m = kNegInf, o[8] = {};
-    bool bad = at.slot < 0;
-    if (!bad) {
-        for (int d = lane; d < hd; d += 32) {
-            const int64_t src = (int64_t)r * a.q_stride + (int64_t)h * hd + d;
-            qs[warp][d] = a.typ == LC_TYPE_F32 ? ((const float*)a.q)[src] : a.typ == LC_TYPE_F16 ? elem_f(((const __half*)a.q)[src]) : elem_f(((const __nv_bfloat16*)a.q)[src]);
+template <int HD, int NG, bool F32> struct Run4Shape {
+    static constexpr int kRows = 8 * NG;
+    static constexpr int kTiles = NG == 1 ? 1 : NG / 2 * (F32 ? 2 : 1);   // operand tiles of 16 rows of queries
+    static constexpr int kHalf = kStep * HD / 2;                          // bytes of a step's keys
+    static constexpr int kStageBytes = 2 * kHalf + 2 * HD;                // keys, values, their scales
+    static constexpr int kStages = HD == 256 && NG > 1 ? 3 : 4;
+    static constexpr bool kQueriesShared = HD == 256 || kTiles > 1;       // operand fragments of the queries in shared memory, not in registers
+    static constexpr int kQueries = kQueriesShared ? kTiles * (HD / 16) * 512 : 0;
+    static constexpr int kWarp = kStages * kStageBytes + kQueries;
+    static constexpr int kByRegisters = HD == 256 ? 2 : NG == 1 ? 4 : NG == 2 ? 3 : 2;
+    static constexpr int kByMemory = (220 << 10) / (kRunWarps * kWarp + 2048);
+    static constexpr int kBlocks = kByRegisters < kByMemory ? kByRegisters : kByMemory;
+};
+// Where values' 16-byte chunk ch of row r of a step lies (in chunks), so that the threads of a quad, whose keys are 2c, 2c + 1, 8 + 2c, 9 + 2c, read other banks: rows in the
+// order of the quads, and chunks swapped where two of these rows begin at the same bank.
+template <int HD> __device__ __forceinline__ int value_chunk(int r, int ch) {
+    constexpr int N = HD / 32;
+    const int slot = (r >> 1) + (r & 1) * 8;
+    return slot * N + (HD == 256 ? ch ^ ((slot & 3) * 2) : HD == 128 ? ch ^ (slot & 2) : ch);
+}
+template <int N> __device__ __forceinline__ void lds_words(const unsigned char* p, uint32_t (&w)[N]) {  // N: 1, 2, 4 or 8 words, aligned to 16 bytes or their size
+    if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+    else if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x; w[1] = u.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+            w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
         }
-        __syncwarp();
-        const int limit = seqs.ctx[at.seq] + at.index, from = a.window > 0 ? max(0, limit - a.window + 1) : 0, mask = (1 << pool.page_shift) - 1;
+    }
+}
+// the same, aligned to 8 bytes
+template <int N> __device__ __forceinline__ void lds_words8(const unsigned char* p, uint32_t (&w)[N]) {
+    if constexpr (N <= 2) lds_words<N>(p, w);
+    else
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            const uint2 u = reinterpret_cast<const uint2*>(p)[i];
+            w[2 * i] = u.x; w[2 * i + 1] = u.y;
+        }
+}
+
+template <int HD, int NG, bool F32, bool FULL>
+__global__ void __launch_bounds__(kRunWarps * 32, Run4Shape<HD, NG, F32>::kBlocks)
+kv4_runs_kernel(Kv4Pool pool, Kv8Seqs seqs, AttnArgs a) {
+    using Shape = Run4Shape<HD, NG, F32>;
+    constexpr int RB = Shape::kRows, S = Shape::kStages, TILES = Shape::kTiles;
+    constexpr int KS = HD / 16;             // k steps of the scores
+    constexpr int NT = HD / 16;             // tiles of 16 dims of the output
+    constexpr int KW = HD / 32;             // words of a key that a thread has
+    constexpr int VW = HD / 64;             // words of a value
+    constexpr bool LOW_ROWS = F32 && NG == 1;   // the low parts are rows 8 .. 15 of the tile
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ uint2 warp_sums[kRunWarps];
+    uint32_t* cum = reinterpret_cast<uint32_t*>(smem + kRunWarps * Shape::kWarp);
+    pdl_launch_dependents();
+    if (blockIdx.x == 0) kv8_check_seqs(seqs, pool);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const uint32_t total = line_up<RB>(seqs, pool, a, cum, nullptr, warp_sums);
+    const Runs runs(total, gridDim.x * kRunWarps);
+    const uint32_t run = blockIdx.x * kRunWarps + warp;
+    if (lane == 0) a.records[run].row_n = 0;
+    if (run >= runs.n) return;
+    uint32_t t = runs.start(run);
+    const uint32_t t_end = runs.start(run + 1);
+    unsigned char* const mine = smem + warp * Shape::kWarp;
+    const uint32_t ring = smem_u32(mine);
+    uint4* const qs = reinterpret_cast<uint4*>(mine + S * Shape::kStageBytes);
+    const int hd = FULL ? HD : pool.hd, page_mask = (1 << pool.page_shift) - 1;
+
+    while (t < t_end) {
+        // a segment: this run's steps of one unit
+        Place at;
+        place_at<RB>(at, seqs, pool, a, cum, t);
+        const SeqWork& w = at.w;
+        const int end = min(w.steps + kUnitCost, at.in + (int)(t_end - t)), s0 = max(0, at.in - kUnitCost), s1 = end - kUnitCost;
+        t += (uint32_t)(end - at.in);
+        if (s1 <= s0) continue;  // the unit's steps are the next run's
+        if (s0 == 0 && s1 < w.steps && lane == 0) {
+            a.records[run].last = (int)min(runs.run_of(t + (uint32_t)(w.steps - s1) - 1), runs.n - 1);
+            *reinterpret_cast<int4*>(&a.records[run]) = make_int4(w.first, at.kvh, at.rb * RB, min(RB, w.n * a.group - at.rb * RB));
+        }
         const int32_t* table = seqs.table + (size_t)at.seq * seqs.width;
-        const float gk = pool.k_scale[kvh], gv = pool.v_scale[kvh];
-        for (int key0 = from & ~31; key0 <= limit; key0 += 32) {
-            const int key = key0 + lane;
-            const bool sees = key >= from && key <= limit;
-            const int number = sees ? table[key >> pool.page_shift] : 0;
-            const bool held = number >= 0 && number < pool.n_pages;
-            if (sees && !held) { bad = true; kv8_raise(seqs, at.seq); }
-            const size_t row = (((size_t)(held ? number : 0) * pool.n_kv + kvh) << pool.page_shift) + (key & mask);
-            float s = kNegInf;
-            if (sees && held) {
-                s = 0.0f;
-                for (int b = 0; b < blocks; b++) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(pool.k + row * (hd >> 1) + 8 * b);
-                    float part = 0.0f;
-                    for (int e = 0; e < 16; e++) part = fmaf((float)(int)(((e < 8 ? w.x : w.y) >> (4 * (e & 7)) & 15u) - 8u), qs[warp][16 * b + e], part);
-                    s = fmaf(part, scale4_f(pool.k_block[row * blocks + b]), s);
+        const int row_lo = at.rb * RB, row_n = min(RB, w.n * a.group - row_lo);
+
+        // pages of 32 steps on, one per lane
+        int pages_at = s0, pages = -1;
+        auto look_up = [&]() {
+            const int st = pages_at + lane;
+            pages = w.inside && st < s1 ? table[((w.step0 + st) * kStep) >> pool.page_shift] : -1;
+        };
+        look_up();
+        uint32_t outside = 0;                // bit st % 32: that step's page is outside the pool
+        auto fetch = [&](int st) {
+            if (st - pages_at == 32) { pages_at += 32; look_up(); }
+            if (st < s1 && w.inside) {
+                const int number = __shfl_sync(0xffffffffu, pages, st - pages_at);
+                if (number < 0 || number >= pool.n_pages) {
+                    outside |= 1u << (st & 31);
+                    if (lane == 0) kv8_raise(seqs, at.seq);
+                } else {
+                    outside &= ~(1u << (st & 31));
+                    const uint32_t dst = ring + (uint32_t)(st % S) * Shape::kStageBytes;
+                    const size_t row = ((((size_t)number * pool.n_kv + at.kvh) << pool.page_shift) + (((w.step0 + st) * kStep) & page_mask));
+                    const int8_t* ks = pool.k + row * (hd >> 1);
+                    const int8_t* vs = pool.v + row * (hd >> 1);
+                    if (FULL) {
+#pragma unroll
+                        for (int i = 0; i < KW * kStep / 32; i++) {
+                            const int ch = i * 32 + lane;
+                            cp_async16(dst + ch * 16, ks + ch * 16);
+                            cp_async16(dst + Shape::kHalf + value_chunk<HD>(ch / KW, ch % KW) * 16, vs + ch * 16);
+                        }
+                    } else {
+                        for (int ch = lane; ch < hd >> 1; ch += 32) {
+                            cp_async16(dst + ch * 16, ks + ch * 16);
+                            cp_async16(dst + Shape::kHalf + ch * 16, vs + ch * 16);
+                        }
+                    }
+                    const int pieces = hd >> 4;
+                    if (lane < 2 * pieces) {
+                        const bool v = lane >= pieces;
+                        const int ch = v ? lane - pieces : lane;
+                        cp_async16(dst + 2 * Shape::kHalf + (v ? HD : 0) + ch * 16, (v ? pool.v_block : pool.k_block) + row * pieces + ch * 16);
+                    }
                 }
-                s *= a.scale * gk;
             }
-            const float top = fmaxf(m, warp_max(s)), ref = top == kNegInf ? 0.0f : top, corr = expf(m - ref), p = expf(s - ref);
-            m = top;
-            l = l * corr + warp_sum(p);
-            for (int i = 0; i < 8; i++) o[i] *= corr;
-            for (int x = 0; x < 32; x++) {
-                const float w = __shfl_sync(0xffffffffu, p, x);
-                const size_t vrow = __shfl_sync(0xffffffffu, (unsigned long long)row, x);
-                if (w == 0.0f) continue;
-                for (int i = 0; i < 8; i++) {
-                    const int d = lane + 32 * i;
-                    if (d < hd) {
-                        const int n = (int)((uint8_t)pool.v[vrow * (hd >> 1) + (d >> 1)] >> (4 * (d & 1)) & 15) - 8;
-                        o[i] = fmaf(w, (float)n * scale4_f(pool.v_block[vrow * blocks + (d >> 4)]) * gv, o[i]);
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int k = 0; k < S - 1; k++) fetch(s0 + k);
+
+        // The queries as operand fragments.  A thread's dims are HD / 4 in a row, eight of which make two k steps: (0, 4), (1, 5) and (2, 6), (3, 7), as the keys' words give them.
+        uint32_t qf[Shape::kQueriesShared ? 1 : KS][4];
+        float rf[NG];                        // what a row's scores are multiplied by
+        int limit[NG];                       // last slot that the row sees (-1: no row)
+        {
+            const float head = kUnit4 * pool.k_scale[at.kvh];
+#pragma unroll
+            for (int pair = 0; pair < (NG + 1) / 2; pair++) {
+                float v[2][HD / 4], up[2];
+#pragma unroll
+                for (int x = 0; x < (NG == 1 ? 1 : 2); x++) {
+                    const int gr = 2 * pair + x, r = 8 * gr + g;
+                    const bool has = r < row_n;
+                    const int tok = has ? (row_lo + r) / a.group : 0, hq = has ? (row_lo + r) - tok * a.group : 0;
+                    const int64_t src = (int64_t)(w.first + tok) * a.q_stride + (int64_t)(at.kvh * a.group + hq) * hd;
+                    limit[gr] = has ? w.ctx + tok : -1;
+                    float top = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < HD / 64; j++) {
+                        const int d = c * (HD / 4) + 16 * j;
+                        float* u = v[x] + 16 * j;
+                        if (has && (FULL || d < hd)) load16(a.q, src + d, a.typ, a.q_vec, u);
+                        else
+#pragma unroll
+                            for (int e = 0; e < 16; e++) u[e] = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) top = max_nan(top, fabsf(u[e]));
+                    }
+                    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    float down;
+                    row_scale(top, up[x], down);
+                    rf[gr] = top < INFINITY ? a.scale_log2 * down * head : __int_as_float(0x7fffffff);  // not finite: the row is NaN
+                }
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    uint32_t hi[2][2] = {}, lo[2][2] = {};
+#pragma unroll
+                    for (int x = 0; x < (NG == 1 ? 1 : 2); x++)
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            const int e = 8 * (ks >> 1) + 2 * (ks & 1) + y;
+                            const float p = v[x][e] * up[x], q = v[x][e + 4] * up[x];
+                            if (F32) h2_split(p, q, hi[x][y], lo[x][y]);
+                            else hi[x][y] = h2_pack(p, q);
+                        }
+                    // (row g, row g + 8) of the first two dims, then of the others
+                    const uint4 f = LOW_ROWS ? make_uint4(hi[0][0], lo[0][0], hi[0][1], lo[0][1]) : make_uint4(hi[0][0], hi[1][0], hi[0][1], hi[1][1]);
+                    if (Shape::kQueriesShared) {
+                        qs[((F32 && NG > 1 ? 2 * pair : pair) * KS + ks) * 32 + lane] = f;
+                        if (F32 && NG > 1) qs[((2 * pair + 1) * KS + ks) * 32 + lane] = make_uint4(lo[0][0], lo[1][0], lo[0][1], lo[1][1]);
+                    } else {
+                        uint32_t(&q4)[4] = qf[Shape::kQueriesShared ? 0 : ks];
+                        q4[0] = f.x; q4[1] = f.y; q4[2] = f.z; q4[3] = f.w;
                     }
                 }
             }
         }
+
+        // o: dims 2 t (places 0, 1) and 2 t + 1 (places 2, 3) of the thread's, of rows 2c, 2c + 1 of the group; m, l: of row g
+        float o[NG][NT][4], m[NG], l[NG];
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[gr][t][e] = 0.0f;
+            m[gr] = kNegInf;
+            l[gr] = 0.0f;
+        }
+        // rows see all keys up to the first row's slot (with a window, from the last row's on)
+        const int sees = w.ctx + row_lo / a.group, from = a.window > 0 ? w.ctx + (row_lo + row_n - 1) / a.group - a.window : -1;
+        for (int st = s0; st < s1; st++) {
+            cp_async_wait<S - 2>();
+            __syncwarp();
+            fetch(st + S - 1);  // into the place of the step before
+            const int key0 = (w.step0 + st) * kStep;
+            const bool plain = key0 + kStep - 1 <= sees && key0 > from;
+            const unsigned char* kp = mine + (st % S) * Shape::kStageBytes;
+            const unsigned char* scales = kp + 2 * Shape::kHalf;
+            float s[NG][2][2];               // [group][tile of 8 keys][two keys]
+            {
+                float dot[TILES][2][4];
+#pragma unroll
+                for (int tl = 0; tl < 2; tl++) {
+                    const int row = 8 * tl + g;
+                    uint32_t kw[KW];
+                    if (FULL) lds_words<KW>(kp + row * (HD / 2) + c * (HD / 8), kw);
+                    else lds_words8<KW>(kp + row * (hd >> 1) + c * (HD / 8), kw);
+                    const unsigned char* sc = scales + row * (hd >> 4) + c * (HD / 64);
+                    uint32_t bytes = 0;
+                    if (HD == 64) bytes = *sc;
+                    else if (FULL) bytes = HD == 128 ? *reinterpret_cast<const uint16_t*>(sc) : *reinterpret_cast<const uint32_t*>(sc);
+                    else
+#pragma unroll
+                        for (int j = 0; j < HD / 64; j++) bytes |= (uint32_t)sc[j] << (8 * j);
+#pragma unroll
+                    for (int j = 0; j < HD / 64; j++) {   // 16 dims: two words, four k steps
+                        const uint32_t b = (bytes >> (8 * j)) & 0xffu;
+                        const Scale4 k4 = scale4(b | b << 16);
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            uint32_t kv[4];
+                            values8(kw[2 * j + x], k4, kv);
+#pragma unroll
+                            for (int y = 0; y < 2; y++) {
+                                const int ks = 4 * j + 2 * x + y;
+#pragma unroll
+                                for (int tile = 0; tile < TILES; tile++) {
+                                    uint4 f;
+                                    if (Shape::kQueriesShared) f = qs[(tile * KS + ks) * 32 + lane];
+                                    else {
+                                        const uint32_t(&q4)[4] = qf[Shape::kQueriesShared ? 0 : ks];
+                                        f = make_uint4(q4[0], q4[1], q4[2], q4[3]);
+                                    }
+                                    const uint32_t fa[4] = {f.x, f.y, f.z, f.w};
+                                    if (ks == 0) mma_f16_first(dot[tile][tl], fa, kv[2 * y], kv[2 * y + 1]);
+                                    else mma_f16(dot[tile][tl], fa, kv[2 * y], kv[2 * y + 1]);
+                                }
+                            }
+                        }
+                    }
+                }
+                // Products are rounded by themselves, as the reference is: far from 0 their difference is then exact near it.
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                    for (int tl = 0; tl < 2; tl++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            float v;
+                            if (LOW_ROWS) v = __fadd_rn(dot[0][tl][k], dot[0][tl][2 + k]);
+                            else if (F32) v = __fadd_rn(dot[gr / 2 * 2][tl][2 * (gr & 1) + k], dot[TILES > 1 ? gr / 2 * 2 + 1 : 0][tl][2 * (gr & 1) + k]);
+                            else v = dot[gr / 2][tl][2 * (gr & 1) + k];
+                            s[gr][tl][k] = __fmul_rn(v, rf[gr]);
+                        }
+            }
+            if (outside && (outside >> (st & 31) & 1)) {  // the rows that see its keys are NaN
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[gr][e >> 1][e & 1] = __int_as_float(0x7fffffff);
+            }
+            float mx[NG];
+            bool raise = false;
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+                if (!plain) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int key = key0 + 8 * (e >> 1) + 2 * c + (e & 1);
+                        if (key > limit[gr] || (a.window > 0 && key <= limit[gr] - a.window)) s[gr][e >> 1][e & 1] = kNegInf;
+                    }
+                }
+                mx[gr] = fmaxf(fmaxf(s[gr][0][0], s[gr][0][1]), fmaxf(s[gr][1][0], s[gr][1][1]));
+            }
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) mx[gr] = fmaxf(mx[gr], __shfl_xor_sync(0xffffffffu, mx[gr], 1));
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+                mx[gr] = fmaxf(mx[gr], __shfl_xor_sync(0xffffffffu, mx[gr], 2));
+                raise = raise || mx[gr] > m[gr] + 4.0f;
+            }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) {
+                    const float top = fmaxf(mx[gr], m[gr]), corr = top == kNegInf ? 1.0f : exp2_fast(m[gr] - top);
+                    l[gr] *= corr;
+                    m[gr] = top;
+                    const float c0 = __shfl_sync(0xffffffffu, corr, 8 * c), c1 = __shfl_sync(0xffffffffu, corr, 8 * c + 4);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) { o[gr][t][0] *= c0; o[gr][t][1] *= c1; o[gr][t][2] *= c0; o[gr][t][3] *= c1; }
+                }
+            }
+            uint32_t ph[NG][2], pl[NG][2];   // weights, and what their rounding lost: keys 2c, 2c + 1 and 8 + 2c, 9 + 2c of row g
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+                const float ref = m[gr] == kNegInf ? 0.0f : m[gr];
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = exp2_fast(__fadd_rn(__fsub_rn(s[gr][e >> 1][e & 1], ref), kWeightUp));
+                l[gr] += (v[0] + v[1]) + (v[2] + v[3]);
+                if (F32) {
+                    h2_split(v[0], v[1], ph[gr][0], pl[gr][0]);
+                    h2_split(v[2], v[3], ph[gr][1], pl[gr][1]);
+                } else {
+                    ph[gr][0] = h2_pack(v[0], v[1]);
+                    ph[gr][1] = h2_pack(v[2], v[3]);
+                }
+            }
+            // values: a thread's keys are 2c, 2c + 1, 8 + 2c, 9 + 2c, its dims HD / 8 in a row
+            const unsigned char* vp = kp + Shape::kHalf;
+            uint32_t vw[4][VW], vb[4][HD == 256 ? 2 : 1];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int row = (x >> 1) * 8 + 2 * c + (x & 1);
+                if (FULL) lds_words<VW>(vp + value_chunk<HD>(row, HD == 256 ? g : HD == 128 ? g >> 1 : g >> 2) * 16 + (HD == 256 ? 0 : HD == 128 ? (g & 1) * 8 : (g & 3) * 4), vw[x]);
+                else lds_words8<VW>(vp + row * (hd >> 1) + g * (HD / 16), vw[x]);
+                const unsigned char* sc = scales + HD + row * (hd >> 4) + (HD == 256 ? 2 * g : HD == 128 ? g : g >> 1);
+                vb[x][0] = sc[0];
+                if (HD == 256) vb[x][HD == 256 ? 1 : 0] = sc[1];
+            }
+#pragma unroll
+            for (int half = 0; half < (HD == 256 ? 2 : 1); half++) {
+                const Scale4 sa = scale4(vb[0][half] | vb[1][half] << 16), sb = scale4(vb[2][half] | vb[3][half] << 16);
+#pragma unroll
+                for (int wd = 0; wd < (VW < 2 ? 1 : 2); wd++) {
+                    const int word = 2 * half + wd;
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {   // four dims
+                        const uint32_t xa = __byte_perm(vw[0][word], vw[1][word], q ? 0x7632 : 0x5410), xb = __byte_perm(vw[2][word], vw[3][word], q ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (int b = 0; b < 2; b++) {   // two dims: a tile
+                            const uint32_t ya = b ? xa >> 8 : xa, yb = b ? xb >> 8 : xb;
+                            const uint32_t vf[4] = {value_lo(ya, sa), value_hi(ya, sa), value_lo(yb, sb), value_hi(yb, sb)};
+#pragma unroll
+                            for (int gr = 0; gr < NG; gr++) {
+                                float(&oo)[4] = o[gr][4 * word + 2 * q + b];
+                                if (F32) {
+                                    float acc[4];
+                                    mma_f16_first(acc, vf, pl[gr][0], pl[gr][1]);
+                                    mma_f16(acc, vf, ph[gr][0], ph[gr][1]);
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) oo[e] += acc[e];
+                                } else {
+                                    mma_f16(oo, vf, ph[gr][0], ph[gr][1]);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        cp_async_wait<0>();
+
+        const bool starts = s0 == 0, ends = s1 == w.steps, whole = starts && ends;
+        const float unit = kUnit4 * pool.v_scale[at.kvh];
+        float* part = a.part + (size_t)(2 * run + (starts ? 1 : 0)) * part_floats<HD, RB>();
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++) {
+            float sum = l[gr];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (!w.inside) sum = __int_as_float(0x7fffffff);
+            if (c == 0 && 8 * gr + g < row_n) {
+                const int r = 8 * gr + g;
+                if (!whole) { part[r] = m[gr]; part[RB + r] = sum; }
+                else if (a.lse) {
+                    const int tok = (row_lo + r) / a.group;
+                    a.lse[(int64_t)(w.first + tok) * a.lse_stride + at.kvh * a.group + row_lo + r - tok * a.group] = (m[gr] + (log2f(sum) - kWeightUp)) * 0.693147180559945f;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int r = 8 * gr + 2 * c + x;
+                const float total = __shfl_sync(0xffffffffu, sum, 8 * c + 4 * x);
+                if (r >= row_n) continue;
+                const float by = whole ? unit / total : unit;   // a NaN sum makes all of the row NaN
+                const int tok = (row_lo + r) / a.group, hq = (row_lo + r) - tok * a.group;
+                const int64_t dst = (int64_t)(w.first + tok) * a.out_stride + (int64_t)(at.kvh * a.group + hq) * hd;
+                constexpr int N = HD == 64 ? 8 : 16;  // dims stored at a time
+#pragma unroll
+                for (int half = 0; half < (HD == 256 ? 2 : 1); half++) {
+                    float v[N];
+#pragma unroll
+                    for (int e = 0; e < N; e++) v[e] = o[gr][8 * half + (e >> 1)][2 * (e & 1) + x] * by;
+                    const int d = HD == 64 ? 8 * g : HD == 128 ? 16 * g : 32 * g + 16 * half;
+                    if (!whole) store_run<N>(part + 2 * RB + r * HD + d, true, v);
+                    else if (FULL || d < hd) store_run<N>(a.out, dst + d, a.typ, a.out_vec, v);
+                }
+            }
+        }
+        __syncwarp();
     }
-    bad = __any_sync(0xffffffffu, bad);
-    if (bad) l = __int_as_float(0x7fffffff);
-    for (int i = 0; i < 8; i++) {
-        const int d = lane + 32 * i;
-        if (d < hd) store1(a.out, dst + d, a.typ, o[i] / l);
-    }
-    if (a.lse && lane == 0) a.lse[(int64_t)r * a.lse_stride + h] = m + logf(l);
+}
+
+struct Run4Plan {
+    int hd, groups, blocks;
+    size_t bytes;
+};
+template <int HD, bool F32> int run_blocks(int groups) {
+    if (HD < 256 && groups == 4) return Run4Shape<HD, HD < 256 ? 4 : 1, F32>::kBlocks;
+    return groups == 2 ? Run4Shape<HD, 2, F32>::kBlocks : Run4Shape<HD, 1, F32>::kBlocks;
+}
+// As many groups of 8 rows share a step's keys and values as a unit has rows for: four at most, whose sums are 128 registers (two for heads of 256).
+int run_groups(const Kv4Pool& pool, int group, int max_rows) {
+    const int64_t rows = (int64_t)group * (max_rows < 1 ? 1 : max_rows);
+    return rows <= 8 ? 1 : rows <= 16 || pool.hd > 128 ? 2 : 4;
+}
+int most_groups(const Kv4Pool& pool) { return pool.hd > 128 ? 2 : 4; }
+Run4Plan plan_runs(const Kv4Pool& pool, uint32_t typ, int groups) {
+    Run4Plan p;
+    p.hd = pool.hd <= 64 ? 64 : pool.hd <= 128 ? 128 : 256;
+    p.groups = groups;
+    const bool f32 = typ == LC_TYPE_F32;
+    p.blocks = sm_count() * (p.hd == 64    ? (f32 ? run_blocks<64, true>(p.groups) : run_blocks<64, false>(p.groups))
+                             : p.hd == 128 ? (f32 ? run_blocks<128, true>(p.groups) : run_blocks<128, false>(p.groups))
+                                           : (f32 ? run_blocks<256, true>(p.groups) : run_blocks<256, false>(p.groups)));
+    p.bytes = (size_t)p.blocks * kRunWarps * (sizeof(UnitRecord) + (size_t)2 * 8 * p.groups * (p.hd + 2) * sizeof(float));
+    return p;
+}
+// As many groups as it takes for the line to be counted in 31 bits.
+Run4Plan plan_call(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows) {
+    int groups = run_groups(pool, group, max_rows);
+    while (groups < most_groups(pool) && !line_fits(pool, seqs, group, 8 * groups)) groups *= 2;
+    return plan_runs(pool, typ, groups);
+}
+// The most that a call with at most these arguments needs: fewer rows may take fewer groups, whose runs are more.
+size_t most_bytes(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows) {
+    const bool any = !line_fits(pool, seqs, group, 8);  // then a smaller max_rows may take any number of groups
+    size_t most = 16;
+    for (int groups = any ? most_groups(pool) : run_groups(pool, group, max_rows); groups >= 1; groups /= 2) most = std::max(most, plan_runs(pool, typ, groups).bytes);
+    return most;
+}
+
+template <int HD, int NG, bool F32, bool FULL>
+int32_t runs_as(const Kv4Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int blocks, cudaStream_t s) {
+    using Shape = Run4Shape<HD, NG, F32>;
+    const size_t cum = (size_t)(seqs.n_seqs + 1) * 4, smem = kRunWarps * Shape::kWarp + cum;
+    LC_CUDA(ensure_smem_limit((const void*)kv4_runs_kernel<HD, NG, F32, FULL>, smem));
+    kv4_runs_kernel<HD, NG, F32, FULL><<<blocks, kRunWarps * 32, smem, s>>>(pool, seqs, a);
+    LC_CUDA(cudaGetLastError());
+    LC_CUDA(launch_pdl(kv_join_kernel<HD, Shape::kRows>, dim3((unsigned)blocks * kRunWarps, (Shape::kRows + kJoinRows - 1) / kJoinRows), dim3(kJoinThreads), 0, s, a, pool.hd));
+    return LC_OK;
+}
+template <int HD, int NG>
+int32_t runs_full(const Kv4Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, int blocks, cudaStream_t s) {
+    if (a.typ == LC_TYPE_F32) return pool.hd == HD ? runs_as<HD, NG, true, true>(pool, seqs, a, blocks, s) : runs_as<HD, NG, true, false>(pool, seqs, a, blocks, s);
+    return pool.hd == HD ? runs_as<HD, NG, false, true>(pool, seqs, a, blocks, s) : runs_as<HD, NG, false, false>(pool, seqs, a, blocks, s);
+}
+template <int HD>
+int32_t runs_of(const Kv4Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const Run4Plan& p, cudaStream_t s) {
+    if constexpr (HD < 256)
+        if (p.groups == 4) return runs_full<HD, 4>(pool, seqs, a, p.blocks, s);
+    return p.groups == 2 ? runs_full<HD, 2>(pool, seqs, a, p.blocks, s) : runs_full<HD, 1>(pool, seqs, a, p.blocks, s);
+}
+
+int32_t check_heads(const char* call, const Kv4Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {
+    LC_CHECK(n_heads > 0 && n_heads <= 65536 && n_heads % pool.n_kv == 0, LC_ERR_INVALID, "%s: %d heads over %d kv heads", call, n_heads, pool.n_kv);
+    const int group = n_heads / pool.n_kv;
+    // a sequence outside its table may have all rows: what a call's rows are in the kernels' 32 bits
+    LC_CHECK((int64_t)seqs.n_rows * group < (int64_t)0x7fffffff - kTileRows2, LC_ERR_INVALID, "%s: %d rows of %d heads are too many for one call", call, seqs.n_rows, n_heads);
+    LC_CHECK(line_fits(pool, seqs, group, 8 * most_groups(pool)), LC_ERR_INVALID, "%s: %d rows of %d heads over tables of %d pages are too many for one call", call, seqs.n_rows, n_heads, seqs.width);
+    return LC_OK;
 }
 
 }  // namespace
 }  // namespace lc
 
 using namespace lc;
-
-namespace {
-int32_t check_heads(const char* call, const Kv4Pool& pool, const Kv8Seqs& seqs, int32_t n_heads) {
-    LC_CHECK(n_heads > 0 && n_heads <= 65536 && n_heads % pool.n_kv == 0, LC_ERR_INVALID, "%s: %d heads over %d kv heads", call, n_heads, pool.n_kv);
-    LC_CHECK((int64_t)seqs.n_rows * n_heads <= (int64_t)1 << 30, LC_ERR_INVALID, "%s: %d rows of %d heads are too many for one call", call, seqs.n_rows, n_heads);
-    return LC_OK;
-}
-}  // namespace
 
 extern "C" {
 
@@ -108,7 +513,13 @@ int32_t lc_attention_kv4_workspace(const lc_kv4_cache* cache, const lc_kv8_rows*
     LC_CHECK(out_bytes, LC_ERR_INVALID, "%s: null output", call);
     LC_TRY(kv4_check(call, cache, rows, typ, n_rows, &pool, &seqs));
     LC_TRY(check_heads(call, pool, seqs, n_heads));
-    *out_bytes = 16;
+    if (n_rows == 0 || seqs.n_seqs == 0) {  // nothing to do, as for the call itself
+        *out_bytes = 16;
+        return LC_OK;
+    }
+    DeviceScope dev;
+    LC_TRY(dev.enter(cache->k_dev, call));
+    *out_bytes = most_bytes(pool, seqs, typ, n_heads / pool.n_kv, rows->max_rows);
     return LC_OK;
 }
 
@@ -126,13 +537,19 @@ int32_t lc_attention_kv4_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows,
     LC_CHECK(q_stride >= (int64_t)n_heads * pool.hd && out_stride >= (int64_t)n_heads * pool.hd && (!lse_dev || lse_stride >= n_heads), LC_ERR_INVALID, "%s: rows overlap", call);
     DeviceScope dev;
     LC_TRY(dev.enter(cache->k_dev, call));
-    LC_CHECK(workspace_dev && workspace_bytes >= 16 && (uintptr_t)workspace_dev % 16 == 0, LC_ERR_INVALID, "%s: needs a workspace of 16 bytes, 16-byte aligned (got %zu)", call, workspace_bytes);
+    const int group = n_heads / pool.n_kv;
+    const Run4Plan plan = plan_call(pool, seqs, typ, group, rows->max_rows);
+    LC_CHECK(workspace_dev && workspace_bytes >= plan.bytes && (uintptr_t)workspace_dev % 16 == 0, LC_ERR_INVALID, "%s: needs a workspace of %zu bytes, 16-byte aligned (got %zu)", call, plan.bytes,
+             workspace_bytes);
     if (scale == 0.0f) scale = 1.0f / sqrtf((float)pool.hd);
-    const Attn4Args a{q_dev, out_dev, lse_dev, q_stride, out_stride, lse_stride, (int)typ, n_heads, n_heads / pool.n_kv, std::min(window, 1 << 30), scale};
-    const int64_t units = (int64_t)n_rows * n_heads;
-    kv4_attention_kernel<<<(unsigned)((units + kWarps - 1) / kWarps), kWarps * 32, 0, stream_or_own(stream_)>>>(pool, seqs, a);
-    LC_CUDA(cudaGetLastError());
-    return LC_OK;
+    window = std::min(window, 1 << 30);  // the kernels' differences of slots stay in 32 bits
+    const size_t elem = typ == LC_TYPE_F32 ? 4 : 2;
+    const AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16), scale * 1.44269504088896f,
+                     (float*)((char*)workspace_dev + (size_t)plan.blocks * kRunWarps * sizeof(UnitRecord)), (UnitRecord*)workspace_dev, lse_dev, lse_stride, kWeightUp};
+    cudaStream_t s = stream_or_own(stream_);
+    if (plan.hd == 64) return runs_of<64>(pool, seqs, a, plan, s);
+    if (plan.hd == 128) return runs_of<128>(pool, seqs, a, plan, s);
+    return runs_of<256>(pool, seqs, a, plan, s);
 }
 
 }  // extern "C"
