@@ -454,16 +454,31 @@ Run4Plan plan_runs(const Kv4Pool& pool, uint32_t typ, int groups) {
     p.bytes = (size_t)p.blocks * kRunWarps * (sizeof(UnitRecord) + (size_t)2 * 8 * p.groups * (p.hd + 2) * sizeof(float));
     return p;
 }
-// As many groups as it takes for the line to be counted in 31 bits.
-Run4Plan plan_call(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows) {
-    int groups = run_groups(pool, group, max_rows);
-    while (groups < most_groups(pool) && !line_fits(pool, seqs, group, 8 * groups)) groups *= 2;
-    return plan_runs(pool, typ, groups);
+bool tiles_fit(const Kv4Pool& pool, const Kv8Seqs& seqs, int group) {
+    TilePlan tiles;
+    return line_fits(pool, seqs, group, kTileRows2) && kv8_tiles_plan(pool, seqs, group, &tiles);
 }
-// The most that a call with at most these arguments needs: fewer rows may take fewer groups, whose runs are more.
+struct Plan {
+    bool by_tiles;
+    TilePlan tiles;
+    Run4Plan runs;
+    size_t bytes() const { return by_tiles ? tiles.bytes : runs.bytes; }
+};
+// The faster kernel, unless its line does not fit: a call with many more rows than its max_rows says goes by tiles then, or by as many groups as it takes.
+Plan plan_call(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows) {
+    Plan p;
+    int groups = run_groups(pool, group, max_rows);
+    p.by_tiles = kv8_tiles_plan(pool, seqs, group, &p.tiles) && line_fits(pool, seqs, group, kTileRows2) &&
+                 (kv8_tiles_pay(pool, seqs, typ, group, max_rows, p.tiles) || !line_fits(pool, seqs, group, 8 * groups));
+    while (!p.by_tiles && groups < most_groups(pool) && !line_fits(pool, seqs, group, 8 * groups)) groups *= 2;
+    p.runs = plan_runs(pool, typ, groups);
+    return p;
+}
+// The most that a call with at most these arguments needs: fewer rows, sequences or pages may go by runs instead of tiles, take fewer groups (whose
+// runs are more), or have their keys cut where larger ones are not, so the answer goes by none of them.
 size_t most_bytes(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows) {
-    const bool any = !line_fits(pool, seqs, group, 8);  // then a smaller max_rows may take any number of groups
-    size_t most = 16;
+    const bool any = !line_fits(pool, seqs, group, 8);  // then a smaller max_rows may lead to every kernel
+    size_t most = kv8_tiles_most_bytes(pool, any ? 1 << 30 : (int64_t)group * max_rows);
     for (int groups = any ? most_groups(pool) : run_groups(pool, group, max_rows); groups >= 1; groups /= 2) most = std::max(most, plan_runs(pool, typ, groups).bytes);
     return most;
 }
@@ -495,7 +510,7 @@ int32_t check_heads(const char* call, const Kv4Pool& pool, const Kv8Seqs& seqs, 
     const int group = n_heads / pool.n_kv;
     // a sequence outside its table may have all rows: what a call's rows are in the kernels' 32 bits
     LC_CHECK((int64_t)seqs.n_rows * group < (int64_t)0x7fffffff - kTileRows2, LC_ERR_INVALID, "%s: %d rows of %d heads are too many for one call", call, seqs.n_rows, n_heads);
-    LC_CHECK(line_fits(pool, seqs, group, 8 * most_groups(pool)), LC_ERR_INVALID, "%s: %d rows of %d heads over tables of %d pages are too many for one call", call, seqs.n_rows, n_heads, seqs.width);
+    LC_CHECK(line_fits(pool, seqs, group, 8 * most_groups(pool)) || tiles_fit(pool, seqs, group), LC_ERR_INVALID, "%s: %d rows of %d heads over tables of %d pages are too many for one call", call, seqs.n_rows, n_heads, seqs.width);
     return LC_OK;
 }
 
@@ -538,18 +553,20 @@ int32_t lc_attention_kv4_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows,
     DeviceScope dev;
     LC_TRY(dev.enter(cache->k_dev, call));
     const int group = n_heads / pool.n_kv;
-    const Run4Plan plan = plan_call(pool, seqs, typ, group, rows->max_rows);
-    LC_CHECK(workspace_dev && workspace_bytes >= plan.bytes && (uintptr_t)workspace_dev % 16 == 0, LC_ERR_INVALID, "%s: needs a workspace of %zu bytes, 16-byte aligned (got %zu)", call, plan.bytes,
-             workspace_bytes);
+    const Plan plan = plan_call(pool, seqs, typ, group, rows->max_rows);
+    const size_t need = plan.bytes();
+    LC_CHECK(workspace_dev && workspace_bytes >= need && (uintptr_t)workspace_dev % 16 == 0, LC_ERR_INVALID, "%s: needs a workspace of %zu bytes, 16-byte aligned (got %zu)", call, need, workspace_bytes);
     if (scale == 0.0f) scale = 1.0f / sqrtf((float)pool.hd);
     window = std::min(window, 1 << 30);  // the kernels' differences of slots stay in 32 bits
     const size_t elem = typ == LC_TYPE_F32 ? 4 : 2;
-    const AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16), scale * 1.44269504088896f,
-                     (float*)((char*)workspace_dev + (size_t)plan.blocks * kRunWarps * sizeof(UnitRecord)), (UnitRecord*)workspace_dev, lse_dev, lse_stride, kWeightUp};
+    AttnArgs a{q_dev, out_dev, q_stride, out_stride, (int)typ, group, window, rows_aligned(q_dev, q_stride, elem, 16), rows_aligned(out_dev, out_stride, elem, 16), scale * 1.44269504088896f,
+               (float*)workspace_dev, (UnitRecord*)workspace_dev, lse_dev, lse_stride, kWeightUp};
     cudaStream_t s = stream_or_own(stream_);
-    if (plan.hd == 64) return runs_of<64>(pool, seqs, a, plan, s);
-    if (plan.hd == 128) return runs_of<128>(pool, seqs, a, plan, s);
-    return runs_of<256>(pool, seqs, a, plan, s);
+    if (plan.by_tiles) return launch_kv4_tiles(pool, seqs, a, plan.tiles, s);
+    a.part = (float*)((char*)workspace_dev + (size_t)plan.runs.blocks * kRunWarps * sizeof(UnitRecord));
+    if (plan.runs.hd == 64) return runs_of<64>(pool, seqs, a, plan.runs, s);
+    if (plan.runs.hd == 128) return runs_of<128>(pool, seqs, a, plan.runs, s);
+    return runs_of<256>(pool, seqs, a, plan.runs, s);
 }
 
 }  // extern "C"

@@ -23,7 +23,7 @@
 #include <algorithm>
 #include "lc_kernels.h"
 #include "lc_kv8_attn.cuh"
-#include "lc_umma.cuh"
+#include "lc_attn_tiles.cuh"
 
 namespace lc {
 
@@ -63,30 +63,6 @@ template <int HD, bool SPLIT> struct TileShape {
     static constexpr int kRaw = kKeys * HD;                   // keys, values as they are in the cache
     static constexpr int kBytes = kQ + kK + kVs * kV + 2 * kRaw + 1024;
 };
-
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
-    tmem_ld16(taddr, r);
-    tmem_ld16(taddr + 16, r + 16);
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-}
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// products issued by the lane whose `by` is set, in a warp that goes through this together
-__device__ __forceinline__ void mma_ss_by(uint32_t by, uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(da), "l"(db),
-                 "r"(idesc), "r"(accumulate), "r"(by)
-                 : "memory");
-}
-__device__ __forceinline__ void mma_ts_by(uint32_t by, uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(db),
-                 "r"(idesc), "r"(accumulate), "r"(by)
-                 : "memory");
-}
-// 16-byte chunk `ch` (of 8) of a row of 128 bytes
-__device__ __forceinline__ int sw128(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
 
 template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a, int splits) {
@@ -614,44 +590,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
     if (warp == 0) tmem_free(tmem, 512);
 }
 
-// Joins the parts of units whose keys are cut: a warp per row.
-template <int HD>
-__global__ void __launch_bounds__(256) kv8_tiles_join_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a, int splits) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint2 sums[8];
-    uint32_t* units = reinterpret_cast<uint32_t*>(smem);
-    uint32_t* cum = units + seqs.n_seqs + 1;
-    line_up<kTileRows2>(seqs, pool, a, cum, units, sums);
-    pdl_wait();
-    if (blockIdx.x >= units[seqs.n_seqs]) return;
-    const int seq = seq_at(units, seqs.n_seqs, blockIdx.x), in = blockIdx.x - units[seq];
-    const SeqWork w = seq_work<kTileRows2>(seqs, pool, a, seq);
-    const int kvh = in % pool.n_kv, row_lo = (w.blocks - 1 - in / pool.n_kv) * kTileRows2, row_n = min(kTileRows2, w.n * a.group - row_lo);
-    const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (r >= row_n) return;
-    constexpr int PER = HD / 32;
-    float mx = kNegInf, sum = 0.0f, v[PER];
-#pragma unroll
-    for (int e = 0; e < PER; e++) v[e] = 0.0f;
-    for (int s = 0; s < splits; s++) {
-        const float* p = a.part + (size_t)(blockIdx.x * splits + s) * (kTileRows2 * (HD + 2));
-        const float pm = p[r], ps = p[kTileRows2 + r];
-        if (pm == kNegInf && ps == 0.0f) continue;      // no keys: its sums are not there
-        const float m2 = fmaxf(mx, pm), ref = m2 == kNegInf ? 0.0f : m2;
-        const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(pm - ref);
-        sum = f0 * sum + (isnan(ps) ? ps : f1 * ps);
-#pragma unroll
-        for (int e = 0; e < PER; e++) v[e] = fmaf(f0, v[e], f1 * p[2 * kTileRows2 + (size_t)r * HD + lane * PER + e]);
-        mx = m2;
-    }
-    const int tok = (row_lo + r) / a.group;
-    const int64_t dst = (int64_t)(w.first + tok) * a.out_stride + ((int64_t)kvh * a.group + (row_lo + r - tok * a.group)) * pool.hd;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int e = 0; e < PER; e++)
-        if (lane * PER + e < pool.hd) store1(a.out, dst + lane * PER + e, a.typ, v[e] * inv);
-}
-
 template <int HD, bool SPLIT>
 int32_t tiles_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const TilePlan& plan, cudaStream_t s) {
     using Shape = TileShape<HD, SPLIT>;
@@ -667,7 +605,7 @@ int32_t tiles_as(const Kv8Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, co
     LC_CUDA(cudaGetLastError());
     if (plan.splits > 1) {
         const size_t cum = (size_t)2 * (seqs.n_seqs + 1) * 4;
-        LC_CUDA(launch_pdl(kv8_tiles_join_kernel<HD>, dim3((unsigned)plan.units, kTileRows2 / 8), dim3(256), cum, s, pool, seqs, a, plan.splits));
+        LC_CUDA(launch_pdl(kv_tiles_join_kernel<HD>, dim3((unsigned)plan.units, kTileRows2 / 8), dim3(256), cum, s, pool, seqs, a, plan.splits));
     }
     return LC_OK;
 }

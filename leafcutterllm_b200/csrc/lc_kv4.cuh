@@ -15,6 +15,11 @@ struct Kv4Pool : Kv8Pool {
 // kv4.cu: the arguments that all calls over the cache have
 int32_t kv4_check(const char* call, const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, Kv4Pool* view, Kv8Seqs* seqs);
 
+struct AttnArgs;
+struct TilePlan;
+// attention_kv4_tiles.cu: many rows per sequence, by the plan of kv8_tiles_plan
+int32_t launch_kv4_tiles(const Kv4Pool& pool, const Kv8Seqs& seqs, const AttnArgs& a, const TilePlan& plan, cudaStream_t s);
+
 constexpr float kUnit4 = 8.0f;  // what the f16 values below are to be multiplied by
 
 #ifdef __CUDACC__
