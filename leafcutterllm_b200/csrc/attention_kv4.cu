@@ -39,30 +39,6 @@ template <int HD> __device__ __forceinline__ int value_chunk(int r, int ch) {
     const int slot = (r >> 1) + (r & 1) * 8;
     return slot * N + (HD == 256 ? ch ^ ((slot & 3) * 2) : HD == 128 ? ch ^ (slot & 2) : ch);
 }
-template <int N> __device__ __forceinline__ void lds_words(const unsigned char* p, uint32_t (&w)[N]) {  // N: 1, 2, 4 or 8 words, aligned to 16 bytes or their size
-    if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
-    else if constexpr (N == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[0] = u.x; w[1] = u.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N / 4; i++) {
-            const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-            w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
-        }
-    }
-}
-// the same, aligned to 8 bytes
-template <int N> __device__ __forceinline__ void lds_words8(const unsigned char* p, uint32_t (&w)[N]) {
-    if constexpr (N <= 2) lds_words<N>(p, w);
-    else
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) {
-            const uint2 u = reinterpret_cast<const uint2*>(p)[i];
-            w[2 * i] = u.x; w[2 * i + 1] = u.y;
-        }
-}
-
 template <int HD, int NG, bool F32, bool FULL>
 __global__ void __launch_bounds__(kRunWarps * 32, Run4Shape<HD, NG, F32>::kBlocks)
 kv4_runs_kernel(Kv4Pool pool, Kv8Seqs seqs, AttnArgs a) {

@@ -57,6 +57,30 @@ __device__ __forceinline__ void values8(uint32_t x, const Scale4& s, uint32_t (&
     v[2] = value_lo(x >> 8, s);
     v[3] = value_hi(x >> 8, s);
 }
+template <int N> __device__ __forceinline__ void lds_words(const unsigned char* p, uint32_t (&w)[N]) {  // N: 1, 2, 4 or 8 words, aligned to 16 bytes or their size
+    if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t*>(p);
+    else if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x; w[1] = u.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+            w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+        }
+    }
+}
+// the same, aligned to 8 bytes
+template <int N> __device__ __forceinline__ void lds_words8(const unsigned char* p, uint32_t (&w)[N]) {
+    if constexpr (N <= 2) lds_words<N>(p, w);
+    else
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            const uint2 u = reinterpret_cast<const uint2*>(p)[i];
+            w[2 * i] = u.x; w[2 * i + 1] = u.y;
+        }
+}
+
 // a block scale as a number
 __device__ __forceinline__ float scale4_f(uint32_t b) { return __half2float(__ushort_as_half((unsigned short)((b & 0x7fu) << 7))) * 256.0f; }
 
