@@ -431,6 +431,33 @@ def test_evict(gpu, case, ties):
     assert s.status.item() == 0
 
 
+@pytest.mark.parametrize("length,keep", [(450_000, 300_000), (449_999, 17), (100, 50)])
+def test_evict_of_contexts_beyond_shared_memory(gpu, length, keep):
+    """Tables of more slots than a cluster's shared memory has sums for."""
+    page, pages = 16, 30_000
+    rng = np.random.default_rng(keep)
+    table = rng.permutation(pages).astype(np.int32)[None]
+    pools = [rng.integers(0, 256, (pages, 1, page, n)).astype(np.uint8) for n in (8, 8, 1, 1)]
+    on_gpu = [cuda(a) for a in pools]
+    cache = gpu.Kv4Cache(*on_gpu, torch.ones(1, device="cuda"), torch.ones(1, device="cuda"))
+    rows = gpu.Kv8Rows(cuda(table), cuda(np.array([length], np.int32)), cuda(np.zeros(2, np.int32)), 0)
+    mass = rng.lognormal(0, 2, (1, 1, page * pages)).astype(np.float32)
+    got = cuda(mass)
+    kept, ctx = cache.evict(rows, got, keep, recent=5, first=3)
+    order = np.lexsort((np.arange(3, length - 5), -mass[0, 0, 3:length - 5]))[:keep - 8] + 3
+    stays = np.sort(np.concatenate((np.arange(3), order, np.arange(length - 5, length))))
+    assert ctx.item() == keep and (kept[0, 0].cpu().numpy() == stays).all()
+    want = mass[0, 0].copy()
+    want[:length] = 0.0
+    want[:keep] = mass[0, 0][stays]
+    assert (got[0, 0].cpu().numpy() == want).all()
+    at = lambda slots: table[0][slots // page]  # noqa: E731
+    for t, old in zip(on_gpu, pools):
+        new = old.copy()
+        new[at(np.arange(keep)), 0, np.arange(keep) % page] = old[at(stays), 0, stays % page]
+        assert (t.cpu().numpy() == new).all()
+
+
 def test_evict_leaves_bad_sequences_alone(gpu):
     s = Setup(gpu, [(100, 0), (100, 0), (100, 0), (100, 0)], 2, 64, 16)
     table, ctx = s.table.copy(), s.ctx.copy()
