@@ -291,8 +291,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
                 uint32_t first[4] = {0, 0, 0, 0}, second[4] = {0, 0, 0, 0};
                 if (ch * 16 < hd) {
                     const uint2 x = *reinterpret_cast<const uint2*>(rk + key * row_ints + ch * 8);
-                    const uint32_t b = rk[kKeys * HD / 2 + key * row_scales + ch];
-                    const Scale4 s = scale4(b | b << 16);
+                    const uint32_t b = rk[kKeys * HD / 2 + key * row_scales + ch] & 0x7fu;
+                    const Scale4 s = scale4_both(b, 0);
                     values8(x.x, s, first);
                     values8(x.y, s, second);
                 }
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
                         su = rv[kKeys * HD / 2 + key * row_scales + (word >> 1)];
                         sv2 = rv[kKeys * HD / 2 + (key + 1) * row_scales + (word >> 1)];
                     }
-                    const Scale4 s = scale4(su | sv2 << 16);
+                    const Scale4 s = scale4_pair(su, sv2);
                     const uint32_t x = __byte_perm(u, v, pick0), y = __byte_perm(u, v, pick1);  // (key, key + 1) of dims 0 - 3, of 4 - 7
                     out[0][k] = value_lo(x, s); out[1][k] = value_hi(x, s); out[2][k] = value_lo(x >> 8, s); out[3][k] = value_hi(x >> 8, s);
                     out[4][k] = value_lo(y, s); out[5][k] = value_hi(y, s); out[6][k] = value_lo(y >> 8, s); out[7][k] = value_hi(y >> 8, s);

@@ -25,11 +25,11 @@ struct WeightArgs {
 template <int HD, int NG, bool F32> struct WeightShape {
     static constexpr int kRows = 8 * NG;
     static constexpr int kTerms = F32 ? 2 : 1;
-    static constexpr int kStageBytes = kStep * HD / 2 + HD;               // keys, their scales
-    static constexpr int kStages = 6;
+    static constexpr int kStages = HD == 64 ? 8 : 4;
+    static constexpr int kRing = kStages * Ring4<HD, true, false, kStages>::kPlace;
     static constexpr bool kQueriesShared = HD == 256 || NG > 1;           // operand fragments of the queries in shared memory, not in registers
     static constexpr int kQueries = kQueriesShared ? NG * kTerms * (HD / 32) * 512 : 0;
-    static constexpr int kWarp = kStages * kStageBytes + kQueries;
+    static constexpr int kWarp = kRing + kQueries;
     static constexpr int kByRegisters = HD == 256 ? 2 : F32 ? 4 : 5;
     static constexpr int kByMemory = (220 << 10) / (kRunWarps * kWarp + 2048);
     static constexpr int kBlocks = kByRegisters < kByMemory ? kByRegisters : kByMemory;
@@ -106,8 +106,9 @@ kv4_weights_kernel(Kv4Pool pool, Kv8Seqs seqs, WeightArgs a) {
     const uint32_t t_end = runs.start(run + 1);
     unsigned char* const mine = smem + warp * Shape::kWarp;
     const uint32_t ring = smem_u32(mine);
-    uint4* const qs = reinterpret_cast<uint4*>(mine + S * Shape::kStageBytes);
-    const int hd = FULL ? HD : pool.hd, page_mask = (1 << pool.page_shift) - 1;
+    uint4* const qs = reinterpret_cast<uint4*>(mine + Shape::kRing);
+    const int hd = FULL ? HD : pool.hd;
+    using Ring = Ring4<HD, FULL, false, S>;
 
     while (t < t_end) {
         // a segment: this run's steps of one sequence and kv head.  A step is the run's that has its first place.
@@ -128,38 +129,10 @@ kv4_weights_kernel(Kv4Pool pool, Kv8Seqs seqs, WeightArgs a) {
             // the block's steps: from its first row's window to its last row's slot
             const int b0 = max(s0, (a.window > 0 ? max(0, w.ctx + tok_first - a.window + 1) : 0) / kStep - w.step0), b1 = min(s1, (w.ctx + tok_last) / kStep + 1 - w.step0);
             if (b0 >= b1) continue;
-            int pages_at = b0, pages = -1;
-            auto look_up = [&]() {
-                const int st = pages_at + lane;
-                pages = st < b1 ? table[((w.step0 + st) * kStep) >> pool.page_shift] : -1;
-            };
-            look_up();
-            uint32_t outside = 0;                // bit st % 32: that step's page is outside the pool
-            auto fetch = [&](int st) {
-                if (st - pages_at == 32) { pages_at += 32; look_up(); }
-                if (st < b1) {
-                    const int number = __shfl_sync(0xffffffffu, pages, st - pages_at);
-                    if (number < 0 || number >= pool.n_pages) {
-                        outside |= 1u << (st & 31);
-                        if (lane == 0) kv8_raise(seqs, seq);
-                    } else {
-                        outside &= ~(1u << (st & 31));
-                        const uint32_t dst = ring + (uint32_t)(st % S) * Shape::kStageBytes;
-                        const size_t row = ((((size_t)number * pool.n_kv + kvh) << pool.page_shift) + (((w.step0 + st) * kStep) & page_mask));
-                        const int8_t* ks = pool.k + row * (hd >> 1);
-                        if (FULL) {
+            Ring keys(pool, hd, table, kvh, w.step0, ring, lane);
+            bool bad = keys.begin(b0, b1);
 #pragma unroll
-                            for (int i = 0; i < KW * kStep / 32; i++) cp_async16(dst + (i * 32 + lane) * 16, ks + (i * 32 + lane) * 16);
-                        } else {
-                            for (int ch = lane; ch < hd >> 1; ch += 32) cp_async16(dst + ch * 16, ks + ch * 16);
-                        }
-                        if (lane < hd >> 4) cp_async16(dst + kStep * HD / 2 + lane * 16, pool.k_block + row * (hd >> 4) + lane * 16);
-                    }
-                }
-                cp_async_commit();
-            };
-#pragma unroll
-            for (int k = 0; k < S - 1; k++) fetch(b0 + k);
+            for (int k = 0; k < S - 1; k++) bad = keys.fetch(b0 + k, k == 0) || bad;
 
             // The queries as operand fragments.  A thread's dims are HD / 4 in a row, eight of which make two k steps: (0, 4), (1, 5) and (2, 6), (3, 7), as the keys' words give them.
             uint32_t qf[Shape::kQueriesShared ? 1 : TERMS * KS][2];
@@ -226,18 +199,19 @@ kv4_weights_kernel(Kv4Pool pool, Kv8Seqs seqs, WeightArgs a) {
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) all_rows = all_rows && limit[gr][0] >= 0 && limit[gr][1] >= 0;
             all_rows = __all_sync(0xffffffffu, all_rows);
+            const int plain0 = !all_rows ? b1 : from < 0 ? 0 : from / kStep + 1 - w.step0, plain1 = (sees + 1) / kStep - w.step0;   // steps whose keys all rows see
             for (int st = b0; st < b1; st++) {
                 cp_async_wait<S - 2>();
                 __syncwarp();
-                fetch(st + S - 1);  // into the place of the step before
-                if (outside >> (st & 31) & 1) continue;
+                bad = keys.fetch(st + S - 1) || bad;  // into the place of the step before
+                if (keys.any_bad && keys.outside(st)) continue;
                 const int key0 = (w.step0 + st) * kStep, key = key0 + g + 8 * (c & 1);
-                const bool plain = all_rows && key0 + kStep - 1 <= sees && key0 > from;
+                const bool plain = st >= plain0 && st < plain1;
                 // the sums' own threads: c = 0 has key g, c = 1 key g + 8
                 const bool writes = c < 2 && key < w.ctx + w.n;
                 float* const to = mass + key;
                 const float before = writes ? *to : 0.0f;
-                const unsigned char* kp = mine + (st % S) * Shape::kStageBytes;
+                const unsigned char* kp = mine + (st & (S - 1)) * Ring::kPlace;
                 uint32_t kf[KS][4];
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
@@ -245,17 +219,17 @@ kv4_weights_kernel(Kv4Pool pool, Kv8Seqs seqs, WeightArgs a) {
                     uint32_t kw[KW];
                     if (FULL) lds_words<KW>(kp + row * (HD / 2) + c * (HD / 8), kw);
                     else lds_words8<KW>(kp + row * (hd >> 1) + c * (HD / 8), kw);
-                    const unsigned char* sc = kp + kStep * HD / 2 + row * (hd >> 4) + c * (HD / 64);
+                    const unsigned char* sc = kp + Ring::kScales + row * (hd >> 4) + c * (HD / 64);
                     uint32_t bytes = 0;
                     if (HD == 64) bytes = *sc;
                     else if (FULL) bytes = HD == 128 ? *reinterpret_cast<const uint16_t*>(sc) : *reinterpret_cast<const uint32_t*>(sc);
                     else
 #pragma unroll
                         for (int j = 0; j < HD / 64; j++) bytes |= (uint32_t)sc[j] << (8 * j);
+                    bytes &= 0x7f7f7f7fu;
 #pragma unroll
                     for (int j = 0; j < HD / 64; j++) {
-                        const uint32_t b = (bytes >> (8 * j)) & 0xffu;
-                        const Scale4 k4 = scale4(b | b << 16);
+                        const Scale4 k4 = scale4_both(bytes, j);
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
                             uint32_t kv[4];
@@ -289,8 +263,7 @@ kv4_weights_kernel(Kv4Pool pool, Kv8Seqs seqs, WeightArgs a) {
                         }
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        // products are rounded by themselves: far from 0 their difference to lse is then exact near it
-                        float y = __fsub_rn(__fmul_rn(dot[0][e] + dot[1][e], f[gr][e & 1]), less[gr][e & 1]);
+                        float y = fmaf(dot[0][e] + dot[1][e], f[gr][e & 1], -less[gr][e & 1]);
                         if (!plain) {
                             const int k = key0 + g + 8 * (e >> 1);
                             if (k > limit[gr][e & 1] || (a.window > 0 && k <= limit[gr][e & 1] - a.window)) y = kNegInf;
@@ -307,6 +280,7 @@ kv4_weights_kernel(Kv4Pool pool, Kv8Seqs seqs, WeightArgs a) {
             }
             cp_async_wait<0>();
             __syncwarp();
+            if (bad && lane == 0) kv8_raise(seqs, seq);
         }
     }
 }

@@ -243,70 +243,6 @@ __device__ __forceinline__ void place_at(Place& at, const Kv8Seqs& s, const Kv8P
     at.rb = unit - at.kvh * at.w.blocks;
 }
 
-// Joins the partial results of units that lie in several runs.  grid: (runs, slices of kJoinRows rows); a run's record says which unit begins in it.  Threads
-// take four dims of a row each, and what threads are left over shares of the partial results.
-constexpr int kJoinThreads = 128, kJoinRows = 4;
-template <int HD, int RB>
-__global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(AttnArgs a, int hd) {
-    __shared__ float4 s_val[kJoinThreads];
-    __shared__ float s_m[kJoinThreads], s_sum[kJoinThreads];
-    constexpr int P = part_floats<HD, RB>(), Q = HD / 4;
-    pdl_wait();  // every block: this kernel's end then means that of the one before
-    const int b = blockIdx.x;
-    const int4 at = *reinterpret_cast<const int4*>(&a.records[b]);
-    const int last = a.records[b].last, row0 = blockIdx.y * kJoinRows, rows = min(kJoinRows, at.w - row0);
-    if (rows <= 0) return;
-    const int cells = rows * Q, per = min(cells, kJoinThreads), shares = kJoinThreads / per, share = threadIdx.x / per;
-    for (int e0 = 0; e0 < cells; e0 += per) {
-        const int e = e0 + threadIdx.x - share * per, r = row0 + e / Q, d = (e % Q) * 4;
-        const bool here = share < shares && e < cells;
-        float mx = kNegInf, sum = 0.0f;
-        float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (here) {
-            const float* p = a.part + (size_t)(2 * b + 1) * P;  // of the run itself the second place, of the later ones the first
-#pragma unroll 8
-            for (int x = b + share; x <= last; x += shares) {
-                const float* q = x == b ? p : a.part + (size_t)(2 * x) * P;
-                const float pm = q[r], ps = q[RB + r];
-                const float4 v = *reinterpret_cast<const float4*>(q + 2 * RB + r * HD + d);
-                const float m2 = fmaxf(mx, pm), ref = m2 == kNegInf ? 0.0f : m2;
-                const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(pm - ref);
-                sum = f0 * sum + (isnan(ps) ? ps : f1 * ps);
-                val.x = fmaf(f0, val.x, f1 * v.x); val.y = fmaf(f0, val.y, f1 * v.y);
-                val.z = fmaf(f0, val.z, f1 * v.z); val.w = fmaf(f0, val.w, f1 * v.w);
-                mx = m2;
-            }
-        }
-        if (shares > 1) {
-            __syncthreads();
-            s_val[threadIdx.x] = val; s_m[threadIdx.x] = mx; s_sum[threadIdx.x] = sum;
-            __syncthreads();
-            if (share == 0 && here) {
-                for (int x = 1; x < shares; x++) {
-                    const int k = x * per + threadIdx.x;
-                    const float m2 = fmaxf(mx, s_m[k]), ref = m2 == kNegInf ? 0.0f : m2;
-                    const float f0 = exp2_fast(mx - ref), f1 = exp2_fast(s_m[k] - ref);
-                    const float4 v = s_val[k];
-                    sum = f0 * sum + f1 * s_sum[k];
-                    val.x = fmaf(f0, val.x, f1 * v.x); val.y = fmaf(f0, val.y, f1 * v.y);
-                    val.z = fmaf(f0, val.z, f1 * v.z); val.w = fmaf(f0, val.w, f1 * v.w);
-                    mx = m2;
-                }
-            }
-        }
-        if (share == 0 && here && d < hd) {
-            const int tok = (at.z + r) / a.group, hq = (at.z + r) - tok * a.group;
-            if (a.lse && d == 0) a.lse[(int64_t)(at.x + tok) * a.lse_stride + at.y * a.group + hq] = (mx + (log2f(sum) - a.lse_less)) * 0.693147180559945f;
-            const int64_t dst = (int64_t)(at.x + tok) * a.out_stride + (int64_t)(at.y * a.group + hq) * hd + d;
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            store1(a.out, dst, a.typ, val.x * inv);
-            store1(a.out, dst + 1, a.typ, val.y * inv);
-            store1(a.out, dst + 2, a.typ, val.z * inv);
-            store1(a.out, dst + 3, a.typ, val.w * inv);
-        }
-    }
-}
-
 // Whether the places of the line, with row blocks of so many rows, are sure to stay in 31 bits: every context as long as its table.
 inline bool line_fits(const Kv8Pool& pool, const Kv8Seqs& seqs, int group, int block_rows) {
     const double steps = (double)((int64_t)seqs.width << pool.page_shift) / kStep + 2 + kUnitCost;
