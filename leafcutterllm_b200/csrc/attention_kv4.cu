@@ -378,17 +378,17 @@ __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a, int 
     pdl_wait();  // every block: this kernel's end then means that of the one before
     const int b0 = blockIdx.x * kJoinRuns, row0 = blockIdx.y * kJoinRows, cell = threadIdx.x % CELLS, share = threadIdx.x / CELLS;
     const int r = row0 + cell / Q, d = (cell % Q) * 4;
-    int rows[kJoinRuns];
-#pragma unroll
-    for (int k = 0; k < kJoinRuns; k++) rows[k] = b0 + k < runs ? a.records[b0 + k].row_n : 0;
-#pragma unroll 1
-    for (int k = 0; k < kJoinRuns; k++) {
-        int n = 0;
-#pragma unroll
-        for (int x = 0; x < kJoinRuns; x++) n = x == k ? rows[x] : n;
-        if (n <= row0) continue;
-        const int b = b0 + k, last = a.records[b].last;
-        const int4 at = *reinterpret_cast<const int4*>(&a.records[b]);
+    // the runs' records, one per lane
+    const int lane = threadIdx.x & 31;
+    UnitRecord mine;
+    mine.row_n = 0;
+    if (lane < kJoinRuns && b0 + lane < runs) {
+        *reinterpret_cast<int4*>(&mine) = *reinterpret_cast<const int4*>(&a.records[b0 + lane]);
+        mine.last = a.records[b0 + lane].last;
+    }
+    for (uint32_t which = __ballot_sync(0xffffffffu, mine.row_n > row0); which; which &= which - 1) {
+        const int k = __ffs(which) - 1, b = b0 + k, last = __shfl_sync(0xffffffffu, mine.last, k), n = __shfl_sync(0xffffffffu, mine.row_n, k);
+        const int4 at = make_int4(__shfl_sync(0xffffffffu, mine.first, k), __shfl_sync(0xffffffffu, mine.kvh, k), __shfl_sync(0xffffffffu, mine.row_lo, k), n);
         float mx = kNegInf, sum = 0.0f;
         float4 val = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         auto add = [&](float pm, float ps, const float4& v) {

@@ -1,8 +1,8 @@
 // The key/value cache in 4 bits: appending rows (with the position rotation on the way), reading rows back.
 //
 // A row's 16 dims x have the block scale s = e4m3(max |x| / (7 g)) and the integers n = rint(x / (s g)), all as if in 64 bits, so that the cache's bytes depend on the definition alone.
-// Rotations are in 64 bits (the GPU has half as many such units as of f32); quotients are in f32, 2^-22 off, and what lies too near a border between two integers or two scales
-// is compared with the border in 64 bits, where both are exact.  A thread has the 16 dims of one block and loads the 16 that they are paired with, so rows pass once.
+// f32 decides them wherever its error bounds allow; a block with a number or a scale too near a border between two, with infinities, NaN or sizes beyond f32's relative errors is done again in 64 bits.
+// A thread has the 16 dims of one block and loads the 16 that they are paired with, so rows pass once.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -46,50 +46,116 @@ struct Block4 {
     uint2 words;
     uint32_t scale;
 };
-// y: the numbers in 64 bits (in f32 where these are all there is)
-template <typename Y>
-__device__ __forceinline__ Block4 quantised(const Y (&y)[16], float g) {
-    float x[16], most = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-        x[e] = (float)y[e];
-        if (sizeof(Y) == 8 && isinf(x[e]) && !isinf(y[e])) x[e] = copysignf(FLT_MAX, x[e]);  // two large ones together
-        const float a = fabsf(x[e]);
-        most = a < INFINITY ? fmaxf(most, a) : most;
+// s is `k` steps of the numbers of its size, 2^size to 2^(size + 1): 2^(size - 3) each; k = 16 is the next size's 8
+__device__ __forceinline__ float block_scale(float k, int size) { return fminf(k * __int_as_float((127 + size - 3) << 23), 448.0f); }
+__device__ __forceinline__ int size_of(float want) { return min(max((__float_as_int(want) >> 23) - 127, -6), 9); }
+__device__ __forceinline__ uint32_t scale_byte(float s) { return s >= 0x1p-6f ? (__float_as_uint(s) >> 20) - (120u << 3) : (uint32_t)(s * 512.0f); }
+
+// Where a block's numbers come from: dims d0 .. d0 + 15 of a head at x, turned by the row of a table (cosines and sines, then what their f32 lost) where they are before 2 * half.
+template <typename T> struct BlockFrom {
+    const T* x;
+    const float2* row;
+    const float2* low;
+    int d0, half, n8;
+    bool interleaved;
+    __device__ __forceinline__ double number(int e) const {
+        const int d = d0 + e;
+        const double own = elem_f(x[d]);
+        if (d >= 2 * half) return own;
+        const int p = interleaved ? d >> 1 : d < half ? d : d - half, at = turn_place(p, n8);
+        const bool second = interleaved ? d & 1 : d >= half;
+        const double other = elem_f(x[interleaved ? d ^ 1 : second ? d - half : d + half]);
+        const double c = (double)row[at].x + (double)low[at].x, si = (double)row[at].y + (double)low[at].y;
+        return own * c + other * (second ? si : -si);
     }
-    // s: k steps of the numbers of its size, 2^-9 at the least; k = 16 is the next size's 8
-    const float want = most * (1.0f / (7.0f * g));
-    const int size = min(max((__float_as_int(want) >> 23) - 127, -6), 9);
+};
+template <typename P> __device__ __forceinline__ P* from_lane(P* p, int lane) { return reinterpret_cast<P*>(__shfl_sync(0xffffffffu, (unsigned long long)p, lane)); }
+// The definition, in 64 bits, for the block of one lane, by the whole warp: a number per lane, twice.  Its own lane gets the result.
+template <typename T> __device__ __noinline__ Block4 quantised64(const T* x, int d0, int half, const float2* row, const float2* low, int n8, bool interleaved, float head, int whose, Block4 out) {
+    const int lane = threadIdx.x & 31;
+    const BlockFrom<T> f{from_lane(x, whose), row, low, __shfl_sync(0xffffffffu, d0, whose), __shfl_sync(0xffffffffu, half, whose), n8, interleaved};
+    const float g = __shfl_sync(0xffffffffu, head, whose);
+    const double y = f.number(lane & 15), z = fabs(y);
+    double top = z < (double)INFINITY ? z : 0.0;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // f32 says which two scales and integers are near; the border between them, exact in 64 bits, says which it is
+    const float want = (float)fmin(top, (double)FLT_MAX) * (1.0f / (7.0f * g));
+    const int size = size_of(want);
     const float r = want * __int_as_float((127 + 3 - size) << 23);
     float k = rintf(r);
     if (fabsf(fabsf(r - k) - 0.5f) < 0x1p-15f) {
-        double top = 0.0;
-#pragma unroll
-        for (int e = 0; e < 16; e++) top = fabs((double)y[e]) < (double)INFINITY ? fmax(top, fabs((double)y[e])) : top;
         const float below = rintf(r - 0.5f);
         const double border = ((double)below + 0.5) * (double)__int_as_float((127 + size - 3) << 23) * (7.0 * (double)g);
         k = top > border ? below + 1.0f : top < border ? below : 2.0f * rintf(0.5f * (below + 0.5f));
     }
-    const float s = fminf(k * __int_as_float((127 + size - 3) << 23), 448.0f);
-    Block4 out;
-    out.scale = s >= 0x1p-6f ? (__float_as_uint(s) >> 20) - (120u << 3) : (uint32_t)(s * 512.0f);
-    const float inv = s > 0.0f ? 1.0f / (s * g) : 0.0f;
+    const float s = block_scale(k, size);
     const double step = (double)s * (double)g;
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 16; e++) {
-        const float a = fabsf(x[e] * inv);
-        float n = rintf(a);
-        if (fabsf(fabsf(a - n) - 0.5f) < 1e-5f) {
-            const float below = rintf(a - 0.5f);
-            const double border = ((double)below + 0.5) * step, z = fabs((double)y[e]);
-            n = z > border ? below + 1.0f : z < border ? below : 2.0f * rintf(0.5f * (below + 0.5f));
-        }
-        const int m = a == a ? (int)fminf(n, 7.0f) : 0;
-        w[e >> 3] |= (uint32_t)(x[e] < 0.0f ? 8 - m : 8 + m) << (4 * (e & 7));
+    const float a = fminf((float)fmin(z, (double)FLT_MAX) * (s > 0.0f ? 1.0f / (s * g) : 0.0f), 8.0f);
+    float n = rintf(a);
+    if (fabsf(fabsf(a - n) - 0.5f) < 1e-5f) {
+        const float below = rintf(a - 0.5f);
+        const double border = ((double)below + 0.5) * step;
+        n = z > border ? below + 1.0f : z < border ? below : 2.0f * rintf(0.5f * (below + 0.5f));
     }
-    out.words = make_uint2(w[0], w[1]);
+    const int m = s > 0.0f && !isnan(y) ? (int)fminf(n, 7.0f) : 0;
+    uint32_t w = (uint32_t)(y < 0.0 ? 8 - m : 8 + m) << (4 * (lane & 7));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
+    const uint32_t w0 = __shfl_sync(0xffffffffu, w, 0), w1 = __shfl_sync(0xffffffffu, w, 8);
+    if (lane == whose) {
+        out.words = make_uint2(w0, w1);
+        out.scale = scale_byte(s);
+    }
     return out;
+}
+// The same in f32, for numbers that are off by `off` at most: false where one, or their scale, lies too near a border, where one is not finite, and for sizes that f32's relative errors do not
+// hold for.  Numbers that are exact (off 0) often lie on borders, bf16 under a scale that is a power of two; these are compared in 64 bits.
+__device__ __forceinline__ bool quantised32(const float (&y)[16], float off, float g, Block4& out) {
+    float most = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; e++) most = max_nan(most, fabsf(y[e]));
+    const float want = most * (1.0f / (7.0f * g));
+    const int size = size_of(want);
+    const float up = __int_as_float((127 + 3 - size) << 23), r = want * up;
+    float k = rintf(r);
+    // r is off by 2^-21 of itself besides; quotients, up to 7.5, by 2^-19
+    bool sure = fabsf(r - k) < 0.5f - (off * (1.0f / (7.0f * g)) * up + r * 0x1p-21f);
+    if (!sure && off == 0.0f) {
+        const float below = rintf(r - 0.5f);
+        const double border = ((double)below + 0.5) * (double)__int_as_float((127 + size - 3) << 23) * (7.0 * (double)g);
+        k = (double)most > border ? below + 1.0f : (double)most < border ? below : 2.0f * rintf(0.5f * (below + 0.5f));
+        sure = true;
+    }
+    const float s = block_scale(k, size), inv = 1.0f / (s * g);
+    float least = 0.0f;
+    uint32_t w[2] = {0, 0};
+    // of eight sums' upper bits, 0x4b400000, what eight multiplications by 16 leave
+    constexpr uint32_t kUpper = 0x3f400000u;
+#pragma unroll
+    for (int e = 15; e >= 0; e--) {
+        // added to 1.5 2^23 + 8, a small number is rounded to a whole one, to the nearest even, and 8 more are in the sum's low bits
+        const float q = y[e] * inv, t = q + 12582920.0f;
+        least = fmaxf(least, fabsf(q - (t - 12582920.0f)));
+        w[e >> 3] = w[e >> 3] * 16u + __float_as_uint(t);
+    }
+    sure = sure && most * inv < 7.49f && most > 1e-30f && s > 0.0f;
+    if (!(least < 0.5f - (off * inv + 0x1p-19f)) && sure) {
+        if (off != 0.0f) return false;
+        const double step = (double)s * (double)g, middle = 0.5 * step;
+        w[0] = w[1] = 0;
+#pragma unroll
+        for (int e = 15; e >= 0; e--) {
+            const float n = (y[e] * inv + 12582912.0f) - 12582912.0f;
+            const double rest = fma((double)-n, step, (double)y[e]);   // compared with what 64 bits hold, its one rounding does not matter
+            const bool odd = ((int)n & 1) != 0;
+            const float to = rest > middle || (rest == middle && odd) ? n + 1.0f : rest < -middle || (rest == -middle && odd) ? n - 1.0f : n;
+            w[e >> 3] = w[e >> 3] * 16u + __float_as_uint(to + 12582920.0f);
+        }
+    }
+    out.words = make_uint2(w[0] - kUpper, w[1] - kUpper);
+    out.scale = scale_byte(s);
+    return sure;
 }
 
 // Sixteen elements in a row as f32
@@ -106,23 +172,26 @@ template <typename T, bool VEC> __device__ __forceinline__ void load16f(const T*
     }
 }
 
-// Dims d0 .. d0 + 15 of a head of keys, turned.  VEC: they lie on one side of the middle and of the end of the rotated part, and 16-byte accesses are possible.
+// Dims d0 .. d0 + 15 of a head of keys, turned in f32; returns how far one may be off.  VEC: they lie on one side of the middle and of the end of the rotated part, and 16-byte accesses are possible.
 template <typename T, bool VEC>
-__device__ __forceinline__ void turned16(const T* x, int d0, int half, bool interleaved, const double2* row, int n8, double (&y)[16]) {
-    float v[16];
+__device__ __forceinline__ float turned16(const T* x, int d0, int half, bool interleaved, const float2* row, int n8, float (&y)[16]) {
+    float v[16], big = 0.0f, other_big = 0.0f;
     load16f<T, VEC>(x + d0, v);
+#pragma unroll
+    for (int e = 0; e < 16; e++) big = fmaxf(big, fabsf(v[e]));
     if (VEC) {
         if (d0 >= 2 * half) {
 #pragma unroll
             for (int e = 0; e < 16; e++) y[e] = v[e];
-        } else if (interleaved) {
+            return 0.0f;
+        }
+        if (interleaved) {
             const int p8 = d0 >> 4;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const double2 t = row[k * n8 + p8];
-                const double a = v[2 * k], b = v[2 * k + 1];
-                y[2 * k] = a * t.x - b * t.y;
-                y[2 * k + 1] = a * t.y + b * t.x;
+                const float2 t = row[k * n8 + p8];
+                y[2 * k] = v[2 * k] * t.x - v[2 * k + 1] * t.y;
+                y[2 * k + 1] = v[2 * k] * t.y + v[2 * k + 1] * t.x;
             }
         } else {
             const bool second = d0 >= half;
@@ -131,9 +200,9 @@ __device__ __forceinline__ void turned16(const T* x, int d0, int half, bool inte
             const int p8 = (second ? d0 - half : d0) >> 3;
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const double2 t = row[(e & 7) * n8 + p8 + (e >> 3)];
-                const double own = v[e], other = w[e];
-                y[e] = own * t.x + other * (second ? t.y : -t.y);
+                const float2 t = row[(e & 7) * n8 + p8 + (e >> 3)];
+                y[e] = v[e] * t.x + w[e] * (second ? t.y : -t.y);
+                other_big = fmaxf(other_big, fabsf(w[e]));
             }
         }
     } else {
@@ -144,17 +213,20 @@ __device__ __forceinline__ void turned16(const T* x, int d0, int half, bool inte
             if (d < 2 * half) {
                 const int p = interleaved ? d >> 1 : d < half ? d : d - half;
                 const bool second = interleaved ? d & 1 : d >= half;
-                const double other = elem_f(x[interleaved ? d ^ 1 : second ? d - half : d + half]);
-                const double2 t = row[turn_place(p, n8)];
+                const float other = elem_f(x[interleaved ? d ^ 1 : second ? d - half : d + half]);
+                const float2 t = row[turn_place(p, n8)];
                 y[e] = y[e] * t.x + other * (second ? t.y : -t.y);
+                other_big = fmaxf(other_big, fabsf(other));
             }
         }
     }
+    // sine and cosine are off by 2^-25 of themselves (magnitude 1), products and their sum by 2^-24 each, of the two numbers together
+    return (big + fmaxf(big, other_big)) * 0x1p-22f;
 }
 
 // grid: (groups of rows, slices of kv heads and then of query heads)
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(Kv4Pool pool, Kv8Seqs seqs, Append4Args a) {
+__global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(Kv4Pool pool, Kv8Seqs seqs, Append4Args a) {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ RowPlace place[kAppendRows];
     if (blockIdx.x == 0 && blockIdx.y == 0) kv8_check_seqs(seqs, pool);
@@ -167,58 +239,92 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_append_kernel(Kv4Pool pool
             if (at.seq >= 0 && at.page < 0) kv8_raise(seqs, at.seq);
         }
     }
-    __syncthreads();
     const bool kv = (int)blockIdx.y < a.kv_slices;
     const int slices = kv ? a.kv_slices : gridDim.y - a.kv_slices, sl = kv ? blockIdx.y : blockIdx.y - a.kv_slices, heads = kv ? pool.n_kv : a.n_heads;
-    const int h0 = heads * sl / slices, mine = heads * (sl + 1) / slices - h0;
+    const int h0 = heads * sl / slices, h1 = heads * (sl + 1) / slices;
     const int hd = pool.hd, half = a.half, n8 = (half + 7) >> 3;
+    float2* const tab = reinterpret_cast<float2*>(smem);       // cosines and sines of the rows' pairs, then what f32 lost of them
+    float2* const low = tab + rows * 8 * n8;
+    if (VEC && tid < rows) {
+        const uint32_t head = (uint32_t)(hd * sizeof(T));
+        if (kv) {
+            prefetch_l2((const T*)a.k + (row0 + tid) * a.k_stride + (int64_t)h0 * hd, (h1 - h0) * head);
+            prefetch_l2((const T*)a.v + (row0 + tid) * a.v_stride + (int64_t)h0 * hd, (h1 - h0) * head);
+        } else {
+            prefetch_l2((const T*)a.q + (row0 + tid) * a.q_stride + (int64_t)h0 * hd, (h1 - h0) * head);
+        }
+    }
+    __syncthreads();
+    const Divider by_half(half);
     for (int e = tid; e < rows * half; e += kAppendThreads) {
-        const int j = e / half, p = e - j * half;
+        const int j = by_half(e), p = e - j * half;
         const RowPlace& at = place[j];
         if (at.seq < 0) continue;
         double2 t = turn_of(a.turns[p], (a.positions ? a.positions[at.seq] : (int64_t)seqs.ctx[at.seq]) + at.index);
         t.x *= a.magnitude;
         t.y *= a.magnitude;
         const int to = j * 8 * n8 + turn_place(p, n8);
-        if (kv) reinterpret_cast<double2*>(smem)[to] = t;
-        else put_turn(reinterpret_cast<typename TurnEntry<T>::type*>(smem)[to], t);
+        const float2 high = make_float2((float)t.x, (float)t.y);
+        tab[to] = high;
+        low[to] = make_float2((float)(t.x - high.x), (float)(t.y - high.y));
     }
     __syncthreads();
+    // a row has its own share of the threads, whole warps
+    const int share = kAppendThreads / a.rows, j = tid / share, mine = tid - j * share;
+    if (j >= rows) return;
+    const RowPlace at = place[j];
+    const float2* const row = tab + j * 8 * n8;
     if (kv) {
-        // blocks of 16 dims: of the rows' keys, then of their values
-        const int blocks = hd >> 4, per_row = mine * blocks, all = rows * per_row;
-        for (int e = tid; e < 2 * all; e += kAppendThreads) {
-            const bool is_k = e < all;
-            const int f = is_k ? e : e - all, j = f / per_row, g = f - j * per_row, h = h0 + g / blocks, b = g % blocks;
-            const RowPlace& at = place[j];
-            if (at.page < 0) continue;
-            const T* x = (const T*)(is_k ? a.k : a.v) + (int64_t)(row0 + j) * (is_k ? a.k_stride : a.v_stride) + (int64_t)h * hd;
+        if (at.page < 0) return;
+        // blocks of 16 dims, of the row's keys, then of its values; a warp's lanes go through this together
+        const int blocks = hd >> 4, all = (h1 - h0) * blocks;
+        const Divider by_blocks(blocks);
+        const float by_magnitude = fmaxf(1.0f, fabsf((float)a.magnitude));
+        const T* const k_row = (const T*)a.k + (int64_t)(row0 + j) * a.k_stride;
+        const T* const v_row = (const T*)a.v + (int64_t)(row0 + j) * a.v_stride;
+        for (int e0 = mine & ~31; e0 < 2 * all; e0 += share) {
+            const int e = min(e0 + lane, 2 * all - 1);
+            const bool here = e0 + lane < 2 * all, is_k = e < all;
+            const int f = is_k ? e : e - all, g = by_blocks(f), h = h0 + g, b = f - g * blocks;
+            const float head = (is_k ? pool.k_scale : pool.v_scale)[h];
+            const T* const x = (is_k ? k_row : v_row) + h * hd;
             Block4 out;
-            if (is_k && half > 0) {
-                double y[16];
-                turned16<T, VEC>(x, 16 * b, half, a.interleaved, reinterpret_cast<const double2*>(smem) + j * 8 * n8, n8, y);
-                out = quantised(y, pool.k_scale[h]);
-            } else {
-                float y[16];
-                load16f<T, VEC>(x + 16 * b, y);
-                out = quantised(y, (is_k ? pool.k_scale : pool.v_scale)[h]);
+            float y[16], off = 0.0f;
+            if (is_k && half > 0) off = turned16<T, VEC>(x, 16 * b, half, a.interleaved, row, n8, y) * by_magnitude;
+            else load16f<T, VEC>(x + 16 * b, y);
+            const bool sure = quantised32(y, off, head, out);
+            for (uint32_t left = __ballot_sync(0xffffffffu, here && !sure); left; left &= left - 1)
+                out = quantised64(x, 16 * b, is_k ? half : 0, row, low + j * 8 * n8, n8, a.interleaved, head, __ffs(left) - 1, out);
+            if (here) {
+                const size_t to = (((size_t)at.page * pool.n_kv + h) << pool.page_shift) + at.slot;
+                *reinterpret_cast<uint2*>((is_k ? pool.k : pool.v) + to * (hd >> 1) + 8 * b) = out.words;
+                (is_k ? pool.k_block : pool.v_block)[to * blocks + b] = (uint8_t)out.scale;
             }
-            const size_t row = (((size_t)at.page * pool.n_kv + h) << pool.page_shift) + at.slot;
-            *reinterpret_cast<uint2*>((is_k ? pool.k : pool.v) + row * (hd >> 1) + 8 * b) = out.words;
-            (is_k ? pool.k_block : pool.v_block)[row * blocks + b] = (uint8_t)out.scale;
         }
-    } else {
-        using Entry = typename TurnEntry<T>::type;
-        const int items = VEC ? turn_items(hd, half) : hd - half, per_row = mine * items;
-        for (int e = tid; e < rows * per_row; e += kAppendThreads) {
-            const int j = e / per_row, g = e - j * per_row, h = h0 + g / items, i = g % items;
-            const RowPlace& at = place[j];
-            if (at.seq < 0 || at.slot < 0) continue;
-            const T* in = (const T*)a.q + (int64_t)(row0 + j) * a.q_stride + (int64_t)h * hd;
-            T* out = (T*)a.q_out + (int64_t)(row0 + j) * a.qo_stride + (int64_t)h * hd;
-            const Entry* row = reinterpret_cast<const Entry*>(smem) + j * 8 * n8;
-            if constexpr (VEC) turn_item(in, out, i, half, a.interleaved, row, n8);
-            else turn_item_plain(in, out, i, half, a.interleaved, row, n8);
+    } else if (at.slot >= 0) {
+        const T* const q_in = (const T*)a.q + (int64_t)(row0 + j) * a.q_stride + (int64_t)h0 * hd;
+        T* const q_out = (T*)a.q_out + (int64_t)(row0 + j) * a.qo_stride + (int64_t)h0 * hd;
+        const TurnRow<T> turns{row, low + j * 8 * n8};
+        const int heads = h1 - h0;
+        if constexpr (VEC) {
+            constexpr int B = kTurnHeads<T>;
+            const int groups = (heads + B - 1) / B, pairs = half >> 3, copies = (hd - 2 * half) >> 3;
+            const Divider by_pairs(pairs), by_copies(copies);
+            for (int e = mine; e < groups * pairs; e += share) {
+                const int gr = by_pairs(e), h = gr * B;
+                turn_item(q_in + h * hd, q_out + h * hd, hd, min(B, heads - h), e - gr * pairs, half, a.interleaved, turns, n8);
+            }
+            for (int e = mine; e < heads * copies; e += share) {
+                const int h = by_copies(e);
+                if (q_in != q_out) copy_item(q_in + h * hd, q_out + h * hd, e - h * copies, half);
+            }
+        } else {
+            const int items = hd - half;
+            const Divider by_items(items);
+            for (int e = mine; e < heads * items; e += share) {
+                const int h = by_items(e);
+                turn_item_plain(q_in + h * hd, q_out + h * hd, e - h * items, half, a.interleaved, turns, n8);
+            }
         }
     }
 }
@@ -232,7 +338,7 @@ struct Read4Args {
 };
 // A block takes a few rows, a thread 16 dims of them at a time: of the keys, then of the values.
 template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) kv4_read_kernel(Kv4Pool pool, Kv8Seqs seqs, Read4Args a) {
+__global__ void __launch_bounds__(kAppendThreads, 5) kv4_read_kernel(Kv4Pool pool, Kv8Seqs seqs, Read4Args a) {
     __shared__ RowPlace place[kAppendRows];
     if (blockIdx.x == 0 && blockIdx.y == 0) kv8_check_seqs(seqs, pool);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -245,32 +351,50 @@ __global__ void __launch_bounds__(kAppendThreads) kv4_read_kernel(Kv4Pool pool, 
         }
     }
     __syncthreads();
-    const int h0 = pool.n_kv * blockIdx.y / gridDim.y, mine = pool.n_kv * (blockIdx.y + 1) / gridDim.y - h0;
-    const int blocks = pool.hd >> 4, per_row = mine * blocks, all = rows * per_row;
-    for (int e = tid; e < 2 * all; e += kAppendThreads) {
-        const bool is_k = e < all;
-        T* out = (T*)(is_k ? a.k : a.v);
-        const int f = is_k ? e : e - all, j = f / per_row, g = f - j * per_row, h = h0 + g / blocks, b = g % blocks;
-        const RowPlace& at = place[j];
-        if (at.seq < 0 || !out) continue;
-        float scale = __int_as_float(0x7fffffff), head = 1.0f;
-        uint2 w = make_uint2(0, 0);
-        if (at.page >= 0) {
-            const size_t row = (((size_t)at.page * pool.n_kv + h) << pool.page_shift) + at.slot;
-            w = *reinterpret_cast<const uint2*>((is_k ? pool.k : pool.v) + row * (pool.hd >> 1) + 8 * b);
-            scale = scale4_f((is_k ? pool.k_block : pool.v_block)[row * blocks + b]);
-            head = (is_k ? pool.k_scale : pool.v_scale)[h];
+    const int h0 = pool.n_kv * blockIdx.y / gridDim.y, h1 = pool.n_kv * (blockIdx.y + 1) / gridDim.y;
+    // a row has its own share of the threads; four blocks of 16 dims a thread, whose loads go out together
+    const int share = kAppendThreads / a.rows, j = tid / share, mine = tid - j * share;
+    if (j >= rows) return;
+    const RowPlace at = place[j];
+    if (at.seq < 0) return;
+    const int blocks = pool.hd >> 4, all = (h1 - h0) * blocks;
+    const Divider by_blocks(blocks);
+    constexpr int B = 4;
+    for (int e0 = mine; e0 < 2 * all; e0 += B * share) {
+        uint2 w[B];
+        float scale[B], head[B];
+#pragma unroll
+        for (int x = 0; x < B; x++) {
+            const int e = min(e0 + x * share, 2 * all - 1);
+            const bool is_k = e < all;
+            const int f = is_k ? e : e - all, g = by_blocks(f), h = h0 + g, b = f - g * blocks;
+            w[x] = make_uint2(0, 0);
+            scale[x] = __int_as_float(0x7fffffff);
+            head[x] = (is_k ? pool.k_scale : pool.v_scale)[h];
+            if (at.page >= 0) {
+                const size_t row = (((size_t)at.page * pool.n_kv + h) << pool.page_shift) + at.slot;
+                w[x] = *reinterpret_cast<const uint2*>((is_k ? pool.k : pool.v) + row * (pool.hd >> 1) + 8 * b);
+                scale[x] = scale4_f((is_k ? pool.k_block : pool.v_block)[row * blocks + b]);
+            }
         }
-        __align__(16) T t[16];
 #pragma unroll
-        for (int x = 0; x < 16; x++) t[x] = to_elem<T>((float)(int)(((x < 8 ? w.x : w.y) >> (4 * (x & 7)) & 15u) - 8u) * scale * head);
-        out += (int64_t)(row0 + j) * (is_k ? a.k_stride : a.v_stride) + (int64_t)h * pool.hd + 16 * b;
-        if (a.vec) {
+        for (int x = 0; x < B; x++) {
+            const int e = e0 + x * share;
+            const bool is_k = e < all;
+            const int f = is_k ? e : e - all;
+            T* out = (T*)(is_k ? a.k : a.v);
+            if (e >= 2 * all || !out) continue;
+            __align__(16) T t[16];
 #pragma unroll
-            for (int x = 0; x < (int)sizeof(T); x++) reinterpret_cast<uint4*>(out)[x] = reinterpret_cast<const uint4*>(t)[x];
-        } else {
+            for (int y = 0; y < 16; y++) t[y] = to_elem<T>((float)(int)(((y < 8 ? w[x].x : w[x].y) >> (4 * (y & 7)) & 15u) - 8u) * scale[x] * head[x]);
+            out += (int64_t)(row0 + j) * (is_k ? a.k_stride : a.v_stride) + (int64_t)h0 * pool.hd + 16 * f;
+            if (a.vec) {
 #pragma unroll
-            for (int x = 0; x < 16; x++) out[x] = t[x];
+                for (int y = 0; y < (int)sizeof(T); y++) reinterpret_cast<uint4*>(out)[y] = reinterpret_cast<const uint4*>(t)[y];
+            } else {
+#pragma unroll
+                for (int y = 0; y < 16; y++) out[y] = t[y];
+            }
         }
     }
 }
@@ -281,7 +405,8 @@ struct RowGrid {
 };
 RowGrid row_grid(int n_rows) {
     RowGrid g;
-    g.rows = std::max(1, std::min(kAppendRows, n_rows / (2 * sm_count())));
+    g.rows = 1;
+    while (2 * g.rows <= kAppendRows && 2 * g.rows <= n_rows / (2 * sm_count())) g.rows *= 2;
     g.groups = (n_rows + g.rows - 1) / g.rows;
     return g;
 }
@@ -295,7 +420,7 @@ int32_t append4_as(const Kv4Pool& pool, const Kv8Seqs& seqs, Append4Args a, cuda
     const int slices = a.kv_slices + (a.q ? slices_of(grid.groups, a.n_heads, 4) : 0);
     const bool vec = a.half % (a.interleaved ? 8 : 16) == 0 && rows_aligned(a.k, a.k_stride, sizeof(T), 16) && rows_aligned(a.v, a.v_stride, sizeof(T), 16) &&
                      (!a.q || (rows_aligned(a.q, a.q_stride, sizeof(T), 16) && rows_aligned(a.q_out, a.qo_stride, sizeof(T), 16)));
-    const size_t smem = (size_t)a.rows * ((a.half + 7) / 8 * 8) * sizeof(double2);
+    const size_t smem = (size_t)a.rows * ((a.half + 7) / 8 * 8) * sizeof(float4);
     const auto kern = vec ? kv4_append_kernel<T, true> : kv4_append_kernel<T, false>;
     kern<<<dim3((unsigned)grid.groups, (unsigned)slices), kAppendThreads, smem, s>>>(pool, seqs, a);
     LC_CUDA(cudaGetLastError());

@@ -85,7 +85,7 @@ __device__ __forceinline__ bool begins_cut(const Kv4Pool& pool, const Kv8Seqs& s
 __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seqs, EvictArgs a, int per) {
     constexpr int W = kSelectThreads / 32;
     extern __shared__ float sum[];               // [per]
-    __shared__ int hist[3][2048];
+    __shared__ __align__(16) int hist[3][2048];
     __shared__ int sums[32], flag, chosen[2];
     __shared__ int2 warp_counts[W], block_counts;
     cg::cluster_group cluster = cg::this_cluster();
@@ -115,14 +115,15 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4Pool pool
                 if (d == 0 || v >> (shift + bits[d]) == value >> (shift + bits[d])) atomicAdd(&hist[d][v >> shift & ((1u << bits[d]) - 1)], 1);
             }
             cluster.sync();
-            // counts from the top: a thread has four places
-            int c[4], mysum = 0;
+            // counts from the top: a thread has four places, of all blocks at once
+            int4 part[kMostCluster];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                c[k] = 0;
-                for (int r = 0; r < size; r++) c[k] += *cluster.map_shared_rank(&hist[d][2047 - 4 * tid - k], r);
-                mysum += c[k];
-            }
+            for (int r = 0; r < kMostCluster; r++)
+                part[r] = r < size ? *cluster.map_shared_rank(reinterpret_cast<const int4*>(&hist[d][2044 - 4 * tid]), r) : make_int4(0, 0, 0, 0);
+            int c[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int r = 0; r < kMostCluster; r++) { c[0] += part[r].w; c[1] += part[r].z; c[2] += part[r].y; c[3] += part[r].x; }
+            const int mysum = (c[0] + c[1]) + (c[2] + c[3]);
             int all, before = before_me(mysum, sums, all);
 #pragma unroll
             for (int k = 0; k < 4; k++) {

@@ -50,8 +50,14 @@ __device__ __forceinline__ Scale4 scale4_both(uint32_t b, int j) { return scale4
 // two keys' scales, a byte each
 __device__ __forceinline__ Scale4 scale4_pair(uint32_t a, uint32_t b) { return scale4_of((a * 128u + b * 0x800000u) & 0x3f803f80u); }
 // the integers in bits 0-3 and 16-19, 4-7 and 20-23 of x (and 8 higher, after a shift) as values
-__device__ __forceinline__ uint32_t value_lo(uint32_t x, const Scale4& s) { return h2_fma4((x & 0x000f000fu) | 0x64006400u, s.by, s.lo_less); }
-__device__ __forceinline__ uint32_t value_hi(uint32_t x, const Scale4& s) { return h2_fma4((x & 0x00f000f0u) | 0x54005400u, s.by, s.hi_less); }
+// (x & keep) | with, in one instruction: left to itself the compiler takes two
+template <uint32_t KEEP> __device__ __forceinline__ uint32_t bits_with(uint32_t x, uint32_t with) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "n"(KEEP), "r"(with));
+    return r;
+}
+__device__ __forceinline__ uint32_t value_lo(uint32_t x, const Scale4& s) { return h2_fma4(bits_with<0x000f000fu>(x, 0x64006400u), s.by, s.lo_less); }
+__device__ __forceinline__ uint32_t value_hi(uint32_t x, const Scale4& s) { return h2_fma4(bits_with<0x00f000f0u>(x, 0x54005400u), s.by, s.hi_less); }
 // eight neighbouring dims: (0, 4), (1, 5), (2, 6), (3, 7)
 __device__ __forceinline__ void values8(uint32_t x, const Scale4& s, uint32_t (&v)[4]) {
     v[0] = value_lo(x, s);

@@ -5,6 +5,16 @@
 namespace lc {
 
 #ifdef __CUDACC__
+// Quotients by a number that a kernel learns when it runs, for dividends below 2^32 over it.
+struct Divider {
+    uint32_t d, m;
+    __device__ __forceinline__ explicit Divider(int by) : d((uint32_t)max(by, 1)), m(0xffffffffu / d + 1) {}
+    __device__ __forceinline__ int operator()(int n) const { return d == 1 ? n : (int)__umulhi((uint32_t)n, m); }
+};
+// Brings bytes that will be read soon into L2: a multiple of 16, 16-byte aligned.
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+    if (bytes) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes));
+}
 // (cosine, sine) of `positions` times an entry of turns: the product wraps around by itself, and what is left is the angle's fraction of a turn to 2^-64 of one,
 // however far the position is (cos and sin of an f32 angle lose 2^-24 of the ANGLE: 0.06 at 10^6).
 __device__ __forceinline__ double2 turn_of(uint64_t per_position, int64_t positions) {
@@ -40,6 +50,15 @@ __device__ __forceinline__ void turn_pair(float u, float w, const float2& t, flo
     a = u * t.x - w * t.y;
     b = u * t.y + w * t.x;
 }
+// A row of a table that is kept as cosines and sines in f32 and, apart, what f32 lost of them.
+template <typename T> struct TurnRow {
+    const float2* high;
+    const float2* low;
+    __device__ __forceinline__ typename TurnEntry<T>::type operator[](int at) const {
+        if constexpr (sizeof(T) == 2) return high[at];
+        else return make_float4(high[at].x, low[at].x, high[at].y, low[at].y);
+    }
+};
 template <typename T> __device__ __forceinline__ void load8(const T* p, T (&v)[8]) {
 #pragma unroll
     for (int u = 0; u < (int)sizeof(T) / 2; u++) reinterpret_cast<uint4*>(v)[u] = reinterpret_cast<const uint4*>(p)[u];
@@ -49,42 +68,58 @@ template <typename T> __device__ __forceinline__ void store8(T* p, const T (&v)[
     for (int u = 0; u < (int)sizeof(T) / 2; u++) reinterpret_cast<uint4*>(p)[u] = reinterpret_cast<const uint4*>(v)[u];
 }
 
-// What a thread turns at a time: eight pairs, or copies: eight dims behind them.  hd and half multiples of 8, 16-byte accesses.  A head has turn_items of them, the copies last.
-__device__ __forceinline__ int turn_items(int hd, int half) { return (half >> 3) + ((hd - 2 * half) >> 3); }
-template <typename T, typename Entry>
-__device__ __forceinline__ void turn_item(const T* in, T* out, int i, int half, bool interleaved, const Entry* row, int n8) {
-    const int pairs = half >> 3;
-    __align__(16) T u[8], w[8];
-    if (i >= pairs) {
-        const int d = 2 * half + 8 * (i - pairs);
-        load8(in + d, u);
-        store8(out + d, u);
-        return;
-    }
+// What a thread turns at a time: eight pairs (8 i ..) of kTurnHeads neighbouring heads, of which n are there; their loads go out together and share what the table says.  half and the heads' dims multiples
+// of 8, 16-byte accesses.
+template <typename T> constexpr int kTurnHeads = sizeof(T) == 2 ? 4 : 2;
+template <typename T, typename Row>
+__device__ __forceinline__ void turn_item(const T* in, T* out, int hd, int n, int i, int half, bool interleaved, const Row& row, int n8) {
+    constexpr int B = kTurnHeads<T>;
     const int d0 = interleaved ? 16 * i : 8 * i, d1 = interleaved ? d0 + 8 : half + d0;
-    load8(in + d0, u);
-    load8(in + d1, w);
+    __align__(16) T u[B][8], w[B][8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-        const Entry at = row[k * n8 + i];
-        const int k2 = 2 * (k & 3);
-        const T p = interleaved ? (k < 4 ? u[k2] : w[k2]) : u[k], q = interleaved ? (k < 4 ? u[k2 + 1] : w[k2 + 1]) : w[k];
-        float y0, y1;
-        turn_pair(elem_f(p), elem_f(q), at, y0, y1);
-        if (interleaved) {
-            (k < 4 ? u : w)[k2] = to_elem<T>(y0);
-            (k < 4 ? u : w)[k2 + 1] = to_elem<T>(y1);
-        } else {
-            u[k] = to_elem<T>(y0);
-            w[k] = to_elem<T>(y1);
-        }
+    for (int b = 0; b < B; b++) {
+        const T* from = in + min(b, n - 1) * hd;
+        load8(from + d0, u[b]);
+        load8(from + d1, w[b]);
     }
-    store8(out + d0, u);
-    store8(out + d1, w);
+    typename TurnEntry<T>::type t[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) t[k] = row[k * n8 + i];
+#pragma unroll
+    for (int b = 0; b < B; b++) {
+        if (b >= n) break;
+        if (interleaved) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                T(&v)[8] = k < 4 ? u[b] : w[b];
+                const int k2 = 2 * (k & 3);
+                float y0, y1;
+                turn_pair(elem_f(v[k2]), elem_f(v[k2 + 1]), t[k], y0, y1);
+                v[k2] = to_elem<T>(y0);
+                v[k2 + 1] = to_elem<T>(y1);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                float y0, y1;
+                turn_pair(elem_f(u[b][k]), elem_f(w[b][k]), t[k], y0, y1);
+                u[b][k] = to_elem<T>(y0);
+                w[b][k] = to_elem<T>(y1);
+            }
+        }
+        store8(out + b * hd + d0, u[b]);
+        store8(out + b * hd + d1, w[b]);
+    }
+}
+// Eight dims behind the turned ones (8 i ..), copied.
+template <typename T> __device__ __forceinline__ void copy_item(const T* in, T* out, int i, int half) {
+    __align__(16) T u[8];
+    load8(in + 2 * half + 8 * i, u);
+    store8(out + 2 * half + 8 * i, u);
 }
 // The same for any sizes and alignment: a pair, or one dim behind them (hd - half items).
-template <typename T, typename Entry>
-__device__ __forceinline__ void turn_item_plain(const T* in, T* out, int p, int half, bool interleaved, const Entry* row, int n8) {
+template <typename T, typename Row>
+__device__ __forceinline__ void turn_item_plain(const T* in, T* out, int p, int half, bool interleaved, const Row& row, int n8) {
     if (p >= half) {
         out[half + p] = in[half + p];
         return;

@@ -42,38 +42,61 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeArgs a) {
     const int row0 = blockIdx.x * a.rows, rows = min(a.rows, a.n_rows - row0);
     const int heads = a.x.heads + a.y.heads, h0 = heads * blockIdx.y / gridDim.y, h1 = heads * (blockIdx.y + 1) / gridDim.y, mine = h1 - h0;
     const int n8 = (a.half + 7) >> 3;
+    if (VEC && (int)threadIdx.x < rows) {
+        const int x1 = min(h1, a.x.heads), y0 = max(h0, a.x.heads);
+        if (h0 < x1) prefetch_l2((const T*)a.x.in + (row0 + threadIdx.x) * a.x.in_stride + (int64_t)h0 * a.hd, (uint32_t)((x1 - h0) * a.hd * sizeof(T)));
+        if (y0 < h1) prefetch_l2((const T*)a.y.in + (row0 + threadIdx.x) * a.y.in_stride + (int64_t)(y0 - a.x.heads) * a.hd, (uint32_t)((h1 - y0) * a.hd * sizeof(T)));
+    }
+    const Divider by_half(a.half);
     for (int e = threadIdx.x; e < rows * a.half; e += kRopeThreads) {
-        const int j = e / a.half, p = e - j * a.half;
+        const int j = by_half(e), p = e - j * a.half;
         double2 t = turn_of(a.turns[p], a.positions[row0 + j]);
         t.x *= a.magnitude;
         t.y *= a.inverse ? -a.magnitude : a.magnitude;
         put_turn(tab[j * 8 * n8 + turn_place(p, n8)], t);
     }
     __syncthreads();
-    auto head_at = [&](int j, int h, const T*& in, T*& out) {
-        const RopeTensor& t = h < a.x.heads ? a.x : a.y;
-        const int64_t off = (int64_t)(h < a.x.heads ? h : h - a.x.heads) * a.hd;
-        in = (const T*)t.in + (int64_t)(row0 + j) * t.in_stride + off;
-        out = (T*)t.out + (int64_t)(row0 + j) * t.out_stride + off;
+    // a row has its own share of the threads, whole warps
+    const int share = kRopeThreads / a.rows, j = threadIdx.x / share, at = threadIdx.x - j * share;
+    if (j >= rows) return;
+    const Entry* const row = tab + j * 8 * n8;
+    const T* const x_in = (const T*)a.x.in + (int64_t)(row0 + j) * a.x.in_stride;
+    const T* const y_in = (const T*)a.y.in + (int64_t)(row0 + j) * a.y.in_stride;
+    T* const x_out = (T*)a.x.out + (int64_t)(row0 + j) * a.x.out_stride;
+    T* const y_out = (T*)a.y.out + (int64_t)(row0 + j) * a.y.out_stride;
+    auto head_at = [&](int h, const T*& in, T*& out) {
+        const bool x = h < a.x.heads;
+        const int64_t off = (int64_t)(x ? h : h - a.x.heads) * a.hd;
+        in = (x ? x_in : y_in) + off;
+        out = (x ? x_out : y_out) + off;
     };
+    const T* in;
+    T* out;
     if constexpr (VEC) {
-        // items of a head: eight pairs, then eight elements that are copied
-        const int items = turn_items(a.hd, a.half), per_row = mine * items;
-        for (int e = threadIdx.x; e < rows * per_row; e += kRopeThreads) {
-            const int j = e / per_row, r = e - j * per_row, h = h0 + r / items, i = r % items;
-            const T* in;
-            T* out;
-            head_at(j, h, in, out);
-            turn_item(in, out, i, a.half, a.interleaved, tab + j * 8 * n8, n8);
+        // groups of heads of one tensor: x's that are in [h0, h1), then y's
+        constexpr int B = kTurnHeads<T>;
+        const int x0 = min(h0, a.x.heads), x1 = min(h1, a.x.heads), groups_x = (x1 - x0 + B - 1) / B;
+        const int y0 = max(h0, a.x.heads), y1 = max(h1, a.x.heads), groups = groups_x + (y1 - y0 + B - 1) / B;
+        const int pairs = a.half >> 3, copies = (a.hd - 2 * a.half) >> 3;
+        const Divider by_pairs(pairs), by_copies(copies);
+        for (int e = at; e < groups * pairs; e += share) {
+            const int gr = by_pairs(e), h = gr < groups_x ? x0 + gr * B : y0 + (gr - groups_x) * B, n = min(B, (gr < groups_x ? x1 : y1) - h);
+            head_at(h, in, out);
+            turn_item(in, out, a.hd, n, e - gr * pairs, a.half, a.interleaved, row, n8);
+        }
+        // what is not turned
+        for (int e = at; e < mine * copies; e += share) {
+            const int h = by_copies(e);
+            head_at(h0 + h, in, out);
+            if (in != out) copy_item(in, out, e - h * copies, a.half);
         }
     } else {
-        const int items = a.hd - a.half, per_row = mine * items;
-        for (int e = threadIdx.x; e < rows * per_row; e += kRopeThreads) {
-            const int j = e / per_row, r = e - j * per_row, h = h0 + r / items, p = r % items;
-            const T* in;
-            T* out;
-            head_at(j, h, in, out);
-            turn_item_plain(in, out, p, a.half, a.interleaved, tab + j * 8 * n8, n8);
+        const int items = a.hd - a.half;
+        const Divider by_items(items);
+        for (int e = at; e < mine * items; e += share) {
+            const int h = by_items(e);
+            head_at(h0 + h, in, out);
+            turn_item_plain(in, out, e - h * items, a.half, a.interleaved, row, n8);
         }
     }
 }
@@ -81,7 +104,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeArgs a) {
 template <typename T> int32_t rope_as(RopeArgs a, cudaStream_t s) {
     const int heads = a.x.heads + a.y.heads;
     // a block's table is made once for all of its heads, so it has all heads of its rows, and as many rows (8 at most) as leave four blocks for each SM; few rows: heads apart
-    a.rows = std::max(1, std::min(8, a.n_rows / (4 * sm_count())));
+    a.rows = 1;
+    while (a.rows < 8 && 2 * a.rows <= a.n_rows / (4 * sm_count())) a.rows *= 2;
     while (a.rows > 1 && (size_t)a.rows * (a.half + 7) * sizeof(typename TurnEntry<T>::type) > 24 * 1024) a.rows /= 2;
     const int groups = (a.n_rows + a.rows - 1) / a.rows;
     const int slices = std::max(1, std::min({(2 * sm_count() + groups - 1) / groups, (heads + 7) / 8, 64}));
