@@ -289,18 +289,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
             for (int e = ct; e < kKeys * KC; e += 32 * kConvWarps) {
                 const int key = e / KC, ch = e % KC;
                 uint32_t first[4] = {0, 0, 0, 0}, second[4] = {0, 0, 0, 0};
+                // the upper half of a row's chunks writes its second piece first: eight lanes then meet all banks
+                const int swap = ch >= 4;
                 if (ch * 16 < hd) {
                     const uint2 x = *reinterpret_cast<const uint2*>(rk + key * row_ints + ch * 8);
-                    const uint32_t b = rk[kKeys * HD / 2 + key * row_scales + ch] & 0x7fu;
-                    const Scale4 s = scale4_both(b, 0);
-                    values8(x.x, s, first);
-                    values8(x.y, s, second);
+                    const Scale4 s = scale4_both(rk[kKeys * HD / 2 + key * row_scales + ch] & 0x7fu, 0);
+                    values8(swap ? x.y : x.x, s, first);
+                    values8(swap ? x.x : x.y, s, second);
                 }
                 unsigned char* dst = sk + (ch >> 2) * (128 * 128);
-                // the upper half of a row's chunks writes its second piece first: eight lanes then meet all banks
-                const bool swap = ch >= 4;
-                *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + (swap ? 1 : 0))) = swap ? make_uint4(second[0], second[1], second[2], second[3]) : make_uint4(first[0], first[1], first[2], first[3]);
-                *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + (swap ? 0 : 1))) = swap ? make_uint4(first[0], first[1], first[2], first[3]) : make_uint4(second[0], second[1], second[2], second[3]);
+                *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + swap)) = make_uint4(first[0], first[1], first[2], first[3]);
+                *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + 1 - swap)) = make_uint4(second[0], second[1], second[2], second[3]);
             }
             fence_async();
             __syncwarp();

@@ -6,21 +6,12 @@
 #include <algorithm>
 #include "lc_kernels.h"
 #include "lc_kv4.cuh"
+#include "lc_kv4_weights.cuh"
 #include "lc_kv8_attn.cuh"
 
 namespace lc {
 
 namespace {
-
-struct WeightArgs {
-    const void* q;
-    const float* lse;
-    float* mass;
-    int64_t q_stride, lse_stride, mass_stride, mass_head_stride;
-    int typ, group, window, capacity;
-    bool q_vec;
-    float scale_log2;
-};
 
 template <int HD, int NG, bool F32> struct WeightShape {
     static constexpr int kRows = 8 * NG;
@@ -91,13 +82,7 @@ kv4_weights_kernel(Kv4Pool pool, Kv8Seqs seqs, WeightArgs a) {
     __shared__ uint32_t warp_sums[kRunWarps];
     uint32_t* cum = reinterpret_cast<uint32_t*>(smem + kRunWarps * Shape::kWarp);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    if (blockIdx.x == 0) {
-        kv8_check_seqs(seqs, pool);
-        for (int i = threadIdx.x; i < seqs.n_seqs; i += blockDim.x) {
-            int first, n;
-            if (kv8_span(seqs, i, first, n) && n > 0 && (long long)seqs.ctx[i] + n > a.capacity) kv8_raise(seqs, i);
-        }
-    }
+    if (blockIdx.x == 0) weights_check_seqs(pool, seqs, a);
     const uint32_t total = weight_line<RB>(seqs, pool, a, cum, warp_sums);
     const Runs runs(total, gridDim.x * kRunWarps);
     const uint32_t run = blockIdx.x * kRunWarps + warp;
@@ -299,6 +284,7 @@ int32_t weights_full(const Kv4Pool& pool, const Kv8Seqs& seqs, const WeightArgs&
     if (a.typ == LC_TYPE_F32) return pool.hd == HD ? weights_as<HD, NG, true, true>(pool, seqs, a, s) : weights_as<HD, NG, true, false>(pool, seqs, a, s);
     return pool.hd == HD ? weights_as<HD, NG, false, true>(pool, seqs, a, s) : weights_as<HD, NG, false, false>(pool, seqs, a, s);
 }
+constexpr int kTileWeightRows = 64;  // of a sequence and kv head, from which on tiles are faster
 // As many groups of 8 rows share a step's keys as a sequence and kv head has rows for, four at most.
 template <int HD>
 int32_t weights_of(const Kv4Pool& pool, const Kv8Seqs& seqs, const WeightArgs& a, int64_t rows, cudaStream_t s) {
@@ -340,6 +326,7 @@ extern "C" int32_t lc_kv4_weights_dev(const lc_kv4_cache* cache, const lc_kv8_ro
                        scale * 1.44269504088896f};
     cudaStream_t s = stream_or_own(stream_);
     const int64_t most = (int64_t)group * std::max(1, rows->max_rows);
+    if (pool.hd <= 128 && most >= kTileWeightRows) return launch_kv4_weights_tiles(pool, seqs, a, s);
     if (pool.hd <= 64) return weights_of<64>(pool, seqs, a, most, s);
     if (pool.hd <= 128) return weights_of<128>(pool, seqs, a, most, s);
     return weights_of<256>(pool, seqs, a, most, s);
