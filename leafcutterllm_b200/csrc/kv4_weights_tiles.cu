@@ -21,10 +21,11 @@ struct WeightShared {
     uint64_t done[2];                  // scores of the two tiles of keys
     uint32_t tmem;
     uint32_t sums[kWeightThreads / 32];
-    float4 row[kWeightRows / 2];       // (f, f, -L, -L) of two rows
     int64_t at[kUnitKeys];             // the keys' rows in the pool; -1: none
-    int64_t from[kWeightRows];         // of a row's queries; -1: none
-    int limit[kWeightRows];            // last slot that the row sees; -1: none
+    // of two tiles of rows, in turn
+    float4 row[2][kWeightRows / 2];    // (f, f, -L, -L) of two rows
+    int64_t from[2][kWeightRows];      // of a row's queries; -1: none
+    int limit[2][kWeightRows];         // last slot that the row sees; -1: none
 };
 template <int HD, bool SPLIT> struct WeightTiles {
     static constexpr int kPart = HD * 256;                      // 128 rows of HD f16
@@ -97,6 +98,24 @@ __global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 4 ? 1 : 2) kv4_we
         const int chunks = of_seq / pool.n_kv, kvh = in / chunks, key0 = (chunk0 + (int)(in - (uint32_t)kvh * chunks)) * kUnitKeys;
         const int rows = n * a.group;
 
+        // rows in front of the keys see none of them, and rows whose window begins behind them
+        const int r_from = max(0, key0 - ctx) * a.group / kWeightRows * kWeightRows;
+        const int r_end = a.window > 0 ? (int)min((int64_t)rows, ((int64_t)key0 + kUnitKeys - 1 + a.window - ctx) * a.group) : rows;
+        // the rows' numbers, a thread each (of the half that does not issue the products): those behind the last row, and those without a finite lse, are zeros that add nothing
+        auto numbers = [&](int r0, int to) {
+            const int at = tid - (kWeightThreads - kWeightRows);
+            if (at < 0 || r0 >= r_end) return;
+            const int mine = min(kWeightRows, rows - r0), r = r0 + min(at, mine - 1), tok = r / a.group, hq = kvh * a.group + r - tok * a.group;
+            const float lse = a.lse[(int64_t)(first + tok) * a.lse_stride + hq];
+            const bool counts = at < mine && fabsf(lse) < INFINITY;
+            sh.from[to][at] = counts ? (int64_t)(first + tok) * a.q_stride + (int64_t)hq * hd : -1;
+            sh.limit[to][at] = counts ? ctx + tok : -1;
+            float* const k = reinterpret_cast<float*>(&sh.row[to][at >> 1]) + (at & 1);
+            k[0] = 0.0f;
+            k[2] = counts ? -lse * 1.44269504088896f : kNegInf;
+        };
+        numbers(r_from, 0);
+
         // a key per thread
         const int key = key0 + tid;
         bool held = key < ctx + n;
@@ -112,7 +131,7 @@ __global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 4 ? 1 : 2) kv4_we
         {
             // 16 dims of a key at a time: neighbours read neighbouring bytes
             constexpr int C = HD / 16;
-#pragma unroll 4
+#pragma unroll 8
             for (int e = tid; e < kUnitKeys * C; e += kWeightThreads) {
                 const int r = e / C, ch = e % C;
                 const int64_t row = sh.at[r];
@@ -134,31 +153,16 @@ __global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 4 ? 1 : 2) kv4_we
         float* const mass = a.mass + (int64_t)seq * a.mass_stride + (int64_t)kvh * a.mass_head_stride + key;
         const float before = held ? *mass : 0.0f;
         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        // rows in front of the keys see none of them, and rows whose window begins behind them
-        const int r_from = max(0, key0 - ctx) * a.group / kWeightRows * kWeightRows;
-        const int r_end = a.window > 0 ? (int)min((int64_t)rows, ((int64_t)key0 + kUnitKeys - 1 + a.window - ctx) * a.group) : rows;
-        for (int r0 = r_from; r0 < r_end && ok; r0 += kWeightRows) {
+        for (int r0 = r_from, turn = 0; r0 < r_end && ok; r0 += kWeightRows, turn ^= 1) {
             const int mine = min(kWeightRows, rows - r0);
-            // the rows' numbers, a thread each: those behind the last row, and those without a finite lse, are zeros that add nothing
-            if (tid < kWeightRows) {
-                const int r = r0 + min(tid, mine - 1), tok = r / a.group, hq = kvh * a.group + r - tok * a.group;
-                const float lse = a.lse[(int64_t)(first + tok) * a.lse_stride + hq];
-                const bool counts = tid < mine && fabsf(lse) < INFINITY;
-                sh.from[tid] = counts ? (int64_t)(first + tok) * a.q_stride + (int64_t)hq * hd : -1;
-                sh.limit[tid] = counts ? ctx + tok : -1;
-                float* const k = reinterpret_cast<float*>(&sh.row[tid >> 1]) + (tid & 1);
-                k[0] = 0.0f;
-                k[2] = counts ? -lse * 1.44269504088896f : kNegInf;
-            }
-            __syncthreads();
             // the queries: HD / 16 threads a row
             constexpr int C = HD / 16;
-#pragma unroll 2
+#pragma unroll(SPLIT ? 2 : 4)
             for (int e = tid; e < kWeightRows * C; e += kWeightThreads) {
                 const int r = e / C, ch = e % C;
-                const int64_t at_q = sh.from[r];
+                const int64_t at_q = sh.from[turn][r];
                 const bool here = at_q >= 0 && ch * 16 < hd;
-                float* const k = reinterpret_cast<float*>(&sh.row[r >> 1]) + (r & 1);
+                float* const k = reinterpret_cast<float*>(&sh.row[turn][r >> 1]) + (r & 1);
                 const int at0 = (ch >> 2) * (128 * 128) + sw128(r, 2 * (ch & 3)), at1 = (ch >> 2) * (128 * 128) + sw128(r, 2 * (ch & 3) + 1);
                 if constexpr (!SPLIT) {
                     // pairs of 16 bits: the largest magnitude of a row by pairs; f16 as it is, bf16 times a power of two
@@ -186,7 +190,7 @@ __global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 4 ? 1 : 2) kv4_we
                     if (!std::is_same<T, __half>::value) row_scale(top, up, down);
                     if (ch == 0) {
                         if (finite) k[0] = a.scale_log2 * down * head;
-                        else { sh.limit[r] = -1; k[2] = kNegInf; }   // a row that is not finite adds nothing either
+                        else { sh.limit[turn][r] = -1; k[2] = kNegInf; }   // a row that is not finite adds nothing either
                     }
                     uint32_t w[8];
 #pragma unroll
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 4 ? 1 : 2) kv4_we
                     row_scale(top, up, down);
                     if (ch == 0) {
                         if (finite) k[0] = a.scale_log2 * down * head;
-                        else { sh.limit[r] = -1; k[2] = kNegInf; }
+                        else { sh.limit[turn][r] = -1; k[2] = kNegInf; }
                     }
                     uint32_t hi[8], lo[8];
 #pragma unroll
@@ -253,6 +257,7 @@ __global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 4 ? 1 : 2) kv4_we
                     umma_commit(&sh.done[t]);
                 }
             }
+            numbers(r0 + kWeightRows, turn ^ 1);   // the next ones, while the products run
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.done[warp >> 2], phase));
             phase ^= 1;
             tc_fence_after();
@@ -268,12 +273,12 @@ __global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 4 ? 1 : 2) kv4_we
                 if (!plain)
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
-                        const int limit = sh.limit[c + e];
+                        const int limit = sh.limit[turn][c + e];
                         if (key > limit || (a.window > 0 && key <= limit - a.window)) x[e] = __float_as_uint(kNegInf);
                     }
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
-                    const float4 k = sh.row[(c + e) / 2];
+                    const float4 k = sh.row[turn][(c + e) / 2];
                     float2 y = fma2(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(k.x, k.y), make_float2(k.z, k.w));
                     if (!plain) {  // a masked score times a factor that is 0
                         if (x[e] == 0xff800000u) y.x = kNegInf;
