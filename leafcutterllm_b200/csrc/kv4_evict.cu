@@ -22,8 +22,8 @@ struct EvictArgs {
     int32_t* kept;
     int32_t* ctx_out;
 };
-constexpr int kSelectThreads = 512, kFarThreads = 1024, kMoveThreads = 512, kMovePieces = 8, kMostCluster = 8;
-constexpr size_t kSelectSmem = 196 * 1024;  // of a block's sums, at most
+constexpr int kFarThreads = 1024, kMoveThreads = 512, kMovePieces = 4, kMostCluster = 8;
+constexpr size_t kSelectSmem = 190 * 1024;  // of a block's sums and slots, at most
 
 // whole numbers in the order of f32, NaN at the bottom
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -81,28 +81,58 @@ __device__ __forceinline__ bool begins_cut(const Kv4Pool& pool, const Kv8Seqs& s
     return cut;
 }
 
-// grid: (cluster, sequences * kv heads); `per`: slots of a block, a multiple of 32
-__global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seqs, EvictArgs a, int per) {
-    constexpr int W = kSelectThreads / 32;
-    extern __shared__ float sum[];               // [per]
-    __shared__ __align__(16) int hist[3][2048];
-    __shared__ int sums[32], flag, chosen[2];
+// What a thread of a block of T has before it, of all threads' v; `totals`: of the warps, for this call alone.
+template <int T> __device__ __forceinline__ int before_thread(int v, int* totals) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int incl = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += u;
+    }
+    if (lane == 31) totals[warp] = incl;
+    __syncthreads();
+    int off = incl - v;
+#pragma unroll
+    for (int w = 0; w < T / 32; w += 4) {
+        const int4 u = *reinterpret_cast<const int4*>(totals + w);
+        off += (w < warp ? u.x : 0) + (w + 1 < warp ? u.y : 0) + (w + 2 < warp ? u.z : 0) + (w + 3 < warp ? u.w : 0);
+    }
+    return off;
+}
+// grid: (cluster, sequences * kv heads); `per`: slots of a block, a multiple of 128
+template <int T>
+__global__ void __launch_bounds__(T) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seqs, EvictArgs a, int per) {
+    constexpr int W = T / 32, PLACES = 2048 / T;
+    extern __shared__ __align__(16) uint32_t key[];              // [per], sums as whole numbers of their order
+    uint16_t* const list = reinterpret_cast<uint16_t*>(key + per);   // [per], the block's slots that stay
+    __shared__ __align__(16) uint32_t hist[3][1024];             // counts of 16 bits, two in a word: a block has fewer sums than that
+    __shared__ __align__(16) int totals[3][W];
+    __shared__ int flag, chosen[3][2];
     __shared__ int2 warp_counts[W], block_counts;
     cg::cluster_group cluster = cg::this_cluster();
     const int size = cluster.num_blocks(), rank = cluster.block_rank();
     const int i = blockIdx.y / pool.n_kv, h = blockIdx.y - i * pool.n_kv, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int32_t* kept = a.kept + ((int64_t)i * pool.n_kv + h) * a.limit;
-    const int length = evict_length(seqs, pool, i, a.capacity, &flag);
-    if (!begins_cut(pool, seqs, a, i, h, length, kept, rank == 0 && tid == 0, rank * kSelectThreads + tid, size * kSelectThreads)) return;  // the whole cluster
     float* mass = a.mass + (int64_t)i * a.mass_stride + (int64_t)h * a.mass_head_stride;
+    const int base = rank * per;
+    {
+        // the sums set out while the pages are looked at: of a length that may turn out to be none
+        const int maybe = min(max(seqs.ctx[i] + seqs.row_start[i + 1] - seqs.row_start[i], 0), a.capacity), mine = max(0, min(per, maybe - base));
+        if (maybe > a.limit)
+#pragma unroll 8
+            for (int x = tid; x < ((mine + 3) & ~3); x += T) key[x] = x < mine ? ordered(mass[base + x]) : 0;
+    }
+    for (int x = tid; x < 3 * 256; x += T) reinterpret_cast<int4*>(&hist[0][0])[x] = make_int4(0, 0, 0, 0);
+    const int length = evict_length(seqs, pool, i, a.capacity, &flag);
+    if (!begins_cut(pool, seqs, a, i, h, length, kept, rank == 0 && tid == 0, rank * T + tid, size * T)) return;  // the whole cluster
     const int lo = a.first, hi = length - a.recent, most = a.keep - a.first - a.recent;
-    const int base = rank * per, mine = max(0, min(per, length - base));
-    for (int x = tid; x < 3 * 2048; x += kSelectThreads) (&hist[0][0])[x] = 0;
-    for (int x = tid; x < mine; x += kSelectThreads) sum[x] = mass[base + x];
+    const int mine = max(0, min(per, length - base)), quads = (mine + 3) >> 2;
     // the most-th largest of [lo, hi): its digits one after the other; `left`: how many of those that share the digits so far stay
     uint32_t value = 0;
     int left = most;
     const int in0 = max(lo - base, 0), in1 = min(hi - base, mine);  // the block's part of [lo, hi)
+    const uint4* const key4 = reinterpret_cast<const uint4*>(key);
     if (most > 0) {
         const int bits[3] = {11, 11, 10};
         int shift = 32;
@@ -110,78 +140,127 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4Pool pool
         for (int d = 0; d < 3; d++) {
             shift -= bits[d];
             __syncthreads();
-            for (int x = in0 + tid; x < in1; x += kSelectThreads) {
-                const uint32_t v = ordered(sum[x]);
-                if (d == 0 || v >> (shift + bits[d]) == value >> (shift + bits[d])) atomicAdd(&hist[d][v >> shift & ((1u << bits[d]) - 1)], 1);
+            auto count = [&](uint32_t v) {
+                if (d == 0 || v >> (shift + bits[d]) == value >> (shift + bits[d])) {
+                    const uint32_t digit = v >> shift & ((1u << bits[d]) - 1);
+                    atomicAdd(&hist[d][digit >> 1], digit & 1 ? 0x10000u : 1u);
+                }
+            };
+            const int f0 = (in0 + 3) >> 2, f1 = in1 >> 2;   // quads of nothing else
+#pragma unroll 2
+            for (int q = f0 + tid; q < f1; q += T) {
+                const uint4 v = key4[q];
+                count(v.x);
+                count(v.y);
+                count(v.z);
+                count(v.w);
+            }
+            if (tid < 8) {
+                const int x = tid < 4 ? 4 * f0 - 4 + tid : 4 * max(f1, f0) + tid - 4;   // around them
+                if (x >= in0 && x < in1) count(key[x]);
             }
             cluster.sync();
-            // counts from the top: a thread has four places, of all blocks at once
-            int4 part[kMostCluster];
+            // counts from the top: a thread has some places in a row, of all blocks at once
+            int c[PLACES];
 #pragma unroll
-            for (int r = 0; r < kMostCluster; r++)
-                part[r] = r < size ? *cluster.map_shared_rank(reinterpret_cast<const int4*>(&hist[d][2044 - 4 * tid]), r) : make_int4(0, 0, 0, 0);
-            int c[4] = {0, 0, 0, 0};
+            for (int k = 0; k < PLACES; k += 2) {
+                uint32_t part[kMostCluster];
 #pragma unroll
-            for (int r = 0; r < kMostCluster; r++) { c[0] += part[r].w; c[1] += part[r].z; c[2] += part[r].y; c[3] += part[r].x; }
-            const int mysum = (c[0] + c[1]) + (c[2] + c[3]);
-            int all, before = before_me(mysum, sums, all);
+                for (int r = 0; r < kMostCluster; r++) part[r] = r < size ? *cluster.map_shared_rank(&hist[d][1023 - (PLACES / 2) * tid - k / 2], r) : 0;
+                c[k] = c[k + 1] = 0;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (before < left && before + c[k] >= left) { chosen[0] = 2047 - 4 * tid - k; chosen[1] = left - before; }
+                for (int r = 0; r < kMostCluster; r++) { c[k] += part[r] >> 16; c[k + 1] += part[r] & 0xffff; }
+            }
+            int all = 0;
+#pragma unroll
+            for (int k = 0; k < PLACES; k++) all += c[k];
+            int before = before_thread<T>(all, totals[d]);
+#pragma unroll
+            for (int k = 0; k < PLACES; k++) {
+                if (before < left && before + c[k] >= left) { chosen[d][0] = 2047 - PLACES * tid - k; chosen[d][1] = left - before; }
                 before += c[k];
             }
             __syncthreads();
-            value |= (uint32_t)chosen[0] << shift;
-            left = chosen[1];
+            value |= (uint32_t)chosen[d][0] << shift;
+            left = chosen[d][1];
         }
+    } else {
+        __syncthreads();
     }
-    // Slots in ascending order: all above the value, and the first `left` equal to it.  A warp counts those of its stretch, then knows what is before it and goes over it again.
-    __syncthreads();
-    const int stretch = ((mine + W - 1) / W + 31) & ~31, x0 = min(warp * stretch, mine), x1 = min(x0 + stretch, mine);
-    auto kind = [&](int x, bool& above, bool& equal) {
-        const bool here = x < x1, in = x >= in0 && x < in1;
-        const uint32_t v = here ? ordered(sum[x]) : 0;
-        above = here && (!in || (most > 0 && v > value));
-        equal = here && in && most > 0 && v == value;
+    // Slots in ascending order: all above the value, and the first `left` equal to it.  A warp counts those of its stretch, four in a row a lane, then knows what is before it and goes over it again.
+    const int stretch = ((quads + W - 1) / W + 31) & ~31, q0 = min(warp * stretch, quads), q1 = min(q0 + stretch, quads);
+    // bits 0-3: of a lane's four those above, 4-7: those equal
+    auto kinds = [&](int q) {
+        uint32_t bits = 0;
+        if (q + lane >= q1) return bits;
+        const uint4 k4 = key4[q + lane];
+        const uint32_t v[4] = {k4.x, k4.y, k4.z, k4.w};
+        if (most > 0)
+#pragma unroll
+            for (int e = 0; e < 4; e++) bits |= (v[e] > value ? 1u << e : 0u) | (v[e] == value ? 16u << e : 0u);
+        const int x0 = 4 * (q + lane);
+        if (x0 < in0 || x0 + 4 > in1) {  // some are not chosen by their sums
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int x = x0 + e;
+                if (x < in0 || x >= in1) bits = (bits & ~(17u << e)) | (x < mine ? 1u << e : 0u);
+            }
+        }
+        return bits;
     };
-    int2 mc = make_int2(0, 0);
-    for (int x = x0; x < x1; x += 32) {
-        bool above, equal;
-        kind(x + lane, above, equal);
-        mc.x += __popc(__ballot_sync(0xffffffffu, above));
-        mc.y += __popc(__ballot_sync(0xffffffffu, equal));
+    int n_both = 0;                                              // above, and in the upper half equal: 16 bits are enough for a block's
+    for (int q = q0; q < q1; q += 32) {
+        const uint32_t b = kinds(q);
+        n_both += __popc(b & 15u) + (__popc(b & 240u) << 16);
     }
+    const int2 mc = make_int2(__reduce_add_sync(0xffffffffu, n_both & 0xffff), __reduce_add_sync(0xffffffffu, n_both >> 16));
     if (lane == 0) warp_counts[warp] = mc;
     __syncthreads();
-    if (tid == 0) {
-        int2 t = make_int2(0, 0);
-        for (int w = 0; w < W; w++) { t.x += warp_counts[w].x; t.y += warp_counts[w].y; }
-        block_counts = t;
+    if (warp == 0) {
+        const int2 t = lane < W ? warp_counts[lane] : make_int2(0, 0);
+        const int x = __reduce_add_sync(0xffffffffu, t.x), y = __reduce_add_sync(0xffffffffu, t.y);
+        if (lane == 0) block_counts = make_int2(x, y);
     }
     cluster.sync();  // and every sum is in shared memory
-    int equals = 0, out = 0;
-    auto pass = [&](const int2& n) {
-        out += n.x + min(max(left - equals, 0), n.y);
-        equals += n.y;
-    };
-    for (int r = 0; r < rank; r++) pass(*cluster.map_shared_rank(&block_counts, r));
-    for (int w = 0; w < warp; w++) pass(warp_counts[w]);
-    for (int x = x0; x < x1; x += 32) {
-        bool above, equal;
-        kind(x + lane, above, equal);
-        const uint32_t below = (1u << lane) - 1, eq = __ballot_sync(0xffffffffu, equal);
-        const bool stays = above || (equal && equals + __popc(eq & below) < left);
-        const uint32_t st = __ballot_sync(0xffffffffu, stays);
-        if (stays) {
-            const int to = out + __popc(st & below);
-            kept[to] = base + x + lane;
-            mass[to] = sum[x + lane];
+    // what is in front: above and equal of the blocks before, of the warps before
+    int2 mine_before = lane < rank ? *cluster.map_shared_rank(&block_counts, lane) : make_int2(0, 0);
+    const int b_above = __reduce_add_sync(0xffffffffu, mine_before.x), b_equal = __reduce_add_sync(0xffffffffu, mine_before.y);
+    mine_before = lane < warp ? warp_counts[lane] : make_int2(0, 0);
+    int above = b_above + __reduce_add_sync(0xffffffffu, mine_before.x), equals = b_equal + __reduce_add_sync(0xffffffffu, mine_before.y);
+    // of the equal ones the first `left` stay: out = above + min(equals, left)
+    const int begin = b_above + min(b_equal, left);              // of the block
+    for (int q = q0; q < q1; q += 32) {
+        const uint32_t b = kinds(q);
+        const int n = __popc(b & 15u) + (__popc(b & 240u) << 16);
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += u;
         }
-        equals += __popc(eq);
-        out += __popc(st);
+        const int before = incl - n, total = __shfl_sync(0xffffffffu, incl, 31);
+        int e_before = equals + (before >> 16), to = above + (before & 0xffff) + min(e_before, left) - begin;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool eq = b >> (4 + e) & 1, stays = (b >> e & 1) || (eq && e_before < left);
+            if (stays) list[to++] = (uint16_t)(4 * (q + lane) + e);
+            e_before += eq;
+        }
+        above += total & 0xffff;
+        equals += total >> 16;
     }
-    for (int x = a.keep + rank * kSelectThreads + tid; x < length; x += size * kSelectThreads) mass[x] = 0.0f;
-    for (int x = a.keep + rank * kSelectThreads + tid; x < a.limit; x += size * kSelectThreads) kept[x] = -1;
+    if (warp == W - 1 && lane == 0) chosen[0][0] = above + min(equals, left) - begin;   // the last warp knows how many there are
+    __syncthreads();
+    const int n_list = chosen[0][0];
+#pragma unroll 4
+    for (int o = tid; o < n_list; o += T) {
+        const int x = list[o];
+        const uint32_t v = key[x];
+        kept[begin + o] = base + x;
+        mass[begin + o] = v == 0 ? __int_as_float(0x7fffffff) : __uint_as_float(v & 0x80000000u ? v & 0x7fffffffu : ~v);
+    }
+    for (int x = a.keep + rank * T + tid; x < length; x += size * T) mass[x] = 0.0f;
+    for (int x = a.keep + rank * T + tid; x < a.limit; x += size * T) kept[x] = -1;
     cluster.sync();  // no block leaves while another reads its counts
 }
 
@@ -247,40 +326,45 @@ __global__ void __launch_bounds__(kFarThreads) kv4_select_far_kernel(Kv4Pool poo
     for (int x = a.keep + tid; x < a.limit; x += kFarThreads) kept[x] = -1;
 }
 
-// Rows of pieces (T) by one cluster: slot j of the sequence from kept[j].
+// Rows of pieces (T) by one cluster: slot j of the sequence from kept[j].  A thread has the same piece of some rows.
 template <typename T>
 __device__ __forceinline__ void move_rows(const Kv4Pool& pool, const int32_t* table, const int32_t* kept, int keep, int h, uint8_t* base, int row_bytes) {
     cg::cluster_group cluster = cg::this_cluster();
-    const int threads = kMoveThreads * cluster.num_blocks(), me = cluster.block_rank() * kMoveThreads + threadIdx.x;
-    const int pieces = row_bytes / (int)sizeof(T), mask = (1 << pool.page_shift) - 1;
-    const int all = keep * pieces;               // in 31 bits: checked by the call
-    auto at = [&](int slot, int piece) {
-        return reinterpret_cast<T*>(base + ((((size_t)table[slot >> pool.page_shift] * pool.n_kv + h) << pool.page_shift) + (slot & mask)) * row_bytes) + piece;
-    };
-    for (int e0 = 0; e0 < all; e0 += threads * kMovePieces) {
+    const int blocks = cluster.num_blocks(), mask = (1 << pool.page_shift) - 1;
+    const int pieces = row_bytes / (int)sizeof(T), rows = kMoveThreads / pieces;   // rows of a block at a time
+    const int mine = threadIdx.x / pieces, piece = threadIdx.x - mine * pieces, step = blocks * rows;
+    T* const from0 = reinterpret_cast<T*>(base) + piece;
+    auto at = [&](int number, int slot) { return from0 + ((((size_t)(uint32_t)number * (uint32_t)pool.n_kv + h) << pool.page_shift) + (slot & mask)) * (uint32_t)pieces; };
+    for (int j0 = 0; j0 < keep; j0 += step * kMovePieces) {
+        const int j = j0 + (int)cluster.block_rank() * rows + mine;
+        // all loads of a kind go out together: rows that are not there, or in their place, read slot 0
         T v[kMovePieces];
-        int from[kMovePieces];
+        int from[kMovePieces], page[kMovePieces];
+#pragma unroll
+        for (int u = 0; u < kMovePieces; u++) from[u] = kept[mine < rows && j + u * step < keep ? j + u * step : 0];
+#pragma unroll
+        for (int u = 0; u < kMovePieces; u++) page[u] = table[from[u] >> pool.page_shift];
+#pragma unroll
+        for (int u = 0; u < kMovePieces; u++) v[u] = *at(page[u], from[u]);
+        T* to[kMovePieces];
 #pragma unroll
         for (int u = 0; u < kMovePieces; u++) {
-            const int e = e0 + u * threads + me;
-            from[u] = e < all ? kept[e / pieces] : -1;
+            const bool moves = mine < rows && j + u * step < keep && from[u] != j + u * step;
+            to[u] = moves ? at(table[(j + u * step) >> pool.page_shift], j + u * step) : nullptr;
         }
+        if (blocks == 1) __syncthreads();
+        else cluster.sync();
 #pragma unroll
-        for (int u = 0; u < kMovePieces; u++) {
-            const int e = e0 + u * threads + me;
-            if (from[u] >= 0 && from[u] != e / pieces) v[u] = *at(from[u], e % pieces);
+        for (int u = 0; u < kMovePieces; u++)
+            if (to[u]) *to[u] = v[u];
+        if (j0 + step * kMovePieces < keep) {
+            if (blocks == 1) __syncthreads();
+            else cluster.sync();
         }
-        cluster.sync();
-#pragma unroll
-        for (int u = 0; u < kMovePieces; u++) {
-            const int e = e0 + u * threads + me;
-            if (from[u] >= 0 && from[u] != e / pieces) *at(e / pieces, e % pieces) = v[u];
-        }
-        if (e0 + threads * kMovePieces < all) cluster.sync();
     }
 }
 // grid: (cluster, sequences * kv heads, planes: keys, values, their scales)
-__global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4Pool pool, Kv8Seqs seqs, EvictArgs a) {
+__global__ void __launch_bounds__(kMoveThreads, 3) kv4_move_kernel(Kv4Pool pool, Kv8Seqs seqs, EvictArgs a) {
     const int i = blockIdx.y / pool.n_kv, h = blockIdx.y - i * pool.n_kv, hd = pool.hd;
     // sequences that are cut, and not left alone: only these have a new length
     if ((long long)seqs.ctx[i] + seqs.row_start[i + 1] - seqs.row_start[i] <= a.limit || a.ctx_out[i] != a.keep) return;
@@ -325,7 +409,7 @@ extern "C" int32_t lc_kv4_evict_dev(const lc_kv4_cache* cache, const lc_kv8_rows
              (long long)mass_head_stride);
     LC_CHECK(seqs.n_seqs <= 1 || pool.n_kv == 1 || mass_stride >= (int64_t)(pool.n_kv - 1) * mass_head_stride + capacity || mass_head_stride >= (int64_t)(seqs.n_seqs - 1) * mass_stride + capacity,
              LC_ERR_INVALID, "%s: the sums of sequences and heads overlap (strides %lld and %lld)", call, (long long)mass_stride, (long long)mass_head_stride);
-    LC_CHECK((int64_t)keep * (pool.hd / 16) < 0x70000000, LC_ERR_INVALID, "%s: keep=%d rows of %d dims are too many for one call", call, keep, pool.hd);
+    LC_CHECK(limit <= 1 << 30, LC_ERR_INVALID, "%s: limit=%d (2^30 at most)", call, limit);
     LC_CHECK((int64_t)seqs.n_seqs * pool.n_kv <= 65535, LC_ERR_INVALID, "%s: %d sequences of %d kv heads are too many for one call", call, seqs.n_seqs, pool.n_kv);
     if (seqs.n_seqs == 0) return LC_OK;
     LC_CHECK(seqs.table && seqs.ctx && seqs.row_start && mass_dev && kept_dev && ctx_out_dev, LC_ERR_INVALID, "%s: null pointer", call);
@@ -337,14 +421,16 @@ extern "C" int32_t lc_kv4_evict_dev(const lc_kv4_cache* cache, const lc_kv8_rows
     cudaLaunchAttribute attr[1];
     // blocks of a cluster: as many as leave all sequences and heads about two blocks for each SM, and at least what holds the longest context's sums
     const int64_t slots = std::min<int64_t>((int64_t)seqs.width << pool.page_shift, capacity), units = (int64_t)seqs.n_seqs * pool.n_kv;
-    auto per_block = [&](int size) { return (slots + 32 * size - 1) / (32 * size) * 32; };
+    auto per_block = [&](int size) { return (slots + 128 * size - 1) / (128 * size) * 128; };
+    auto bytes = [&](int size) { return (size_t)per_block(size) * 6; };
     int size = 1;
-    while (size < kMostCluster && (2 * size * units <= 2 * sm_count() || per_block(size) * sizeof(float) > kSelectSmem)) size *= 2;
-    if (per_block(size) * sizeof(float) <= kSelectSmem) {
-        const size_t smem = per_block(size) * sizeof(float);
-        LC_CUDA(ensure_smem_limit((const void*)kv4_select_kernel, smem));
-        const cudaLaunchConfig_t cfg = clusters(dim3((unsigned)size, (unsigned)units), kSelectThreads, smem, s, attr);
-        LC_CUDA(cudaLaunchKernelEx(&cfg, kv4_select_kernel, pool, seqs, a, (int)per_block(size)));
+    while (size < kMostCluster && (2 * size * units <= 2 * sm_count() || bytes(size) > kSelectSmem)) size *= 2;
+    if (bytes(size) <= kSelectSmem) {
+        const bool wide = per_block(size) > 8192;   // blocks of so many sums are one for an SM
+        const auto kern = wide ? kv4_select_kernel<1024> : kv4_select_kernel<512>;
+        LC_CUDA(ensure_smem_limit((const void*)kern, bytes(size)));
+        const cudaLaunchConfig_t cfg = clusters(dim3((unsigned)size, (unsigned)units), wide ? 1024 : 512, bytes(size), s, attr);
+        LC_CUDA(cudaLaunchKernelEx(&cfg, kern, pool, seqs, a, (int)per_block(size)));
     } else {
         kv4_select_far_kernel<<<dim3((unsigned)seqs.n_seqs, (unsigned)pool.n_kv), kFarThreads, 0, s>>>(pool, seqs, a);
         LC_CUDA(cudaGetLastError());
