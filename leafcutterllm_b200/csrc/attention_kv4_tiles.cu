@@ -32,8 +32,8 @@ struct TileShared {
     uint64_t s_full[2], p_full[2], o_full[2];  // scores, weights, sums of a row tile
     uint64_t c_full[kSlots];                   // `outside` of a key tile
     uint64_t raw_full[2][2], raw_free[2][2];   // copied keys, values, of a place
-    uint64_t k_full, v_full[2];                // unpacked keys, values (a barrier for each place: the next tile's values may be there before this one's are waited for);
-    uint64_t v_free[2];                        // the keys' place is free when the last row tile's scores are done, the values' when its sums are
+    uint64_t k_full[2], v_full[2];             // unpacked keys, values (a barrier for each place: the next tile's may be there before this one's are waited for);
+    uint64_t k_free[2], v_free[2];             // a place of keys is free when the last row tile's scores are done, one of values when its sums are
     uint2 sums[kTileThreads / 32];
     uint32_t outside[kSlots];                  // bit g: the key tile's group g of 16 lies on a page outside the pool
     uint32_t tmem;
@@ -46,10 +46,10 @@ template <int HD, bool SPLIT> struct TileShape {
     static constexpr int kK = HD * 256, kV = HD * 256;
     static constexpr int kSoftRegs = SPLIT ? 176 : 184, kOtherRegs = 256 - kSoftRegs;  // of the softmax's 256 threads, of the other 256
     static_assert(256 * (kSoftRegs + kOtherRegs) <= kLaunchRegs * kTileThreads, "setmaxnreg waits for registers that the launch does not have");
-    static constexpr int kVs = SPLIT ? 1 : 2;                 // places for unpacked values, for copied tiles: f32 queries leave room for one
-    static constexpr int kRaws = SPLIT ? 1 : 2;
+    static constexpr int kVs = SPLIT ? 1 : 2;                 // places for unpacked keys, values: f32 queries leave room for one
+    static constexpr int kRaws = 1;                           // and for copied ones
     static constexpr int kRawHalf = kKeys * HD / 2 + kKeys * HD / 16;  // integers and scales of a tile's keys or values
-    static constexpr int kBytes = kQ + kK + kVs * kV + kRaws * 2 * kRawHalf + 1024;
+    static constexpr int kBytes = kQ + kVs * (kK + kV) + kRaws * 2 * kRawHalf + 1024;
 };
 
 template <int HD, bool SPLIT>
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
     unsigned char* const smem = (unsigned char*)(((uintptr_t)raw_smem + 1023) & ~(uintptr_t)1023);
     unsigned char* const sq = smem;
     unsigned char* const sk = sq + Shape::kQ;
-    unsigned char* const sv = sk + Shape::kK;
+    unsigned char* const sv = sk + Shape::kVs * Shape::kK;
     unsigned char* const raws = sv + Shape::kVs * Shape::kV;   // [place][keys, values][integers, then scales]
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (blockIdx.x == 0 && blockIdx.y == 0) kv8_check_seqs(seqs, pool);
@@ -115,15 +115,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
         for (int t = 0; t < 2; t++) {
             mbar_init(&sh.s_full[t], 1);
             mbar_init(&sh.o_full[t], 1);
+            mbar_init(&sh.k_free[t], 1);
             mbar_init(&sh.v_free[t], 1);
             mbar_init(&sh.p_full[t], 128);
             for (int x = 0; x < 2; x++) {
                 mbar_init(&sh.raw_full[t][x], 1);
                 mbar_init(&sh.raw_free[t][x], kConvWarps);
             }
+            mbar_init(&sh.k_full[t], kConvWarps);
             mbar_init(&sh.v_full[t], kConvWarps);
         }
-        mbar_init(&sh.k_full, kConvWarps);
         for (int t = 0; t < kSlots; t++) mbar_init(&sh.c_full[t], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
@@ -178,41 +179,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
       if (warp == 12 || warp == 13) {
         if (warp == 12) {
             // ------------------------------------------------------------------------------------------------ products
-            // All lanes go the same way and one of them issues: descriptors then are the warp's and not a thread's.
-            const uint32_t q_at = smem_u32(sq), k_at = smem_u32(sk), v_at = smem_u32(sv), base = __shfl_sync(0xffffffffu, tmem, 0);
-            const uint32_t one = lane == 0;
-            auto scores = [&](int t) {
-                const uint32_t d = base + 128 * t;
+            // All lanes go the same way and one of them issues.  The allocation is of all columns, so it begins at 0, and the places in shared memory are counted from its base: operands that are the warp's.
+            const uint32_t q_at = (smem_u32(raw_smem) + 1023u) & ~1023u, k_at = q_at + Shape::kQ, v_at = k_at + Shape::kVs * Shape::kK;
+            const uint32_t one = elect_lane();
+            auto scores = [&](int t, int i) {
 #pragma unroll
                 for (int term = TERMS - 1; term >= 0; term--) {  // the low parts first: what is cut off then is small
-                    const uint64_t dq = umma_desc_sw128(q_at + (t * TERMS + term) * Shape::kPart), dk = umma_desc_sw128(k_at);
+                    const uint32_t dq = desc_low(q_at + (t * TERMS + term) * Shape::kPart), dk = desc_low(k_at + (i % Shape::kVs) * Shape::kK);
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ks++) {
-                        const uint64_t off = ((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4;
-                        mma_ss_by(one, d, dq + off, dk + off, idesc_f16(kKeys), term < TERMS - 1 || ks > 0);
+                        const uint32_t off = ((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4;
+                        mma_ss_low(one, 128 * t, dq + off, dk + off, idesc_f16(kKeys), term < TERMS - 1 || ks > 0);
                     }
                 }
-                if (one) umma_commit(&sh.s_full[t]);
+                if (one) {
+                    umma_commit(&sh.s_full[t]);
+                    if (t == last) umma_commit(&sh.k_free[i % Shape::kVs]);
+                }
                 __syncwarp();
             };
             auto sums = [&](int t, int i) {
-                const uint32_t d = base + 256 + 128 * t, p = base + 128 * t;
-                const uint64_t dv = umma_desc_sw128(v_at + (i % Shape::kVs) * Shape::kV);
-                const uint32_t on = !SPLIT && i > 0;
+                const uint32_t dv = desc_low(v_at + (i % Shape::kVs) * Shape::kV), on = !SPLIT && i > 0;
 #pragma unroll
                 for (int term = TERMS - 1; term >= 0; term--)
 #pragma unroll
                     for (int ks = 0; ks < kKeys / 16; ks++)
-                        mma_ts_by(one, d, p + 16 * ks + 8 * term, dv + (((ks >> 2) * (HD * 128) + (ks & 3) * 32) >> 4), idesc_f16(HD), term < TERMS - 1 || ks > 0 ? 1u : on);
+                        mma_ts_low(one, 256 + 128 * t, 128 * t + 16 * ks + 8 * term, dv + (((ks >> 2) * (HD * 128) + (ks & 3) * 32) >> 4), idesc_f16(HD), term < TERMS - 1 || ks > 0 ? 1u : on);
                 if (one) {
                     umma_commit(&sh.o_full[t]);
                     if (t == last) umma_commit(&sh.v_free[i % Shape::kVs]);
                 }
                 __syncwarp();
             };
-            bool ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_full, 0));
+            bool ok = __all_sync(0xffffffffu, tmem == 0 && mbar_wait(&sh.k_full[0], 0));
             tc_fence_after();
-            for (int t = 0; t < n_tiles && ok; t++) scores(t);
+            for (int t = 0; t < n_tiles && ok; t++) scores(t, 0);
             for (int i = 0; i < n && ok; i++) {
                 const bool more = i + 1 < n;
                 ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_full[i % Shape::kVs], (i / Shape::kVs) & 1));
@@ -222,10 +223,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
                     if (!ok) break;
                     sums(t, i);
                     if (more) {
-                        if (t == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_full, (i + 1) & 1));
+                        if (t == 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.k_full[(i + 1) % Shape::kVs], ((i + 1) / Shape::kVs) & 1));
                         if (!ok) break;
                         tc_fence_after();
-                        scores(t);
+                        scores(t, i + 1);
                     }
                 }
             }
@@ -276,18 +277,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
         const int cw = warp < 12 ? warp - 8 : warp - 10, ct = cw * 32 + lane;
         constexpr int KC = HD / 16, VC = HD / 8;     // K: pieces of 16 dims of a key; V: words of 8 dims of a key
         const int row_ints = hd >> 1, row_scales = hd >> 4;
+        // Rounds of 32 pieces: the keys' are 32 or 16, the values', twice as long, 8 or 4.  Warps with more of the values' have fewer of the keys'.
+        constexpr int K_MORE = HD == 128 ? 6 : 4, K_LESS = HD == 128 ? 4 : 2, LESS = HD == 128 ? 2 : 4;   // the first LESS warps have K_LESS rounds of keys
+        static_assert(LESS * K_LESS + (kConvWarps - LESS) * K_MORE == kKeys * KC / 32, "every round has a warp");
+        const int k_from = cw < LESS ? cw * K_LESS : LESS * K_LESS + (cw - LESS) * K_MORE, k_to = k_from + (cw < LESS ? K_LESS : K_MORE);
         bool ok = true;
         for (int i = 0; i < n && ok; i++) {
             const int st = i % RS;
             const unsigned char* const rk = raws + 2 * st * Shape::kRawHalf;
             const unsigned char* const rv = rk + Shape::kRawHalf;
             ok = mbar_wait(&sh.raw_full[st][0], (i / RS) & 1);
-            if (i > 0) ok = ok && mbar_wait(&sh.s_full[last], (i - 1) & 1);  // the keys' place is free
+            if (i >= Shape::kVs) ok = ok && mbar_wait(&sh.k_free[i % Shape::kVs], (i / Shape::kVs - 1) & 1);  // the keys' place is free
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
+            unsigned char* const k_to_place = sk + (i % Shape::kVs) * Shape::kK;
 #pragma unroll 2
-            for (int e = ct; e < kKeys * KC; e += 32 * kConvWarps) {
-                const int key = e / KC, ch = e % KC;
+            for (int round = k_from; round < k_to; round++) {
+                const int e = round * 32 + lane, key = e / KC, ch = e % KC;
                 uint32_t first[4] = {0, 0, 0, 0}, second[4] = {0, 0, 0, 0};
                 // the upper half of a row's chunks writes its second piece first: eight lanes then meet all banks
                 const int swap = ch >= 4;
@@ -297,13 +303,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
                     values8(swap ? x.y : x.x, s, first);
                     values8(swap ? x.x : x.y, s, second);
                 }
-                unsigned char* dst = sk + (ch >> 2) * (128 * 128);
+                unsigned char* dst = k_to_place + (ch >> 2) * (128 * 128);
                 *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + swap)) = make_uint4(first[0], first[1], first[2], first[3]);
                 *reinterpret_cast<uint4*>(dst + sw128(key, 2 * (ch & 3) + 1 - swap)) = make_uint4(second[0], second[1], second[2], second[3]);
             }
             fence_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(&sh.k_full); mbar_arrive(&sh.raw_free[st][0]); }
+            if (lane == 0) { mbar_arrive(&sh.k_full[i % Shape::kVs]); mbar_arrive(&sh.raw_free[st][0]); }
 
             ok = mbar_wait(&sh.raw_full[st][1], (i / RS) & 1);
             if (i >= Shape::kVs) ok = ok && mbar_wait(&sh.v_free[i % Shape::kVs], (i / Shape::kVs - 1) & 1);  // the values' place is free

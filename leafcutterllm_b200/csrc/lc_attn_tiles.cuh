@@ -27,6 +27,25 @@ __device__ __forceinline__ void mma_ts_by(uint32_t by, uint32_t d, uint32_t a, u
                  "r"(idesc), "r"(accumulate), "r"(by)
                  : "memory");
 }
+// The same with descriptors as their lower words, for an issuing lane that elect_lane has chosen.  Both let the compiler keep the operands in the warp's registers: a product then takes 50 cycles
+// to issue, less than it runs, instead of 105 to 155 (64-bit descriptors, lane 0 by its number), which made the issue the bottleneck of attention in tiles.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(r));
+    return r;
+}
+// of umma_desc_sw128, whose upper word is 0x40004040
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr) { return ((saddr >> 4) & 0x3fffu) | 0x10000u; }
+__device__ __forceinline__ void mma_ss_low(uint32_t by, uint32_t d, uint32_t da, uint32_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p, q;\n .reg .b64 x, y;\n mov.b64 x, {%1, 0x40004040};\n mov.b64 y, {%2, 0x40004040};\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d), "r"(da), "r"(db), "r"(idesc), "r"(accumulate), "r"(by)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts_low(uint32_t by, uint32_t d, uint32_t a, uint32_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p, q;\n .reg .b64 y;\n mov.b64 y, {%2, 0x40004040};\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(db), "r"(idesc), "r"(accumulate), "r"(by)
+                 : "memory");
+}
 // 16-byte chunk `ch` (of 8) of a row of 128 bytes
 __device__ __forceinline__ int sw128(int row, int ch) { return row * 128 + ((ch ^ (row & 7)) << 4); }
 
