@@ -459,6 +459,7 @@ bool tiles_fit(const Kv4Pool& pool, const Kv8Seqs& seqs, int group) {
     TilePlan tiles;
     return line_fits(pool, seqs, group, kTileRows2) && kv8_tiles_plan(pool, seqs, group, &tiles);
 }
+bool tiles_pay(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, const TilePlan& plan) { return kv8_tiles_pay(pool, seqs, typ, group, max_rows, plan); }
 struct Plan {
     bool by_tiles;
     TilePlan tiles;
@@ -470,7 +471,7 @@ Plan plan_call(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group
     Plan p;
     int groups = run_groups(pool, group, max_rows);
     p.by_tiles = kv8_tiles_plan(pool, seqs, group, &p.tiles) && line_fits(pool, seqs, group, kTileRows2) &&
-                 (kv8_tiles_pay(pool, seqs, typ, group, max_rows, p.tiles) || !line_fits(pool, seqs, group, 8 * groups));
+                 (tiles_pay(pool, seqs, typ, group, max_rows, p.tiles) || !line_fits(pool, seqs, group, 8 * groups));
     while (!p.by_tiles && groups < most_groups(pool) && !line_fits(pool, seqs, group, 8 * groups)) groups *= 2;
     p.runs = plan_runs(pool, typ, groups);
     return p;
