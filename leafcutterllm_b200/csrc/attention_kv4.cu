@@ -459,7 +459,12 @@ bool tiles_fit(const Kv4Pool& pool, const Kv8Seqs& seqs, int group) {
     TilePlan tiles;
     return line_fits(pool, seqs, group, kTileRows2) && kv8_tiles_plan(pool, seqs, group, &tiles);
 }
-bool tiles_pay(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, const TilePlan& plan) { return kv8_tiles_pay(pool, seqs, typ, group, max_rows, plan); }
+// Whether tiles are faster than runs, us in runs / in tiles.  128 rows (tokens x heads of a group) of a sequence and kv head: bf16, 32 heads over 8 of 128, one sequence behind 4,000 tokens 30 / 31, 16 behind 2,000
+// 100 / 49, 64 behind 1,000 199 / 138; f32 138 / 77, 278 / 206; heads of 64, 64 sequences 84 / 51.  64 rows: 16-bit types where units are no more than SMs, one sequence 27 / 29 (32 kv heads 39 / 36), 16
+// 60 / 49, but 64 sequences 116 / 118, 16 of 32 kv heads 186 / 206; f32 158 / 172; heads of 64 29 / 41.  32 rows: 39 / 48.
+bool tiles_pay(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, const TilePlan& plan) {
+    return (int64_t)group * max_rows >= (typ != LC_TYPE_F32 && pool.hd > 64 && plan.units <= sm_count() ? 64 : 128);
+}
 struct Plan {
     bool by_tiles;
     TilePlan tiles;

@@ -284,7 +284,14 @@ int32_t weights_full(const Kv4Pool& pool, const Kv8Seqs& seqs, const WeightArgs&
     if (a.typ == LC_TYPE_F32) return pool.hd == HD ? weights_as<HD, NG, true, true>(pool, seqs, a, s) : weights_as<HD, NG, true, false>(pool, seqs, a, s);
     return pool.hd == HD ? weights_as<HD, NG, false, true>(pool, seqs, a, s) : weights_as<HD, NG, false, false>(pool, seqs, a, s);
 }
-constexpr int kTileWeightRows = 64;  // of a sequence and kv head, from which on tiles are faster
+// Whether tiles are faster than runs, us in runs / in tiles, with so many stretches of 256 keys (as long as the tables are).  256 rows (tokens x heads of a group) of a sequence and kv head: always, bf16 214 / 157
+// with 2,048 stretches and 798 / 703 with 8,192, f32 351 / 330 and 1,329 / 1,379.  128 rows: bf16 28 / 12 with 128, 114 / 99 with 2,048, 388 / 450 with 8,192; f32 108 / 73 with 1,024, 312 / 396 with 4,096.  64
+// rows: bf16 17 / 12 with 128, 39 / 42 with 1,024, 59 / 85 with 2,048; f32 23 / 14 and 56 / 68.  32 rows: bf16 12 / 12 and 21 / 41.
+bool tiles_pay(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int64_t rows) {
+    const int64_t stretches = (((int64_t)seqs.width << pool.page_shift) + 255) / 256 * seqs.n_seqs * pool.n_kv;
+    const bool f32 = typ == LC_TYPE_F32;
+    return pool.hd <= 128 && (rows >= 256 || (rows >= 128 && stretches <= (f32 ? 8 : 16) * sm_count()) || (rows >= 64 && stretches <= (f32 ? 2 : 7) * sm_count()));
+}
 // As many groups of 8 rows share a step's keys as a sequence and kv head has rows for, four at most.
 template <int HD>
 int32_t weights_of(const Kv4Pool& pool, const Kv8Seqs& seqs, const WeightArgs& a, int64_t rows, cudaStream_t s) {
@@ -326,7 +333,7 @@ extern "C" int32_t lc_kv4_weights_dev(const lc_kv4_cache* cache, const lc_kv8_ro
                        scale * 1.44269504088896f};
     cudaStream_t s = stream_or_own(stream_);
     const int64_t most = (int64_t)group * std::max(1, rows->max_rows);
-    if (pool.hd <= 128 && most >= kTileWeightRows) return launch_kv4_weights_tiles(pool, seqs, a, s);
+    if (tiles_pay(pool, seqs, typ, most)) return launch_kv4_weights_tiles(pool, seqs, a, s);
     if (pool.hd <= 64) return weights_of<64>(pool, seqs, a, most, s);
     if (pool.hd <= 128) return weights_of<128>(pool, seqs, a, most, s);
     return weights_of<256>(pool, seqs, a, most, s);
