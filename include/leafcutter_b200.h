@@ -233,7 +233,7 @@ int32_t lc_rope_turns_scaled(double theta, int32_t rot_dim, int32_t kind, double
                              double* magnitude);
 /* Rows turned by their positions: of each head the first rot_dim dims, pair p by positions_dev[row] * turns_dev[p] (which wraps around), times magnitude; the other dims are copied.
  * inverse != 0: the other way round, which is also the gradient's way.  x is [n_rows][x_heads][head_dim], y (NULL: none) [n_rows][y_heads][head_dim] with the same positions; the outputs may be the
- * inputs themselves (with their strides) and must not overlap them otherwise.  head_dim: 1 to 1024.  Results are within 2^-23 of the turned value (before typ's rounding).  n_rows: 2^24 at most. */
+ * inputs themselves (with their strides) and must not overlap them otherwise.  head_dim: 1 to 1024.  Results are within 2^-22 of the turned value (f32) or of the pair's length (16-bit types, before their rounding).  n_rows: 2^24 at most. */
 int32_t lc_rope_dev(uint32_t typ, int32_t n_rows, const int64_t* positions_dev, const uint64_t* turns_dev, int32_t rot_dim, int32_t head_dim,
                     int32_t layout, int32_t inverse, double magnitude, const void* x_dev, int64_t x_stride, void* x_out_dev, int64_t x_out_stride,
                     int32_t x_heads, const void* y_dev, int64_t y_stride, void* y_out_dev, int64_t y_out_stride, int32_t y_heads, void* stream);
@@ -248,7 +248,7 @@ int32_t lc_kv4_append_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, ui
 int32_t lc_kv4_read_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, void* k_out_dev, int64_t k_stride,
                         void* v_out_dev, int64_t v_stride, void* stream);
 /* Attention as lc_attention_kv8_dev, each row over the slots up to its own.  lse_dev (may be NULL), f32 [n_rows][n_heads], lse_stride between rows, receives
- * ln sum exp of a row's scores.  Queries of 16-bit types are exact down to 2^-24 of their row's largest element, f32 ones have 22 bits; weights 11 bits (f32: 22) or 2^-35 of the row's largest; sums in f32. */
+ * ln sum exp of a row's scores.  Queries of 16-bit types are exact down to 2^-24 of their row's largest element, f32 ones have 22 bits; weights 11 bits (f32: 22) or 2^-31 of the row's largest; sums in f32. */
 int32_t lc_attention_kv4_workspace(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, int32_t n_heads, size_t* out_bytes);
 int32_t lc_attention_kv4_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, const void* q_dev, int64_t q_stride,
                              int32_t n_heads, float scale, int32_t window, void* out_dev, int64_t out_stride, float* lse_dev, int64_t lse_stride,
@@ -256,14 +256,15 @@ int32_t lc_attention_kv4_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows,
 /* Adds to mass_dev[i * mass_stride + h * mass_head_stride + slot] what weight the rows of sequence i gave the cached key of kv head h in `slot`: the sum over the rows and the heads of the
  * group of exp(q . k * scale - lse), with the lse that attention over the same rows gave (rows whose lse is not finite add nothing).  A sequence with more slots than `capacity`, which
  * is no more than either stride, is left out and raises the status, and so do sequences that leave their table; keys on bad pages are left out.  Sums are in f32, in an order that depends on the arguments and lengths
- * alone.  Sequences never share sums, whatever pages they share; sequences that share rows all count them. */
+ * alone.  Sequences never share sums, whatever pages they share; sequences that share rows all count them.  Refused where the work, every context as long as its table, could not be counted in 31 bits:
+ * (n_rows * heads per kv head / 8 + n_seqs) * n_kv_heads * (positions of a table / 16 + 6). */
 int32_t lc_kv4_weights_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, const void* q_dev, int64_t q_stride,
                            int32_t n_heads, float scale, int32_t window, const float* lse_dev, int64_t lse_stride, float* mass_dev,
                            int64_t mass_stride, int64_t mass_head_stride, int32_t capacity, void* stream);
 /* Cuts sequences whose length (context and rows) is above `limit` to `keep` rows: for each kv head by itself the `first` first and `recent` last rows and, of those between, the ones with the
  * largest mass (equal ones by the lower slot; NaN counts as the smallest).  They move to the front of the sequence's pages in their order, their sums in mass_dev with them; sums behind them become 0.  kept_dev
  * [n_seqs][n_kv_heads][limit] receives the slots that they came from, -1 behind them, and ctx_out_dev [n_seqs] the new lengths (shorter sequences: as they are).
- * first + recent <= keep <= limit <= capacity, keep > 0.  Pages of a sequence that is cut must be its own.  A sequence that leaves its table, has a bad page among those of its length or
+ * first + recent <= keep <= limit <= capacity, keep > 0; n_seqs * n_kv_heads up to 65535; ctx_out_dev is not the rows' ctx_dev.  Pages of a sequence that is cut must be its own.  A sequence that leaves its table, has a bad page among those of its length or
  * is longer than `capacity` raises the status and stays as it is, -1 in kept_dev. */
 int32_t lc_kv4_evict_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, float* mass_dev, int64_t mass_stride, int64_t mass_head_stride,
                          int32_t capacity, int32_t keep, int32_t limit, int32_t recent, int32_t first, int32_t* kept_dev, int32_t* ctx_out_dev,

@@ -98,7 +98,7 @@ template <typename T> __device__ __noinline__ Block4 quantised64(const T* x, int
         const double border = ((double)below + 0.5) * step;
         n = z > border ? below + 1.0f : z < border ? below : 2.0f * rintf(0.5f * (below + 0.5f));
     }
-    const int m = s > 0.0f && !isnan(y) ? (int)fminf(n, 7.0f) : 0;
+    const int m = step > 0.0 && !isnan(y) ? (int)fminf(n, 7.0f) : 0;
     uint32_t w = (uint32_t)(y < 0.0 ? 8 - m : 8 + m) << (4 * (lane & 7));
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
@@ -320,9 +320,8 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv4_append_kernel(Kv4Pool p
             }
         } else {
             const int items = hd - half;
-            const Divider by_items(items);
             for (int e = mine; e < heads * items; e += share) {
-                const int h = by_items(e);
+                const int h = e / items;
                 turn_item_plain(q_in + h * hd, q_out + h * hd, e - h * items, half, a.interleaved, turns, n8);
             }
         }

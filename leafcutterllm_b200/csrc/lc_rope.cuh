@@ -5,7 +5,7 @@
 namespace lc {
 
 #ifdef __CUDACC__
-// Quotients by a number that a kernel learns when it runs, for dividends below 2^32 over it.
+// Quotients by a number d that a kernel learns when it runs, for dividends below 2^32 / d (heads times pieces of 8 or 16 dims of a head: below 2^30).
 struct Divider {
     uint32_t d, m;
     __device__ __forceinline__ explicit Divider(int by) : d((uint32_t)max(by, 1)), m(0xffffffffu / d + 1) {}

@@ -92,9 +92,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(RopeArgs a) {
         }
     } else {
         const int items = a.hd - a.half;
-        const Divider by_items(items);
         for (int e = at; e < mine * items; e += share) {
-            const int h = by_items(e);
+            const int h = e / items;
             head_at(h0 + h, in, out);
             turn_item_plain(in, out, e - h * items, a.half, a.interleaved, row, n8);
         }

@@ -122,12 +122,12 @@ def score_bound(big, dim):
 def attention_bound(out, mass, big, keys, dim, dtype, split):
     """How far an output may be off.  A weight is off by a factor e^(+-d) for a score off by d, so an output by at most 2 d of its mass (the sum of
     weight times |value|), the denominator counted.  A weight is held in 22 bits (split), or rounded to f16: half a step, 2^-11.  In both forms nothing below f16's smallest step, 2^-24, is
-    held, half of which a weight may lose, where the row's largest is 2^10 or more: 2^-35 of it, times the values, for which 8 times the largest mass stands (a split form
+    held, half of which a weight may lose, where the row's largest is 2^6 or more (2^10 where few rows make a sequence): 2^-31 of it, times a value, for which the largest mass stands (a split form
     without this part asks for weights of 1e-39 beside one of 1).  Sums in f32 of steps and warps: 2^-20.  Then the output's own rounding, by way of f32."""
     d = score_bound(big, dim)
     weight = 2.0 ** -22 if split else 2.0 ** -11
     eps = 2 * (d[..., None] + weight) + 2.0 ** -20
-    low = 2.0 ** -34 * keys[:, None, None] * np.abs(mass).max(initial=1.0) * 8
+    low = 2.0 ** -31 * keys[:, None, None] * np.abs(mass).max(initial=1.0)
     return mass * eps + low + np.abs(out) * (EPS[dtype] + 2.0 ** -23) + TINY[dtype]
 
 

@@ -108,6 +108,17 @@ def test_captured_and_on_other_streams(gpu):
     assert (out == other).all() and (out[1:] != x[1:]).any()
 
 
+@pytest.mark.parametrize("heads,dim,rot", [(3001, 33, 18), (2500, 32, 16)])
+def test_many_heads(gpu, heads, dim, rot):
+    x = torch.randn(5, heads, dim, device="cuda")
+    turns, on_gpu = table(gpu, rot)
+    pos = torch.arange(5).cuda() * 1000
+    got = gpu.rope_dev(x, pos, on_gpu)
+    x64 = x.double().cpu().numpy()
+    want = plain.rotate(x64, turns, pos.tolist())
+    assert (np.abs(got.double().cpu().numpy() - want) <= bound(x64, want, "float32")).all()
+
+
 def test_refusals(gpu):
     x, pos = torch.randn(3, 2, 64, device="cuda"), torch.arange(3).cuda()
     _, on_gpu = table(gpu, 64)
