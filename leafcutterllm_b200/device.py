@@ -60,9 +60,12 @@ def _elsewhere(index, *tensors):
 
 def _rows(t, heads, dim, what):
     """Rows [n][heads][dim] whose heads and dims are contiguous: the distance between rows, in elements."""
-    shape, stride = t.shape, t.stride()
+    shape = t.shape
     if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
         raise ValueError(f"{what}: [rows, {heads if heads is not None else 'heads'}, {dim}] expected, got {list(shape)}")
+    if t.is_contiguous():
+        return shape[1] * dim
+    stride = t.stride()
     if shape[0] and (stride[2] != 1 or (shape[1] > 1 and stride[1] != dim)):
         raise ValueError(f"{what}: the heads of a row must be contiguous")
     return stride[0] if shape[0] > 1 else shape[1] * dim
@@ -208,18 +211,19 @@ _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "llama3": 4}
 
 
 def _layout(layout):
-    if layout not in _LAYOUTS:
+    number = _LAYOUTS.get(layout)
+    if number is None:
         raise ValueError(f"layout {layout!r}: one of {sorted(_LAYOUTS)}")
-    return _LAYOUTS[layout]
+    return number
 
 
 def _turns(call, turns, index):
     """Pointer and rotated dims of a table on the GPU"""
-    if turns.element_size() != 8 or turns.is_floating_point() or turns.is_complex() or not turns.is_contiguous() or turns.dim() != 1:
+    if turns.element_size() != 8 or turns.is_floating_point() or turns.is_complex() or turns.dim() != 1 or not turns.is_contiguous():
         raise ValueError(f"{call}: turns are contiguous 64-bit integers")
     if turns.get_device() != index:
         _elsewhere(index, turns)
-    return turns.data_ptr(), 2 * turns.shape[0]
+    return turns.data_ptr(), 2 * turns.numel()
 
 
 def rope_turns_scaled(theta: float, rot_dim: int, scaling: str = "none", factor: float = 1.0, original: int = 0, fast: float = 0.0, slow: float = 0.0):
@@ -237,31 +241,31 @@ def rope_dev(x, positions, turns, layout: str = "half", magnitude: float = 1.0, 
     """Rows of heads x [rows, heads, dim] turned by their positions (int64 [rows]): of each head the first 2 * len(turns) dims, pairs (d, d + half of them) or, interleaved,
     (2 d, 2 d + 1), times `magnitude`; the others are copied.  inverse: the other way round, which is also the way of gradients.  y: a second tensor of the same
     rows.  Outputs that are None are made; they may be the inputs.  Returns out, or (out, y_out) where y is given."""
-    typ, index, n = _typ(x), x.get_device(), x.shape[0]
-    dim = x.shape[-1]
+    typ, index, shape, dtype = _typ(x), x.get_device(), x.shape, x.dtype
+    n, dim = shape[0], shape[-1]
     xs = _rows(x, None, dim, "x")
-    _contiguous("rope_dev", _torch().int64, positions)
-    if tuple(positions.shape) != (n,):
-        raise ValueError("rope_dev: one position per row expected")
-    tp, rot = _turns("rope_dev", turns, index)
+    heads = shape[1]
     if out is None:
-        out = _empty("rope_dev", x, x.shape, x.dtype, stream)
+        out = _empty("rope_dev", x, shape, dtype, stream)
+    if positions.dtype != _torch().int64 or positions.dim() != 1 or positions.shape[0] != n or not positions.is_contiguous():
+        raise ValueError("rope_dev: one position per row expected, contiguous int64")
+    tp, rot = _turns("rope_dev", turns, index)
     yp = ys = op = os = yh = 0
     if y is not None:
         if y_out is None:
             y_out = _empty("rope_dev", y, y.shape, y.dtype, stream)
-        yh = y.shape[1]
-        if y.dtype != x.dtype or y_out.dtype != x.dtype or y.shape[0] != n or y_out.shape[0] != n:
+        ys, yh = _rows(y, None, dim, "y"), y.shape[1]
+        os = _rows(y_out, yh, dim, "y_out")
+        if y.dtype != dtype or y_out.dtype != dtype or y.shape[0] != n or y_out.shape[0] != n:
             raise ValueError("rope_dev: y of x's type and as many rows expected, y_out like y")
-        ys, os = _rows(y, None, dim, "y"), _rows(y_out, yh, dim, "y_out")
         yp, op = y.data_ptr(), y_out.data_ptr()
         if y.get_device() != index or y_out.get_device() != index:
             _elsewhere(index, y, y_out)
-    if out.dtype != x.dtype or out.shape[0] != n:
+    if out.dtype != dtype or out.shape[0] != n:
         raise ValueError("rope_dev: out like x expected")
     if positions.get_device() != index or out.get_device() != index:
         _elsewhere(index, positions, out)
-    check(load().lc_rope_dev(typ, n, positions.data_ptr(), tp, rot, dim, _layout(layout), bool(inverse), magnitude, x.data_ptr(), xs, out.data_ptr(), _rows(out, x.shape[1], dim, "out"), x.shape[1],
+    check(load().lc_rope_dev(typ, n, positions.data_ptr(), tp, rot, dim, _layout(layout), 1 if inverse else 0, magnitude, x.data_ptr(), xs, out.data_ptr(), _rows(out, heads, dim, "out"), heads,
                              yp, ys, op, os, yh, _stream(index, stream)))
     return out if y is None else (out, y_out)
 
