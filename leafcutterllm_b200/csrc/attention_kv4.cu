@@ -111,8 +111,8 @@ kv4_runs_kernel(Kv4Pool pool, Kv8Seqs seqs, AttnArgs a) {
                     top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     float down;
                     row_scale(top, up[x], down);
-                    // not finite: the row is NaN.  A factor of 0 as 2^-100, so that a masked score of minus infinity stays one
-                    rf[gr] = top < INFINITY ? max_nan(a.scale_log2 * down * head, 0x1p-100f) : __int_as_float(0x7fffffff);
+                    // not finite: the row is NaN
+                    rf[gr] = top < INFINITY ? score_factor(a.scale_log2, down, head) : __int_as_float(0x7fffffff);
                 }
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {

@@ -371,8 +371,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
         const uint32_t my_s = col_s[t] + lanes, my_o = col_o[t] + lanes;
         const int limit = w.ctx + (row_lo + min(r, row_n - 1)) / a.group;      // last slot that the row sees
         const int least = __shfl_sync(0xffffffffu, limit, 0), most = __shfl_sync(0xffffffffu, limit, 31);
-        // A factor of 0 as 2^-100, so that a masked score of minus infinity stays one.  NaN for a row that is not finite, whose scores may all be minus infinity, as masked ones are.
-        const float f = sh.down[r] == 255 ? __int_as_float(0x7fffffff) : max_nan(a.scale_log2 * __uint_as_float((uint32_t)sh.down[r] << 23) * (kUnit4 * pool.k_scale[kvh]), 0x1p-100f);
+        // NaN for a row that is not finite, whose scores may all be minus infinity, as masked ones are
+        const float f = sh.down[r] == 255 ? __int_as_float(0x7fffffff) : score_factor(a.scale_log2, __uint_as_float((uint32_t)sh.down[r] << 23), kUnit4 * pool.k_scale[kvh]);
         float o[HD], m = kNegInf, l = 0.0f, corr = 1.0f;
         bool ok = true, far = false;
         // Far from 0 a reference has no bits left for what is added to it, and a product that is rounded with it may be off by more than f16's range

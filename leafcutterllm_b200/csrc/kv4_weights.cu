@@ -145,7 +145,7 @@ kv4_weights_kernel(Kv4Pool pool, Kv8Seqs seqs, WeightArgs a) {
                 top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 row_scale(top, up, down);
-                const float rf = a.scale_log2 * down * head;
+                const float rf = score_factor(a.scale_log2, down, head);
                 const int rl = has && fabsf(lse) < INFINITY && top < INFINITY ? w.ctx + tok : -1;
 #pragma unroll
                 for (int x = 0; x < 2; x++) {

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 4 ? 1 : 2) kv4_we
                     float up = 1.0f, down = 1.0f;
                     if (!std::is_same<T, __half>::value) row_scale(top, up, down);
                     if (ch == 0) {
-                        if (finite) k[0] = a.scale_log2 * down * head;
+                        if (finite) k[0] = score_factor(a.scale_log2, down, head);
                         else { sh.limit[turn][r] = -1; k[2] = kNegInf; }   // a row that is not finite adds nothing either
                     }
                     uint32_t w[8];
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kWeightThreads, sizeof(T) == 4 ? 1 : 2) kv4_we
                     float up, down;
                     row_scale(top, up, down);
                     if (ch == 0) {
-                        if (finite) k[0] = a.scale_log2 * down * head;
+                        if (finite) k[0] = score_factor(a.scale_log2, down, head);
                         else { sh.limit[turn][r] = -1; k[2] = kNegInf; }
                     }
                     uint32_t hi[8], lo[8];

@@ -23,6 +23,12 @@ int32_t launch_kv4_tiles(const Kv4Pool& pool, const Kv8Seqs& seqs, const AttnArg
 constexpr float kUnit4 = 8.0f;  // what the f16 values below are to be multiplied by
 
 #ifdef __CUDACC__
+// What a row's scores are multiplied by: the scale times log2 e, what undoes the row's power of two, the head's scale.  0 as 2^-100, so that a masked score of minus infinity stays one; beyond f32, where a
+// row of zeros has no power of two that brings it back, as f32's largest: its scores stay 0.
+__device__ __forceinline__ float score_factor(float scale_log2, float down, float head) {
+    const float f = max_nan(scale_log2 * down * head, 0x1p-100f);
+    return f == INFINITY ? 0x1.fffffep127f : f;
+}
 __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);

@@ -181,3 +181,26 @@ def test_a_smaller_workspace_is_refused(gpu):
         s.cache.weights(s.batch, q, torch.empty(1, 4, device="cuda"), torch.zeros(1, 3, 200, device="cuda"))
     with pytest.raises(ValueError):
         s.cache.weights(s.batch, q, torch.empty(1, 4, device="cuda"), torch.zeros(1, 2, 400, device="cuda")[..., ::2])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("seqs", [[(300, 1), (40, 1)], [(30, 21)], [(200, 160)]], ids=["few", "some", "many"])
+def test_rows_of_zeros_beside_queries_that_only_a_large_scale_brings_back(gpu, seqs, dtype):
+    """A scale of 2^126 for queries of 2^-130: a row of zeros, and the rows that fill up a tile, have scores of 0 all the same."""
+    s = Setup(gpu, seqs, 1, 128, 16, seed=4)
+    s.pools[4].fill_(1.0)
+    s.plain.k_scale[:] = 1.0
+    q = s.normal(4, "float32")[0].mul_(2.0 ** -130).to(DT[dtype])
+    q[:, 2] = 0.0
+    q64 = q.double().cpu().numpy()
+    out, lse = torch.empty_like(q), torch.empty(s.rows, 4, device="cuda")
+    s.cache.attention(s.batch, q, out, lse=lse, scale=2.0 ** 126)
+    weights = check_attention(s, out, lse, q64, dtype, 2.0 ** 126)
+    _, wlse, _, big, _, _ = s.plain.attention(s.table, s.ctx, s.start, q64, 2.0 ** 126)
+    mass = torch.zeros(len(seqs), 1, s.table.shape[1] * s.page, device="cuda")
+    s.cache.weights(s.batch, q, cuda(wlse.astype(np.float32)), mass, scale=2.0 ** 126)
+    want = np.zeros(mass.shape)
+    for i, r, h, lo, p in weights:
+        want[i, 0, lo:lo + len(p)] += p
+    bound = mass_bound(want, weights, plain.score_bound(big, s.dim), 4, want.shape, np.abs(wlse) * 2.0 ** -23)
+    assert (np.abs(host(mass) - want) <= bound).all()
