@@ -8,6 +8,10 @@
 //   Values  are the operand of 16 rows (dims), weights that of 8 columns (rows of queries), which the scores' layout already is.  Weights are 2^(s - max + 10) in f16; f32: and what that rounding lost, in a second
 //           product, a step's sums added in f32, so that what the matrix unit cuts off when it adds stays within 16 keys.
 // Dims of a score and keys of a sum may stand in any order, so a thread takes neighbouring dims of its key, whose scale they share, and two keys' dims become pairs by one byte permutation for eight of them.
+//
+// 64 sequences of 128 to 4,096 slots, 32 heads over 8 of 128 in bf16: 41 us with the join, 87 MB (a floor of 13).  What bounds it are instructions: 400 a step of 16 keys, of which the matrix unit's are 16; 60 % of the
+// issue slots at 16 warps an SM (128 registers), the rest is the beginning and the end of runs of 16 steps.  Three blocks an SM: 39.1 us without the join, four 39.7, five, whose registers spill, 45.  Two sequences of 60,001 and
+// 131,000 slots, four tokens, 64 heads over 8 in f16: 125 us with the join, 220 MB (34): 32 rows share a step's unpacking, and 8 warps of 235 registers wait for one another's results (two groups of rows instead of four: 172).
 #include <algorithm>
 #include "lc_kernels.h"
 #include "lc_kv4.cuh"
@@ -368,7 +372,7 @@ kv4_runs_kernel(Kv4Pool pool, Kv8Seqs seqs, AttnArgs a) {
 }
 
 // Joins the partial results of units that lie in several runs.  A run's record says which unit begins in it; a block looks through those of kJoinRuns runs, a slice of kJoinRows
-// rows of each.  Threads have four dims of a row each, and shares of the partial results.  (A block per run and four rows: 9.5 us instead of 4 after 64 sequences, 37 instead of 8 after two of 131,000 keys.)
+// rows of each.  Threads have four dims of a row each, and shares of the partial results.  (A block per run and four rows: 12 us more after two sequences of 131,000 keys, 137 instead of 125 with the runs.)
 constexpr int kJoinThreads = 256, kJoinRuns = 8, kJoinRows = 2;
 template <int HD, int RB>
 __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(AttnArgs a, int hd, int runs) {

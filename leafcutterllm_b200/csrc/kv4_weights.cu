@@ -3,6 +3,9 @@
 // By runs, as attention of few rows: the steps of 16 keys of all sequences and kv heads stand in one line, which is cut into equal runs, one per warp.  A step's keys are the operand of 16 rows and
 // queries, 8 at a time, that of 8 columns (mma.sync m16n8k16 in f16, as there); a key's sum over the rows then lies in four threads of a row of the result.  The warp goes over
 // its steps once for every block of 8 NG rows and adds to the sums itself, so that every sum is added to by one warp, in the order of the rows.
+//
+// 64 sequences of 128 to 4,096 slots, one row of 32 heads over 8 of 128 in bf16: 22.6 us, 48 MB (a floor of 7.3).  What bounds it are instructions, 270 to 400 a step of 16 keys: 60 % of the issue slots at 20 warps an SM.  A first,
+// simple kernel: 86.
 #include <algorithm>
 #include "lc_kernels.h"
 #include "lc_kv4.cuh"
