@@ -85,8 +85,8 @@ __device__ __forceinline__ bool begins_cut(const Kv4Pool& pool, const Kv8Seqs& s
     return cut;
 }
 
-// What a thread of a block of T has before it, of all threads' v; `totals`: of the warps, for this call alone.
-template <int T> __device__ __forceinline__ int before_thread(int v, int* totals) {
+// What a thread of the block's first eight warps has before it, of their v; `totals`: of these warps, for this call alone.
+__device__ __forceinline__ int before_thread(int v, int* totals) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int incl = v;
 #pragma unroll
@@ -94,24 +94,18 @@ template <int T> __device__ __forceinline__ int before_thread(int v, int* totals
         const int u = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += u;
     }
-    if (lane == 31) totals[warp] = incl;
+    if (lane == 31 && warp < 8) totals[warp] = incl;
     __syncthreads();
-    int off = incl - v;
-#pragma unroll
-    for (int w = 0; w < T / 32; w += 4) {
-        const int4 u = *reinterpret_cast<const int4*>(totals + w);
-        off += (w < warp ? u.x : 0) + (w + 1 < warp ? u.y : 0) + (w + 2 < warp ? u.z : 0) + (w + 3 < warp ? u.w : 0);
-    }
-    return off;
+    return incl - v + __reduce_add_sync(0xffffffffu, lane < min(warp, 8) ? totals[lane] : 0);
 }
 // grid: (cluster, sequences * kv heads); `per`: slots of a block, a multiple of 128
 template <int T>
-__global__ void __launch_bounds__(T) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seqs, EvictArgs a, int per) {
-    constexpr int W = T / 32, PLACES = 2048 / T;
+__global__ void __launch_bounds__(T, T == 512 ? 4 : 1) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seqs, EvictArgs a, int per) {
+    constexpr int W = T / 32, AT_ONCE = T == 512 ? 2 : kMostCluster;   // AT_ONCE: blocks whose counts are read together; four blocks of 512 on an SM have 32 registers a thread
     extern __shared__ __align__(16) uint32_t key[];              // [per], sums as whole numbers of their order
     uint16_t* const list = reinterpret_cast<uint16_t*>(key + per);   // [per], the block's slots that stay
     __shared__ __align__(16) uint32_t hist[3][1024];             // counts of 16 bits, two in a word: a block has fewer sums than that
-    __shared__ __align__(16) int totals[3][W];
+    __shared__ int totals[3][8];
     __shared__ int flag, chosen[3][2];
     __shared__ int2 warp_counts[W], block_counts;
     cg::cluster_group cluster = cg::this_cluster();
@@ -123,9 +117,16 @@ __global__ void __launch_bounds__(T) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seq
     {
         // the sums set out while the pages are looked at: of a length that may turn out to be none
         const int maybe = min(max(seqs.ctx[i] + seqs.row_start[i + 1] - seqs.row_start[i], 0), a.capacity), mine = max(0, min(per, maybe - base));
-        if (maybe > a.limit)
-#pragma unroll 8
-            for (int x = tid; x < ((mine + 3) & ~3); x += T) key[x] = x < mine ? ordered(mass[base + x]) : 0;
+        if (maybe > a.limit) {
+            const int quads = (uintptr_t)mass % 16 == 0 ? mine >> 2 : 0;
+#pragma unroll 4
+            for (int q = tid; q < quads; q += T) {
+                const float4 v = reinterpret_cast<const float4*>(mass + base)[q];
+                reinterpret_cast<uint4*>(key)[q] = make_uint4(ordered(v.x), ordered(v.y), ordered(v.z), ordered(v.w));
+            }
+#pragma unroll 4
+            for (int x = 4 * quads + tid; x < ((mine + 3) & ~3); x += T) key[x] = x < mine ? ordered(mass[base + x]) : 0;
+        }
     }
     for (int x = tid; x < 3 * 256; x += T) reinterpret_cast<int4*>(&hist[0][0])[x] = make_int4(0, 0, 0, 0);
     const int length = evict_length(seqs, pool, i, a.capacity, &flag);
@@ -164,26 +165,30 @@ __global__ void __launch_bounds__(T) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seq
                 if (x >= in0 && x < in1) count(key[x]);
             }
             cluster.sync();
-            // counts from the top: a thread has some places in a row, of all blocks at once
-            int c[PLACES];
+            // counts from the top, of all blocks at once: a thread of the first eight warps has eight places in a row
+            int c[8] = {}, all = 0;
+            if (tid < 256) {
+                for (int r0 = 0; r0 < size; r0 += AT_ONCE) {
+                    uint4 part[AT_ONCE];
 #pragma unroll
-            for (int k = 0; k < PLACES; k += 2) {
-                uint32_t part[kMostCluster];
+                    for (int r = 0; r < AT_ONCE; r++)
+                        part[r] = r0 + r < size ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&hist[d][1020 - 4 * tid], r0 + r)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                for (int r = 0; r < kMostCluster; r++) part[r] = r < size ? *cluster.map_shared_rank(&hist[d][1023 - (PLACES / 2) * tid - k / 2], r) : 0;
-                c[k] = c[k + 1] = 0;
+                    for (int r = 0; r < AT_ONCE; r++) {
+                        c[0] += part[r].w >> 16; c[1] += part[r].w & 0xffff; c[2] += part[r].z >> 16; c[3] += part[r].z & 0xffff;
+                        c[4] += part[r].y >> 16; c[5] += part[r].y & 0xffff; c[6] += part[r].x >> 16; c[7] += part[r].x & 0xffff;
+                    }
+                }
 #pragma unroll
-                for (int r = 0; r < kMostCluster; r++) { c[k] += part[r] >> 16; c[k + 1] += part[r] & 0xffff; }
+                for (int k = 0; k < 8; k++) all += c[k];
             }
-            int all = 0;
+            int before = before_thread(all, totals[d]);
+            if (tid < 256 && before < left && before + all >= left)
 #pragma unroll
-            for (int k = 0; k < PLACES; k++) all += c[k];
-            int before = before_thread<T>(all, totals[d]);
-#pragma unroll
-            for (int k = 0; k < PLACES; k++) {
-                if (before < left && before + c[k] >= left) { chosen[d][0] = 2047 - PLACES * tid - k; chosen[d][1] = left - before; }
-                before += c[k];
-            }
+                for (int k = 0; k < 8; k++) {
+                    if (before < left && before + c[k] >= left) { chosen[d][0] = 2047 - 8 * tid - k; chosen[d][1] = left - before; }
+                    before += c[k];
+                }
             __syncthreads();
             value |= (uint32_t)chosen[d][0] << shift;
             left = chosen[d][1];
@@ -191,7 +196,7 @@ __global__ void __launch_bounds__(T) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seq
     } else {
         __syncthreads();
     }
-    // Slots in ascending order: all above the value, and the first `left` equal to it.  A warp counts those of its stretch, four in a row a lane, then knows what is before it and goes over it again.
+    // Slots in ascending order: all above the value, and the first `left` equal to it.  A warp counts those of its stretch, four in a row a lane, then knows what is before it.
     const int stretch = ((quads + W - 1) / W + 31) & ~31, q0 = min(warp * stretch, quads), q1 = min(q0 + stretch, quads);
     // bits 0-3: of a lane's four those above, 4-7: those equal
     auto kinds = [&](int q) {
@@ -213,8 +218,10 @@ __global__ void __launch_bounds__(T) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seq
         return bits;
     };
     int n_both = 0;                                              // above, and in the upper half equal: 16 bits are enough for a block's
-    for (int q = q0; q < q1; q += 32) {
+    uint64_t kept_kinds = 0;                                     // a byte for each of the stretch's eight rounds at most (a block's slots are 32,384 at most)
+    for (int q = q0, at = 0; q < q1; q += 32, at += 8) {
         const uint32_t b = kinds(q);
+        kept_kinds |= (uint64_t)b << at;
         n_both += __popc(b & 15u) + (__popc(b & 240u) << 16);
     }
     const int2 mc = make_int2(__reduce_add_sync(0xffffffffu, n_both & 0xffff), __reduce_add_sync(0xffffffffu, n_both >> 16));
@@ -233,25 +240,33 @@ __global__ void __launch_bounds__(T) kv4_select_kernel(Kv4Pool pool, Kv8Seqs seq
     int above = b_above + __reduce_add_sync(0xffffffffu, mine_before.x), equals = b_equal + __reduce_add_sync(0xffffffffu, mine_before.y);
     // of the equal ones the first `left` stay: out = above + min(equals, left)
     const int begin = b_above + min(b_equal, left);              // of the block
-    for (int q = q0; q < q1; q += 32) {
-        const uint32_t b = kinds(q);
-        const int n = __popc(b & 15u) + (__popc(b & 240u) << 16);
-        int incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += u;
-        }
-        const int before = incl - n, total = __shfl_sync(0xffffffffu, incl, 31);
-        int e_before = equals + (before >> 16), to = above + (before & 0xffff) + min(e_before, left) - begin;
+    auto put = [&](int q, uint32_t b, int to, int e_before) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const bool eq = b >> (4 + e) & 1, stays = (b >> e & 1) || (eq && e_before < left);
             if (stays) list[to++] = (uint16_t)(4 * (q + lane) + e);
             e_before += eq;
         }
-        above += total & 0xffff;
-        equals += total >> 16;
+    };
+    for (int q = q0; q < q1; q += 64, kept_kinds >>= 16) {
+        // two rounds at once: four counts of 128 at most in a word
+        const uint32_t b0 = (uint32_t)kept_kinds & 255u, b1 = (uint32_t)kept_kinds >> 8 & 255u;
+        const uint32_t n = __popc(b0 & 15u) | __popc(b0 >> 4) << 8 | __popc(b1 & 15u) << 16 | __popc(b1 >> 4) << 24;
+        uint32_t incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t u = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += u;
+        }
+        const uint32_t before = incl - n, total = __shfl_sync(0xffffffffu, incl, 31);
+        int e_before = equals + (before >> 8 & 255u);
+        put(q, b0, above + (before & 255u) + min(e_before, left) - begin, e_before);
+        above += total & 255u;
+        equals += total >> 8 & 255u;
+        e_before = equals + (before >> 24);
+        put(q + 32, b1, above + (before >> 16 & 255u) + min(e_before, left) - begin, e_before);
+        above += total >> 16 & 255u;
+        equals += total >> 24;
     }
     if (warp == W - 1 && lane == 0) chosen[0][0] = above + min(equals, left) - begin;   // the last warp knows how many there are
     __syncthreads();
@@ -361,10 +376,7 @@ __device__ __forceinline__ void move_rows(const Kv4Pool& pool, const int32_t* ta
 #pragma unroll
         for (int u = 0; u < kMovePieces; u++)
             if (to[u]) *to[u] = v[u];
-        if (j0 + step * kMovePieces < keep) {
-            if (blocks == 1) __syncthreads();
-            else cluster.sync();
-        }
+        // nothing to wait for: the next stretch reads behind what this one writes, and writes when all have read it
     }
 }
 // grid: (cluster, sequences * kv heads, planes: keys, values, their scales)
