@@ -5,8 +5,8 @@
 // places, a cluster per sequence, kv head and plane (keys, values, their scales).  The row that goes to slot j comes from kept[j] >= j, so a stretch of rows is read as a whole, by all threads of the
 // cluster into registers, before it is written, in ascending order, and what a stretch writes is behind no row that a later one still reads.
 //
-// 64 sequences and 8 kv heads of 128 cut to 1,024 slots where they have more than 1,280: 31 us, 56 MB (a floor of 8.5); two of them cut to 16,384: 69 us, 85 MB (12.9).  What bounds it is a chain of waits: the sums, three rounds
-// of digits of 4,500 cycles in clusters of 8, the list, a launch, kept slot -> page -> row.  Of the second kernel's shapes four pieces a thread and three blocks on an SM are the best with L2 cold, 39 and 72 us (eight and
+// 64 sequences and 8 kv heads of 128 cut to 1,024 slots where they have more than 1,280: 27 us, 56 MB (a floor of 8.5); two of them cut to 16,384: 68 us, 85 MB (12.9).  What bounds it is a chain of waits: the sums, three rounds
+// of digits in clusters of 8 (a count of 1,700 to 3,200 cycles, a barrier, other blocks' counts, a scan), the list, a launch, kept slot -> page -> row.  Of the second kernel's shapes four pieces a thread and three blocks on an SM are the best with L2 cold, 39 and 72 us (eight and
 // two: 41 and 72; two and three: 43 and 78).  First kernels, a block for a sequence and head over sums in global memory: 80 and 612.
 #include <cooperative_groups.h>
 #include <algorithm>
@@ -354,28 +354,34 @@ __device__ __forceinline__ void move_rows(const Kv4Pool& pool, const int32_t* ta
     const int mine = threadIdx.x / pieces, piece = threadIdx.x - mine * pieces, step = blocks * rows;
     T* const from0 = reinterpret_cast<T*>(base) + piece;
     auto at = [&](int number, int slot) { return from0 + ((((size_t)(uint32_t)number * (uint32_t)pool.n_kv + h) << pool.page_shift) + (slot & mask)) * (uint32_t)pieces; };
-    for (int j0 = 0; j0 < keep; j0 += step * kMovePieces) {
-        const int j = j0 + (int)cluster.block_rank() * rows + mine;
-        // all loads of a kind go out together: rows that are not there, or in their place, read slot 0
-        T v[kMovePieces];
-        int from[kMovePieces], page[kMovePieces];
+    const int j_first = (int)cluster.block_rank() * rows + mine;
+    // what is not there reads the first slot's row
+    auto there = [&](int j) { return mine < rows && j < keep; };
+    int from[kMovePieces];
 #pragma unroll
-        for (int u = 0; u < kMovePieces; u++) from[u] = kept[mine < rows && j + u * step < keep ? j + u * step : 0];
+    for (int u = 0; u < kMovePieces; u++) from[u] = kept[there(j_first + u * step) ? j_first + u * step : 0];
+    for (int j0 = 0; j0 < keep; j0 += step * kMovePieces) {
+        const int j = j0 + j_first, next = j + step * kMovePieces;
+        // all loads of a kind go out together, the next stretch's first ones too
+        T v[kMovePieces];
+        int page[kMovePieces];
 #pragma unroll
         for (int u = 0; u < kMovePieces; u++) page[u] = table[from[u] >> pool.page_shift];
 #pragma unroll
         for (int u = 0; u < kMovePieces; u++) v[u] = *at(page[u], from[u]);
-        T* to[kMovePieces];
 #pragma unroll
         for (int u = 0; u < kMovePieces; u++) {
-            const bool moves = mine < rows && j + u * step < keep && from[u] != j + u * step;
-            to[u] = moves ? at(table[(j + u * step) >> pool.page_shift], j + u * step) : nullptr;
+            const int to = j + u * step;
+            page[u] = there(to) && from[u] != to ? table[to >> pool.page_shift] : -1;
         }
+        if (j0 + step * kMovePieces < keep)
+#pragma unroll
+            for (int u = 0; u < kMovePieces; u++) from[u] = kept[there(next + u * step) ? next + u * step : 0];
         if (blocks == 1) __syncthreads();
         else cluster.sync();
 #pragma unroll
         for (int u = 0; u < kMovePieces; u++)
-            if (to[u]) *to[u] = v[u];
+            if (page[u] >= 0) *at(page[u], j + u * step) = v[u];
         // nothing to wait for: the next stretch reads behind what this one writes, and writes when all have read it
     }
 }
