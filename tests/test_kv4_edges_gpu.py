@@ -204,3 +204,46 @@ def test_rows_of_zeros_beside_queries_that_only_a_large_scale_brings_back(gpu, s
         want[i, 0, lo:lo + len(p)] += p
     bound = mass_bound(want, weights, plain.score_bound(big, s.dim), 4, want.shape, np.abs(wlse) * 2.0 ** -23)
     assert (np.abs(host(mass) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("ties", ["none", "many", "odd"])
+@pytest.mark.parametrize("length,keep,off", [(259_065, 100_003, 0), (259_072, 17, 1), (70_001, 70_000, 0), (130_000, 64_999, 3)])
+def test_evict_of_as_long_contexts_as_clusters_hold(gpu, length, keep, off, ties):
+    """Blocks of up to 32,384 sums, at any alignment; shorter sequences in the same tables."""
+    page, pages = 16, -(-length // 16)
+    rng = np.random.default_rng(length)
+    table = rng.permutation(pages + 3000).astype(np.int32)[:pages]
+    tables = np.full((2, pages), -1, np.int32)
+    tables[0] = table
+    rest = np.setdiff1d(np.arange(pages + 3000), table)[:2000]
+    tables[1, :2000] = rest
+    lengths = [length, 31_990]
+    pools = [rng.integers(0, 256, (pages + 3000, 1, page, n)).astype(np.uint8) for n in (8, 8, 1, 1)]
+    on_gpu = [cuda(a) for a in pools]
+    cache = gpu.Kv4Cache(*on_gpu, torch.ones(1, device="cuda"), torch.ones(1, device="cuda"))
+    rows = gpu.Kv8Rows(cuda(tables), cuda(np.array(lengths, np.int32)), cuda(np.zeros(3, np.int32)), 0)
+    mass = rng.lognormal(0, 2, (2, 1, page * pages + 4)).astype(np.float32)
+    if ties == "many":
+        mass = np.floor(np.minimum(mass, 3.0))
+    elif ties == "odd":
+        mass = np.where(rng.random(mass.shape) < 0.3, rng.choice(np.array([np.nan, np.inf, -np.inf, 0.0, -0.0, -1.0, 1e-45], np.float32), mass.shape), mass).astype(np.float32)
+    whole = cuda(mass)
+    kept, ctx = cache.evict(rows, whole[:, :, off:off + page * pages], keep, recent=5, first=3)
+    want, pool_want = mass.copy(), [p.copy() for p in pools]
+    for i, n in enumerate(lengths):
+        m, got = mass[i, 0, off:off + n], kept[i, 0].cpu().numpy()
+        if n <= keep:
+            assert ctx[i].item() == n and (got[:n] == np.arange(n)).all() and (got[n:] == -1).all()
+            continue
+        inner = np.arange(3, n - 5)
+        nan = np.isnan(m[inner])
+        order = inner[np.lexsort((inner, -np.where(nan, 0.0, m[inner]), nan))][:keep - 8]   # NaN last, then the larger, then the lower slot
+        stays = np.sort(np.concatenate((np.arange(3), order, np.arange(n - 5, n))))
+        assert ctx[i].item() == keep and (got == stays).all()
+        want[i, 0, off:off + n] = 0.0
+        want[i, 0, off:off + keep] = m[stays]
+        for p, old in zip(pool_want, pools):
+            p[tables[i][np.arange(keep) // page], 0, np.arange(keep) % page] = old[tables[i][stays // page], 0, stays % page]
+    assert np.array_equal(host(whole), want, equal_nan=True)
+    for t, p in zip(on_gpu, pool_want):
+        assert (t.cpu().numpy() == p).all()
