@@ -245,7 +245,7 @@ kv4_runs_kernel(Kv4Pool pool, Kv8Seqs seqs, AttnArgs a) {
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) {
                 mx[gr] = __fmul_rn(fmaxf(mx[gr], __shfl_xor_sync(0xffffffffu, mx[gr], 2)), rf[gr]);
-                raise = raise || mx[gr] > m[gr] + 4.0f;
+                raise = raise || mx[gr] - m[gr] > 4.0f;   // the difference: far from 0, m + 4 may be rounded up to the next number, which mx may be
             }
             // the references are raised when a row's maximum has grown by more than 2^4; one vote for all groups, whose chains of instructions then run side by side
             if (__any_sync(0xffffffffu, raise)) {
