@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv4_tiles_kernel(Kv4Pool pool
                     for (int e = 0; e < kKeys; e++) tops[e & 3] = fmaxf(tops[e & 3], __uint_as_float(x[e]));
                     top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     const float mx = fmaxf(m, __fmul_rn(top, f));
-                    const bool raise = mx > m + 8.0f;  // also from minus infinity
+                    const bool raise = mx - m > 8.0f;  // also from minus infinity; the difference, because far from 0 m + 8 may be rounded up to the next number, which mx may be
                     if (__any_sync(0xffffffffu, raise)) {
                         const float by = raise ? exp2_fast(m - mx) : 1.0f;
                         if (raise) m = mx;
