@@ -248,6 +248,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
             m[gr] = kNegInf;
             l[gr] = 0.0f;
         }
+        bool far = false;                    // a row's reference is so far from 0 that it has no bits left for what is added to it
         float vref = 0.0f, vtop = 0.0f;      // 16-bit types: what the sums' scales are relative to; the largest that was
 
         // rows see all keys up to the first row's position (with a window, from the last row's on)
@@ -353,7 +354,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) {
                 mx[gr] = fmaxf(mx[gr], __shfl_xor_sync(0xffffffffu, mx[gr], 2));
-                raise = raise || mx[gr] > m[gr] + 4.0f;
+                raise = raise || mx[gr] - m[gr] > 4.0f;   // the difference: far from 0, m + 4 may be rounded up to the next number, which mx may be
             }
             // the references are raised when a row's maximum has grown by more than 2^4, so that a weight is 2^10 at most (with its scale 2^14); one vote for all
             // groups, whose chains of instructions then run side by side
@@ -363,10 +364,12 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                     const float top = fmaxf(mx[gr], m[gr]), corr = top == kNegInf ? 1.0f : exp2_fast(m[gr] - top);
                     l[gr] *= corr;
                     m[gr] = top;
+                    far = far || (fabsf(top) > 65536.0f && top != kNegInf);
                     const float c0 = __shfl_sync(0xffffffffu, corr, 8 * c), c1 = __shfl_sync(0xffffffffu, corr, 8 * c + 4);
 #pragma unroll
                     for (int t = 0; t < NT; t++) { o[gr][t][0] *= c0; o[gr][t][1] *= c1; o[gr][t][2] *= c0; o[gr][t][3] *= c1; }
                 }
+                far = __any_sync(0xffffffffu, far);
             }
             uint32_t ph[NG][2], pl[NG][2];   // weights, and what their rounding lost: keys 2c, 2c + 1 and 8 + 2c, 9 + 2c of row g
 #pragma unroll
@@ -374,7 +377,14 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 const float less = m[gr] == kNegInf ? 6.0f : 6.0f - m[gr];
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = exp2_fast(s[gr][e >> 1][e & 1] + less);
+                for (int e = 0; e < 4; e++) v[e] = s[gr][e >> 1][e & 1] + less;
+                if (far) {  // 6 - m may be 4 off there, and as much the other way for another m: the difference first, of rounded scores, as m is; it is exact near m
+                    const float ref = m[gr] == kNegInf ? 0.0f : m[gr];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = __fadd_rn(__fsub_rn(s[gr][e >> 1][e & 1], ref), 6.0f);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = exp2_fast(v[e]);
                 l[gr] += (v[0] + v[1]) + (v[2] + v[3]);
                 if (F32) {
                     h2_split(v[0], v[1], ph[gr][0], pl[gr][0]);
