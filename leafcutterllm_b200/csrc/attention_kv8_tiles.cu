@@ -499,7 +499,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         const GroupConst k = gc[c / 16];
                         mx = fmaxf(mx, exponent(g, factor(k.f), k.lv));
                     }
-                    const bool raise = mx > m + 8.0f;  // also from minus infinity
+                    // Also from minus infinity.  Far from 0 whenever it has grown: there steps of f32 hide S_v in m and in mx, and what a score is over m, up to 8 more, would go to a weight with it.
+                    const bool raise = mx - m > (far ? 0.0f : 8.0f);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float f = raise ? exp2_fast(m - mx) : 1.0f;
                         if (raise) m = mx;

@@ -58,3 +58,12 @@ def check(dtype, out, want):
 @pytest.mark.parametrize("kv,heads,dim,rows", [(2, 8, 64, 1), (2, 4, 128, 1), (2, 32, 128, 1), (2, 8, 64, 6), (2, 8, 128, 5), (2, 4, 256, 1), (2, 12, 256, 2), (2, 2, 80, 3)], ids=str)
 def test_neighbouring_scores_far_from_zero_in_runs(gpu, dtype, exponent, sign, louder, kv, heads, dim, rows):
     check(dtype, *neighbours(gpu, dtype, exponent, sign, kv, heads, dim, rows, 3, 20, louder))
+
+
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("exponent", [24, 25, 26, 27])
+@pytest.mark.parametrize("sign,louder", [(1, 1.0), (-1, 1.0), (1, 16.0), (-1, 0.125)], ids=["above", "below", "above loud", "below quiet"])
+@pytest.mark.parametrize("kv,heads,dim,rows", [(2, 4, 64, 70), (2, 8, 128, 40), (2, 2, 112, 300), (8, 16, 128, 150)], ids=str)
+@pytest.mark.parametrize("second", [20, 150])
+def test_neighbouring_scores_far_from_zero_in_tiles(gpu, dtype, exponent, sign, louder, kv, heads, dim, rows, second):
+    check(dtype, *neighbours(gpu, dtype, exponent, sign, kv, heads, dim, rows, 3, second, louder))
