@@ -177,7 +177,7 @@ typedef struct lc_kv8_rows {
  * own fills such a table itself.  Positions times entries wrap around, so far positions lose nothing. */
 int32_t lc_rope_turns(double theta, int32_t rot_dim, uint64_t* out);
 /* Appends rows of keys and values, each [n_rows][n_kv_heads][head_dim], at their positions, the keys rotated by turns_dev (rot_dim / 2
- * entries; rot_dim 0: no rotation).  Integers and scales are those of rotations and quotients in 64 bits; rotated queries are within 2^-23 of theirs, and rounded to typ.  Per page and head that receives rows: the scale becomes the largest finite
+ * entries; rot_dim 0: no rotation).  Integers and scales are those of rotations and quotients in 64 bits; rotated queries are within 2^-23 of theirs and 2^-45 of their pair's length, and rounded to typ.  Per page and head that receives rows: the scale becomes the largest finite
  * magnitude among the new rows / 127 (rounded to f32) or, where the page already holds rows of the sequence, the larger of that and the scale before; if it grows,
  * the integers of the earlier rows are rounded once more, to the new scale.  New integers are round(x / scale) to the nearest even, infinities
  * become +-127 and NaN 0 (all 0 where the scale is 0).  Slots behind the last row keep what they hold.
@@ -233,7 +233,8 @@ int32_t lc_rope_turns_scaled(double theta, int32_t rot_dim, int32_t kind, double
                              double* magnitude);
 /* Rows turned by their positions: of each head the first rot_dim dims, pair p by positions_dev[row] * turns_dev[p] (which wraps around), times magnitude; the other dims are copied.
  * inverse != 0: the other way round, which is also the gradient's way.  x is [n_rows][x_heads][head_dim], y (NULL: none) [n_rows][y_heads][head_dim] with the same positions; the outputs may be the
- * inputs themselves (with their strides) and must not overlap them otherwise.  head_dim: 1 to 1024.  Results are within 2^-22 of the turned value (f32) or of the pair's length (16-bit types, before their rounding).  n_rows: 2^24 at most. */
+ * inputs themselves (with their strides) and must not overlap them otherwise.  head_dim: 1 to 1024.  For pairs whose length times magnitude f32 holds, results are within 2^-22 of the turned value and
+ * 2^-45 of that length (f32: where the two products cancel, the second is the larger), or within 2^-22 of that length (16-bit types, before their rounding).  n_rows: 2^24 at most. */
 int32_t lc_rope_dev(uint32_t typ, int32_t n_rows, const int64_t* positions_dev, const uint64_t* turns_dev, int32_t rot_dim, int32_t head_dim,
                     int32_t layout, int32_t inverse, double magnitude, const void* x_dev, int64_t x_stride, void* x_out_dev, int64_t x_out_stride,
                     int32_t x_heads, const void* y_dev, int64_t y_stride, void* y_out_dev, int64_t y_out_stride, int32_t y_heads, void* stream);
