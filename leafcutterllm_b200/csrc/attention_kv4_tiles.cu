@@ -55,6 +55,9 @@ template <int HD, bool SPLIT> struct TileShape {
     static constexpr int kRawHalf = kKeys * HD / 2 + kKeys * HD / 16;  // integers and scales of a tile's keys or values
     static constexpr int kBytes = kQ + kVs * (kK + kV) + (kRawKs + kRawVs) * kRawHalf + 1024;
     static_assert(kBytes + 1024 <= 227 * 1024, "shared memory of a block");
+    // A slot of `outside` is written again when the values of the key tile before have been copied, whose place the unpacking of those kRawVs tiles earlier left; these wait for the sums of kVs tiles earlier,
+    // and sums for the softmax that has read its slot.
+    static_assert(kSlots >= 1 + kRawVs + kVs, "a slot that the softmax may still read");
 };
 
 template <int HD, bool SPLIT>

@@ -62,6 +62,9 @@ template <int HD, bool SPLIT> struct TileShape {
     static constexpr int kVs = SPLIT ? 1 : 2;                 // places for unpacked values: f32 queries leave room for one
     static constexpr int kRaw = kKeys * HD;                   // keys, values as they are in the cache
     static constexpr int kBytes = kQ + kK + kVs * kV + 2 * kRaw + 1024;
+    // A slot of `consts` is written again when the values of the key tile before have been copied (one place), whose place the unpacking of those one tile earlier left; these wait for the sums of kVs tiles
+    // earlier, and sums for the softmax that has read its slot.
+    static_assert(kSlots >= 1 + 1 + kVs, "a slot that the softmax may still read");
 };
 
 template <int HD, bool SPLIT>
