@@ -50,6 +50,7 @@ struct TileShared {
     uint2 sums[kTileThreads / 32];
     uint32_t tmem;
     float base;                                // what the values' scales of the unit are relative to
+    int8_t far_lv[kTileRows2];                 // of rows with a reference far from 0: the part of it that stands beside log2 S_v; of others 0
     uint8_t down[kTileRows2];                  // exponents of the factors that undo the rows' powers of two; 255: a row that is not finite
 };
 
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         fence_async();
         sh.base = 1.0f;
     }
+    if (tid < kTileRows2) sh.far_lv[tid] = 0;
     if (warp == 0) tmem_alloc(&sh.tmem, 512);
     tc_fence_before();
     __syncthreads();
@@ -399,9 +401,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
         // Far from 0 a reference has no bits left for what is added to it, and a product that is rounded with it may be off by more than f16's range
         // (scores of 1e8: 2^4).  There a score is rounded by itself, as the reference was, and what remains over it goes on; without loss in a neighbourhood of the reference.
         auto is_far = [](float mx) { return fabsf(mx) > 65536.0f && mx != kNegInf; };
-        auto over = [](float x, float f, float ref, float lv) {
-            const float y = __fsub_rn(__fmul_rn(x, f), ref);
-            return y > 9.0f - lv ? 9.0f - lv : y;  // 2^15 at most; NaN stays
+        auto over = [](float x, float f, float ref) { return __fsub_rn(__fmul_rn(x, f), ref); };
+        // There log2 S_v would vanish beside a score, too, so such a row's reference is a pair: m beside scores, and a whole number beside log2 S_v.  Of two pairs the heavier one, with room for what
+        // the whole number leaves.
+        auto heavier = [](float& m1, float& lv1, float score, float lv) {
+            if (score > kNegInf && (m1 == kNegInf || (score - m1) + (lv - lv1) > 1.0f)) {
+                m1 = score;
+                lv1 = fminf(fmaxf(rintf(lv), -127.0f), 127.0f);
+            }
         };
         auto add_up = [&](int i) {  // o = o corr + the key tile's sums
             ok = mbar_wait(&sh.o_full[t], i & 1) && ok;
@@ -451,11 +458,37 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                             mx = fmaxf(mx, exponent(g, factor(k.f), k.lv));
                         }
                     }
-                    const float ref = mx == kNegInf ? 0.0f : mx;
-                    far = is_far(mx);
-                    const bool any_far = __any_sync(0xffffffffu, far);
-                    const float less = far ? 6.0f : 6.0f - ref;
+                    const int was_lv = sh.far_lv[r];
+                    const bool far = is_far(mx), any_far = __any_sync(0xffffffffu, far || was_lv != 0);
+                    float ref = mx == kNegInf ? 0.0f : mx, less = 6.0f - ref;
                     corr = exp2_fast(m - ref);
+                    if (__builtin_expect(any_far, 0)) {
+                        const float lv0 = (float)was_lv;
+                        float m1 = m, lv1 = lv0;
+#pragma unroll 1
+                        for (int c = 0; c < kKeys; c += 16) {
+                            uint32_t x[16];
+                            tmem_ld16(my_s + c, x);
+                            tmem_wait_ld();
+                            const GroupConst k = gc[c / 16];
+                            float g = kNegInf;
+#pragma unroll
+                            for (int e = 0; e < 16; e++)
+                                if (c + e <= to && c + e >= from) g = fmaxf(g, __uint_as_float(x[e]));
+                            heavier(m1, lv1, __fmul_rn(g, factor(k.f)), k.lv);
+                        }
+                        if (far) {
+                            corr = exp2_fast((m - m1) + (lv0 - lv1));
+                            mx = ref = m1;
+                            less = 6.0f - lv1;
+                        } else {  // near again: one number
+                            if (lv0 != 0.0f) mx = ref = fmaxf(mx, m + lv0);
+                            corr = exp2_fast((m - ref) + lv0);
+                            less = 6.0f - ref;
+                            lv1 = 0.0f;
+                        }
+                        sh.far_lv[r] = (int8_t)lv1;
+                    }
                     m = mx;
                     // 16 keys' weights take the first 8 columns of their scores' 16, their low parts the other 8
 #pragma unroll 2
@@ -469,9 +502,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
 #pragma unroll
                             for (int e = 0; e < 16; e++)
                                 if (c + e > to || c + e < from) x[e] = __float_as_uint(kNegInf);
-                        if (any_far)
+                        if (__builtin_expect(any_far, 0))
 #pragma unroll
-                            for (int e = 0; e < 16; e++) x[e] = far ? __float_as_uint(over(__uint_as_float(x[e]), factor(k.f), ref, k.lv)) : x[e];
+                            for (int e = 0; e < 16; e++) x[e] = far ? __float_as_uint(over(__uint_as_float(x[e]), factor(k.f), ref)) : x[e];
                         const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
                         float2 gs = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -502,12 +535,34 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         const GroupConst k = gc[c / 16];
                         mx = fmaxf(mx, exponent(g, factor(k.f), k.lv));
                     }
-                    // Also from minus infinity.  Far from 0 whenever it has grown: there steps of f32 hide S_v in m and in mx, and what a score is over m, up to 8 more, would go to a weight with it.
-                    const bool raise = mx - m > (far ? 0.0f : 8.0f);
+                    float grown = mx - m;
+                    bool raise = grown > 8.0f;  // also from minus infinity
+                    if (__builtin_expect(__any_sync(0xffffffffu, far || is_far(mx)), 0)) {
+                        const float lv0 = (float)sh.far_lv[r];
+                        float m1 = fmaxf(mx, m + lv0), lv1 = 0.0f;  // near again: one number
+                        far = is_far(mx);
+                        if (far) {
+                            m1 = m;
+                            lv1 = lv0;
+#pragma unroll
+                            for (int c = 0; c < kKeys; c += 16) {
+                                float g = __uint_as_float(x[c]);
+#pragma unroll
+                                for (int e = 1; e < 16; e++) g = fmaxf(g, __uint_as_float(x[c + e]));
+                                const GroupConst k = gc[c / 16];
+                                heavier(m1, lv1, __fmul_rn(g, factor(k.f)), k.lv);
+                            }
+                        }
+                        if (far || lv0 != 0.0f) {
+                            raise = m1 != m || lv1 != lv0;
+                            grown = (m1 - m) + (lv1 - lv0);
+                            mx = m1;
+                            sh.far_lv[r] = (int8_t)lv1;
+                        }
+                    }
                     if (__any_sync(0xffffffffu, raise)) {
-                        const float f = raise ? exp2_fast(m - mx) : 1.0f;
+                        const float f = raise ? exp2_fast(-grown) : 1.0f;
                         if (raise) m = mx;
-                        far = is_far(m);
                         l *= f;
                         if (i > 0) {
                             ok = mbar_wait(&sh.o_full[t], (i - 1) & 1);
@@ -525,20 +580,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         }
                     }
                     const float ref = m == kNegInf ? 0.0f : m;
-                    const float less = far ? 6.0f : 6.0f - ref;
-                    if (__any_sync(0xffffffffu, far))
+                    float less = 6.0f - ref;
+                    if (__builtin_expect(__any_sync(0xffffffffu, far), 0)) {
+                        if (far) less = 6.0f - (float)sh.far_lv[r];
 #pragma unroll
                         for (int c = 0; c < kKeys; c += 16) {
                             const GroupConst k = gc[c / 16];
 #pragma unroll
-                            for (int e = 0; e < 16; e++) x[c + e] = far ? __float_as_uint(over(__uint_as_float(x[c + e]), factor(k.f), ref, k.lv)) : x[c + e];
+                            for (int e = 0; e < 16; e++) x[c + e] = far ? __float_as_uint(over(__uint_as_float(x[c + e]), factor(k.f), ref)) : x[c + e];
                         }
+                    }
 #pragma unroll
                     for (int c = 0; c < kKeys; c += 16) {
                         uint32_t p[8];
                         const GroupConst k = gc[c / 16];
-                        const float off = k.lv + less, f = far ? 1.0f : factor(k.f);
-                        const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
+                        const float off = k.lv + less, by = far ? 1.0f : factor(k.f);
+                        const float2 f2 = make_float2(by, by), off2 = make_float2(off, off);
                         float2 gs = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
@@ -575,13 +632,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_tiles_kernel(Kv8Pool pool
                         if (d < hd) store16(a.out, dst + d, a.typ, a.out_vec, v);
                     }
                 } else {
+                    const float up = exp2f((float)sh.far_lv[r]);  // parts are joined by their m alone
                     part[r] = m;
-                    part[kTileRows2 + r] = l;
+                    part[kTileRows2 + r] = l * up;
 #pragma unroll
                     for (int d = 0; d < HD; d += 16) {
                         float v[16];
 #pragma unroll
-                        for (int e = 0; e < 16; e++) v[e] = o[((d + e) >> 2) + ((d + e) & 3) * (HD / 4)] * base;
+                        for (int e = 0; e < 16; e++) v[e] = o[((d + e) >> 2) + ((d + e) & 3) * (HD / 4)] * base * up;
                         store16(part + 2 * kTileRows2 + (size_t)r * HD + d, true, v);
                     }
                 }

@@ -67,3 +67,90 @@ def test_neighbouring_scores_far_from_zero_in_runs(gpu, dtype, exponent, sign, l
 @pytest.mark.parametrize("second", [20, 150])
 def test_neighbouring_scores_far_from_zero_in_tiles(gpu, dtype, exponent, sign, louder, kv, heads, dim, rows, second):
     check(dtype, *neighbours(gpu, dtype, exponent, sign, kv, heads, dim, rows, 3, second, louder))
+
+
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("exponent", [10, 16, 22, 28, 30, 45])
+@pytest.mark.parametrize("kv,heads,dim,seqs", [(2, 8, 64, [(600, 40), (130, 70)]), (2, 2, 128, [(3000, 150)]), (8, 32, 48, [(200 + 7 * i, 32) for i in range(20)]), (2, 4, 64, [(600, 2)])], ids=["cut", "cut long", "whole", "few"])
+def test_equal_scores_far_from_zero_of_pages_of_other_scales(gpu, dtype, exponent, kv, heads, dim, seqs):
+    """Keys that are all the same, or the opposite: a row's output is the mean of the values of those that it likes, on pages whose scales are far apart."""
+    rng = np.random.default_rng(exponent)
+    s = Setup(gpu, seqs, kv, dim, 16, seed=dim)
+    p = s.plain
+    key = rng.integers(-127, 128, (kv, dim))
+    key[:, 0] = 127
+    p.k_scale[:] = 2.0 ** -7
+    p.v_scale[:] = np.exp2(rng.uniform(-8, 8, p.v_scale.shape)).astype(np.float32)
+    signs = []
+    for i, (c, n) in enumerate(seqs):
+        sign = np.where(rng.random((c + n, kv)) < 0.3, 1, -1)
+        sign[0] = 1
+        for slot in range(c + n):
+            p.k[s.table[i, slot // 16], :, slot % 16] = sign[slot][:, None] * key
+        signs.append(sign)
+    for t, a in zip(s.pools, (p.k, p.v, p.k_scale, p.v_scale)):
+        t.copy_(cuda(a))
+    # queries along the key or against it, each of its own size up to a factor of 4
+    q = np.sign(key).repeat(heads // kv, 0)[None] * np.abs(rng.normal(0, 1, (s.rows, heads, dim))) * np.exp2(rng.uniform(0, 2, (s.rows, heads, 1)))
+    q = torch.from_numpy((q * np.where(rng.random((s.rows, heads, 1)) < 0.8, 1, -1)).astype(np.float32)).to(DT[dtype])
+    q64 = q.double().numpy()
+    out = torch.empty_like(q, device="cuda")
+    s.cache.attention(s.batch, q.cuda(), out, scale=2.0 ** (exponent - 8))
+    got, clear, seen = host(out).astype(np.float64), 0, 0
+    for i, (c, n) in enumerate(seqs):
+        v = p.values("v", s.table[i], c + n)
+        for j in range(0, n, 1 + n // 16):
+            for h in range(heads):
+                g, r = h // (heads // kv), int(s.start[i]) + j
+                score = float(key[g] @ q64[r, h]) * 2.0 ** (exponent - 15)
+                seen += 1
+                mine = signs[i][:c + j + 1, g] * score > 0
+                if not mine.any():
+                    mine = ~mine
+                elif 2 * abs(score) < 200.0:
+                    continue                                    # the others would count as well
+                clear += 1
+                some = v[:c + j + 1, g][mine]
+                want, amp = some.mean(0), np.abs(some).mean(0)
+                # All weights are the same.  Each is off by its exponential, its scale's logarithm (2^-22 of up to 8) and its rounding to 11 bits (f32: 22), or by 2^-31 of the largest weight and scale;
+                # sums in f32, then the output's own rounding.  Near 0 (scores of up to 2^16 powers of two) log2 of a page's scale, 6 and the reference m are added up in f32 before the score is: two
+                # roundings of 2^-24 m each, which differ between pages, so a weight is off by ln 2 x 2^-23 m and an output, numerator and denominator, by twice that, 1.4 x 2^-23 m.
+                m = abs(score) * 1.4427
+                near = m * 2.0 ** -22 if m < 65600.0 else 0.0
+                bound = amp * (2.0 ** -18 + (dtype != "float32") * 2.0 ** -10 + near) + np.abs(v[:c + j + 1, g]).max() * 2.0 ** -31 + np.abs(want) * plain.EPS[dtype] / 2 + plain.TINY[dtype]
+                assert (np.abs(got[r, h] - want) <= bound).all(), (r, h, (np.abs(got[r, h] - want) / bound).max())
+    assert clear > seen / 2
+
+
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("exponent", [17, 20, 30])
+@pytest.mark.parametrize("kv,heads,seqs", [(2, 4, [(300, 300), (390, 150)]), (8, 32, [(380, 40)] * 20), (2, 4, [(420, 3), (390, 2)])], ids=["cut", "whole", "few"])
+def test_scores_that_come_near_and_go_far_again(gpu, dtype, exponent, kv, heads, seqs):
+    """Keys far below 0 in the first 256 slots, keys of 0 up to slot 400, keys far above 0 from there: a row's output is the mean of the last kind's values that it sees."""
+    dim = 64
+    rng = np.random.default_rng(exponent)
+    s = Setup(gpu, seqs, kv, dim, 16, seed=dim)
+    p = s.plain
+    key = rng.integers(-127, 128, (kv, dim))
+    key[:, 0] = 127
+    p.k_scale[:] = 2.0 ** -7
+    p.v_scale[:] = np.exp2(rng.uniform(-8, 8, p.v_scale.shape)).astype(np.float32)
+    for i, (c, n) in enumerate(seqs):
+        for slot in range(c + n):
+            p.k[s.table[i, slot // 16], :, slot % 16] = key * (-1 if slot < 256 else 0 if slot < 400 else 1)
+    for t, a in zip(s.pools, (p.k, p.v, p.k_scale, p.v_scale)):
+        t.copy_(cuda(a))
+    q = torch.from_numpy((np.sign(key).repeat(heads // kv, 0)[None] * np.abs(rng.normal(0, 1, (s.rows, heads, dim)))).astype(np.float32)).to(DT[dtype])
+    out = torch.empty_like(q, device="cuda")
+    s.cache.attention(s.batch, q.cuda(), out, scale=2.0 ** (exponent - 5))
+    got = host(out).astype(np.float64)
+    for i, (c, n) in enumerate(seqs):
+        v = p.values("v", s.table[i], c + n)
+        for j in range(0, n, 1 + n // 16):
+            for h in range(heads):
+                g, r, end = h // (heads // kv), int(s.start[i]) + j, c + j + 1
+                some = v[400 if end > 400 else 256:end, g]
+                want, amp = some.mean(0), np.abs(some).mean(0)
+                # as above, the weights that count have scores of 0 or far ones
+                bound = amp * (2.0 ** -18 + (dtype != "float32") * 2.0 ** -10) + np.abs(v[:end, g]).max() * 2.0 ** -31 + np.abs(want) * plain.EPS[dtype] / 2 + plain.TINY[dtype]
+                assert (np.abs(got[r, h] - want) <= bound).all(), (r, h, (np.abs(got[r, h] - want) / bound).max())
