@@ -155,7 +155,8 @@ kv4_runs_kernel(Kv4Pool pool, Kv8Seqs seqs, AttnArgs a) {
             l[gr] = 0.0f;
             off[gr] = kWeightUp;
         }
-        bool far = false;                    // a row's reference is so far from 0 that it has no bits left for what is added to it
+        auto is_far = [](float top) { return fabsf(top) > 65536.0f && top != kNegInf; };  // so far from 0 that a reference has no bits left for what is added to it
+        bool far = false;                    // some row of the warp's has such a reference
         // rows see all keys up to the first row's slot (with a window, from the last row's on)
         const int sees = w.ctx + row_lo / a.group, from = a.window > 0 ? w.ctx + (row_lo + row_n - 1) / a.group - a.window : -1;
         const int plain0 = from < 0 ? 0 : from / kStep + 1 - w.step0, plain1 = (sees + 1) / kStep - w.step0;   // steps whose keys all rows see
@@ -255,7 +256,7 @@ kv4_runs_kernel(Kv4Pool pool, Kv8Seqs seqs, AttnArgs a) {
                     l[gr] *= corr;
                     m[gr] = top;
                     off[gr] = top == kNegInf ? kWeightUp : kWeightUp - top;
-                    far = far || (fabsf(top) > 65536.0f && top != kNegInf);
+                    far = far || is_far(top);
                     const float c0 = __shfl_sync(0xffffffffu, corr, 8 * c), c1 = __shfl_sync(0xffffffffu, corr, 8 * c + 4);
 #pragma unroll
                     for (int t = 0; t < NT; t++) { o[gr][t][0] *= c0; o[gr][t][1] *= c1; o[gr][t][2] *= c0; o[gr][t][3] *= c1; }
@@ -268,10 +269,9 @@ kv4_runs_kernel(Kv4Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = fmaf(s[gr][e >> 1][e & 1], rf[gr], off[gr]);
-                if (far) {  // products rounded by themselves, as the reference is: their difference is exact near it
-                    const float ref = m[gr] == kNegInf ? 0.0f : m[gr];
+                if (far && is_far(m[gr])) {  // products rounded by themselves, as the reference is: their difference is exact near it
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = __fadd_rn(__fsub_rn(__fmul_rn(s[gr][e >> 1][e & 1], rf[gr]), ref), kWeightUp);
+                    for (int e = 0; e < 4; e++) v[e] = __fadd_rn(__fsub_rn(__fmul_rn(s[gr][e >> 1][e & 1], rf[gr]), m[gr]), kWeightUp);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = exp2_fast(v[e]);

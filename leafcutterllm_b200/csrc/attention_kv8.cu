@@ -248,7 +248,8 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
             m[gr] = kNegInf;
             l[gr] = 0.0f;
         }
-        bool far = false;                    // a row's reference is so far from 0 that it has no bits left for what is added to it
+        auto is_far = [](float top) { return fabsf(top) > 65536.0f && top != kNegInf; };  // so far from 0 that a reference has no bits left for what is added to it
+        bool far = false;                    // some row of the warp's has such a reference
         float vref = 0.0f, vtop = 0.0f;      // 16-bit types: what the sums' scales are relative to; the largest that was
 
         // rows see all keys up to the first row's position (with a window, from the last row's on)
@@ -364,7 +365,7 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                     const float top = fmaxf(mx[gr], m[gr]), corr = top == kNegInf ? 1.0f : exp2_fast(m[gr] - top);
                     l[gr] *= corr;
                     m[gr] = top;
-                    far = far || (fabsf(top) > 65536.0f && top != kNegInf);
+                    far = far || is_far(top);
                     const float c0 = __shfl_sync(0xffffffffu, corr, 8 * c), c1 = __shfl_sync(0xffffffffu, corr, 8 * c + 4);
 #pragma unroll
                     for (int t = 0; t < NT; t++) { o[gr][t][0] *= c0; o[gr][t][1] *= c1; o[gr][t][2] *= c0; o[gr][t][3] *= c1; }
@@ -378,10 +379,9 @@ kv8_runs_kernel(Kv8Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = s[gr][e >> 1][e & 1] + less;
-                if (far) {  // 6 - m may be 4 off there, and as much the other way for another m: the difference first, of rounded scores, as m is; it is exact near m
-                    const float ref = m[gr] == kNegInf ? 0.0f : m[gr];
+                if (far && is_far(m[gr])) {  // 6 - m may be 4 off there, and as much the other way for another m: the difference first, of rounded scores, as m is; it is exact near m
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = __fadd_rn(__fsub_rn(s[gr][e >> 1][e & 1], ref), 6.0f);
+                    for (int e = 0; e < 4; e++) v[e] = __fadd_rn(__fsub_rn(s[gr][e >> 1][e & 1], m[gr]), 6.0f);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = exp2_fast(v[e]);
