@@ -269,9 +269,10 @@ kv4_runs_kernel(Kv4Pool pool, Kv8Seqs seqs, AttnArgs a) {
                 float v[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = fmaf(s[gr][e >> 1][e & 1], rf[gr], off[gr]);
-                if (far && is_far(m[gr])) {  // products rounded by themselves, as the reference is: their difference is exact near it
+                if (far) {  // products rounded by themselves, as the reference is: their difference is exact near it
+                    const bool mine = is_far(m[gr]);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = __fadd_rn(__fsub_rn(__fmul_rn(s[gr][e >> 1][e & 1], rf[gr]), m[gr]), kWeightUp);
+                    for (int e = 0; e < 4; e++) v[e] = mine ? __fadd_rn(__fsub_rn(__fmul_rn(s[gr][e >> 1][e & 1], rf[gr]), m[gr]), kWeightUp) : v[e];
                 }
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = exp2_fast(v[e]);
