@@ -114,7 +114,7 @@ template <typename T> __device__ __noinline__ Block4 quantised64(const T* x, int
     return out;
 }
 // The same in f32, for numbers that are off by `off` at most: false where one, or their scale, lies too near a border, where one is not finite, and for sizes that f32's relative errors do not
-// hold for.  Numbers that are exact (off 0) often lie on borders, bf16 under a scale that is a power of two; these are compared in 64 bits.
+// hold for (0 is one that they do).  Numbers that are exact (off 0) often lie on borders, bf16 under a scale that is a power of two; these are compared in 64 bits.
 __device__ __forceinline__ bool quantised32(const float (&y)[16], float off, float g, Block4& out) {
     float most = 0.0f;
 #pragma unroll
@@ -157,9 +157,10 @@ __device__ __forceinline__ bool quantised32(const float (&y)[16], float off, flo
             w[e >> 3] = w[e >> 3] * 16u + __float_as_uint(to + 12582920.0f);
         }
     }
-    out.words = make_uint2(w[0] - kUpper, w[1] - kUpper);
-    out.scale = scale_byte(s);
-    return sure;
+    const bool zeros = most == 0.0f && off == 0.0f;   // nothing to decide: rows that fill up a batch, heads that are switched off
+    out.words = zeros ? make_uint2(0x88888888u, 0x88888888u) : make_uint2(w[0] - kUpper, w[1] - kUpper);
+    out.scale = zeros ? 0 : scale_byte(s);
+    return sure || zeros;
 }
 
 // Sixteen elements in a row as f32
