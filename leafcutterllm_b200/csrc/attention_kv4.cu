@@ -9,9 +9,13 @@
 //           product, a step's sums added in f32, so that what the matrix unit cuts off when it adds stays within 16 keys.
 // Dims of a score and keys of a sum may stand in any order, so a thread takes neighbouring dims of its key, whose scale they share, and two keys' dims become pairs by one byte permutation for eight of them.
 //
-// 64 sequences of 128 to 4,096 slots, 32 heads over 8 of 128 in bf16: 41 us with the join, 87 MB (a floor of 13).  What bounds it are instructions: 400 a step of 16 keys, of which the matrix unit's are 16; 60 % of the
-// issue slots at 16 warps an SM (128 registers), the rest is the beginning and the end of runs of 16 steps.  Three blocks an SM: 39.1 us without the join, four 39.7, five, whose registers spill, 45.  Two sequences of 60,001 and
-// 131,000 slots, four tokens, 64 heads over 8 in f16: 125 us with the join, 220 MB (34): 32 rows share a step's unpacking, and 8 warps of 235 registers wait for one another's results (two groups of rows instead of four: 172).
+// Why 11 bits are enough for 16-bit types' weights: each is off by up to 2^-11 of itself, either way, and an output is a mean over many keys.  Against 64 bits, and with weights of 32 bits: bf16 1.7e-3 and 1.7e-3,
+// f16 2.5e-4 and 2.0e-4, most of it the outputs' own rounding.  A second product for the low parts, as f32 has it, would double the products with the values.
+//
+// 64 sequences of 128 to 4,096 slots, 32 heads over 8 of 128 in bf16: 37 us with the join, 87 MB (a floor of 13).  What bounds it are instructions: 360 a step of 16 keys, of which the matrix unit's are 16; 50 % of the
+// issue slots at 12 warps an SM (153 registers), the rest is the beginning and the end of runs of 20 steps.  Three blocks an SM for up to 8 rows; four (128 registers) take longer, 38.5 us, 42.7 instead of 41.1 in f32, 98 instead of 94 with
+// 16 sequences of 8,000 to 32,000, and five spill.  Two sequences of 60,001 and 131,000 slots, four tokens, 64 heads over 8 in f16: 123 us with the join, 220 MB (34): 32 rows share a step's unpacking, and 8 warps of
+// 235 registers wait for one another's results (two groups of rows instead of four: 172).
 #include <algorithm>
 #include "lc_kernels.h"
 #include "lc_kv4.cuh"
@@ -31,7 +35,7 @@ template <int HD, int NG, bool F32> struct Run4Shape {
     static constexpr bool kQueriesShared = HD == 256 || kTiles > 1;       // operand fragments of the queries in shared memory, not in registers
     static constexpr int kQueries = kQueriesShared ? kTiles * (HD / 16) * 512 : 0;
     static constexpr int kWarp = kRing + kQueries;
-    static constexpr int kByRegisters = HD == 256 ? 2 : NG == 1 ? 4 : NG == 2 ? 3 : 2;
+    static constexpr int kByRegisters = HD == 256 ? 2 : NG <= 2 ? 3 : 2;   // with 8 rows four take 1 to 8 % longer, see above
     static constexpr int kByMemory = (220 << 10) / (kRunWarps * kWarp + 2048);
     static constexpr int kBlocks = kByRegisters < kByMemory ? kByRegisters : kByMemory;
 };
@@ -464,11 +468,15 @@ bool tiles_fit(const Kv4Pool& pool, const Kv8Seqs& seqs, int group) {
     TilePlan tiles;
     return line_fits(pool, seqs, group, kTileRows2) && kv8_tiles_plan(pool, seqs, group, &tiles);
 }
-// Whether tiles are faster than runs, us in runs / in tiles.  128 rows (tokens x heads of a group) of a sequence and kv head: bf16, 32 heads over 8 of 128, one sequence behind 4,000 tokens 30 / 31, 16 behind 2,000
-// 100 / 49, 64 behind 1,000 199 / 138; f32 138 / 77, 278 / 206; heads of 64, 64 sequences 84 / 51.  64 rows: 16-bit types where units are no more than SMs, one sequence 27 / 29 (32 kv heads 39 / 36), 16
-// 60 / 49, but 64 sequences 116 / 118, 16 of 32 kv heads 186 / 206; f32 158 / 172; heads of 64 29 / 41.  32 rows: 39 / 48.
-bool tiles_pay(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows, const TilePlan& plan) {
-    return (int64_t)group * max_rows >= (typ != LC_TYPE_F32 && pool.hd > 64 && plan.units <= sm_count() ? 64 : 128);
+// Whether tiles are faster than runs, us in runs / in tiles.  128 rows (tokens x heads of a group) of a sequence and kv head: bf16, 32 heads over 8 of 128, one sequence behind 1,000 tokens 20.9 / 24.8, behind
+// 4,000 28.1 / 28.5, behind 16,000 52.3 / 40.6 (how long contexts are is not known here), 4 behind 2,000 36.7 / 32.9, 16 95.5 / 46.1, 64 behind 1,000 197 / 135; f32 one behind 4,000 34.7 / 36.5, 16 135 / 73,
+// 64 275 / 203; heads of 64 one 21.7 / 21.9, 16 69.7 / 40.6.  64 rows, a block for each sequence and kv head, 16-bit types: 8 blocks 17.8 / 23.1, 25.8 / 26.4 and 38.4 / 38.6 (behind 1,000, 4,000, 16,000), 32
+// blocks 27.9 / 29.3 and 36.0 / 34.0, 128 56.4 / 45.6 and 57.4 / 48.0, 144 61.1 / 45.6, but 152, more than SMs, 64.0 / 87.1 and 512 112 / 114; f32 77 / 71 with 128 and 88 / 137 with 152; heads of 64 41.0 / 40.3
+// with 128.  32 rows: 39 / 48.
+bool tiles_pay(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group, int max_rows) {
+    const int64_t blocks = (int64_t)seqs.n_seqs * pool.n_kv;
+    const bool one_wave = blocks <= sm_count() && 2 * blocks >= sm_count();
+    return (int64_t)group * max_rows >= (typ != LC_TYPE_F32 && pool.hd > 64 && one_wave ? 64 : 128);
 }
 struct Plan {
     bool by_tiles;
@@ -481,7 +489,7 @@ Plan plan_call(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int group
     Plan p;
     int groups = run_groups(pool, group, max_rows);
     p.by_tiles = kv8_tiles_plan(pool, seqs, group, &p.tiles) && line_fits(pool, seqs, group, kTileRows2) &&
-                 (tiles_pay(pool, seqs, typ, group, max_rows, p.tiles) || !line_fits(pool, seqs, group, 8 * groups));
+                 (tiles_pay(pool, seqs, typ, group, max_rows) || !line_fits(pool, seqs, group, 8 * groups));
     while (!p.by_tiles && groups < most_groups(pool) && !line_fits(pool, seqs, group, 8 * groups)) groups *= 2;
     p.runs = plan_runs(pool, typ, groups);
     return p;

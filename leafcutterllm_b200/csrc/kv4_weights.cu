@@ -287,9 +287,9 @@ int32_t weights_full(const Kv4Pool& pool, const Kv8Seqs& seqs, const WeightArgs&
     if (a.typ == LC_TYPE_F32) return pool.hd == HD ? weights_as<HD, NG, true, true>(pool, seqs, a, s) : weights_as<HD, NG, true, false>(pool, seqs, a, s);
     return pool.hd == HD ? weights_as<HD, NG, false, true>(pool, seqs, a, s) : weights_as<HD, NG, false, false>(pool, seqs, a, s);
 }
-// Whether tiles are faster than runs, us in runs / in tiles, with so many stretches of 256 keys (as long as the tables are).  256 rows (tokens x heads of a group) of a sequence and kv head: always, bf16 214 / 157
-// with 2,048 stretches and 798 / 703 with 8,192, f32 351 / 330 and 1,329 / 1,379.  128 rows: bf16 28 / 12 with 128, 114 / 99 with 2,048, 388 / 450 with 8,192; f32 108 / 73 with 1,024, 312 / 396 with 4,096.  64
-// rows: bf16 17 / 12 with 128, 39 / 42 with 1,024, 59 / 85 with 2,048; f32 23 / 14 and 56 / 68.  32 rows: bf16 12 / 12 and 21 / 41.
+// Whether tiles are faster than runs, us in runs / in tiles, with so many stretches of 256 keys (as long as the tables are).  256 rows (tokens x heads of a group) of a sequence and kv head: always, bf16 41 / 17 with
+// 72 stretches, 211 / 122 with 2,048, 686 / 528 with 8,192, f32 62 / 20, 328 / 218, 1,120 / 1,028 and 2,131 / 2,008 with 16,384.  128 rows: bf16 28 / 12 with 128, 114 / 99 with 2,048, 388 / 450 with 8,192; f32
+// 108 / 73 with 1,024, 312 / 396 with 4,096.  64 rows: bf16 17 / 12 with 128, 39 / 42 with 1,024, 59 / 85 with 2,048; f32 23 / 14 and 56 / 68.  32 rows: bf16 12 / 12 and 21 / 41.
 bool tiles_pay(const Kv4Pool& pool, const Kv8Seqs& seqs, uint32_t typ, int64_t rows) {
     const int64_t stretches = (((int64_t)seqs.width << pool.page_shift) + 255) / 256 * seqs.n_seqs * pool.n_kv;
     const bool f32 = typ == LC_TYPE_F32;
