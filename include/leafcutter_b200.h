@@ -257,7 +257,7 @@ int32_t lc_attention_kv4_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows,
 /* Adds to mass_dev[i * mass_stride + h * mass_head_stride + slot] what weight the rows of sequence i gave the cached key of kv head h in `slot`: the sum over the rows and the heads of the
  * group of exp(q . k * scale - lse), with the lse that attention over the same rows gave (rows whose lse is not finite add nothing).  A sequence with more slots than `capacity`, which
  * is no more than either stride, is left out and raises the status, and so do sequences that leave their table; keys on bad pages are left out.  Sums are in f32, in an order that depends on the arguments and lengths
- * alone.  Sequences never share sums, whatever pages they share; sequences that share rows all count them.  Refused where the work, every context as long as its table, could not be counted in 31 bits:
+ * alone; a weight is off by its score's rounding, as in attention, and by 2^-22 of the lse's size (of itself).  Sequences never share sums, whatever pages they share; sequences that share rows all count them.  Refused where the work, every context as long as its table, could not be counted in 31 bits:
  * (n_rows * heads per kv head / 8 + n_seqs) * n_kv_heads * (positions of a table / 16 + 6). */
 int32_t lc_kv4_weights_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, uint32_t typ, int32_t n_rows, const void* q_dev, int64_t q_stride,
                            int32_t n_heads, float scale, int32_t window, const float* lse_dev, int64_t lse_stride, float* mass_dev,
@@ -266,7 +266,8 @@ int32_t lc_kv4_weights_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, u
  * largest mass (equal ones by the lower slot; NaN counts as the smallest).  They move to the front of the sequence's pages in their order, their sums in mass_dev with them; sums behind them become 0.  kept_dev
  * [n_seqs][n_kv_heads][limit] receives the slots that they came from, -1 behind them, and ctx_out_dev [n_seqs] the new lengths (shorter sequences: as they are).
  * first + recent <= keep <= limit <= capacity, keep > 0; n_seqs * n_kv_heads up to 65535; ctx_out_dev is not the rows' ctx_dev.  Pages of a sequence that is cut must be its own.  A sequence that leaves its table, has a bad page among those of its length or
- * is longer than `capacity` raises the status and stays as it is, -1 in kept_dev. */
+ * is longer than `capacity` raises the status and stays as it is, -1 in kept_dev.
+ * The call is sized by the smaller of `capacity` and the table's positions, so a capacity not far above `limit` and a call's rows is fastest. */
 int32_t lc_kv4_evict_dev(const lc_kv4_cache* cache, const lc_kv8_rows* rows, float* mass_dev, int64_t mass_stride, int64_t mass_head_stride,
                          int32_t capacity, int32_t keep, int32_t limit, int32_t recent, int32_t first, int32_t* kept_dev, int32_t* ctx_out_dev,
                          void* stream);

@@ -10,7 +10,7 @@
 // Dims of a score and keys of a sum may stand in any order, so a thread takes neighbouring dims of its key, whose scale they share, and two keys' dims become pairs by one byte permutation for eight of them.
 //
 // Why 11 bits are enough for 16-bit types' weights: each is off by up to 2^-11 of itself, either way, and an output is a mean over many keys.  Against 64 bits, and with weights of 32 bits: bf16 1.7e-3 and 1.7e-3,
-// f16 2.5e-4 and 2.0e-4, most of it the outputs' own rounding.  A second product for the low parts, as f32 has it, would double the products with the values.
+// f16 2.7e-4 and 2.1e-4, most of it the outputs' own rounding.  A second product for the low parts, as f32 has it, would double the products with the values.
 //
 // 64 sequences of 128 to 4,096 slots, 32 heads over 8 of 128 in bf16: 37 us with the join, 87 MB (a floor of 13).  What bounds it are instructions: 360 a step of 16 keys, of which the matrix unit's are 16; 50 % of the
 // issue slots at 12 warps an SM (153 registers), the rest is the beginning and the end of runs of 20 steps.  Three blocks an SM for up to 8 rows; four (128 registers) take longer, 38.5 us, 42.7 instead of 41.1 in f32, 98 instead of 94 with

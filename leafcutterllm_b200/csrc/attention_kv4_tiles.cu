@@ -15,8 +15,9 @@
 // Every byte of the cache is a finite number, so keys that no row sees may be anything: their weights are 0.
 //
 // Three sequences of 700 to 2,048 rows behind 1,000 to 6,100 slots, 32 heads over 8 of 128 in bf16: 366 us, 315 GFLOP at 860 TFLOP/s (192 us at the rate of library products).  What bounds it, for 256 rows x 128 keys in 4,440
-// cycles: the unpacking warps work 3,600 of them; a row tile's softmax is 2,200 of its chain; 32 products of 62 cycles each are 2,190 and wait 800 for keys and 1,080 for weights.
+// cycles: the unpacking warps work 3,600 of them; a row tile's softmax is 2,200 of its chain; issuing 32 products is 2,190 (68 each with their commits; the matrix unit runs one in 62), which waits 800 for keys and 1,080 for weights.
 // An issue of 50 cycles a product matters (one elected lane, descriptors of 32 changing bits: 105 to 155 before, 410 us), as do two places for keys and work of unpacking that is even over its warps (379).
+// Weights of 11 bits for 16-bit types: as in attention_kv4.cu, where the reason stands.
 #include <algorithm>
 #include "lc_attn_tiles.cuh"
 #include "lc_kernels.h"

@@ -16,7 +16,7 @@
 //   16-bit types    O stays in tensor memory for all keys (the same error is a hundredth of the outputs' rounding), and so that it rarely
 //                   has to be scaled again, M is raised only when a row's largest exponent has grown by more than 8.
 //
-// What bounds it (a pair of row tiles x 128 keys, head dim 128): products 2,048 cycles (f32: 4,096), exponentials 2,048 on the special-function unit, and 320 KB through
+// What bounds it (a pair of row tiles x 128 keys, head dim 128): products 1,980 cycles (32 of 62; f32: 3,970), exponentials 2,048 on the special-function unit, and 320 KB through
 // shared memory, 2,500 cycles (128 of queries and keys, 64 of values for the products, 128 of copies and unpacking); about 3,900 pass, as a row tile's softmax, its sums
 // and its next scores wait for one another.  Steps of 64 keys, whose scores are under way while the 64 before are weighted, took 571 us instead of 412 (three chunks of 700 - 2,048 tokens behind 1,000 - 6,100, 32 heads over 8, bf16): products half
 // as wide read the queries twice.

@@ -4,9 +4,10 @@
 // f32 decides them wherever its error bounds allow; a block with a number or a scale too near a border between two, with infinities, NaN or sizes beyond f32's relative errors is done again in 64 bits.
 // A thread has the 16 dims of one block and loads the 16 that they are paired with, so rows pass once.
 //
-// 4,970 rows of five sequences, 32 heads over 8 of 128 in bf16: append 29 us (107 MB), read back 12 (26 MB); first kernels 57 together.  What bounds the append is its instructions, 3,500 a row: 60 % of
+// 4,970 rows of five sequences, 32 heads over 8 of 128 in bf16: append 27 us (107 MB), read back 9.2 (26 MB); first kernels 57 together.  What bounds the append is its instructions, 3,500 a row: 60 % of
 // the issue slots, three blocks on an SM for 80 registers, the last wave of blocks half full; keys and values are a block's own work beside the queries' blocks (one block for both: 45).  Read: latency, four blocks of 16 dims
-// a thread under way.  64 sequences of one row, 32 kv heads in f32: both in 14 us, the chain row range -> context -> table -> row of two launches.
+// a thread under way.  64 sequences of one row, 32 kv heads in f32: 7.9 and 4.6 us, 12.4 together, in each the chain row range -> context -> table -> row.
+// Blocks of zeros are answered at once (every eighth row of zeros took 184 us when they went the 64-bit way); a block beyond 448 x 7 times its head's scale still goes it.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>

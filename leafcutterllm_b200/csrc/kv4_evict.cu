@@ -5,9 +5,12 @@
 // places, a cluster per sequence, kv head and plane (keys, values, their scales).  The row that goes to slot j comes from kept[j] >= j, so a stretch of rows is read as a whole, by all threads of the
 // cluster into registers, before it is written, in ascending order, and what a stretch writes is behind no row that a later one still reads.
 //
-// 64 sequences and 8 kv heads of 128 cut to 1,024 slots where they have more than 1,280: 27 us, 56 MB (a floor of 8.5); two of them cut to 16,384: 68 us, 85 MB (12.9).  What bounds it is a chain of waits: the sums, three rounds
-// of digits in clusters of 8 (a count of 1,700 to 3,200 cycles, a barrier, other blocks' counts, a scan), the list, a launch, kept slot -> page -> row.  Of the second kernel's shapes four pieces a thread and three blocks on an SM are the best with L2 cold, 39 and 72 us (eight and
-// two: 41 and 72; two and three: 43 and 78).  First kernels, a block for a sequence and head over sums in global memory: 80 and 612.
+// 64 sequences and 8 kv heads of 128 cut to 1,024 slots where they have more than 1,280, a first eviction with L2 cold: 36 us, 56 MB (a floor of 8.5); two of them cut to 16,384: 70 us, 85 MB (12.9; an empty kernel reads
+// 9 the same way).  What bounds it is a chain of waits: the sums, three rounds of digits in clusters of 8 (a count of 1,700 to 3,200 cycles, a barrier, other blocks' counts, a scan), the list, a launch, kept slot ->
+// page -> row.  Cut again as they are, so that an eighth and a thirtieth of the rows move, replayed: 26 and 66 us; none above the limit: 9.  Of the second kernel's shapes four pieces a thread and three blocks on an SM
+// are the best, 36 and 70 us (eight and two: 40 and 73; two and three: 40 and 73).  First kernels, a block for a sequence and head over sums in global memory: 80 and 612, replayed.
+// Blocks are sized by what sequences may hold, the smaller of the tables' length and the sums' capacity, not by the contexts, which only the device knows: in tables of 131,072 slots the 64 sequences take 209 us (blocks of 16,384 sums, of which one in eight has any), in tables beyond
+// clusters, of 524,288, 63.  One sequence of 500,000 slots cut to 65,536, a block for each head: 1,640.
 #include <cooperative_groups.h>
 #include <algorithm>
 #include "lc_kernels.h"

@@ -5,7 +5,7 @@
 // exchanged between threads, and a sum is in the order of the rows.  Two blocks on an SM take turns on the matrix unit.
 //
 // 64 rows of three sequences of 3,000 to 16,000 slots, 32 heads over 8 of 128 in f16: 51 us, 13.6 GFLOP (8.3 us at the rate of library products; by runs 123).  What bounds it are instructions, and a block's phases one
-// after the other: keys to values 4,400 cycles once, then for 128 rows their conversion 3,000, the products 1,900 (of the unit, 1,024) and 32,768 exponentials with their sums 2,300 to 2,700 (of the unit, 2,048).
+// after the other: keys to values 4,400 cycles once, then for 128 rows their conversion 3,000, the products 1,900 (of the unit, 990: 16 of 62) and 32,768 exponentials with their sums 2,300 to 2,700 (of the unit, 2,048).
 // Bringing the next stretch into L2 early gained nothing.
 #include <algorithm>
 #include <type_traits>

@@ -355,7 +355,7 @@ class Kv4Cache:
 
     def attention(self, rows: Kv8Rows, q, out=None, lse=None, scale: float = None, window: int = 0, workspace=None, stream=None):
         """Attention of q [rows, heads, head_dim], already turned, over the cache: each row attends to the slots up to its own (with window > 0 to the last
-        `window` of them), which the cache already holds.  scale None: 1 / sqrt(head_dim).  Returns out.  lse: float32 [rows, heads], which receives ln sum exp of the scores.  workspace: a uint8 tensor of
+        `window` of them), which the cache already holds.  scale None (or 0): 1 / sqrt(head_dim).  Returns out.  lse: float32 [rows, heads], which receives ln sum exp of the scores.  workspace: a uint8 tensor of
         attention_workspace bytes (None: a new one); calls that may run at the same time need one each."""
         typ, index = _typ(q), self.index
         qs = _rows(q, None, self.head_dim, "q")
@@ -401,7 +401,7 @@ class Kv4Cache:
     def evict(self, rows: Kv8Rows, mass, keep: int, limit: int = None, recent: int = 0, first: int = 0, kept=None, ctx_out=None, stream=None):
         """Cuts sequences that hold more than `limit` rows (None: keep), their context and the call's rows, to `keep`: for each kv head the `first` first, the `recent` last and the heaviest between
         move to the front, in their order, and their sums in mass with them.  Returns (kept int32 [n_seqs, kv heads, limit], the slots that they came from, -1 behind them; ctx_out int32 [n_seqs], the new
-        lengths).  The pages of a sequence that is cut must be its own."""
+        lengths).  The pages of a sequence that is cut must be its own.  Fastest where mass's capacity is not far above limit and a call's rows."""
         torch, index, n = _torch(), self.index, rows.struct.n_seqs
         limit = keep if limit is None else limit
         mp, ms, mh, cap = self._mass("evict", rows, mass)
